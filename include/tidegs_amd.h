@@ -13,7 +13,8 @@
  *     negative TGS_ERR_* code for an argument error; tgs_last_error() then
  *     describes it (the reference raises through TORCH_CHECK / AT_ERROR,
  *     bindings.h:7-13).
- *   - Floating point is fp32 throughout.
+ *   - Floating point is fp32 throughout; the decoder operators also take
+ *     bfloat16 and half tensors (and compute in fp32).
  */
 #ifndef TIDEGS_AMD_H
 #define TIDEGS_AMD_H
@@ -793,6 +794,61 @@ int tgs_cull_blocks(const float* centers, const float* radii, const int64_t* blo
 int tgs_cull_blocks_cone(const float* centers, uint32_t nb, double cam_x, double cam_y,
                          double cam_z, double fwd_x, double fwd_y, double fwd_z,
                          double threshold, uint8_t* visible, tgs_stream_t stream);
+
+/* ---- decoder operators -------------------------------------------------- */
+/* The parts of a network over per-Gaussian features.  dtype: the tensors'
+ * element type; every sum is taken in 32 bits or more and a result rounded to
+ * nearest even where it is stored.  Matrices are row-major; a pitch is the
+ * distance of two rows in values.  Sums over rows are joined in a fixed order:
+ * the same call gives the same bits. */
+#define TGS_F32 0
+#define TGS_BF16 1
+#define TGS_F16 2
+
+/* Layer norm over the last dimension of x [rows, width]:
+ * y = (x - mean) / sqrt(var + eps) * weight + bias, y [rows, width] dense.
+ * weight and bias [width] are nullable (1 and 0) and of type weight_dtype: x's or
+ * TGS_F32. */
+int tgs_layer_norm_fwd(uint64_t rows, uint32_t width, int32_t dtype, const void* x,
+                       int64_t x_pitch, const void* weight, const void* bias,
+                       int32_t weight_dtype, float eps, void* y, tgs_stream_t stream);
+/* Its gradients, each nullable: dx [rows, width] dense, dweight and dbias [width] of
+ * weight_dtype.  Mean and variance are computed again from x.  The workspace is
+ * needed for dweight or dbias. */
+uint64_t tgs_layer_norm_bwd_workspace_size(uint64_t rows, uint32_t width);
+int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, const void* x,
+                       int64_t x_pitch, const void* dy, int64_t dy_pitch, const void* weight,
+                       int32_t weight_dtype, float eps, void* dx, void* dweight, void* dbias,
+                       void* workspace, uint64_t workspace_bytes, tgs_stream_t stream);
+
+/* Dropout: y[i] = (draw[i] >= threshold ? x[i] * 65536 / (65536 - threshold) : 0)
+ * + residual[i] (nullable), threshold <= 65536 in 65536ths.  draw[i]: 16 bits of
+ * Philox4x32-10 with key `seed` and counter (i >> 3, offset), word (i & 7) >> 1, low
+ * half first.  The gradient is the same call on dy without a residual. */
+int tgs_dropout(uint64_t n, int32_t dtype, const void* x, const void* residual, void* y,
+                uint32_t threshold, uint64_t seed, uint64_t offset, tgs_stream_t stream);
+
+/* Gated feed-forward block: y = h Wd' + bd, h = act(x Wg' + bg) * (x Wu' + bu);
+ * x [rows, width], w_gate and w_up [hidden, width], w_down [out, hidden], biases
+ * (each nullable) [hidden], [hidden], [out], y [rows, out] dense, all of `dtype`.
+ * activation: 0 silu, 1 gelu (with the error function), 2 relu. */
+uint64_t tgs_gated_ffn_fwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
+                                          uint32_t out, int32_t dtype);
+int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out, int32_t dtype,
+                      int32_t activation, const void* x, int64_t x_pitch, const void* w_gate,
+                      const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                      const void* b_down, void* y, void* workspace, uint64_t workspace_bytes,
+                      tgs_stream_t stream);
+/* Its gradients, each nullable, of the shapes of what they are gradients of (dx
+ * dense).  g = x Wg' + bg and u = x Wu' + bu are computed again. */
+uint64_t tgs_gated_ffn_bwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
+                                          uint32_t out, int32_t dtype);
+int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out, int32_t dtype,
+                      int32_t activation, const void* x, int64_t x_pitch, const void* w_gate,
+                      const void* w_up, const void* w_down, const void* b_gate, const void* b_up,
+                      const void* dy, int64_t dy_pitch, void* dx, void* dw_gate, void* dw_up,
+                      void* dw_down, void* db_gate, void* db_up, void* db_down, void* workspace,
+                      uint64_t workspace_bytes, tgs_stream_t stream);
 
 /* ---- on-disk block store (host code, no GPU) ------------------------------ */
 /* Parallel reads of n blocks of the base/patch files (replaces the per-block

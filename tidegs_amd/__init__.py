@@ -11,6 +11,9 @@ Drop-in surfaces (same names and call conventions as the reference):
 * ``ResidentWorkingSet``: GPU materialization and writeback of the resident
   block set (the Triton movers of TideGS's double-buffered working set)
 
+Beside them, for decoders over per-Gaussian features: ``layer_norm``, ``dropout``
+and ``gated_ffn`` (``decoder_ops``).
+
 All compute runs in hand-written HIP kernels in ``libtidegs_amd.so`` behind a
 plain C ABI (``include/tidegs_amd.h``); PyTorch only provides device memory and
 streams.
@@ -24,6 +27,7 @@ from .gsplat_ops import (
     spherical_harmonics,
 )
 from .clm_ops import FusedSSIMMap, fused_ssim
+from .decoder_ops import dropout, gated_ffn, layer_norm
 from .resident_optim import GPUResidentAdam, GPUResidentSophia
 from .working_set import BlockLayout, ResidentBuffer, ResidentWorkingSet
 
@@ -41,4 +45,7 @@ __all__ = [
     "ResidentWorkingSet",
     "ResidentBuffer",
     "BlockLayout",
+    "layer_norm",
+    "dropout",
+    "gated_ffn",
 ]

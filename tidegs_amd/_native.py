@@ -207,6 +207,20 @@ SIGNATURES = {
     "tgs_ws_block_bounds": (ctypes.c_int, [P, U32, P, P, U32, U32, P, P]),
     "tgs_ws_build_block_starts": (ctypes.c_int, [P, P, U32, P, U32, P]),
     "tgs_ws_global_to_local": (ctypes.c_int, [P, U64, P, U32, U32, P, P]),
+    "tgs_layer_norm_fwd": (ctypes.c_int, [U64, U32, I32, P, I64, P, P, I32, F32, P, P]),
+    "tgs_layer_norm_bwd_workspace_size": (U64, [U64, U32]),
+    "tgs_layer_norm_bwd": (
+        ctypes.c_int, [U64, U32, I32, P, I64, P, I64, P, I32, F32, P, P, P, P, U64, P]),
+    "tgs_dropout": (ctypes.c_int, [U64, I32, P, P, P, U32, U64, U64, P]),
+    "tgs_gated_ffn_fwd_workspace_size": (U64, [U64, U32, U32, U32, I32]),
+    "tgs_gated_ffn_fwd": (
+        ctypes.c_int,
+        [U64, U32, U32, U32, I32, I32, P, I64, P, P, P, P, P, P, P, P, U64, P]),
+    "tgs_gated_ffn_bwd_workspace_size": (U64, [U64, U32, U32, U32, I32]),
+    "tgs_gated_ffn_bwd": (
+        ctypes.c_int,
+        [U64, U32, U32, U32, I32, I32, P, I64, P, P, P, P, P, P, I64, P, P, P, P, P, P, P, P, U64,
+         P]),
     "tgs_io_read_blocks": (ctypes.c_int, [U32, P, P, P, P, P, U32]),
     "tgs_init_scene_bounds": (ctypes.c_int, [P, U64, P, P, P]),
     "tgs_init_morton_codes": (ctypes.c_int, [P, U64, P, P, P]),

@@ -1,0 +1,403 @@
+// Layer norm over the last dimension, forward and backward.
+//
+//   mean = sum x / n, rstd = 1 / sqrt(sum (x - mean)^2 / n + eps), xhat = (x - mean) rstd
+//   y = xhat w + b
+//   with g = dy w:  dx = rstd (g - mean(g) - xhat mean(g xhat)),
+//                   dw = sum_rows dy xhat, db = sum_rows dy
+//
+// Memory bound.  A row is read once: 8 to 64 lanes hold it in registers (the variance
+// is the second pass over them, not a difference of moments) and the backward computes
+// mean and rstd again from the x it reads anyway, so nothing is kept between the two.
+// The weight's gradient is a sum over rows: every lane adds up its columns over the
+// rows of its wavefront, the workgroup joins its wavefronts through LDS into one
+// partial row, and a second launch adds the partial rows, all in a fixed order.
+#include "decoder_common.cuh"
+
+// How LANES lanes hold a row of up to LANES * E values.  VEC: lane l has runs of 16
+// bytes, the runs of one load next to each other (every row 16-byte aligned and a
+// whole number of runs); otherwise values l, l + LANES, ...
+template <typename T, int LANES, int E, bool VEC>
+struct RowMap {
+  static constexpr int R = VEC ? Vec16<T>::N : 1;  // values of a run
+  static_assert(E % R == 0, "whole runs");
+  __device__ static __forceinline__ int column(int lane, int e) {
+    return (e / R * LANES + lane) * R + e % R;
+  }
+  __device__ static __forceinline__ void load(const T* row, int lane, uint32_t n, float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e += R) {
+      const uint32_t c = column(lane, e);
+      if constexpr (VEC) {
+        Vec16<T> t = {};
+        if (c < n) t = *(const Vec16<T>*)(row + c);
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[e + k] = to_f32(t.v[k]);
+      } else {
+        v[e] = c < n ? to_f32(row[c]) : 0.f;
+      }
+    }
+  }
+  __device__ static __forceinline__ void store(T* row, int lane, uint32_t n, const float (&v)[E]) {
+#pragma unroll
+    for (int e = 0; e < E; e += R) {
+      const uint32_t c = column(lane, e);
+      if (c >= n) continue;
+      if constexpr (VEC) {
+        Vec16<T> t;
+#pragma unroll
+        for (int k = 0; k < R; ++k) t.v[k] = from_f32<T>(v[e + k]);
+        *(Vec16<T>*)(row + c) = t;
+      } else {
+        row[c] = from_f32<T>(v[e]);
+      }
+    }
+  }
+};
+
+template <int LANES>
+__device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int off = 1; off < LANES; off <<= 1) v += __shfl_xor(v, off, 64);
+  return v;
+}
+
+// x becomes xhat; returns rstd.  Lanes past the row's end hold zeros.
+template <typename Map, int LANES, int E>
+__device__ __forceinline__ float normalise(float (&x)[E], int lane, uint32_t n, float eps) {
+  float s = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) s += x[e];
+  const float mean = group_sum<LANES>(s) / (float)n;
+  float q = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    x[e] = (uint32_t)Map::column(lane, e) < n ? x[e] - mean : 0.f;
+    q = fmaf(x[e], x[e], q);
+  }
+  const float rstd = 1.f / sqrtf(group_sum<LANES>(q) / (float)n + eps);
+#pragma unroll
+  for (int e = 0; e < E; ++e) x[e] *= rstd;
+  return rstd;
+}
+
+// The weight's or bias's values of this lane's columns; `other` where there are none.
+template <typename Map, typename W, int E>
+__device__ __forceinline__ void load_columns(const W* w, int lane, uint32_t n, float other,
+                                             float (&v)[E]) {
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const uint32_t c = Map::column(lane, e);
+    v[e] = w && c < n ? to_f32(w[c]) : other;
+  }
+}
+
+template <typename T, typename W, int LANES, int E, bool VEC>
+__global__ void __launch_bounds__(256) layer_norm_fwd_kernel(
+    uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const W* __restrict__ weight,
+    const W* __restrict__ bias, float eps, T* __restrict__ y) {
+  using Map = RowMap<T, LANES, E, VEC>;
+  constexpr int PER = 256 / LANES;  // rows of a workgroup at once
+  const int lane = threadIdx.x % LANES;
+  float w[E], b[E];
+  load_columns<Map>(weight, lane, n, 1.f, w);
+  load_columns<Map>(bias, lane, n, 0.f, b);
+  // (the shuffles stay inside the lanes of one row, so a wavefront whose last rows
+  // are missing needs no barrier)
+  for (uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES; r < rows;
+       r += (uint64_t)gridDim.x * PER) {
+    float v[E];
+    Map::load(x + (int64_t)r * pitch, lane, n, v);
+    normalise<Map, LANES, E>(v, lane, n, eps);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = fmaf(v[e], w[e], b[e]);
+    Map::store(y + r * n, lane, n, v);
+  }
+}
+
+template <typename T, typename W, int LANES, int E, bool VEC>
+__global__ void __launch_bounds__(256) layer_norm_bwd_kernel(
+    uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const T* __restrict__ dy,
+    int64_t dy_pitch, const W* __restrict__ weight, float eps, T* __restrict__ dx,
+    float* __restrict__ partial) {
+  using Map = RowMap<T, LANES, E, VEC>;
+  constexpr int PER = 256 / LANES;
+  __shared__ float s_part[2][LANES * E];
+  const int lane = threadIdx.x % LANES;
+  float w[E], dw[E] = {}, db[E] = {};
+  load_columns<Map>(weight, lane, n, 1.f, w);
+  for (uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES; r < rows;
+       r += (uint64_t)gridDim.x * PER) {
+    float v[E], g[E];
+    Map::load(x + (int64_t)r * pitch, lane, n, v);
+    Map::load(dy + (int64_t)r * dy_pitch, lane, n, g);
+    const float rstd = normalise<Map, LANES, E>(v, lane, n, eps);
+    float s = 0.f, q = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      dw[e] = fmaf(g[e], v[e], dw[e]);
+      db[e] += g[e];
+      g[e] *= w[e];
+      s += g[e];
+      q = fmaf(g[e], v[e], q);
+    }
+    if (dx) {
+      s = group_sum<LANES>(s) / (float)n;
+      q = group_sum<LANES>(q) / (float)n;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = rstd * (g[e] - s - v[e] * q);
+      Map::store(dx + r * n, lane, n, v);
+    }
+  }
+  if (!partial) return;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int off = LANES; off < 64; off <<= 1) {
+      dw[e] += __shfl_xor(dw[e], off, 64);
+      db[e] += __shfl_xor(db[e], off, 64);
+    }
+  for (uint32_t wave = 0; wave < 4; ++wave) {
+    if (threadIdx.x / 64 == wave && threadIdx.x % 64 < LANES) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int c = Map::column(lane, e);
+        s_part[0][c] = wave ? s_part[0][c] + dw[e] : dw[e];
+        s_part[1][c] = wave ? s_part[1][c] + db[e] : db[e];
+      }
+    }
+    __syncthreads();
+  }
+  for (uint32_t i = threadIdx.x; i < 2 * n; i += 256)
+    partial[(uint64_t)blockIdx.x * 2 * n + i] = i < n ? s_part[0][i] : s_part[1][i - n];
+}
+
+// A row of any width, one workgroup per row, read again for each of its sums (rows
+// that 64 lanes do not hold in registers: 4096 values).
+__device__ __forceinline__ float block_sum(float v, float* s) {
+  v = tgs_wave_sum(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return (s[0] + s[1]) + (s[2] + s[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ void row_stats(const T* x, uint32_t n, float eps, float* s, float& mean,
+                                          float& rstd) {
+  float a = 0.f;
+  for (uint32_t c = threadIdx.x; c < n; c += 256) a += to_f32(x[c]);
+  mean = block_sum(a, s) / (float)n;
+  a = 0.f;
+  for (uint32_t c = threadIdx.x; c < n; c += 256) {
+    const float d = to_f32(x[c]) - mean;
+    a = fmaf(d, d, a);
+  }
+  rstd = 1.f / sqrtf(block_sum(a, s) / (float)n + eps);
+}
+
+template <typename T, typename W>
+__global__ void __launch_bounds__(256) layer_norm_fwd_wide_kernel(
+    uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const W* __restrict__ weight,
+    const W* __restrict__ bias, float eps, T* __restrict__ y) {
+  __shared__ float s[4];
+  for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* row = x + (int64_t)r * pitch;
+    float mean, rstd;
+    row_stats(row, n, eps, s, mean, rstd);
+    for (uint32_t c = threadIdx.x; c < n; c += 256)
+      y[r * n + c] = from_f32<T>(fmaf((to_f32(row[c]) - mean) * rstd,
+                                      weight ? to_f32(weight[c]) : 1.f,
+                                      bias ? to_f32(bias[c]) : 0.f));
+  }
+}
+
+// The workgroup's partial row is its own in memory: thread t adds to columns t, t + 256, ...
+template <typename T, typename W>
+__global__ void __launch_bounds__(256) layer_norm_bwd_wide_kernel(
+    uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const T* __restrict__ dy,
+    int64_t dy_pitch, const W* __restrict__ weight, float eps, T* __restrict__ dx,
+    float* __restrict__ partial) {
+  __shared__ float s[4];
+  float* dw = partial ? partial + (uint64_t)blockIdx.x * 2 * n : nullptr;
+  if (dw)
+    for (uint32_t c = threadIdx.x; c < n; c += 256) dw[c] = dw[n + c] = 0.f;
+  for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
+    const T* row = x + (int64_t)r * pitch;
+    const T* grad = dy + (int64_t)r * dy_pitch;
+    float mean, rstd, a = 0.f, q = 0.f;
+    row_stats(row, n, eps, s, mean, rstd);
+    for (uint32_t c = threadIdx.x; c < n; c += 256) {
+      const float d = to_f32(grad[c]), xh = (to_f32(row[c]) - mean) * rstd;
+      if (dw) {
+        dw[c] = fmaf(d, xh, dw[c]);
+        dw[n + c] += d;
+      }
+      const float g = d * (weight ? to_f32(weight[c]) : 1.f);
+      a += g;
+      q = fmaf(g, xh, q);
+    }
+    a = block_sum(a, s) / (float)n;
+    q = block_sum(q, s) / (float)n;
+    if (!dx) continue;
+    for (uint32_t c = threadIdx.x; c < n; c += 256) {
+      const float g = to_f32(grad[c]) * (weight ? to_f32(weight[c]) : 1.f);
+      dx[r * n + c] = from_f32<T>(rstd * (g - a - (to_f32(row[c]) - mean) * rstd * q));
+    }
+  }
+}
+
+// dw and db: the partial rows' sums, 32 columns by 32 interleaved runs of rows.
+template <typename W>
+__global__ void __launch_bounds__(1024) layer_norm_join_kernel(uint32_t parts, uint32_t n,
+                                                               const float* __restrict__ partial,
+                                                               W* __restrict__ dweight,
+                                                               W* __restrict__ dbias) {
+  __shared__ float s[32][33];
+  const uint32_t c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
+  float a = 0.f;
+  if (c < 2 * n)
+    for (uint32_t p = k; p < parts; p += 32) a += partial[(uint64_t)p * 2 * n + c];
+  s[k][threadIdx.x % 32] = a;
+  __syncthreads();
+  for (uint32_t h = 16; h > 0; h >>= 1) {
+    if (k < h) s[k][threadIdx.x % 32] += s[k + h][threadIdx.x % 32];
+    __syncthreads();
+  }
+  if (k == 0 && c < 2 * n) {
+    W* out = c < n ? dweight : dbias;
+    if (out) out[c < n ? c : c - n] = from_f32<W>(s[0][threadIdx.x % 32]);
+  }
+}
+
+#define LN_MAX_HELD 4096  // values of a row that 64 lanes hold in registers
+
+// Workgroups of a launch: enough to fill the chip, few enough that a workgroup's rows
+// pay for its loads of the weights.
+static uint32_t norm_groups(uint64_t rows) {
+  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>((rows + 3) / 4, 1), 2048);
+}
+
+// Calls f(LANES, E) as constants: the fewest lanes that hold n values.
+template <typename T, bool VEC, typename F>
+static void with_row_map(uint32_t n, F&& f) {
+  constexpr int R = VEC ? Vec16<T>::N : 1;
+#define LN_MAP(LANES, E) \
+  if (n <= (LANES) * (E)) return f(std::integral_constant<int, LANES>(), std::integral_constant<int, E>())
+  if constexpr (R > 1) {
+    LN_MAP(8, R);
+    LN_MAP(16, R);
+    LN_MAP(32, R);
+  }
+  if constexpr (R < 2) {
+    LN_MAP(16, 1);
+    LN_MAP(64, 1);
+    LN_MAP(64, 2);
+  }
+  if constexpr (R < 8) LN_MAP(64, 4);
+  LN_MAP(64, 8);
+  LN_MAP(64, 16);
+  LN_MAP(64, 32);
+  LN_MAP(64, 64);
+#undef LN_MAP
+}
+
+extern "C" int tgs_layer_norm_fwd(uint64_t rows, uint32_t width, int32_t dtype, const void* x,
+                                  int64_t x_pitch, const void* weight, const void* bias,
+                                  int32_t weight_dtype, float eps, void* y, hipStream_t stream) {
+  return with_dtype(dtype, "tgs_layer_norm_fwd", [&](auto tag) -> int {
+    using T = decltype(tag);
+    TGS_CHECK_ARG(width > 0 && width <= (1u << 30), "tgs_layer_norm_fwd: width %u", width);
+    TGS_CHECK_ARG(weight_dtype == dtype || weight_dtype == TGS_F32,
+                  "tgs_layer_norm_fwd: the weights have x's type or float32");
+    if (rows == 0) return TGS_OK;
+    TGS_CHECK_ARG(x && y, "tgs_layer_norm_fwd: null pointer");
+    TGS_CHECK_ARG(x_pitch >= (int64_t)width || rows == 1, "tgs_layer_norm_fwd: pitch below width");
+    const auto typed = [&](auto wtag) {
+      using W = decltype(wtag);
+      const auto launch = [&](auto kernel, uint64_t groups) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(256), 0, stream, rows, width,
+                           (const T*)x, x_pitch, (const W*)weight, (const W*)bias, eps, (T*)y);
+      };
+      const auto held = [&](auto vec) {
+        with_row_map<T, vec.value>(width, [&](auto lanes, auto e) {
+          const uint64_t per = 256 / lanes.value;
+          launch(layer_norm_fwd_kernel<T, W, lanes.value, e.value, vec.value>,
+                 std::min<uint64_t>((rows + per - 1) / per, 2048));
+        });
+      };
+      if (width > LN_MAX_HELD)
+        launch(layer_norm_fwd_wide_kernel<T, W>, norm_groups(rows));
+      else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
+               aligned16((const T*)y, width))
+        held(std::true_type());
+      else
+        held(std::false_type());
+    };
+    if (weight_dtype == dtype)
+      typed(T{});
+    else
+      typed(float{});
+    TGS_RETURN_LAUNCH("tgs_layer_norm_fwd");
+  });
+}
+
+extern "C" uint64_t tgs_layer_norm_bwd_workspace_size(uint64_t rows, uint32_t width) {
+  return (uint64_t)norm_groups(rows) * 2 * width * sizeof(float);
+}
+
+extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, const void* x,
+                                  int64_t x_pitch, const void* dy, int64_t dy_pitch,
+                                  const void* weight, int32_t weight_dtype, float eps, void* dx,
+                                  void* dweight, void* dbias, void* workspace,
+                                  uint64_t workspace_bytes, hipStream_t stream) {
+  return with_dtype(dtype, "tgs_layer_norm_bwd", [&](auto tag) -> int {
+    using T = decltype(tag);
+    TGS_CHECK_ARG(width > 0 && width <= (1u << 30), "tgs_layer_norm_bwd: width %u", width);
+    TGS_CHECK_ARG(weight_dtype == dtype || weight_dtype == TGS_F32,
+                  "tgs_layer_norm_bwd: the weights have x's type or float32");
+    const bool sums = dweight || dbias;
+    TGS_CHECK_ARG(rows == 0 || (x && dy), "tgs_layer_norm_bwd: null pointer");
+    TGS_CHECK_ARG((x_pitch >= (int64_t)width && dy_pitch >= (int64_t)width) || rows <= 1,
+                  "tgs_layer_norm_bwd: pitch below width");
+    const uint32_t groups = rows ? norm_groups(rows) : 0;
+    if (sums && workspace_bytes < tgs_layer_norm_bwd_workspace_size(rows, width)) {
+      tgs_set_error("tgs_layer_norm_bwd: workspace too small");
+      return TGS_ERR_WORKSPACE;
+    }
+    TGS_CHECK_ARG(!sums || workspace, "tgs_layer_norm_bwd: null workspace");
+    if (!sums && (!dx || rows == 0)) return TGS_OK;
+    float* partial = sums ? (float*)workspace : nullptr;
+    const auto typed = [&](auto wtag) {
+      using W = decltype(wtag);
+      const auto launch = [&](auto kernel, uint32_t g) {
+        hipLaunchKernelGGL(kernel, dim3(g), dim3(256), 0, stream, rows, width, (const T*)x,
+                           x_pitch, (const T*)dy, dy_pitch, (const W*)weight, eps, (T*)dx, partial);
+      };
+      uint32_t parts = groups;
+      const auto held = [&](auto vec) {
+        with_row_map<T, vec.value>(width, [&](auto lanes, auto e) {
+          const uint64_t per = 256 / lanes.value;
+          parts = (uint32_t)std::min<uint64_t>((rows + per - 1) / per, groups);
+          launch(layer_norm_bwd_kernel<T, W, lanes.value, e.value, vec.value>, parts);
+        });
+      };
+      if (rows) {
+        if (width > LN_MAX_HELD)
+          launch(layer_norm_bwd_wide_kernel<T, W>, groups);
+        else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
+                 aligned16((const T*)dy, dy_pitch) && (!dx || aligned16((const T*)dx, width)))
+          held(std::true_type());
+        else
+          held(std::false_type());
+      }
+      if (sums)
+        hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((2 * width + 31) / 32), dim3(1024), 0,
+                           stream, parts, width, partial, (W*)dweight, (W*)dbias);
+    };
+    if (weight_dtype == dtype)
+      typed(T{});
+    else
+      typed(float{});
+    TGS_RETURN_LAUNCH("tgs_layer_norm_bwd");
+  });
+}
