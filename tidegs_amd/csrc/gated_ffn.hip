@@ -6,7 +6,7 @@
 //
 // x [rows, width], Wg and Wu [hidden, width], Wd [out, hidden], row-major (x and dy at
 // a pitch).  The backward computes g and u again.
-#include "decoder_common.cuh"
+#include "matrix.cuh"
 
 enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
 
@@ -21,86 +21,331 @@ __device__ __forceinline__ float2 activation(int act, float g) {
   return make_float2(g * phi, phi + g * 0.39894228040143268f * expf(-0.5f * g * g));
 }
 
-// A matrix by its strides, of the call's element type or of 32-bit values.
-struct Mat {
-  const void* p;
-  int64_t row, col;  // strides (values)
-  int wide;          // 32-bit values whatever the call's type
+// ---------------------------------------------------------------------------
+// Operands that the products cannot read where they lie (32-bit values, rows that do
+// not start on 16 bytes, widths that are no multiple of 8) are laid out as planes
+// with rows of a whole number of chunks, zeros behind the last value.
+// ---------------------------------------------------------------------------
+
+struct LayJob {
+  const void* src;
+  void* dst;
+  int64_t rows, pitch, plane;  // plane: values between two planes of dst
+  uint32_t cols, cols8;
+  uint32_t blocks;  // of the launch, up to and with this job's
+};
+#define LAY_JOBS 5
+struct LayJobs {
+  LayJob job[LAY_JOBS];
 };
 
 template <typename T>
-__device__ __forceinline__ float at(const Mat& m, int64_t r, int64_t c) {
-  const int64_t i = r * m.row + c * m.col;
-  return m.wide ? ((const float*)m.p)[i] : to_f32(((const T*)m.p)[i]);
-}
-
-// C[m,n] = sum_k A[m,k] B[k,n] (+ A2 B2) + bias[n], 16 x 16 tiles through LDS.
-template <typename T>
-__global__ void __launch_bounds__(256) ffn_product_kernel(int64_t M, int64_t N, int64_t K, Mat A,
-                                                          Mat B, Mat A2, Mat B2,
-                                                          const T* __restrict__ bias, void* C,
-                                                          int c_wide) {
-  __shared__ float s_a[16][17], s_b[16][17];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t tiles_n = (N + 15) / 16;
-  const int64_t m = blockIdx.x / tiles_n * 16 + ty, n = blockIdx.x % tiles_n * 16 + tx;
-  const int64_t mb = m - ty + tx;  // the row this thread loads of A where k runs along ty
-  double acc = 0.0;
-  for (int pair = 0; pair < (A2.p ? 2 : 1); ++pair) {
-    const Mat& a = pair ? A2 : A;
-    const Mat& b = pair ? B2 : B;
-    for (int64_t k0 = 0; k0 < K; k0 += 16) {
-      s_a[tx][ty] = mb < M && k0 + ty < K ? at<T>(a, mb, k0 + ty) : 0.f;
-      s_b[ty][tx] = n < N && k0 + ty < K ? at<T>(b, k0 + ty, n) : 0.f;
-      __syncthreads();
+__global__ void __launch_bounds__(256) ffn_lay_kernel(LayJobs jobs) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N;
+  int k = 0;
+  uint32_t first = 0;
+  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
+  const LayJob& job = jobs.job[k];
+  const uint32_t chunks = job.cols8 / 8;
+  const uint64_t i = (uint64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+  const int64_t row = (int64_t)(i / chunks);
+  const uint32_t c = (uint32_t)(i % chunks) * 8;
+  if (row >= job.rows) return;
+  const T* src = (const T*)job.src + row * job.pitch;
+  frag_t<E> out[P];
 #pragma unroll
-      for (int k = 0; k < 16; ++k) acc += (double)s_a[ty][k] * (double)s_b[k][tx];
-      __syncthreads();
-    }
+  for (int e = 0; e < 8; ++e) {
+    E p[P];
+    split<T>(c + e < job.cols ? to_f32(src[c + e]) : 0.f, p);
+#pragma unroll
+    for (int q = 0; q < P; ++q) out[q][e] = p[q];
   }
-  if (m >= M || n >= N) return;
-  const float v = (float)acc + (bias ? to_f32(bias[n]) : 0.f);
-  if (c_wide)
-    ((float*)C)[m * N + n] = v;
-  else
-    ((T*)C)[m * N + n] = from_f32<T>(v);
+  E* dst = (E*)job.dst + row * job.cols8 + c;
+#pragma unroll
+  for (int q = 0; q < P; ++q) *(frag_t<E>*)(dst + q * job.plane) = out[q];
 }
 
-// g -> h in place of g (forward); g, u, dh -> dg, du, h in their places (backward).
-__global__ void __launch_bounds__(256) ffn_gate_kernel(uint64_t n, int act, float* __restrict__ g,
-                                                       float* __restrict__ u,
-                                                       float* __restrict__ dh) {
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < n;
-       i += (uint64_t)gridDim.x * 256) {
-    const float2 a = activation(act, g[i]);
-    const float uu = u[i];
-    if (!dh) {
-      g[i] = a.x * uu;
-      continue;
+// ---------------------------------------------------------------------------
+// The hidden products.  A workgroup's tile is 128 rows by 64 hidden columns: its B rows
+// are runs of 16 of Wg and of Wu in turn, so that a lane's accumulators hold g and u
+// of the same row and columns and the gate is taken in registers.  The backward adds
+// dh = dy Wd for the same tile before its gate.
+// ---------------------------------------------------------------------------
+
+#define FT_M 128
+#define FT_F 64
+
+template <typename E>
+struct HiddenArgs {
+  Operand<E> x, wg, wu, dy, wd;
+  int64_t rows;
+  int32_t width8, hidden, hidden8, out, out8, act;
+  const void *bg, *bu;
+  E* h;     // h, plane by plane; backward: its pitch is hidden8 too
+  E* dgu;   // dg | du at a pitch of 2 hidden8
+  float* sums;  // of dg and du over a tile's rows: [tiles_m, 2 hidden8], nullable
+  int64_t plane;  // values between planes of h; dgu's are 2 * plane
+  int32_t add;    // add to sums
+};
+
+template <typename T, bool BACK>
+__global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename Planes<T>::E> a) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N, PAIRS = PlanePairs<T>::N;
+  using SX = Stage<E, FT_M, ALONG, 256>;
+  using SW = Stage<E, 2 * FT_F, ALONG, 256>;
+  using SD = Stage<E, FT_F, ACROSS, 256>;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * (SX::BYTES + SW::BYTES)];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  uint32_t tm, tn;
+  tile_of(blockIdx.x, (uint32_t)((a.rows + FT_M - 1) / FT_M), (a.hidden8 + FT_F - 1) / FT_F, tm, tn);
+  const int64_t m0 = (int64_t)tm * FT_M;
+  const int f0 = tn * FT_F;
+
+  f32x4 gu[4][4] = {};
+  {
+    const int per = (a.width8 + MX_BK - 1) / MX_BK;
+    product_loop<E, SX, SW>(gu, lds, per * PAIRS, wm * 64, wn * 64, [&](int s, char* to) {
+      const int pair = s / per, k0 = (s % per) * MX_BK;
+      const E* x = a.x.p + PlanePairs<T>::a(pair) * a.x.plane;
+      const E* wg = a.wg.p + PlanePairs<T>::b(pair) * a.wg.plane;
+      const E* wu = a.wu.p + PlanePairs<T>::b(pair) * a.wu.plane;
+      SX::load(to, x, a.x.pitch, m0, a.rows, k0, a.width8,
+               [&](int r) { return RowOf<E>{x, r}; });
+      SW::load(to + SX::BYTES, wg, a.wg.pitch, f0, a.hidden, k0, a.width8, [&](int r) {
+        return RowOf<E>{r & 16 ? wu : wg, (r >> 5) * 16 + (r & 15)};
+      });
+    });
+  }
+  f32x4 dh[4][2] = {};
+  if constexpr (BACK) {
+    const int per = (a.out8 + MX_BK - 1) / MX_BK;
+    product_loop<E, SX, SD>(dh, lds, per * PAIRS, wm * 64, wn * 32, [&](int s, char* to) {
+      const int pair = s / per, k0 = (s % per) * MX_BK;
+      const E* dy = a.dy.p + PlanePairs<T>::a(pair) * a.dy.plane;
+      SX::load(to, dy, a.dy.pitch, m0, a.rows, k0, a.out8,
+               [&](int r) { return RowOf<E>{dy, r}; });
+      SD::load(to + SX::BYTES, a.wd.p + PlanePairs<T>::b(pair) * a.wd.plane, a.wd.pitch, f0,
+               a.hidden8, k0, a.out, [&](int r) { return RowOf<E>{nullptr, 0}; });
+    });
+  }
+
+  const int group = lane >> 4;
+  float sg[2][4] = {}, su[2][4] = {};
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int f = f0 + wn * 32 + j * 16 + group * 4;
+    float bg[4], bu[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      bg[r] = a.bg && f + r < a.hidden ? to_f32(((const T*)a.bg)[f + r]) : 0.f;
+      bu[r] = a.bu && f + r < a.hidden ? to_f32(((const T*)a.bu)[f + r]) : 0.f;
     }
-    const float d = dh[i];
-    g[i] = d * uu * a.y;
-    u[i] = d * a.x;
-    dh[i] = a.x * uu;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t m = m0 + wm * 64 + i * 16 + (lane & 15);
+      const bool live = m < a.rows && f < a.hidden8;
+      four_t<E> h[P], dg[P], du[P];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float g = gu[i][2 * j][r] + bg[r], u = gu[i][2 * j + 1][r] + bu[r];
+        const float2 act = activation(a.act, g);
+        E p[P];
+        split<T>(f + r < a.hidden ? act.x * u : 0.f, p);
+#pragma unroll
+        for (int q = 0; q < P; ++q) h[q][r] = p[q];
+        if constexpr (BACK) {
+          const float d = dh[i][j][r];
+          // (behind the last hidden column zeros, whatever x holds)
+          const float vg = f + r < a.hidden ? d * u * act.y : 0.f;
+          const float vu = f + r < a.hidden ? d * act.x : 0.f;
+          if (m < a.rows) {
+            sg[j][r] += vg;
+            su[j][r] += vu;
+          }
+          split<T>(vg, p);
+#pragma unroll
+          for (int q = 0; q < P; ++q) dg[q][r] = p[q];
+          split<T>(vu, p);
+#pragma unroll
+          for (int q = 0; q < P; ++q) du[q][r] = p[q];
+        }
+      }
+      if (!live) continue;
+#pragma unroll
+      for (int q = 0; q < P; ++q) {
+        *(four_t<E>*)(a.h + q * a.plane + m * a.hidden8 + f) = h[q];
+        if constexpr (BACK) {
+          E* at = a.dgu + 2 * (q * a.plane + m * a.hidden8) + f;
+          *(four_t<E>*)at = dg[q];
+          *(four_t<E>*)(at + a.hidden8) = du[q];
+        }
+      }
+    }
+  }
+  if constexpr (BACK) {
+    if (!a.sums) return;
+    float* s = (float*)lds;  // [2 wm][2][64]; the main loop's last barrier freed it
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) {
+          sg[j][r] += __shfl_xor(sg[j][r], off, 64);
+          su[j][r] += __shfl_xor(su[j][r], off, 64);
+        }
+        if ((lane & 15) == 0) {
+          s[wm * 128 + wn * 32 + j * 16 + group * 4 + r] = sg[j][r];
+          s[wm * 128 + 64 + wn * 32 + j * 16 + group * 4 + r] = su[j][r];
+        }
+      }
+    __syncthreads();
+    if (threadIdx.x < 128) {
+      const int f = f0 + (threadIdx.x & 63);
+      if (f < a.hidden8) {
+        float* out = a.sums + (int64_t)tm * 2 * a.hidden8 + (threadIdx.x >> 6) * a.hidden8 + f;
+        const float v = s[threadIdx.x] + s[128 + threadIdx.x];
+        *out = a.add ? *out + v : v;
+      }
+    }
   }
 }
 
-// Sums of a matrix's columns, one wavefront per column.
+// ---------------------------------------------------------------------------
+// Plain products: C = A B' (+ bias), 128 x 128 tiles, either rounded to the call's type
+// or, with the sum over k split, as 32-bit partial sums that a second launch joins.
+// ---------------------------------------------------------------------------
+
+#define GT 128
+
+template <typename E>
+struct ProductArgs {
+  Operand<E> a, b, a2, b2;  // a2, b2: a second pair (null: none)
+  int64_t M, K;             // K: of each pair
+  int32_t N;
+  int64_t a_limit;          // A's other index runs to this (its columns where k runs across)
+  int32_t b_limit;
+  int32_t splits;           // of the steps over k
+  const void* bias;
+  void* c;                  // [M, N] of the call's type
+  float* partial;           // or [splits, M, N]
+  int32_t add;              // add to what `partial` holds
+};
+
+template <typename T, Along KA, Along KB>
+__global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typename Planes<T>::E> g) {
+  using E = typename Planes<T>::E;
+  constexpr int PAIRS = PlanePairs<T>::N;
+  using SA = Stage<E, GT, KA, 256>;
+  using SB = Stage<E, GT, KB, 256>;
+  __shared__ __attribute__((aligned(1024))) char lds[2 * (SA::BYTES + SB::BYTES)];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wm = wave >> 1, wn = wave & 1;
+  const uint32_t tiles_m = (uint32_t)((g.M + GT - 1) / GT), tiles_n = (g.N + GT - 1) / GT;
+  uint32_t tm, tn;
+  const uint32_t split = blockIdx.x / (tiles_m * tiles_n);
+  tile_of(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
+  const int64_t m0 = (int64_t)tm * GT;
+  const int n0 = tn * GT;
+  const int64_t all = (g.K + MX_BK - 1) / MX_BK;
+  const int64_t from = all * split / g.splits, to_ = all * (split + 1) / g.splits;
+  const int per = (int)(to_ - from);
+  const int pairs = PAIRS * (g.a2.p ? 2 : 1);
+
+  f32x4 acc[4][4] = {};
+  if (per)
+    product_loop<E, SA, SB>(acc, lds, per * pairs, wm * 64, wn * 64, [&](int s, char* to) {
+      const int q = s / per, pair = q % PAIRS;
+      const int64_t k0 = (from + s % per) * MX_BK;
+      const bool second = q >= PAIRS;
+      const E* pa = (second ? g.a2.p : g.a.p) + PlanePairs<T>::a(pair) * g.a.plane;
+      const E* pb = (second ? g.b2.p : g.b.p) + PlanePairs<T>::b(pair) * g.b.plane;
+      SA::load(to, pa, g.a.pitch, m0, g.a_limit, k0, g.K, [&](int r) { return RowOf<E>{pa, r}; });
+      SB::load(to + SA::BYTES, pb, g.b.pitch, n0, g.b_limit, k0, g.K,
+               [&](int r) { return RowOf<E>{pb, r}; });
+    });
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t m = m0 + wm * 64 + i * 16 + (lane & 15);
+    if (m >= g.M) continue;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int n = n0 + wn * 64 + j * 16 + (lane >> 4) * 4;
+      if (g.partial) {
+        float* at = g.partial + ((int64_t)split * g.M + m) * g.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < g.N) at[r] = g.add ? at[r] + acc[i][j][r] : acc[i][j][r];
+      } else {
+        T* at = (T*)g.c + m * g.N + n;
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (n + r < g.N)
+            at[r] = from_f32<T>(acc[i][j][r] + (g.bias ? to_f32(((const T*)g.bias)[n + r]) : 0.f));
+      }
+    }
+  }
+}
+
+// Sums of dy's columns over runs of rows: partial[run, column], 64 columns a workgroup.
 template <typename T>
-__global__ void __launch_bounds__(64) ffn_column_sum_kernel(int64_t rows, Mat A,
-                                                            T* __restrict__ out) {
+__global__ void __launch_bounds__(256) ffn_column_sum_kernel(int64_t rows, int32_t cols,
+                                                             const T* __restrict__ p, int64_t pitch,
+                                                             float* __restrict__ partial,
+                                                             int32_t add) {
+  __shared__ float s[4][64];
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
+  const int64_t from = rows * blockIdx.y / gridDim.y, to = rows * (blockIdx.y + 1) / gridDim.y;
   float acc = 0.f;
-  for (int64_t r = threadIdx.x; r < rows; r += 64) acc += at<T>(A, r, blockIdx.x);
-  acc = tgs_wave_sum(acc);
-  if (threadIdx.x == 0) out[blockIdx.x] = from_f32<T>(acc);
+  if (c < cols)
+    for (int64_t r = from + k; r < to; r += 4) acc += to_f32(p[r * pitch + c]);
+  s[k][threadIdx.x & 63] = acc;
+  __syncthreads();
+  if (k == 0 && c < cols) {
+    float* out = partial + (int64_t)blockIdx.y * cols + c;
+    const float v = (s[0][threadIdx.x] + s[1][threadIdx.x]) + (s[2][threadIdx.x] + s[3][threadIdx.x]);
+    *out = add ? *out + v : v;
+  }
 }
 
+// Partial sums joined in a fixed order and rounded: out[r, c] = sum_s partial[s, r, c].
+// The rows are those of up to three tensors one after another in `partial`.
+struct JoinJob {
+  const float* partial;
+  int64_t part;       // values between two partial sums
+  int64_t pitch;      // of a row of them
+  int32_t parts, cols;
+  int64_t rows;
+  void* out;          // [rows, cols]
+  uint32_t blocks;    // of the launch, up to and with this job's
+};
+#define JOIN_JOBS 6
+struct JoinJobs {
+  JoinJob job[JOIN_JOBS];
+};
+
 template <typename T>
-static void product(hipStream_t s, int64_t M, int64_t N, int64_t K, Mat A, Mat B, const T* bias,
-                    void* C, int c_wide, Mat A2 = Mat{}, Mat B2 = Mat{}) {
-  hipLaunchKernelGGL(ffn_product_kernel<T>, dim3((unsigned)(((M + 15) / 16) * ((N + 15) / 16))),
-                     dim3(256), 0, s, M, N, K, A, B, A2, B2, bias, C, c_wide);
+__global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
+  int k = 0;
+  uint32_t first = 0;
+  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
+  const JoinJob& job = jobs.job[k];
+  const int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+  if (i >= job.rows * job.cols) return;
+  const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
+  float acc = 0.f;
+  for (int s = 0; s < job.parts; ++s) acc += p[s * job.part];
+  ((T*)job.out)[i] = from_f32<T>(acc);
 }
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
 
 static int check_sizes(const char* name, uint64_t rows, uint32_t width, uint32_t hidden,
                        uint32_t out, int32_t activation) {
@@ -113,16 +358,127 @@ static int check_sizes(const char* name, uint64_t rows, uint32_t width, uint32_t
   return TGS_OK;
 }
 
+static int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Hands out parts of a workspace; with a null base it only counts.
+struct Carver {
+  char* base;
+  uint64_t used = 0;
+  template <typename U>
+  U* take(int64_t n) {
+    U* p = base ? (U*)(base + used) : nullptr;
+    used += ((uint64_t)n * sizeof(U) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+// Rows of one pass: what keeps the hidden tensors of a pass (six bytes a value and plane)
+// within 64M values; the next rows reuse them.
+static int64_t pass_rows(int64_t rows, int64_t hidden) {
+  const int64_t most = std::max<int64_t>((64 << 20) / round8(hidden) / FT_M * FT_M, FT_M);
+  return std::min(rows, most);
+}
+
+static int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
+
+// Parts that a product's sum over `k` values is split into so that its workgroups fill the
+// chip twice, none shorter than four steps.
+static int splits_of(int64_t tiles_, int64_t k) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles_, k / (4 * MX_BK)));
+}
+
+#define COLUMN_RUNS 64
+
+// Whether a product can read a matrix where it lies.
+template <typename T>
+static bool in_place(const void* p, int64_t cols, int64_t pitch) {
+  return Planes<T>::N == 1 && cols % 8 == 0 && pitch < (1 << 26) && aligned16((const T*)p, pitch);
+}
+
+// Everything a call keeps in its workspace.
+template <typename T>
+struct Plan {
+  using E = typename Planes<T>::E;
+  static constexpr int P = Planes<T>::N;
+  int64_t rows, D, F, O, D8, F8, O8, pass;
+  E *x, *wg, *wu, *wd, *dy, *h, *dgu;
+  float *gu_sums, *dy_sums, *dwgu, *dwd;
+  int split_gu = 1, split_d = 1;
+  uint64_t bytes;
+
+  Plan(void* ws, int64_t rows_, int64_t D_, int64_t F_, int64_t O_, bool back)
+      : rows(rows_), D(D_), F(F_), O(O_), D8(round8(D_)), F8(round8(F_)), O8(round8(O_)) {
+    Carver c{(char*)ws};
+    pass = pass_rows(rows, F);
+    x = c.take<E>(P * pass * D8);
+    wg = c.take<E>(P * F * D8);
+    wu = c.take<E>(P * F * D8);
+    wd = c.take<E>(P * O * F8);
+    h = c.take<E>(P * pass * F8);
+    if (back) {
+      dy = c.take<E>(P * pass * O8);
+      dgu = c.take<E>(2 * P * pass * F8);
+      gu_sums = c.take<float>(tiles(pass, FT_M) * 2 * F8);
+      dy_sums = c.take<float>(COLUMN_RUNS * O);
+      split_gu = splits_of(tiles(2 * F8, GT) * tiles(D, GT), pass);
+      split_d = splits_of(tiles(O, GT) * tiles(F, GT), pass);
+      dwgu = c.take<float>(split_gu * 2 * F8 * D);
+      dwd = c.take<float>(split_d * O * F);
+    }
+    bytes = c.used;
+  }
+};
+
+template <typename T>
+struct Layer {
+  using E = typename Planes<T>::E;
+  LayJobs jobs;
+  int n = 0;
+  uint32_t blocks = 0;
+  // The operand that holds a matrix: itself, or a copy that the next launch lays out.
+  Operand<E> operand(const void* p, int64_t rows, int64_t cols, int64_t pitch, E* copy) {
+    if (in_place<T>(p, cols, pitch)) return {(const E*)p, 0, pitch};
+    const int64_t cols8 = round8(cols);
+    blocks += (uint32_t)tiles(rows * (cols8 / 8), 256);
+    jobs.job[n++] = LayJob{p, copy, rows, pitch, rows * cols8, (uint32_t)cols, (uint32_t)cols8, blocks};
+    return {copy, rows * cols8, cols8};
+  }
+  void launch(hipStream_t s) {
+    if (n) hipLaunchKernelGGL(ffn_lay_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);
+    n = 0;
+    blocks = 0;
+  }
+};
+
+template <typename T>
+static const void* row_at(const void* p, int64_t row, int64_t pitch) {
+  return (const T*)p + row * pitch;
+}
+
+template <typename T, Along KA, Along KB>
+static void product(hipStream_t s, const ProductArgs<typename Planes<T>::E>& g) {
+  const int64_t n = tiles(g.M, GT) * tiles(g.N, GT) * g.splits;
+  hipLaunchKernelGGL((ffn_product_kernel<T, KA, KB>), dim3((unsigned)n), dim3(256), 0, s, g);
+}
+
+static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out,
+                               int32_t dtype, bool back) {
+  uint64_t bytes = 0;
+  with_dtype(dtype, "tgs_gated_ffn workspace", [&](auto tag) -> int {
+    bytes = Plan<decltype(tag)>(nullptr, rows, width, hidden, out, back).bytes;
+    return TGS_OK;
+  });
+  return bytes;
+}
+
 extern "C" uint64_t tgs_gated_ffn_fwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
                                                      uint32_t out, int32_t dtype) {
-  (void)width, (void)out, (void)dtype;
-  return 2 * rows * hidden * sizeof(float);
+  return workspace_size(rows, width, hidden, out, dtype, false);
 }
 
 extern "C" uint64_t tgs_gated_ffn_bwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
                                                      uint32_t out, int32_t dtype) {
-  (void)width, (void)out, (void)dtype;
-  return 3 * rows * hidden * sizeof(float);
+  return workspace_size(rows, width, hidden, out, dtype, true);
 }
 
 extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out,
@@ -132,6 +488,7 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
                                  void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
   return with_dtype(dtype, "tgs_gated_ffn_fwd", [&](auto tag) -> int {
     using T = decltype(tag);
+    using E = typename Planes<T>::E;
     if (const int rc = check_sizes("tgs_gated_ffn_fwd", rows, width, hidden, out, activation))
       return rc;
     if (rows == 0) return TGS_OK;
@@ -141,14 +498,27 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_fwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
-    const int64_t M = rows, D = width, F = hidden, O = out;
-    float *g = (float*)workspace, *u = g + M * F;
-    const Mat X{x, x_pitch, 1, 0};
-    product<T>(stream, M, F, D, X, Mat{w_gate, 1, D, 0}, (const T*)b_gate, g, 1);
-    product<T>(stream, M, F, D, X, Mat{w_up, 1, D, 0}, (const T*)b_up, u, 1);
-    hipLaunchKernelGGL(ffn_gate_kernel, dim3(std::min<int64_t>((M * F + 255) / 256, 65536)),
-                       dim3(256), 0, stream, (uint64_t)(M * F), activation, g, u, (float*)nullptr);
-    product<T>(stream, M, O, F, Mat{g, F, 1, 1}, Mat{w_down, 1, F, 0}, (const T*)b_down, y, 0);
+    const Plan<T> p(workspace, rows, width, hidden, out, false);
+    Layer<T> lay;
+    const Operand<E> wg = lay.operand(w_gate, p.F, p.D, p.D, p.wg);
+    const Operand<E> wu = lay.operand(w_up, p.F, p.D, p.D, p.wu);
+    const Operand<E> wd = lay.operand(w_down, p.O, p.F, p.F, p.wd);
+    for (int64_t r = 0; r < p.rows; r += p.pass) {
+      const int64_t m = std::min(p.pass, p.rows - r);
+      HiddenArgs<E> a{};
+      a.x = lay.operand(row_at<T>(x, r, x_pitch), m, p.D, x_pitch, p.x);
+      lay.launch(stream);
+      a.wg = wg, a.wu = wu;
+      a.rows = m, a.width8 = p.D8, a.hidden = p.F, a.hidden8 = p.F8, a.act = activation;
+      a.bg = b_gate, a.bu = b_up, a.h = p.h, a.plane = m * p.F8;
+      hipLaunchKernelGGL((ffn_hidden_kernel<T, false>),
+                         dim3((unsigned)(tiles(m, FT_M) * tiles(p.F8, FT_F))), dim3(256), 0, stream, a);
+      ProductArgs<E> g{};
+      g.a = {p.h, a.plane, p.F8}, g.b = wd;
+      g.M = m, g.N = p.O, g.K = p.F8, g.a_limit = m, g.b_limit = p.O, g.splits = 1;
+      g.bias = b_down, g.c = (T*)y + r * p.O;
+      product<T, ALONG, ALONG>(stream, g);
+    }
     TGS_RETURN_LAUNCH("tgs_gated_ffn_fwd");
   });
 }
@@ -162,6 +532,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
                                  void* workspace, uint64_t workspace_bytes, hipStream_t stream) {
   return with_dtype(dtype, "tgs_gated_ffn_bwd", [&](auto tag) -> int {
     using T = decltype(tag);
+    using E = typename Planes<T>::E;
     if (const int rc = check_sizes("tgs_gated_ffn_bwd", rows, width, hidden, out, activation))
       return rc;
     TGS_CHECK_ARG(w_gate && w_up && w_down && (rows == 0 || (x && dy)),
@@ -172,32 +543,71 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_bwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
-    const int64_t M = rows, D = width, F = hidden, O = out;
-    float *g = (float*)workspace, *u = g + M * F, *dh = u + M * F;
-    const Mat X{x, x_pitch, 1, 0}, DY{dy, dy_pitch, 1, 0};
-    const Mat G{g, F, 1, 1}, U{u, F, 1, 1}, H{dh, F, 1, 1};
-    if (M) {
-      product<T>(stream, M, F, D, X, Mat{w_gate, 1, D, 0}, (const T*)b_gate, g, 1);
-      product<T>(stream, M, F, D, X, Mat{w_up, 1, D, 0}, (const T*)b_up, u, 1);
-      product<T>(stream, M, F, O, DY, Mat{w_down, F, 1, 0}, (const T*)nullptr, dh, 1);
-      hipLaunchKernelGGL(ffn_gate_kernel, dim3(std::min<int64_t>((M * F + 255) / 256, 65536)),
-                         dim3(256), 0, stream, (uint64_t)(M * F), activation, g, u, dh);
-      if (dx)
-        product<T>(stream, M, D, F, G, Mat{w_gate, D, 1, 0}, (const T*)nullptr, dx, 0, U,
-                   Mat{w_up, D, 1, 0});
+    const Plan<T> p(workspace, rows, width, hidden, out, true);
+    Layer<T> lay;
+    const Operand<E> wg = lay.operand(w_gate, p.F, p.D, p.D, p.wg);
+    const Operand<E> wu = lay.operand(w_up, p.F, p.D, p.D, p.wu);
+    const Operand<E> wd = lay.operand(w_down, p.O, p.F, p.F, p.wd);
+    const bool hidden_sums = db_gate || db_up;
+    for (int64_t r = 0; r < p.rows; r += p.pass) {
+      const int64_t m = std::min(p.pass, p.rows - r);
+      HiddenArgs<E> a{};
+      a.x = lay.operand(row_at<T>(x, r, x_pitch), m, p.D, x_pitch, p.x);
+      a.dy = lay.operand(row_at<T>(dy, r, dy_pitch), m, p.O, dy_pitch, p.dy);
+      lay.launch(stream);
+      a.wg = wg, a.wu = wu, a.wd = wd;
+      a.rows = m, a.width8 = p.D8, a.hidden = p.F, a.hidden8 = p.F8, a.out = p.O, a.out8 = p.O8;
+      a.act = activation, a.bg = b_gate, a.bu = b_up;
+      a.h = p.h, a.dgu = p.dgu, a.plane = m * p.F8;
+      a.sums = hidden_sums ? p.gu_sums : nullptr, a.add = r > 0;
+      hipLaunchKernelGGL((ffn_hidden_kernel<T, true>),
+                         dim3((unsigned)(tiles(m, FT_M) * tiles(p.F8, FT_F))), dim3(256), 0, stream, a);
+      if (dx) {
+        ProductArgs<E> g{};
+        g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.a2 = {p.dgu + p.F8, 2 * a.plane, 2 * p.F8};
+        g.b = wg, g.b2 = wu;
+        // (k runs to the weights' last row; behind it dg and du are zero)
+        g.M = m, g.N = p.D, g.K = p.F, g.a_limit = m, g.b_limit = p.D8, g.splits = 1;
+        g.c = (T*)dx + r * p.D;
+        product<T, ALONG, ACROSS>(stream, g);
+      }
+      if (dw_gate || dw_up) {
+        ProductArgs<E> g{};
+        g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.b = a.x;
+        g.M = 2 * p.F8, g.N = p.D, g.K = m, g.a_limit = 2 * p.F8, g.b_limit = p.D8;
+        g.splits = p.split_gu, g.partial = p.dwgu, g.add = r > 0;
+        product<T, ACROSS, ACROSS>(stream, g);
+      }
+      if (dw_down) {
+        ProductArgs<E> g{};
+        g.a = a.dy, g.b = {p.h, a.plane, p.F8};
+        g.M = p.O, g.N = p.F, g.K = m, g.a_limit = p.O8, g.b_limit = p.F8;
+        g.splits = p.split_d, g.partial = p.dwd, g.add = r > 0;
+        product<T, ACROSS, ACROSS>(stream, g);
+      }
+      if (db_down)
+        hipLaunchKernelGGL(ffn_column_sum_kernel<T>, dim3((unsigned)tiles(p.O, 64), COLUMN_RUNS),
+                           dim3(256), 0, stream, m, (int32_t)p.O,
+                           (const T*)row_at<T>(dy, r, dy_pitch), dy_pitch, p.dy_sums, r > 0);
     }
-    const T* none = nullptr;
-    if (dw_gate) product<T>(stream, F, D, M, Mat{g, 1, F, 1}, X, none, dw_gate, 0);
-    if (dw_up) product<T>(stream, F, D, M, Mat{u, 1, F, 1}, X, none, dw_up, 0);
-    if (dw_down) product<T>(stream, O, F, M, Mat{dy, 1, dy_pitch, 0}, H, none, dw_down, 0);
-    const auto sums = [&](const Mat& A, int64_t n, void* db) {
-      if (db)
-        hipLaunchKernelGGL(ffn_column_sum_kernel<T>, dim3((unsigned)n), dim3(64), 0, stream, M, A,
-                           (T*)db);
+    JoinJobs join;
+    int n = 0;
+    uint32_t blocks = 0;
+    const auto add = [&](const float* partial, int64_t part, int64_t pitch, int64_t parts,
+                         int64_t rows_, int64_t cols, void* to) {
+      if (!to) return;
+      blocks += (uint32_t)tiles(rows_ * cols, 256);
+      join.job[n++] = JoinJob{partial, part, pitch, p.rows ? (int32_t)parts : 0, (int32_t)cols, rows_,
+                              to, blocks};
     };
-    sums(G, F, db_gate);
-    sums(U, F, db_up);
-    sums(DY, O, db_down);
+    add(p.dwgu, 2 * p.F8 * p.D, p.D, p.split_gu, p.F, p.D, dw_gate);
+    add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, p.split_gu, p.F, p.D, dw_up);
+    add(p.dwd, p.O * p.F, p.F, p.split_d, p.O, p.F, dw_down);
+    const int64_t row_tiles = tiles(p.pass, FT_M);
+    add(p.gu_sums, 2 * p.F8, p.F8, row_tiles, 1, p.F, db_gate);
+    add(p.gu_sums + p.F8, 2 * p.F8, p.F8, row_tiles, 1, p.F, db_up);
+    add(p.dy_sums, p.O, p.O, COLUMN_RUNS, 1, p.O, db_down);
+    if (n) hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, stream, join);
     TGS_RETURN_LAUNCH("tgs_gated_ffn_bwd");
   });
 }
