@@ -6,20 +6,7 @@
 //
 // x [rows, width], Wg and Wu [hidden, width], Wd [out, hidden], row-major (x and dy at
 // a pitch).  The backward computes g and u again.
-#include "matrix.cuh"
-
-enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
-
-// act(g) and its derivative.
-__device__ __forceinline__ float2 activation(int act, float g) {
-  if (act == ACT_RELU) return g > 0.f ? make_float2(g, 1.f) : make_float2(0.f * g, 0.f);
-  if (act == ACT_SILU) {
-    const float s = 1.f / (1.f + expf(-g));
-    return make_float2(g * s, s * (1.f + g * (1.f - s)));
-  }
-  const float phi = 0.5f * (1.f + erff(g * 0.70710678118654752f));
-  return make_float2(g * phi, phi + g * 0.39894228040143268f * expf(-0.5f * g * g));
-}
+#include "gated_ffn.cuh"
 
 // ---------------------------------------------------------------------------
 // Operands that the products cannot read where they lie (32-bit values, rows that do
@@ -135,6 +122,7 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
 
   const int group = lane >> 4;
   float sg[2][4] = {}, su[2][4] = {};
+  with_activation(a.act, [&](auto kind) {
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     const int f = f0 + wn * 32 + j * 16 + group * 4;
@@ -152,7 +140,7 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const float g = gu[i][2 * j][r] + bg[r], u = gu[i][2 * j + 1][r] + bu[r];
-        const float2 act = activation(a.act, g);
+        const float2 act = activation<T, kind.value>(g);
         E p[P];
         split<T>(f + r < a.hidden ? act.x * u : 0.f, p);
 #pragma unroll
@@ -186,6 +174,7 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
       }
     }
   }
+  });
   if constexpr (BACK) {
     if (!a.sums) return;
     float* s = (float*)lds;  // [2 wm][2][64]; the main loop's last barrier freed it
@@ -465,7 +454,10 @@ static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, u
                                int32_t dtype, bool back) {
   uint64_t bytes = 0;
   with_dtype(dtype, "tgs_gated_ffn workspace", [&](auto tag) -> int {
-    bytes = Plan<decltype(tag)>(nullptr, rows, width, hidden, out, back).bytes;
+    using T = decltype(tag);
+    bytes = Plan<T>(nullptr, rows, width, hidden, out, back).bytes;
+    if (!back && RowKernels<T>::takes(rows, width, hidden, out))
+      bytes = RowKernels<T>::workspace(width, hidden, out);
     return TGS_OK;
   });
   return bytes;
@@ -497,6 +489,14 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
     if (workspace_bytes < tgs_gated_ffn_fwd_workspace_size(rows, width, hidden, out, dtype)) {
       tgs_set_error("tgs_gated_ffn_fwd: workspace too small");
       return TGS_ERR_WORKSPACE;
+    }
+    if (RowKernels<T>::takes(rows, width, hidden, out)) {
+      FfnCall c{};
+      c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
+      c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
+      c.bg = b_gate, c.bu = b_up, c.bd = b_down, c.y = y;
+      RowKernels<T>::forward(c, workspace, stream);
+      TGS_RETURN_LAUNCH("tgs_gated_ffn_fwd");
     }
     const Plan<T> p(workspace, rows, width, hidden, out, false);
     Layer<T> lay;
