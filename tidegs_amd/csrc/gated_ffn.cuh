@@ -57,11 +57,156 @@ struct FfnCall {
   void *y, *dx, *dwg, *dwu, *dwd, *dbg, *dbu, *dbd;
 };
 
+// ---------------------------------------------------------------------------
+// Operands that the products cannot read where they lie (32-bit values, rows that do
+// not start on 16 bytes, widths that are no multiple of 8) are laid out as planes
+// with rows of a whole number of chunks, zeros behind the last value.
+// ---------------------------------------------------------------------------
+
+struct LayJob {
+  const void* src;
+  void* dst;
+  int64_t rows, pitch, plane;  // plane: values between two planes of dst
+  uint32_t cols, cols8;
+  uint32_t blocks;  // of the launch, up to and with this job's
+};
+#define LAY_JOBS 5
+struct LayJobs {
+  LayJob job[LAY_JOBS];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_lay_kernel(LayJobs jobs) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N;
+  int k = 0;
+  uint32_t first = 0;
+  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
+  const LayJob& job = jobs.job[k];
+  const uint32_t chunks = job.cols8 / 8;
+  const uint64_t i = (uint64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+  const int64_t row = (int64_t)(i / chunks);
+  const uint32_t c = (uint32_t)(i % chunks) * 8;
+  if (row >= job.rows) return;
+  const T* src = (const T*)job.src + row * job.pitch;
+  frag_t<E> out[P];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    E p[P];
+    split<T>(c + e < job.cols ? to_f32(src[c + e]) : 0.f, p);
+#pragma unroll
+    for (int q = 0; q < P; ++q) out[q][e] = p[q];
+  }
+  E* dst = (E*)job.dst + row * job.cols8 + c;
+#pragma unroll
+  for (int q = 0; q < P; ++q) *(frag_t<E>*)(dst + q * job.plane) = out[q];
+}
+
+// Partial sums joined in a fixed order and rounded: out[r, c] = sum_s partial[s, r, c].
+// The rows are those of up to three tensors one after another in `partial`.
+struct JoinJob {
+  const float* partial;
+  int64_t part;       // values between two partial sums
+  int64_t pitch;      // of a row of them
+  int32_t parts, cols;
+  int64_t rows;
+  void* out;          // [rows, cols]
+  uint32_t blocks;    // of the launch, up to and with this job's
+};
+#define JOIN_JOBS 6
+struct JoinJobs {
+  JoinJob job[JOIN_JOBS];
+};
+
+template <typename T>
+__global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
+  int k = 0;
+  uint32_t first = 0;
+  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
+  const JoinJob& job = jobs.job[k];
+  const int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
+  if (i >= job.rows * job.cols) return;
+  const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
+  float acc = 0.f;
+  for (int s = 0; s < job.parts; ++s) acc += p[s * job.part];
+  ((T*)job.out)[i] = from_f32<T>(acc);
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
+static inline int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// Hands out parts of a workspace; with a null base it only counts.
+struct Carver {
+  char* base;
+  uint64_t used = 0;
+  template <typename U>
+  U* take(int64_t n) {
+    U* p = base ? (U*)(base + used) : nullptr;
+    used += ((uint64_t)n * sizeof(U) + 255) / 256 * 256;
+    return p;
+  }
+};
+
+static inline int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
+
+// Whether a product can read a matrix where it lies.
+template <typename T>
+static bool in_place(const void* p, int64_t cols, int64_t pitch) {
+  return Planes<T>::N == 1 && cols % 8 == 0 && pitch < (1 << 26) && aligned16((const T*)p, pitch);
+}
+
+template <typename T>
+struct Layer {
+  using E = typename Planes<T>::E;
+  LayJobs jobs;
+  int n = 0;
+  uint32_t blocks = 0;
+  // The operand that holds a matrix: itself, or a copy that the next launch lays out.
+  Operand<E> operand(const void* p, int64_t rows, int64_t cols, int64_t pitch, E* copy) {
+    if (in_place<T>(p, cols, pitch)) return {(const E*)p, 0, pitch};
+    const int64_t cols8 = round8(cols);
+    blocks += (uint32_t)tiles(rows * (cols8 / 8), 256);
+    jobs.job[n++] = LayJob{p, copy, rows, pitch, rows * cols8, (uint32_t)cols, (uint32_t)cols8, blocks};
+    return {copy, rows * cols8, cols8};
+  }
+  void launch(hipStream_t s) {
+    if (n) hipLaunchKernelGGL(ffn_lay_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);
+    n = 0;
+    blocks = 0;
+  }
+};
+
+template <typename T>
+static const void* row_at(const void* p, int64_t row, int64_t pitch) {
+  return (const T*)p + row * pitch;
+}
+
+// The join of a call's partial sums, one launch.
+template <typename T>
+struct Joiner {
+  JoinJobs jobs;
+  int n = 0;
+  uint32_t blocks = 0;
+  void add(const float* partial, int64_t part, int64_t pitch, int64_t parts, int64_t rows,
+           int64_t cols, void* to) {
+    if (!to) return;
+    blocks += (uint32_t)tiles(rows * cols, 256);
+    jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, rows, to, blocks};
+  }
+  void launch(hipStream_t s) {
+    if (n) hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);
+  }
+};
+
 // Narrow rows (gated_ffn_rows.cuh): whether a call's sizes are theirs, the workspace they
 // take and their launches.
 template <typename T>
 struct RowKernels {
   static bool takes(int64_t rows, int32_t width, int32_t hidden, int32_t out);
-  static uint64_t workspace(int32_t width, int32_t hidden, int32_t out);
+  static uint64_t workspace(int64_t rows, int32_t width, int32_t hidden, int32_t out, bool back);
   static void forward(const FfnCall& c, void* workspace, hipStream_t stream);
+  static void backward(const FfnCall& c, void* workspace, hipStream_t stream);
 };

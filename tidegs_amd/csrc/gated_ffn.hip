@@ -9,51 +9,6 @@
 #include "gated_ffn.cuh"
 
 // ---------------------------------------------------------------------------
-// Operands that the products cannot read where they lie (32-bit values, rows that do
-// not start on 16 bytes, widths that are no multiple of 8) are laid out as planes
-// with rows of a whole number of chunks, zeros behind the last value.
-// ---------------------------------------------------------------------------
-
-struct LayJob {
-  const void* src;
-  void* dst;
-  int64_t rows, pitch, plane;  // plane: values between two planes of dst
-  uint32_t cols, cols8;
-  uint32_t blocks;  // of the launch, up to and with this job's
-};
-#define LAY_JOBS 5
-struct LayJobs {
-  LayJob job[LAY_JOBS];
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) ffn_lay_kernel(LayJobs jobs) {
-  using E = typename Planes<T>::E;
-  constexpr int P = Planes<T>::N;
-  int k = 0;
-  uint32_t first = 0;
-  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
-  const LayJob& job = jobs.job[k];
-  const uint32_t chunks = job.cols8 / 8;
-  const uint64_t i = (uint64_t)(blockIdx.x - first) * 256 + threadIdx.x;
-  const int64_t row = (int64_t)(i / chunks);
-  const uint32_t c = (uint32_t)(i % chunks) * 8;
-  if (row >= job.rows) return;
-  const T* src = (const T*)job.src + row * job.pitch;
-  frag_t<E> out[P];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    E p[P];
-    split<T>(c + e < job.cols ? to_f32(src[c + e]) : 0.f, p);
-#pragma unroll
-    for (int q = 0; q < P; ++q) out[q][e] = p[q];
-  }
-  E* dst = (E*)job.dst + row * job.cols8 + c;
-#pragma unroll
-  for (int q = 0; q < P; ++q) *(frag_t<E>*)(dst + q * job.plane) = out[q];
-}
-
-// ---------------------------------------------------------------------------
 // The hidden products.  A workgroup's tile is 128 rows by 64 hidden columns: its B rows
 // are runs of 16 of Wg and of Wu in turn, so that a lane's accumulators hold g and u
 // of the same row and columns and the gate is taken in registers.  The backward adds
@@ -302,36 +257,6 @@ __global__ void __launch_bounds__(256) ffn_column_sum_kernel(int64_t rows, int32
   }
 }
 
-// Partial sums joined in a fixed order and rounded: out[r, c] = sum_s partial[s, r, c].
-// The rows are those of up to three tensors one after another in `partial`.
-struct JoinJob {
-  const float* partial;
-  int64_t part;       // values between two partial sums
-  int64_t pitch;      // of a row of them
-  int32_t parts, cols;
-  int64_t rows;
-  void* out;          // [rows, cols]
-  uint32_t blocks;    // of the launch, up to and with this job's
-};
-#define JOIN_JOBS 6
-struct JoinJobs {
-  JoinJob job[JOIN_JOBS];
-};
-
-template <typename T>
-__global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
-  int k = 0;
-  uint32_t first = 0;
-  while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
-  const JoinJob& job = jobs.job[k];
-  const int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
-  if (i >= job.rows * job.cols) return;
-  const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
-  float acc = 0.f;
-  for (int s = 0; s < job.parts; ++s) acc += p[s * job.part];
-  ((T*)job.out)[i] = from_f32<T>(acc);
-}
-
 // ---------------------------------------------------------------------------
 // Host side
 // ---------------------------------------------------------------------------
@@ -347,28 +272,12 @@ static int check_sizes(const char* name, uint64_t rows, uint32_t width, uint32_t
   return TGS_OK;
 }
 
-static int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
-
-// Hands out parts of a workspace; with a null base it only counts.
-struct Carver {
-  char* base;
-  uint64_t used = 0;
-  template <typename U>
-  U* take(int64_t n) {
-    U* p = base ? (U*)(base + used) : nullptr;
-    used += ((uint64_t)n * sizeof(U) + 255) / 256 * 256;
-    return p;
-  }
-};
-
 // Rows of one pass: what keeps the hidden tensors of a pass (six bytes a value and plane)
 // within 64M values; the next rows reuse them.
 static int64_t pass_rows(int64_t rows, int64_t hidden) {
   const int64_t most = std::max<int64_t>((64 << 20) / round8(hidden) / FT_M * FT_M, FT_M);
   return std::min(rows, most);
 }
-
-static int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
 
 // Parts that a product's sum over `k` values is split into so that its workgroups fill the
 // chip twice, none shorter than four steps.
@@ -377,12 +286,6 @@ static int splits_of(int64_t tiles_, int64_t k) {
 }
 
 #define COLUMN_RUNS 64
-
-// Whether a product can read a matrix where it lies.
-template <typename T>
-static bool in_place(const void* p, int64_t cols, int64_t pitch) {
-  return Planes<T>::N == 1 && cols % 8 == 0 && pitch < (1 << 26) && aligned16((const T*)p, pitch);
-}
 
 // Everything a call keeps in its workspace.
 template <typename T>
@@ -418,32 +321,6 @@ struct Plan {
   }
 };
 
-template <typename T>
-struct Layer {
-  using E = typename Planes<T>::E;
-  LayJobs jobs;
-  int n = 0;
-  uint32_t blocks = 0;
-  // The operand that holds a matrix: itself, or a copy that the next launch lays out.
-  Operand<E> operand(const void* p, int64_t rows, int64_t cols, int64_t pitch, E* copy) {
-    if (in_place<T>(p, cols, pitch)) return {(const E*)p, 0, pitch};
-    const int64_t cols8 = round8(cols);
-    blocks += (uint32_t)tiles(rows * (cols8 / 8), 256);
-    jobs.job[n++] = LayJob{p, copy, rows, pitch, rows * cols8, (uint32_t)cols, (uint32_t)cols8, blocks};
-    return {copy, rows * cols8, cols8};
-  }
-  void launch(hipStream_t s) {
-    if (n) hipLaunchKernelGGL(ffn_lay_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);
-    n = 0;
-    blocks = 0;
-  }
-};
-
-template <typename T>
-static const void* row_at(const void* p, int64_t row, int64_t pitch) {
-  return (const T*)p + row * pitch;
-}
-
 template <typename T, Along KA, Along KB>
 static void product(hipStream_t s, const ProductArgs<typename Planes<T>::E>& g) {
   const int64_t n = tiles(g.M, GT) * tiles(g.N, GT) * g.splits;
@@ -456,8 +333,8 @@ static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, u
   with_dtype(dtype, "tgs_gated_ffn workspace", [&](auto tag) -> int {
     using T = decltype(tag);
     bytes = Plan<T>(nullptr, rows, width, hidden, out, back).bytes;
-    if (!back && RowKernels<T>::takes(rows, width, hidden, out))
-      bytes = RowKernels<T>::workspace(width, hidden, out);
+    if (RowKernels<T>::takes(rows, width, hidden, out))
+      bytes = RowKernels<T>::workspace(rows, width, hidden, out, back);
     return TGS_OK;
   });
   return bytes;
@@ -543,6 +420,16 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_bwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
+    if (rows && RowKernels<T>::takes(rows, width, hidden, out)) {
+      FfnCall c{};
+      c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
+      c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
+      c.bg = b_gate, c.bu = b_up, c.dy = dy, c.dy_pitch = dy_pitch;
+      c.dx = dx, c.dwg = dw_gate, c.dwu = dw_up, c.dwd = dw_down;
+      c.dbg = db_gate, c.dbu = db_up, c.dbd = db_down;
+      RowKernels<T>::backward(c, workspace, stream);
+      TGS_RETURN_LAUNCH("tgs_gated_ffn_bwd");
+    }
     const Plan<T> p(workspace, rows, width, hidden, out, true);
     Layer<T> lay;
     const Operand<E> wg = lay.operand(w_gate, p.F, p.D, p.D, p.wg);
@@ -590,24 +477,16 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
                            dim3(256), 0, stream, m, (int32_t)p.O,
                            (const T*)row_at<T>(dy, r, dy_pitch), dy_pitch, p.dy_sums, r > 0);
     }
-    JoinJobs join;
-    int n = 0;
-    uint32_t blocks = 0;
-    const auto add = [&](const float* partial, int64_t part, int64_t pitch, int64_t parts,
-                         int64_t rows_, int64_t cols, void* to) {
-      if (!to) return;
-      blocks += (uint32_t)tiles(rows_ * cols, 256);
-      join.job[n++] = JoinJob{partial, part, pitch, p.rows ? (int32_t)parts : 0, (int32_t)cols, rows_,
-                              to, blocks};
-    };
-    add(p.dwgu, 2 * p.F8 * p.D, p.D, p.split_gu, p.F, p.D, dw_gate);
-    add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, p.split_gu, p.F, p.D, dw_up);
-    add(p.dwd, p.O * p.F, p.F, p.split_d, p.O, p.F, dw_down);
+    Joiner<T> join;
+    const int64_t some = p.rows > 0;  // no rows: sums of nothing
+    join.add(p.dwgu, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_gate);
+    join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up);
+    join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down);
     const int64_t row_tiles = tiles(p.pass, FT_M);
-    add(p.gu_sums, 2 * p.F8, p.F8, row_tiles, 1, p.F, db_gate);
-    add(p.gu_sums + p.F8, 2 * p.F8, p.F8, row_tiles, 1, p.F, db_up);
-    add(p.dy_sums, p.O, p.O, COLUMN_RUNS, 1, p.O, db_down);
-    if (n) hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, stream, join);
+    join.add(p.gu_sums, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_gate);
+    join.add(p.gu_sums + p.F8, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_up);
+    join.add(p.dy_sums, p.O, p.O, some * COLUMN_RUNS, 1, p.O, db_down);
+    join.launch(stream);
     TGS_RETURN_LAUNCH("tgs_gated_ffn_bwd");
   });
 }

@@ -15,18 +15,23 @@
 
 #include "gated_ffn.cuh"
 
-// KB of a chunk of 32 hidden columns: fragments and 1 KB for the biases.
+// A chunk of 32 hidden columns: fragments (times the planes) and 1 KB for the biases.
+// DK, OK: k steps of 32 of the width and of the out; OT, DT: tiles of 16.
 template <typename T, int DK, int OT>
-struct ForwardChunk {
-  static constexpr int P = Planes<T>::N;
-  static constexpr int FRAGMENTS = 4 * DK + OT;  // Wg and Wu: two tiles by DK each; Wd: OT
-  static constexpr int KB = FRAGMENTS * P + 1;
+struct ForwardChunk {  // Wg, Wu: two tiles by DK; Wd: OT tiles
+  static constexpr int FRAGMENTS = 4 * DK + OT;
+  static constexpr int KB = FRAGMENTS * Planes<T>::N + 1;
+};
+template <typename T, int DK, int OK>
+struct BackwardChunk {  // Wg, Wu: two tiles by DK; Wd': two tiles by OK; Wg', Wu': 2 DK tiles
+  static constexpr int FRAGMENTS = 8 * DK + 2 * OK;
+  static constexpr int KB = FRAGMENTS * Planes<T>::N + 1;
 };
 
 struct PackArgs {
   const void *wg, *wu, *wd, *bg, *bu;
   char* out;
-  int32_t width, hidden, out_n, chunks, dk, ot, kb;
+  int32_t width, hidden, out_n, dk, ot, ok, kb;  // ot: forward; ok: backward
 };
 
 // The hidden column of row r of tile t of a chunk.
@@ -35,13 +40,14 @@ __device__ __forceinline__ int dealt(int chunk, int t, int r) {
 }
 
 // One wavefront per fragment (and one per chunk for its biases).
-template <typename T>
+template <typename T, bool BACK>
 __global__ void __launch_bounds__(64) ffn_pack_kernel(PackArgs a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N;
-  const int lane = threadIdx.x;
-  const int per = 4 * a.dk + a.ot + 1;
-  const int chunk = blockIdx.x / per, q = blockIdx.x % per;
+  const int lane = threadIdx.x, row = lane & 15;
+  const int per = (BACK ? 8 * a.dk + 2 * a.ok : 4 * a.dk + a.ot) + 1;
+  const int chunk = blockIdx.x / per;
+  const int q = blockIdx.x % per;
   char* base = a.out + (int64_t)chunk * a.kb * 1024;
   if (q == per - 1) {
     const int f = chunk * 32 + (lane & 31);
@@ -53,17 +59,29 @@ __global__ void __launch_bounds__(64) ffn_pack_kernel(PackArgs a) {
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int k = (lane >> 4) * 8 + j;
-    float v = 0.f;
+    const void* w;
+    int r, c, rows, cols;  // of the weight's element
     if (q < 4 * a.dk) {  // [gate, up][tile][k step]
-      const T* w = (const T*)(q < 2 * a.dk ? a.wg : a.wu);
-      const int f = dealt(chunk, q / a.dk & 1, lane & 15), d = q % a.dk * 32 + k;
-      if (f < a.hidden && d < a.width) v = to_f32(w[(int64_t)f * a.width + d]);
-    } else {
-      const int o = (q - 4 * a.dk) * 16 + (lane & 15), f = chunk * 32 + k;
-      if (o < a.out_n && f < a.hidden) v = to_f32(((const T*)a.wd)[(int64_t)o * a.hidden + f]);
+      w = q < 2 * a.dk ? a.wg : a.wu;
+      r = dealt(chunk, q / a.dk & 1, row), c = q % a.dk * 32 + k;
+      rows = a.hidden, cols = a.width;
+    } else if (!BACK) {
+      w = a.wd;
+      r = (q - 4 * a.dk) * 16 + row, c = chunk * 32 + k;
+      rows = a.out_n, cols = a.hidden;
+    } else if (q < 4 * a.dk + 2 * a.ok) {  // Wd' [tile][k step]
+      const int i = q - 4 * a.dk;
+      w = a.wd;
+      r = i % a.ok * 32 + k, c = dealt(chunk, i / a.ok, row);
+      rows = a.out_n, cols = a.hidden;
+    } else {  // Wg', Wu' [gate, up][tile]
+      const int i = q - 4 * a.dk - 2 * a.ok;
+      w = i < 2 * a.dk ? a.wg : a.wu;
+      r = chunk * 32 + k, c = i % (2 * a.dk) * 16 + row;
+      rows = a.hidden, cols = a.width;
     }
     E p[P];
-    split<T>(v, p);
+    split<T>(r < rows && c < cols ? to_f32(((const T*)w)[(int64_t)r * cols + c]) : 0.f, p);
 #pragma unroll
     for (int s = 0; s < P; ++s) out[s][j] = p[s];
   }
@@ -241,6 +259,406 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
   }
 }
 
+// ---------------------------------------------------------------------------
+// dx: the forward's walk with dh = dy Wd beside g and u, and dx' = Wg' dg' + Wu' du' in
+// place of y.
+// ---------------------------------------------------------------------------
+
+template <typename T>
+struct BackwardArgs {
+  const T *x, *dy;
+  T* dx;
+  const char* packed;
+  int64_t rows, x_pitch, dy_pitch;
+  int32_t width, out, chunks, act;
+  int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
+};
+
+template <typename T, int DK, int OK, int RT>
+__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs<T> a) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N, DT = 2 * DK;
+  using C = BackwardChunk<T, DK, OK>;
+  constexpr int BUFFERS = C::KB <= 80 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * C::KB * 1024];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  constexpr int TILE = 16 * RT * FR_WAVES;
+  const int64_t tiles = (a.rows + TILE - 1) / TILE;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const int64_t m0 = tile * TILE + wave * 16 * RT + (lane & 15);
+    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
+    frag_t<E> x[RT][DK][P], dy[RT][OK][P];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const int64_t m = m0 + i * 16;
+      const int c = (lane >> 4) * 8;
+#pragma unroll
+      for (int k = 0; k < DK; ++k)
+        load_fragment<T>(a.x + m * a.x_pitch, k * 32 + c, a.width, m < a.rows, a.wide, x[i][k]);
+#pragma unroll
+      for (int k = 0; k < OK; ++k)
+        load_fragment<T>(a.dy + m * a.dy_pitch, k * 32 + c, a.out, m < a.rows, a.wide_dy, dy[i][k]);
+    }
+    f32x4 dx[DT][RT] = {};
+    for (int c = 0; c < a.chunks; ++c) {
+      if (BUFFERS == 1 && c) {
+        __syncthreads();
+        copy_chunk<C::KB, FR_WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
+      }
+      __syncthreads();  // the chunk is there, and nobody reads the one before it
+      const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
+      if (BUFFERS == 2 && c + 1 < a.chunks)
+        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
+                                    a.packed + (int64_t)(c + 1) * C::KB * 1024);
+      const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
+#pragma unroll
+        for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
+      };
+      const float* bias = (const float*)(cur + (C::KB - 1) * 1024) + (lane >> 4) * 8;
+      frag_t<E> dg[RT][P], du[RT][P];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 g[RT], u[RT], dh[RT] = {};
+        const f32x4 bg = *(const f32x4*)(bias + t * 4), bu = *(const f32x4*)(bias + 32 + t * 4);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) g[i] = bg, u[i] = bu;
+        frag_t<E> w[P];
+#pragma unroll
+        for (int k = 0; k < DK; ++k) {
+          fragment(t * DK + k, w);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) g[i] = mfma_planes<T>(w, x[i][k], g[i]);
+          fragment((2 + t) * DK + k, w);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < OK; ++k) {
+          fragment(4 * DK + t * OK + k, w);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) dh[i] = mfma_planes<T>(w, dy[i][k], dh[i]);
+        }
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float2 v = activation<T, act.value>(g[i][r]);
+              E p[P];
+              split<T>(dh[i][r] * u[i][r] * v.y, p);
+#pragma unroll
+              for (int s = 0; s < P; ++s) dg[i][s][t * 4 + r] = p[s];
+              split<T>(dh[i][r] * v.x, p);
+#pragma unroll
+              for (int s = 0; s < P; ++s) du[i][s][t * 4 + r] = p[s];
+            }
+        });
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        frag_t<E> w[P];
+        fragment(4 * DK + 2 * OK + d, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, dg[i], dx[d][i]);
+        fragment(4 * DK + 2 * OK + DT + d, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, du[i], dx[d][i]);
+      }
+    }
+    __syncthreads();  // (the next rows' first chunk goes where the last one lay)
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      const int n = d * 16 + (lane >> 4) * 4;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        const int64_t m = m0 + i * 16;
+        if (m >= a.rows || n >= a.width) continue;
+        T* at = a.dx + m * a.width + n;
+        if (a.wide_dx) {
+          four_t<T> v;
+#pragma unroll
+          for (int r = 0; r < 4; ++r) v[r] = from_f32<T>(dx[d][i][r]);
+          *(four_t<T>*)at = v;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < a.width) at[r] = from_f32<T>(dx[d][i][r]);
+        }
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The weights' gradients.  A wavefront owns 16 FT hidden columns: their weights and the
+// accumulators of their gradients stay in its registers while it walks the rows, 32 at a
+// time.  g, u and dh are taken with the rows first (the same fragments, exchanged), so a
+// lane holds, of one hidden column, the rows that the second operand of
+// dWg' = x' dg wants of it; x' and dy' come out of LDS by the transposing read from the
+// tile that x and dy are read from as they lie.  The wavefronts of a workgroup share the
+// tile; the rows are dealt over gridDim.x workgroups, whose partial sums a second launch
+// joins.  db of the hidden products adds up beside, dbd is dy' times ones.
+// ---------------------------------------------------------------------------
+
+template <typename T>
+struct WeightArgs {
+  using E = typename Planes<T>::E;
+  Operand<E> x, dy;
+  const T *wg, *wu, *wd, *bg, *bu;
+  float *dwgu, *dwd, *sums, *dy_sums;  // [gridDim.x, ...]; dy_sums nullable
+  int64_t rows;
+  int32_t width, hidden, out, act, add;
+};
+
+// Rows of a tile in LDS, of STEPS k steps of 32 (64 bytes each), and what its 16-byte
+// chunks are exchanged with: the rows that one read touches together differ in bits 0, 1
+// and 3.
+template <int STEPS>
+struct RowTile {
+  static constexpr int PITCH = STEPS * 64, CHUNKS = STEPS * 4;
+  __device__ static __forceinline__ int turn(int row) {
+    if constexpr (STEPS == 1) return ((row >> 1) & 1) | ((row >> 2) & 2);
+    if constexpr (STEPS == 2) return (row & 3) | ((row >> 1) & 4);
+    return ((row & 3) | ((row >> 1) & 4)) << 1;
+  }
+  template <typename E, int ROWS>
+  __device__ static __forceinline__ void load(char* lds, const E* p, int64_t pitch, int64_t m0,
+                                              int64_t rows, int32_t cols8, int waves) {
+    constexpr int PER = 64 / CHUNKS;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int j = wave; j < ROWS / PER; j += waves) {
+      const int first = j * PER;
+      const int64_t left = rows - m0 - first;
+      const rsrc_t r = buffer_of(
+          p + (m0 + first) * pitch,
+          left > 0 ? (uint32_t)(((left < PER ? left : PER) - 1) * pitch + cols8) * 2 : 0);
+      const int row = first + lane / CHUNKS, c = (lane % CHUNKS) ^ turn(row);
+      uint32_t off = (uint32_t)(lane / CHUNKS * pitch + c * 8) * 2;
+      if (c * 8 >= cols8) off = MX_OUTSIDE;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + first * PITCH), 16, off, 0, 0, 0);
+    }
+  }
+  // Rows first: tile t of the 32 rows from `row` on, dealt as a chunk's hidden columns are.
+  template <typename E>
+  __device__ static __forceinline__ frag_t<E> rows(const char* lds, int row, int t, int k) {
+    const int lane = threadIdx.x & 63;
+    const int r = row + dealt(0, t, lane & 15);
+    return *(const frag_t<E>*)(lds + r * PITCH + ((k * 4 + (lane >> 4)) ^ turn(r)) * 16);
+  }
+  // Columns first: 16 columns from `col` on by the 32 rows.
+  template <typename E>
+  __device__ static __forceinline__ frag_t<E> columns(const char* lds, int row, int col) {
+    const int lane = threadIdx.x & 63;
+    const int r = row + (lane >> 4) * 8 + ((lane >> 2) & 3), c = (col >> 3) + ((lane >> 1) & 1);
+    typedef short s4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s4 lds_s4;
+    const char* at = lds + (lane & 1) * 8;
+    union {
+      s4 h[2];
+      frag_t<E> f;
+    } u;
+    u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(at + r * PITCH + (c ^ turn(r)) * 16));
+    u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        (lds_s4*)(at + (r + 4) * PITCH + (c ^ turn(r + 4)) * 16));
+    return u.f;
+  }
+};
+
+template <typename T>
+constexpr int weight_rows() {  // of a staged tile
+  return Planes<T>::N == 1 ? 64 : 32;
+}
+
+template <typename T, int DK, int OK, int FT>
+__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T> a) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N, DT = 2 * DK, OT = 2 * OK, ROWS = weight_rows<T>();
+  using X = RowTile<DK>;
+  using Y = RowTile<OK>;
+  constexpr int XB = ROWS * X::PITCH, YB = ROWS * Y::PITCH, BYTES = P * (XB + YB);
+  __shared__ __attribute__((aligned(1024))) char lds[2 * BYTES];
+  const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int f0 = (blockIdx.y * waves + wave) * 16 * FT;
+  const bool sum_dy = a.dy_sums && blockIdx.y == 0 && wave == 0;
+  const int width8 = (a.width + 7) & ~7, out8 = (a.out + 7) & ~7;
+
+  frag_t<E> wg[FT][DK][P], wu[FT][DK][P], wd[FT][OK][P];
+  float bg[FT], bu[FT];
+#pragma unroll
+  for (int i = 0; i < FT; ++i) {
+    const int f = f0 + i * 16 + (lane & 15);
+    const bool live = f < a.hidden;
+    bg[i] = a.bg && live ? to_f32(a.bg[f]) : 0.f;
+    bu[i] = a.bu && live ? to_f32(a.bu[f]) : 0.f;
+#pragma unroll
+    for (int k = 0; k < DK; ++k) {
+      const int c = k * 32 + (lane >> 4) * 8;
+      load_fragment<T>(a.wg + (int64_t)f * a.width, c, a.width, live, false, wg[i][k]);
+      load_fragment<T>(a.wu + (int64_t)f * a.width, c, a.width, live, false, wu[i][k]);
+    }
+#pragma unroll
+    for (int k = 0; k < OK; ++k)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int o = k * 32 + (lane >> 4) * 8 + j;
+        E p[P];
+        split<T>(live && o < a.out ? to_f32(a.wd[(int64_t)o * a.hidden + f]) : 0.f, p);
+#pragma unroll
+        for (int s = 0; s < P; ++s) wd[i][k][s][j] = p[s];
+      }
+  }
+  frag_t<E> ones;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) ones[j] = (E)1.f;
+
+  f32x4 dwg[FT][DT] = {}, dwu[FT][DT] = {}, dwd[FT][OT] = {}, dys[OT] = {};
+  float sg[FT] = {}, su[FT] = {};
+  const int64_t tiles = (a.rows + ROWS - 1) / ROWS;
+  const auto stage = [&](int64_t tile, char* to) {
+#pragma unroll
+    for (int s = 0; s < P; ++s) {
+      X::template load<E, ROWS>(to + s * XB, a.x.p + s * a.x.plane, a.x.pitch, tile * ROWS, a.rows,
+                                width8, waves);
+      Y::template load<E, ROWS>(to + P * XB + s * YB, a.dy.p + s * a.dy.plane, a.dy.pitch,
+                                tile * ROWS, a.rows, out8, waves);
+    }
+  };
+  if (blockIdx.x < tiles) stage(blockIdx.x, lds);
+  int turn = 0;
+  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
+    __syncthreads();  // the tile is there, and nobody reads the one before it
+    const char* xs = lds + turn * BYTES;
+    const char* ys = xs + P * XB;
+    if (tile + gridDim.x < tiles) stage(tile + gridDim.x, lds + (turn ^ 1) * BYTES);
+    if (f0 >= a.hidden) continue;
+#pragma unroll 1
+    for (int row = 0; row < ROWS; row += 32) {
+      frag_t<E> dg[FT][P], du[FT][P], h[FT][P];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        f32x4 g[FT], u[FT], dh[FT] = {};
+#pragma unroll
+        for (int i = 0; i < FT; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) g[i][r] = bg[i], u[i][r] = bu[i];
+#pragma unroll
+        for (int k = 0; k < DK; ++k) {
+          frag_t<E> x[P];
+#pragma unroll
+          for (int s = 0; s < P; ++s) x[s] = X::template rows<E>(xs + s * XB, row, t, k);
+#pragma unroll
+          for (int i = 0; i < FT; ++i) {
+            g[i] = mfma_planes<T>(x, wg[i][k], g[i]);
+            u[i] = mfma_planes<T>(x, wu[i][k], u[i]);
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < OK; ++k) {
+          frag_t<E> y[P];
+#pragma unroll
+          for (int s = 0; s < P; ++s) y[s] = Y::template rows<E>(ys + s * YB, row, t, k);
+#pragma unroll
+          for (int i = 0; i < FT; ++i) dh[i] = mfma_planes<T>(y, wd[i][k], dh[i]);
+        }
+        with_activation(a.act, [&](auto act) {
+#pragma unroll
+          for (int i = 0; i < FT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              const float2 v = activation<T, act.value>(g[i][r]);
+              const float vg = dh[i][r] * u[i][r] * v.y, vu = dh[i][r] * v.x;
+              sg[i] += vg;
+              su[i] += vu;
+              E p[P];
+              split<T>(vg, p);
+#pragma unroll
+              for (int s = 0; s < P; ++s) dg[i][s][t * 4 + r] = p[s];
+              split<T>(vu, p);
+#pragma unroll
+              for (int s = 0; s < P; ++s) du[i][s][t * 4 + r] = p[s];
+              split<T>(v.x * u[i][r], p);
+#pragma unroll
+              for (int s = 0; s < P; ++s) h[i][s][t * 4 + r] = p[s];
+            }
+        });
+      }
+#pragma unroll
+      for (int d = 0; d < DT; ++d) {
+        frag_t<E> x[P];
+#pragma unroll
+        for (int s = 0; s < P; ++s) x[s] = X::template columns<E>(xs + s * XB, row, d * 16);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+          dwg[i][d] = mfma_planes<T>(x, dg[i], dwg[i][d]);
+          dwu[i][d] = mfma_planes<T>(x, du[i], dwu[i][d]);
+        }
+      }
+#pragma unroll
+      for (int o = 0; o < OT; ++o) {
+        frag_t<E> y[P];
+#pragma unroll
+        for (int s = 0; s < P; ++s) y[s] = Y::template columns<E>(ys + s * YB, row, o * 16);
+#pragma unroll
+        for (int i = 0; i < FT; ++i) dwd[i][o] = mfma_planes<T>(h[i], y, dwd[i][o]);
+        if (sum_dy)
+#pragma unroll
+          for (int s = P - 1; s >= 0; --s) dys[o] = mfma32(y[s], ones, dys[o]);
+      }
+    }
+  }
+
+  const auto put = [&](float* at, float v) { *at = a.add ? *at + v : v; };
+  float* gu_part = a.dwgu + (int64_t)blockIdx.x * 2 * a.hidden * a.width;
+  float* d_part = a.dwd + (int64_t)blockIdx.x * a.out * a.hidden;
+  float* s_part = a.sums + (int64_t)blockIdx.x * 2 * a.hidden;
+#pragma unroll
+  for (int i = 0; i < FT; ++i) {
+    const int f = f0 + i * 16 + (lane & 15);
+    sg[i] += __shfl_xor(sg[i], 16, 64);
+    sg[i] += __shfl_xor(sg[i], 32, 64);
+    su[i] += __shfl_xor(su[i], 16, 64);
+    su[i] += __shfl_xor(su[i], 32, 64);
+    if (lane < 16 && f < a.hidden) {
+      put(s_part + f, sg[i]);
+      put(s_part + a.hidden + f, su[i]);
+    }
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = d * 16 + (lane >> 4) * 4 + r;
+        if (f < a.hidden && n < a.width) {
+          put(gu_part + (int64_t)f * a.width + n, dwg[i][d][r]);
+          put(gu_part + (int64_t)(a.hidden + f) * a.width + n, dwu[i][d][r]);
+        }
+      }
+#pragma unroll
+    for (int o = 0; o < OT; ++o) {
+      const int n = o * 16 + (lane & 15);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int ff = f0 + i * 16 + (lane >> 4) * 4 + r;
+        if (n < a.out && ff < a.hidden) put(d_part + (int64_t)n * a.hidden + ff, dwd[i][o][r]);
+      }
+    }
+  }
+  if (sum_dy && (lane & 15) == 0)
+#pragma unroll
+    for (int o = 0; o < OT; ++o)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int n = o * 16 + (lane >> 4) * 4 + r;
+        if (n < a.out) put(a.dy_sums + (int64_t)blockIdx.x * a.out + n, dys[o][r]);
+      }
+}
+
+// ---------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------
+
 // Calls f(DK, OT) as constants.
 template <typename F>
 static void with_narrow(int width, int out, F&& f) {
@@ -264,36 +682,157 @@ bool RowKernels<T>::takes(int64_t rows, int32_t width, int32_t hidden, int32_t o
   return width <= NARROW && out <= NARROW;
 }
 
+// Calls f(DK, OK) as constants.
+template <typename F>
+static void with_narrow_back(int width, int out, F&& f) {
+  const auto by_out = [&](auto dk) {
+    if (out <= 32) return f(dk, std::integral_constant<int, 1>());
+    if (out <= 64) return f(dk, std::integral_constant<int, 2>());
+    return f(dk, std::integral_constant<int, 4>());
+  };
+  if (width <= 32) return by_out(std::integral_constant<int, 1>());
+  if (width <= 64) return by_out(std::integral_constant<int, 2>());
+  return by_out(std::integral_constant<int, 4>());
+}
+
+#define ROW_PASS (1 << 20)  // rows whose x and dy are laid out at a time
+
+// The backward's workspace.
+template <typename T, int DK, int OK>
+struct RowPlan {
+  using E = typename Planes<T>::E;
+  static constexpr int FT = Planes<T>::N == 1 && DK <= 2 && OK <= 2 ? 2 : 1;
+  int64_t pass;
+  int waves, columns, runs;  // of a workgroup; workgroups along hidden and along rows
+  char* packed;
+  E *x, *dy;
+  float *dwgu, *dwd, *sums, *dy_sums;
+  uint64_t bytes;
+  RowPlan(void* ws, int64_t rows, int64_t width, int64_t hidden, int64_t out) {
+    constexpr int P = Planes<T>::N;
+    pass = std::min<int64_t>(rows, ROW_PASS);
+    const int64_t slices = tiles(hidden, 16 * FT);
+    waves = (int)std::min<int64_t>(slices, FR_WAVES);
+    columns = (int)tiles(slices, waves);
+    // workgroups that the chip holds at once: 256 of eight wavefronts
+    runs = (int)std::max<int64_t>(
+        1, std::min<int64_t>(tiles(pass, weight_rows<T>()), 256 * FR_WAVES / (waves * columns)));
+    Carver c{(char*)ws};
+    packed = c.take<char>(BackwardChunk<T, DK, OK>::KB * 1024 * tiles(hidden, 32));
+    x = c.take<E>(P * pass * round8(width));
+    dy = c.take<E>(P * pass * round8(out));
+    dwgu = c.take<float>(runs * 2 * hidden * width);
+    dwd = c.take<float>(runs * hidden * out);
+    sums = c.take<float>(runs * 2 * hidden);
+    dy_sums = c.take<float>(runs * out);
+    bytes = c.used;
+  }
+};
+
 template <typename T>
-uint64_t RowKernels<T>::workspace(int32_t width, int32_t hidden, int32_t out) {
-  uint64_t kb = 0;
-  with_narrow(width, out, [&](auto dk, auto ot) { kb = ForwardChunk<T, dk.value, ot.value>::KB; });
-  return kb * 1024 * ((hidden + 31) / 32);
+uint64_t RowKernels<T>::workspace(int64_t rows, int32_t width, int32_t hidden, int32_t out,
+                                  bool back) {
+  uint64_t bytes = 0;
+  if (back)
+    with_narrow_back(width, out, [&](auto dk, auto ok) {
+      bytes = RowPlan<T, dk.value, ok.value>(nullptr, rows, width, hidden, out).bytes;
+    });
+  else
+    with_narrow(width, out, [&](auto dk, auto ot) {
+      bytes = ForwardChunk<T, dk.value, ot.value>::KB * 1024 * tiles(hidden, 32);
+    });
+  return bytes;
+}
+
+// Whether rows can be read 16 bytes at a time.
+template <typename T>
+static bool wide_rows(const void* p, int64_t cols, int64_t pitch) {
+  return cols % Vec16<T>::N == 0 && aligned16((const T*)p, pitch);
+}
+template <typename T>
+static bool wide_stores(const void* p, int64_t cols) {
+  return cols % 4 == 0 && aligned16((const T*)p, 0);
+}
+
+// Rows that fill the chip with wavefronts of 16 RT rows take them (RT as a constant), fewer
+// take 16.
+template <int MANY, typename F>
+static void with_rows(int64_t rows, F&& f) {
+  const auto launch = [&](auto rt) {
+    f(rt, (unsigned)std::min<int64_t>(tiles(rows, 16 * rt.value * FR_WAVES), 512));
+  };
+  if (rows >= 16 * MANY * FR_WAVES * 256)
+    launch(std::integral_constant<int, MANY>());
+  else
+    launch(std::integral_constant<int, 1>());
 }
 
 template <typename T>
 void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t stream) {
-  const int chunks = (c.hidden + 31) / 32;
+  const int chunks = (int)tiles(c.hidden, 32);
   with_narrow(c.width, c.out, [&](auto dk, auto ot) {
     constexpr int DK = dk.value, OT = ot.value;
     using C = ForwardChunk<T, DK, OT>;
     const PackArgs pack{c.wg, c.wu, c.wd, c.bg, c.bu, (char*)workspace, c.width, c.hidden, c.out,
-                        chunks, DK, OT, C::KB};
-    hipLaunchKernelGGL(ffn_pack_kernel<T>, dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0, stream,
-                       pack);
+                        DK, OT, 0, C::KB};
+    hipLaunchKernelGGL((ffn_pack_kernel<T, false>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
+                       stream, pack);
     const ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
                            c.x_pitch, c.width, c.out, chunks, c.act,
-                           c.width % Vec16<T>::N == 0 && aligned16((const T*)c.x, c.x_pitch),
-                           c.out % 4 == 0 && aligned16((const T*)c.y, 0)};
-    const auto launch = [&](auto kernel, int rt) {
-      const int64_t tiles = (c.rows + 16 * rt * FR_WAVES - 1) / (16 * rt * FR_WAVES);
-      hipLaunchKernelGGL(kernel, dim3((unsigned)std::min<int64_t>(tiles, 512)), dim3(64 * FR_WAVES),
-                         0, stream, a);
-    };
+                           wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
     constexpr int MANY = Planes<T>::N == 1 && DK <= 2 && OT <= 4 ? 4 : 2;
-    if (c.rows >= 16 * MANY * FR_WAVES * 256)
-      launch(ffn_rows_fwd_kernel<T, DK, OT, MANY>, MANY);
-    else
-      launch(ffn_rows_fwd_kernel<T, DK, OT, 1>, 1);
+    with_rows<MANY>(c.rows, [&](auto rt, unsigned groups) {
+      hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value>), dim3(groups),
+                         dim3(64 * FR_WAVES), 0, stream, a);
+    });
+  });
+}
+
+template <typename T>
+void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stream) {
+  with_narrow_back(c.width, c.out, [&](auto dk, auto ok) {
+    constexpr int DK = dk.value, OK = ok.value;
+    using C = BackwardChunk<T, DK, OK>;
+    const RowPlan<T, DK, OK> p(workspace, c.rows, c.width, c.hidden, c.out);
+    const int chunks = (int)tiles(c.hidden, 32);
+    if (c.dx) {
+      const PackArgs pack{c.wg, c.wu, c.wd, c.bg, c.bu, p.packed, c.width, c.hidden, c.out,
+                          DK, 0, OK, C::KB};
+      hipLaunchKernelGGL((ffn_pack_kernel<T, true>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
+                         stream, pack);
+      const BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
+                              c.dy_pitch, c.width, c.out, chunks, c.act,
+                              wide_rows<T>(c.x, c.width, c.x_pitch),
+                              wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
+      constexpr int MANY = 2;
+      with_rows<MANY>(c.rows, [&](auto rt, unsigned groups) {
+        hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value>), dim3(groups),
+                           dim3(64 * FR_WAVES), 0, stream, a);
+      });
+    }
+    if (!(c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd)) return;
+    Layer<T> lay;
+    for (int64_t r = 0; r < c.rows; r += p.pass) {
+      const int64_t m = std::min(p.pass, c.rows - r);
+      WeightArgs<T> a{};
+      a.x = lay.operand(row_at<T>(c.x, r, c.x_pitch), m, c.width, c.x_pitch, p.x);
+      a.dy = lay.operand(row_at<T>(c.dy, r, c.dy_pitch), m, c.out, c.dy_pitch, p.dy);
+      lay.launch(stream);
+      a.wg = (const T*)c.wg, a.wu = (const T*)c.wu, a.wd = (const T*)c.wd;
+      a.bg = (const T*)c.bg, a.bu = (const T*)c.bu;
+      a.dwgu = p.dwgu, a.dwd = p.dwd, a.sums = p.sums, a.dy_sums = c.dbd ? p.dy_sums : nullptr;
+      a.rows = m, a.width = c.width, a.hidden = c.hidden, a.out = c.out, a.act = c.act, a.add = r > 0;
+      hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT>),
+                         dim3(p.runs, p.columns), dim3(64 * p.waves), 0, stream, a);
+    }
+    const int64_t F = c.hidden, D = c.width, O = c.out;
+    Joiner<T> join;
+    join.add(p.dwgu, 2 * F * D, D, p.runs, F, D, c.dwg);
+    join.add(p.dwgu + F * D, 2 * F * D, D, p.runs, F, D, c.dwu);
+    join.add(p.dwd, O * F, F, p.runs, O, F, c.dwd);
+    join.add(p.sums, 2 * F, F, p.runs, 1, F, c.dbg);
+    join.add(p.sums + F, 2 * F, F, p.runs, 1, F, c.dbu);
+    join.add(p.dy_sums, O, O, p.runs, 1, O, c.dbd);
+    join.launch(stream);
   });
 }
