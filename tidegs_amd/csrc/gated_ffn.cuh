@@ -37,9 +37,55 @@ __device__ __forceinline__ float2 activation(float g) {
   }
 }
 
-// Calls f with the activation as a constant (the branch is the same for all lanes).
+// Eight values of a row from column c on (zeros past the width), as planes.
+template <typename T>
+__device__ __forceinline__ void load_fragment(const T* row, int c, int width, bool live, bool wide,
+                                              frag_t<typename Planes<T>::E> (&out)[Planes<T>::N]) {
+  using E = typename Planes<T>::E;
+  constexpr int P = Planes<T>::N, V = Vec16<T>::N;
+  T v[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v[e] = (T)0.f;
+  if (live) {
+    if (wide) {  // rows on 16 bytes, a whole number of 16-byte runs
+#pragma unroll
+      for (int e = 0; e < 8; e += V)
+        if (c + e < width) *(Vec16<T>*)(v + e) = *(const Vec16<T>*)(row + c + e);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < width) v[e] = row[c + e];
+    }
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    E p[P];
+    split<T>(to_f32(v[e]), p);
+#pragma unroll
+    for (int s = 0; s < P; ++s) out[s][e] = p[s];
+  }
+}
+
+// a b over the pairs of planes.
+template <typename T>
+__device__ __forceinline__ f32x4 mfma_planes(const frag_t<typename Planes<T>::E> (&a)[Planes<T>::N],
+                                             const frag_t<typename Planes<T>::E> (&b)[Planes<T>::N],
+                                             f32x4 c) {
+  if constexpr (Planes<T>::N == 1) {
+    return mfma32(a[0], b[0], c);
+  } else {
+    c = mfma32(a[2], b[0], c);
+    c = mfma32(a[0], b[2], c);
+    c = mfma32(a[1], b[1], c);
+    c = mfma32(a[1], b[0], c);
+    c = mfma32(a[0], b[1], c);
+    return mfma32(a[0], b[0], c);
+  }
+}
+
+// Calls f with the activation as a constant.
 template <typename F>
-__device__ __forceinline__ void with_activation(int act, F&& f) {
+__host__ __device__ __forceinline__ void with_activation(int act, F&& f) {
   if (act == ACT_SILU)
     f(std::integral_constant<int, ACT_SILU>());
   else if (act == ACT_GELU)
@@ -108,7 +154,7 @@ struct JoinJob {
   const float* partial;
   int64_t part;       // values between two partial sums
   int64_t pitch;      // of a row of them
-  int32_t parts, cols;
+  int32_t parts, cols, groups;  // groups: threads of a value
   int64_t rows;
   void* out;          // [rows, cols]
   uint32_t blocks;    // of the launch, up to and with this job's
@@ -118,18 +164,31 @@ struct JoinJobs {
   JoinJob job[JOIN_JOBS];
 };
 
+// A job's workgroup takes 256 / groups values, each summed by `groups` threads over parts g,
+// g + groups, ... and then over the threads: one thread per value took 62 us for 256 parts of
+// 49k values, a load after another, 32 take 12.
 template <typename T>
 __global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
+  __shared__ float s[256];
   int k = 0;
   uint32_t first = 0;
   while (blockIdx.x >= jobs.job[k].blocks) first = jobs.job[k++].blocks;
   const JoinJob& job = jobs.job[k];
-  const int64_t i = (int64_t)(blockIdx.x - first) * 256 + threadIdx.x;
-  if (i >= job.rows * job.cols) return;
-  const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
+  const int each = 256 / job.groups, e = threadIdx.x % each, g = threadIdx.x / each;
+  const int64_t i = (int64_t)(blockIdx.x - first) * each + e;
+  const bool live = i < job.rows * job.cols;
   float acc = 0.f;
-  for (int s = 0; s < job.parts; ++s) acc += p[s * job.part];
-  ((T*)job.out)[i] = from_f32<T>(acc);
+  if (live) {
+    const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
+#pragma unroll 4
+    for (int part = g; part < job.parts; part += job.groups) acc += p[part * job.part];
+  }
+  s[threadIdx.x] = acc;
+  for (int h = job.groups >> 1; h > 0; h >>= 1) {
+    __syncthreads();
+    if (g < h) s[threadIdx.x] += s[threadIdx.x + h * each];
+  }
+  if (live && g == 0) ((T*)job.out)[i] = from_f32<T>(s[threadIdx.x]);
 }
 
 // ---------------------------------------------------------------------------
@@ -193,19 +252,29 @@ struct Joiner {
   void add(const float* partial, int64_t part, int64_t pitch, int64_t parts, int64_t rows,
            int64_t cols, void* to) {
     if (!to) return;
-    blocks += (uint32_t)tiles(rows * cols, 256);
-    jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, rows, to, blocks};
+    const int groups = parts > 32 ? 32 : parts > 4 ? 8 : 1;
+    blocks += (uint32_t)tiles(rows * cols, 256 / groups);
+    jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, groups, rows, to,
+                            blocks};
   }
   void launch(hipStream_t s) {
     if (n) hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);
   }
 };
 
+// Few rows (gated_ffn_few.hip): the weights' bytes are the work.
+#define FEW_ROWS 64
+template <typename T>
+struct FewKernels {
+  static uint64_t workspace(int64_t rows, int32_t hidden);
+  static void forward(const FfnCall& c, void* workspace, hipStream_t stream);
+};
+
 // Narrow rows (gated_ffn_rows.cuh): whether a call's sizes are theirs, the workspace they
 // take and their launches.
 template <typename T>
 struct RowKernels {
-  static bool takes(int64_t rows, int32_t width, int32_t hidden, int32_t out);
+  static bool takes(int32_t width, int32_t out);
   static uint64_t workspace(int64_t rows, int32_t width, int32_t hidden, int32_t out, bool back);
   static void forward(const FfnCall& c, void* workspace, hipStream_t stream);
   static void backward(const FfnCall& c, void* workspace, hipStream_t stream);

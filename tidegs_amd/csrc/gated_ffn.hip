@@ -175,7 +175,10 @@ struct ProductArgs {
   int32_t b_limit;
   int32_t splits;           // of the steps over k
   const void* bias;
-  void* c;                  // [M, N] of the call's type
+  void* c;                  // [M, N] of the call's type, or, of its first and second half of
+  void* c2;                 // rows, `each` to c and to c2 (each: 0 or less than M / 2; null: left out)
+  int64_t each;
+  int32_t wide;             // c is written four values at a time
   float* partial;           // or [splits, M, N]
   int32_t add;              // add to what `partial` holds
 };
@@ -226,11 +229,22 @@ __global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typenam
         for (int r = 0; r < 4; ++r)
           if (n + r < g.N) at[r] = g.add ? at[r] + acc[i][j][r] : acc[i][j][r];
       } else {
-        T* at = (T*)g.c + m * g.N + n;
+        const bool upper = g.each && m >= g.M / 2;
+        const int64_t row = upper ? m - g.M / 2 : m;
+        T* c = (T*)(upper ? g.c2 : g.c);
+        if (!c || (g.each && row >= g.each)) continue;
+        T* at = c + row * g.N + n;
+        four_t<T> v;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          if (n + r < g.N)
-            at[r] = from_f32<T>(acc[i][j][r] + (g.bias ? to_f32(((const T*)g.bias)[n + r]) : 0.f));
+          v[r] = from_f32<T>(acc[i][j][r] + (g.bias && n + r < g.N ? to_f32(((const T*)g.bias)[n + r]) : 0.f));
+        if (g.wide) {
+          if (n < g.N) *(four_t<T>*)at = v;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (n + r < g.N) at[r] = v[r];
+        }
       }
     }
   }
@@ -314,15 +328,17 @@ struct Plan {
       dy_sums = c.take<float>(COLUMN_RUNS * O);
       split_gu = splits_of(tiles(2 * F8, GT) * tiles(D, GT), pass);
       split_d = splits_of(tiles(O, GT) * tiles(F, GT), pass);
-      dwgu = c.take<float>(split_gu * 2 * F8 * D);
-      dwd = c.take<float>(split_d * O * F);
+      // (one sum over all rows is rounded where it is taken)
+      dwgu = split_gu > 1 || pass < rows ? c.take<float>(split_gu * 2 * F8 * D) : nullptr;
+      dwd = split_d > 1 || pass < rows ? c.take<float>(split_d * O * F) : nullptr;
     }
     bytes = c.used;
   }
 };
 
 template <typename T, Along KA, Along KB>
-static void product(hipStream_t s, const ProductArgs<typename Planes<T>::E>& g) {
+static void product(hipStream_t s, ProductArgs<typename Planes<T>::E> g) {
+  g.wide = g.N % 4 == 0 && aligned16((const T*)g.c, 0) && aligned16((const T*)g.c2, 0);
   const int64_t n = tiles(g.M, GT) * tiles(g.N, GT) * g.splits;
   hipLaunchKernelGGL((ffn_product_kernel<T, KA, KB>), dim3((unsigned)n), dim3(256), 0, s, g);
 }
@@ -333,8 +349,9 @@ static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, u
   with_dtype(dtype, "tgs_gated_ffn workspace", [&](auto tag) -> int {
     using T = decltype(tag);
     bytes = Plan<T>(nullptr, rows, width, hidden, out, back).bytes;
-    if (RowKernels<T>::takes(rows, width, hidden, out))
+    if (RowKernels<T>::takes(width, out))
       bytes = RowKernels<T>::workspace(rows, width, hidden, out, back);
+    if (!back) bytes = std::max(bytes, FewKernels<T>::workspace(std::min<int64_t>(rows, FEW_ROWS), hidden));
     return TGS_OK;
   });
   return bytes;
@@ -367,11 +384,15 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_fwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
-    if (RowKernels<T>::takes(rows, width, hidden, out)) {
-      FfnCall c{};
-      c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
-      c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
-      c.bg = b_gate, c.bu = b_up, c.bd = b_down, c.y = y;
+    FfnCall c{};
+    c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
+    c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
+    c.bg = b_gate, c.bu = b_up, c.bd = b_down, c.y = y;
+    if (rows <= FEW_ROWS) {
+      FewKernels<T>::forward(c, workspace, stream);
+      TGS_RETURN_LAUNCH("tgs_gated_ffn_fwd");
+    }
+    if (RowKernels<T>::takes(width, out)) {
       RowKernels<T>::forward(c, workspace, stream);
       TGS_RETURN_LAUNCH("tgs_gated_ffn_fwd");
     }
@@ -420,7 +441,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_bwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
-    if (rows && RowKernels<T>::takes(rows, width, hidden, out)) {
+    if (rows && RowKernels<T>::takes(width, out)) {
       FfnCall c{};
       c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
       c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
@@ -463,13 +484,14 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
         g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.b = a.x;
         g.M = 2 * p.F8, g.N = p.D, g.K = m, g.a_limit = 2 * p.F8, g.b_limit = p.D8;
         g.splits = p.split_gu, g.partial = p.dwgu, g.add = r > 0;
+        g.c = dw_gate, g.c2 = dw_up, g.each = p.F;
         product<T, ACROSS, ACROSS>(stream, g);
       }
       if (dw_down) {
         ProductArgs<E> g{};
         g.a = a.dy, g.b = {p.h, a.plane, p.F8};
         g.M = p.O, g.N = p.F, g.K = m, g.a_limit = p.O8, g.b_limit = p.F8;
-        g.splits = p.split_d, g.partial = p.dwd, g.add = r > 0;
+        g.splits = p.split_d, g.partial = p.dwd, g.add = r > 0, g.c = dw_down;
         product<T, ACROSS, ACROSS>(stream, g);
       }
       if (db_down)
@@ -479,9 +501,11 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
     }
     Joiner<T> join;
     const int64_t some = p.rows > 0;  // no rows: sums of nothing
-    join.add(p.dwgu, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_gate);
-    join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up);
-    join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down);
+    if (p.dwgu || !some) {
+      join.add(p.dwgu, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_gate);
+      join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up);
+    }
+    if (p.dwd || !some) join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down);
     const int64_t row_tiles = tiles(p.pass, FT_M);
     join.add(p.gu_sums, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_gate);
     join.add(p.gu_sums + p.F8, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_up);

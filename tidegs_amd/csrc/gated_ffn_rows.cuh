@@ -89,35 +89,6 @@ __global__ void __launch_bounds__(64) ffn_pack_kernel(PackArgs a) {
   for (int s = 0; s < P; ++s) ((frag_t<E>*)(base + (q * P + s) * 1024))[lane] = out[s];
 }
 
-// Eight values of a row from column c on (zeros past the width), as planes.
-template <typename T>
-__device__ __forceinline__ void load_fragment(const T* row, int c, int width, bool live, bool wide,
-                                              frag_t<typename Planes<T>::E> (&out)[Planes<T>::N]) {
-  using E = typename Planes<T>::E;
-  constexpr int P = Planes<T>::N, V = Vec16<T>::N;
-  T v[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = (T)0.f;
-  if (live) {
-    if (wide) {  // rows on 16 bytes, a whole number of 16-byte runs
-#pragma unroll
-      for (int e = 0; e < 8; e += V)
-        if (c + e < width) *(Vec16<T>*)(v + e) = *(const Vec16<T>*)(row + c + e);
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < width) v[e] = row[c + e];
-    }
-  }
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    E p[P];
-    split<T>(to_f32(v[e]), p);
-#pragma unroll
-    for (int s = 0; s < P; ++s) out[s][e] = p[s];
-  }
-}
-
 template <typename T>
 struct ForwardArgs {
   const T* x;
@@ -125,27 +96,10 @@ struct ForwardArgs {
   const char* packed;
   const T* bd;
   int64_t rows, x_pitch;
-  int32_t width, out, chunks, act;
+  int32_t width, out, chunks;
   int32_t wide;      // x is read 16 bytes at a time
   int32_t wide_out;  // y is written four values at a time
 };
-
-// a b over the pairs of planes.
-template <typename T>
-__device__ __forceinline__ f32x4 mfma_planes(const frag_t<typename Planes<T>::E> (&a)[Planes<T>::N],
-                                             const frag_t<typename Planes<T>::E> (&b)[Planes<T>::N],
-                                             f32x4 c) {
-  if constexpr (Planes<T>::N == 1) {
-    return mfma32(a[0], b[0], c);
-  } else {
-    c = mfma32(a[2], b[0], c);
-    c = mfma32(a[0], b[2], c);
-    c = mfma32(a[1], b[1], c);
-    c = mfma32(a[1], b[0], c);
-    c = mfma32(a[0], b[1], c);
-    return mfma32(a[0], b[0], c);
-  }
-}
 
 // KB kilobytes to LDS by WAVES wavefronts, without registers.
 template <int KB, int WAVES>
@@ -161,19 +115,18 @@ __device__ __forceinline__ void copy_chunk(char* lds, const char* src) {
 
 #define FR_WAVES 8
 
-template <typename T, int DK, int OT, int RT>
-__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
+template <typename T, int DK, int OT, int RT, int ACT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N;
   using C = ForwardChunk<T, DK, OT>;
   __shared__ __attribute__((aligned(1024))) char lds[2 * C::KB * 1024];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int TILE = 16 * RT * FR_WAVES;
-  const int64_t tiles = (a.rows + TILE - 1) / TILE;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t m0 = tile * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
+  constexpr int TILE = 16 * RT * WAVES;
+  {
+    const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
+    copy_chunk<C::KB, WAVES>(lds, a.packed);
     frag_t<E> x[RT][DK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -188,7 +141,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
       __syncthreads();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (c & 1) * C::KB * 1024;
       if (c + 1 < a.chunks)
-        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
+        copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
                                     a.packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
@@ -212,17 +165,15 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
 #pragma unroll
           for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
         }
-        with_activation(a.act, [&](auto act) {
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               E p[P];
-              split<T>(activation<T, act.value>(g[i][r]).x * u[i][r], p);
+              split<T>(activation<T, ACT>(g[i][r]).x * u[i][r], p);
 #pragma unroll
               for (int s = 0; s < P; ++s) h[i][s][t * 4 + r] = p[s];
             }
-        });
       }
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
@@ -232,7 +183,6 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
         for (int i = 0; i < RT; ++i) y[o][i] = mfma_planes<T>(w, h[i], y[o][i]);
       }
     }
-    __syncthreads();  // (the next rows' first chunk goes where the last one lay)
 #pragma unroll
     for (int o = 0; o < OT; ++o) {
       const int n = o * 16 + (lane >> 4) * 4;
@@ -270,12 +220,12 @@ struct BackwardArgs {
   T* dx;
   const char* packed;
   int64_t rows, x_pitch, dy_pitch;
-  int32_t width, out, chunks, act;
+  int32_t width, out, chunks;
   int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
 };
 
-template <typename T, int DK, int OK, int RT>
-__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs<T> a) {
+template <typename T, int DK, int OK, int RT, int ACT, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) ffn_rows_dx_kernel(BackwardArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK;
   using C = BackwardChunk<T, DK, OK>;
@@ -283,11 +233,10 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * C::KB * 1024];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int TILE = 16 * RT * FR_WAVES;
-  const int64_t tiles = (a.rows + TILE - 1) / TILE;
-  for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const int64_t m0 = tile * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
+  constexpr int TILE = 16 * RT * WAVES;
+  {
+    const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
+    copy_chunk<C::KB, WAVES>(lds, a.packed);
     frag_t<E> x[RT][DK][P], dy[RT][OK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -304,12 +253,12 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
     for (int c = 0; c < a.chunks; ++c) {
       if (BUFFERS == 1 && c) {
         __syncthreads();
-        copy_chunk<C::KB, FR_WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
+        copy_chunk<C::KB, WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
       }
       __syncthreads();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
       if (BUFFERS == 2 && c + 1 < a.chunks)
-        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
+        copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
                                     a.packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
@@ -339,12 +288,11 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
 #pragma unroll
           for (int i = 0; i < RT; ++i) dh[i] = mfma_planes<T>(w, dy[i][k], dh[i]);
         }
-        with_activation(a.act, [&](auto act) {
 #pragma unroll
           for (int i = 0; i < RT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float2 v = activation<T, act.value>(g[i][r]);
+              const float2 v = activation<T, ACT>(g[i][r]);
               E p[P];
               split<T>(dh[i][r] * u[i][r] * v.y, p);
 #pragma unroll
@@ -353,7 +301,6 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
 #pragma unroll
               for (int s = 0; s < P; ++s) du[i][s][t * 4 + r] = p[s];
             }
-        });
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -366,7 +313,6 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
         for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, du[i], dx[d][i]);
       }
     }
-    __syncthreads();  // (the next rows' first chunk goes where the last one lay)
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
       const int n = d * 16 + (lane >> 4) * 4;
@@ -408,7 +354,7 @@ struct WeightArgs {
   const T *wg, *wu, *wd, *bg, *bu;
   float *dwgu, *dwd, *sums, *dy_sums;  // [gridDim.x, ...]; dy_sums nullable
   int64_t rows;
-  int32_t width, hidden, out, act, add;
+  int32_t width, hidden, out, add;
 };
 
 // Rows of a tile in LDS, of STEPS k steps of 32 (64 bytes each), and what its 16-byte
@@ -471,7 +417,7 @@ constexpr int weight_rows() {  // of a staged tile
   return Planes<T>::N == 1 ? 64 : 32;
 }
 
-template <typename T, int DK, int OK, int FT>
+template <typename T, int DK, int OK, int FT, int ACT>
 __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK, OT = 2 * OK, ROWS = weight_rows<T>();
@@ -563,12 +509,11 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
 #pragma unroll
           for (int i = 0; i < FT; ++i) dh[i] = mfma_planes<T>(y, wd[i][k], dh[i]);
         }
-        with_activation(a.act, [&](auto act) {
 #pragma unroll
           for (int i = 0; i < FT; ++i)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-              const float2 v = activation<T, act.value>(g[i][r]);
+              const float2 v = activation<T, ACT>(g[i][r]);
               const float vg = dh[i][r] * u[i][r] * v.y, vu = dh[i][r] * v.x;
               sg[i] += vg;
               su[i] += vu;
@@ -583,7 +528,6 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
 #pragma unroll
               for (int s = 0; s < P; ++s) h[i][s][t * 4 + r] = p[s];
             }
-        });
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -677,8 +621,7 @@ static void with_narrow(int width, int out, F&& f) {
 #define NARROW 128
 
 template <typename T>
-bool RowKernels<T>::takes(int64_t rows, int32_t width, int32_t hidden, int32_t out) {
-  (void)rows, (void)hidden;
+bool RowKernels<T>::takes(int32_t width, int32_t out) {
   return width <= NARROW && out <= NARROW;
 }
 
@@ -754,15 +697,13 @@ static bool wide_stores(const void* p, int64_t cols) {
   return cols % 4 == 0 && aligned16((const T*)p, 0);
 }
 
-// Rows that fill the chip with wavefronts of 16 RT rows take them (RT as a constant), fewer
-// take 16.
-template <int MANY, typename F>
+// Rows that fill the chip with wavefronts of 32 rows take them, fewer take 16 (RT as a
+// constant, and the workgroups of WAVES wavefronts).
+template <int WAVES, typename F>
 static void with_rows(int64_t rows, F&& f) {
-  const auto launch = [&](auto rt) {
-    f(rt, (unsigned)std::min<int64_t>(tiles(rows, 16 * rt.value * FR_WAVES), 512));
-  };
-  if (rows >= 16 * MANY * FR_WAVES * 256)
-    launch(std::integral_constant<int, MANY>());
+  const auto launch = [&](auto rt) { f(rt, (unsigned)tiles(rows, 16 * rt.value * WAVES)); };
+  if (rows >= 32 * 8 * 256)
+    launch(std::integral_constant<int, 2>());
   else
     launch(std::integral_constant<int, 1>());
 }
@@ -778,12 +719,14 @@ void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
     hipLaunchKernelGGL((ffn_pack_kernel<T, false>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                        stream, pack);
     const ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
-                           c.x_pitch, c.width, c.out, chunks, c.act,
+                           c.x_pitch, c.width, c.out, chunks,
                            wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
-    constexpr int MANY = Planes<T>::N == 1 && DK <= 2 && OT <= 4 ? 4 : 2;
-    with_rows<MANY>(c.rows, [&](auto rt, unsigned groups) {
-      hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value>), dim3(groups),
-                         dim3(64 * FR_WAVES), 0, stream, a);
+    constexpr int WAVES = Planes<T>::N * (DK + OT) <= 8 ? 8 : 4;
+    with_rows<WAVES>(c.rows, [&](auto rt, unsigned groups) {
+      with_activation(c.act, [&](auto act) {
+        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value, WAVES>),
+                           dim3(groups), dim3(64 * WAVES), 0, stream, a);
+      });
     });
   });
 }
@@ -801,13 +744,15 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       hipLaunchKernelGGL((ffn_pack_kernel<T, true>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                          stream, pack);
       const BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
-                              c.dy_pitch, c.width, c.out, chunks, c.act,
+                              c.dy_pitch, c.width, c.out, chunks,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
                               wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
-      constexpr int MANY = 2;
-      with_rows<MANY>(c.rows, [&](auto rt, unsigned groups) {
-        hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value>), dim3(groups),
-                           dim3(64 * FR_WAVES), 0, stream, a);
+      constexpr int WAVES = Planes<T>::N * (2 * DK + OK) <= 6 ? 8 : 4;
+      with_rows<WAVES>(c.rows, [&](auto rt, unsigned groups) {
+        with_activation(c.act, [&](auto act) {
+          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value, WAVES>),
+                             dim3(groups), dim3(64 * WAVES), 0, stream, a);
+        });
       });
     }
     if (!(c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd)) return;
@@ -821,9 +766,11 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       a.wg = (const T*)c.wg, a.wu = (const T*)c.wu, a.wd = (const T*)c.wd;
       a.bg = (const T*)c.bg, a.bu = (const T*)c.bu;
       a.dwgu = p.dwgu, a.dwd = p.dwd, a.sums = p.sums, a.dy_sums = c.dbd ? p.dy_sums : nullptr;
-      a.rows = m, a.width = c.width, a.hidden = c.hidden, a.out = c.out, a.act = c.act, a.add = r > 0;
-      hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT>),
-                         dim3(p.runs, p.columns), dim3(64 * p.waves), 0, stream, a);
+      a.rows = m, a.width = c.width, a.hidden = c.hidden, a.out = c.out, a.add = r > 0;
+      with_activation(c.act, [&](auto act) {
+        hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value>),
+                           dim3(p.runs, p.columns), dim3(64 * p.waves), 0, stream, a);
+      });
     }
     const int64_t F = c.hidden, D = c.width, O = c.out;
     Joiner<T> join;

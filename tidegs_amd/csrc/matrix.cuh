@@ -21,6 +21,7 @@
 #include "decoder_common.cuh"
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 template <typename E>
 using frag_t = E __attribute__((ext_vector_type(8)));
 template <typename E>
