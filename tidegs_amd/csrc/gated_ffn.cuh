@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
   float acc = 0.f;
   if (live) {
     const float* p = job.partial + i / job.cols * job.pitch + i % job.cols;
-#pragma unroll 4
+#pragma unroll 8
     for (int part = g; part < job.parts; part += job.groups) acc += p[part * job.part];
   }
   s[threadIdx.x] = acc;
@@ -214,7 +214,7 @@ static inline int64_t tiles(int64_t n, int64_t t) { return (n + t - 1) / t; }
 // Whether a product can read a matrix where it lies.
 template <typename T>
 static bool in_place(const void* p, int64_t cols, int64_t pitch) {
-  return Planes<T>::N == 1 && cols % 8 == 0 && pitch < (1 << 26) && aligned16((const T*)p, pitch);
+  return Planes<T>::N == 1 && cols % 8 == 0 && pitch <= MX_PITCH && aligned16((const T*)p, pitch);
 }
 
 template <typename T>
@@ -252,7 +252,7 @@ struct Joiner {
   void add(const float* partial, int64_t part, int64_t pitch, int64_t parts, int64_t rows,
            int64_t cols, void* to) {
     if (!to) return;
-    const int groups = parts > 32 ? 32 : parts > 4 ? 8 : 1;
+    const int groups = parts > 4 ? 8 : 1;
     blocks += (uint32_t)tiles(rows * cols, 256 / groups);
     jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, groups, rows, to,
                             blocks};

@@ -49,30 +49,31 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
 
   f32x4 gu[4][4] = {};
   {
-    const int per = (a.width8 + MX_BK - 1) / MX_BK;
-    product_loop<E, SX, SW>(gu, lds, per * PAIRS, wm * 64, wn * 64, [&](int s, char* to) {
-      const int pair = s / per, k0 = (s % per) * MX_BK;
-      const E* x = a.x.p + PlanePairs<T>::a(pair) * a.x.plane;
-      const E* wg = a.wg.p + PlanePairs<T>::b(pair) * a.wg.plane;
-      const E* wu = a.wu.p + PlanePairs<T>::b(pair) * a.wu.plane;
-      SX::load(to, x, a.x.pitch, m0, a.rows, k0, a.width8,
-               [&](int r) { return RowOf<E>{x, r}; });
-      SW::load(to + SX::BYTES, wg, a.wg.pitch, f0, a.hidden, k0, a.width8, [&](int r) {
-        return RowOf<E>{r & 16 ? wu : wg, (r >> 5) * 16 + (r & 15)};
-      });
-    });
+    SX sx;
+    SW sw;
+    sx.begin(a.x.pitch, m0, a.rows, a.width8);
+    sw.begin(a.wg.pitch, f0, a.hidden, a.width8, [](int r) { return (r >> 5) * 16 + (r & 15); });
+    const E *x = a.x.p + m0 * a.x.pitch, *wg = a.wg.p + f0 * a.wg.pitch, *wu = a.wu.p + f0 * a.wu.pitch;
+    product_loop<E, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * 64, wn * 64,
+                            [&](const Steps& s, char* to) {
+                              const int64_t w = PlanePairs<T>::b(s.pair) * a.wg.plane;
+                              sx.copy(to, x + PlanePairs<T>::a(s.pair) * a.x.plane, s.k);
+                              sw.copy(to + SX::BYTES, wg + w, wu + w, s.k,
+                                      [](int r) { return (r & 16) != 0; });
+                            });
   }
   f32x4 dh[4][2] = {};
   if constexpr (BACK) {
-    const int per = (a.out8 + MX_BK - 1) / MX_BK;
-    product_loop<E, SX, SD>(dh, lds, per * PAIRS, wm * 64, wn * 32, [&](int s, char* to) {
-      const int pair = s / per, k0 = (s % per) * MX_BK;
-      const E* dy = a.dy.p + PlanePairs<T>::a(pair) * a.dy.plane;
-      SX::load(to, dy, a.dy.pitch, m0, a.rows, k0, a.out8,
-               [&](int r) { return RowOf<E>{dy, r}; });
-      SD::load(to + SX::BYTES, a.wd.p + PlanePairs<T>::b(pair) * a.wd.plane, a.wd.pitch, f0,
-               a.hidden8, k0, a.out, [&](int r) { return RowOf<E>{nullptr, 0}; });
-    });
+    SX sy;
+    SD sd;
+    sy.begin(a.dy.pitch, m0, a.rows, a.out8);
+    sd.begin(a.wd.pitch, f0, a.hidden8, a.out);
+    const E *dy = a.dy.p + m0 * a.dy.pitch, *wd = a.wd.p + f0;
+    product_loop<E, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * 64, wn * 32,
+                            [&](const Steps& s, char* to) {
+                              sy.copy(to, dy + PlanePairs<T>::a(s.pair) * a.dy.plane, s.k);
+                              sd.copy(to + SX::BYTES, wd + PlanePairs<T>::b(s.pair) * a.wd.plane, s.k);
+                            });
   }
 
   const int group = lane >> 4;
@@ -200,22 +201,25 @@ __global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typenam
   const int64_t m0 = (int64_t)tm * GT;
   const int n0 = tn * GT;
   const int64_t all = (g.K + MX_BK - 1) / MX_BK;
-  const int64_t from = all * split / g.splits, to_ = all * (split + 1) / g.splits;
-  const int per = (int)(to_ - from);
-  const int pairs = PAIRS * (g.a2.p ? 2 : 1);
+  const int64_t from = all * split / g.splits * MX_BK;
+  const int64_t to = min(all * (split + 1) / g.splits * MX_BK, g.K);
 
+  SA sa;
+  SB sb;
+  sa.begin(g.a.pitch, m0, g.a_limit, g.K);
+  sb.begin(g.b.pitch, n0, g.b_limit, g.K);
+  const int64_t at_a = KA == ALONG ? m0 * g.a.pitch : m0;
+  const int64_t at_b = KB == ALONG ? n0 * g.b.pitch : n0;
   f32x4 acc[4][4] = {};
-  if (per)
-    product_loop<E, SA, SB>(acc, lds, per * pairs, wm * 64, wn * 64, [&](int s, char* to) {
-      const int q = s / per, pair = q % PAIRS;
-      const int64_t k0 = (from + s % per) * MX_BK;
-      const bool second = q >= PAIRS;
-      const E* pa = (second ? g.a2.p : g.a.p) + PlanePairs<T>::a(pair) * g.a.plane;
-      const E* pb = (second ? g.b2.p : g.b.p) + PlanePairs<T>::b(pair) * g.b.plane;
-      SA::load(to, pa, g.a.pitch, m0, g.a_limit, k0, g.K, [&](int r) { return RowOf<E>{pa, r}; });
-      SB::load(to + SA::BYTES, pb, g.b.pitch, n0, g.b_limit, k0, g.K,
-               [&](int r) { return RowOf<E>{pb, r}; });
-    });
+  product_loop<E, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * 64, wn * 64,
+                          [&](const Steps& s, char* to_lds) {
+                            const bool second = s.pair >= PAIRS;
+                            const int pair = second ? s.pair - PAIRS : s.pair;
+                            sa.copy(to_lds, (second ? g.a2.p : g.a.p) + at_a +
+                                                PlanePairs<T>::a(pair) * g.a.plane, s.k);
+                            sb.copy(to_lds + SA::BYTES, (second ? g.b2.p : g.b.p) + at_b +
+                                                            PlanePairs<T>::b(pair) * g.b.plane, s.k);
+                          });
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t m = m0 + wm * 64 + i * 16 + (lane & 15);

@@ -78,8 +78,7 @@ enum Along { ALONG, ACROSS };
 
 #define MX_BK 64  // k of one staged step
 
-// A matrix operand: planes `plane` values apart, rows `pitch` values apart.  k runs to
-// K and the other index to N.
+// A matrix operand: planes `plane` values apart, rows `pitch` values apart.
 template <typename E>
 struct Operand {
   const E* p;
@@ -91,12 +90,14 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __amdgpu_buffer_rsrc_t rsrc_t;
 
 #define MX_OUTSIDE 0x80000000u  // an offset past every buffer here
+#define MX_PITCH (1 << 22)      // of an operand at most: 256 rows stay within such offsets
 
 __device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
 }
 
-// ROWS of an operand by MX_BK of its k, staged by the THREADS of a workgroup.
+// ROWS of an operand by MX_BK of its k, staged by the THREADS of a workgroup.  Where each
+// lane reads is worked out once; a step moves the buffer's base.
 template <typename E, int ROWS, Along K_, int THREADS>
 struct Stage {
   static constexpr int BYTES = ROWS * MX_BK * 2;
@@ -104,6 +105,7 @@ struct Stage {
   static constexpr int PASSES = BYTES / (1024 * WAVES);
   static_assert(PASSES * 1024 * WAVES == BYTES, "whole passes");
   static constexpr int CHUNKS = (K_ == ALONG ? MX_BK : ROWS) / 8;  // of an LDS row
+  static constexpr int PER = 64 / CHUNKS;                          // LDS rows of one KB
 
   // Which unit of 32 bytes an ACROSS row's units are exchanged with: rows that one
   // transposing read touches together (bits 0, 1 and 3) meet different banks.
@@ -112,44 +114,59 @@ struct Stage {
     return ((row >> 1) & 1) | ((row >> 2) & 2);
   }
 
-  // `rows` of the operand are there (from row0 on), k runs from k0 to K.  Row r of the
-  // tile is row of(r) of the operand, the same distance from r for r of a run of 8.
+  int64_t pitch, K;
+  uint32_t off[PASSES];  // bytes, from the tile's first row (ALONG) or column (ACROSS)
+  uint32_t last;         // ALONG: bytes to the last row's start
+  int chunk;             // ALONG: the chunk of this lane
+
+  // The tile is rows row0 .. (ALONG; row r of it is row of(r) of the operand) or columns
+  // row0 .. (ACROSS) of an operand that has `rows` of them; k runs to K.
   template <typename Of>
-  __device__ static __forceinline__ void load(char* lds, const E* p, int64_t pitch, int64_t row0,
-                                              int64_t rows, int64_t k0, int64_t K, Of&& of) {
-    const int lane = threadIdx.x & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    if constexpr (K_ == ALONG) {
+  __device__ __forceinline__ void begin(int64_t pitch_, int64_t row0, int64_t rows, int64_t K_end,
+                                        Of&& of) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    pitch = pitch_;
+    K = K_end;
+    const int left = (int)min((int64_t)ROWS, rows - row0);
 #pragma unroll
-      for (int j = 0; j < PASSES; ++j) {
-        const int first = (j * WAVES + wave) * 8;  // row of lane 0
-        const auto src = of(first);
-        const int64_t at = row0 + src.row;
-        const int64_t left = rows - at;
-        const rsrc_t r = buffer_of(src.p + at * pitch + k0,
-                                   left > 0 ? (uint32_t)(((left < 8 ? left : 8) - 1) * pitch +
-                                                         ((K + 7) & ~7) - k0) * 2 : 0);
-        const int c = (lane & 7) ^ (lane >> 3);
-        uint32_t off = (uint32_t)((lane >> 3) * pitch + c * 8) * 2;
-        if (k0 + c * 8 >= K) off = MX_OUTSIDE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + first * 128), 16, off, 0, 0, 0);
-      }
-    } else {
-      // row0 is this tile's first column of the operand's rows, which are its k
-      constexpr int PER = 64 / CHUNKS;  // k rows of one wavefront's KB
-#pragma unroll
-      for (int j = 0; j < PASSES; ++j) {
-        const int first = (j * WAVES + wave) * PER;
-        const int64_t left = K - k0 - first;
-        const rsrc_t r =
-            buffer_of(p + (k0 + first) * pitch + row0,
-                      left > 0 ? (uint32_t)(((left < PER ? left : PER) - 1) * pitch + rows - row0) * 2 : 0);
-        const int row = first + lane / CHUNKS, pos = lane % CHUNKS;
+    for (int j = 0; j < PASSES; ++j) {
+      const int row = (j * WAVES + wave) * PER + lane / CHUNKS, pos = lane % CHUNKS;
+      if constexpr (K_ == ALONG) {
+        chunk = pos ^ (row & 7);
+        const int r = of(row);
+        off[j] = r < left ? (uint32_t)(r * pitch + chunk * 8) * 2 : MX_OUTSIDE;
+      } else {
         const int c = (((pos >> 1) ^ turn(row)) << 1) | (pos & 1);
-        uint32_t off = (uint32_t)((lane / CHUNKS) * pitch + c * 8) * 2;
-        if (row0 + c * 8 >= rows) off = MX_OUTSIDE;
-        __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_void*)(lds + first * ROWS * 2), 16, off, 0, 0, 0);
+        off[j] = c * 8 < left ? (uint32_t)(row * pitch + c * 8) * 2 : MX_OUTSIDE;
       }
+    }
+    last = (uint32_t)((left - 1) * pitch) * 2;
+  }
+  __device__ __forceinline__ void begin(int64_t pitch_, int64_t row0, int64_t rows, int64_t K_end) {
+    begin(pitch_, row0, rows, K_end, [](int r) { return r; });
+  }
+
+  // Starts the copies of k0 .. k0 + MX_BK - 1; `p` is the tile's first row's or column's
+  // place in the plane, p2 that of the rows that `other` says come from another matrix.
+  __device__ __forceinline__ void copy(char* lds, const E* p, int64_t k0) const {
+    copy(lds, p, p, k0, [](int) { return false; });
+  }
+  template <typename Other>
+  __device__ __forceinline__ void copy(char* lds, const E* p, const E* p2, int64_t k0,
+                                       Other&& other) const {
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int left = (int)min((int64_t)MX_BK, K - k0);
+    const int64_t at = K_ == ALONG ? k0 : k0 * pitch;
+    // ALONG: chunks that start before K are there whole (operands end on chunks)
+    const uint32_t bytes = K_ == ALONG ? last + ((left + 7) & ~7) * 2 : (uint32_t)(left * pitch) * 2;
+    const rsrc_t r = buffer_of(p + at, bytes), r2 = buffer_of(p2 + at, bytes);
+    const bool whole = K_ == ACROSS || chunk * 8 < left;
+#pragma unroll
+    for (int j = 0; j < PASSES; ++j) {
+      const int first = (j * WAVES + wave) * PER;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(other(first) ? r2 : r,
+                                               (lds_void*)(lds + (j * WAVES + wave) * 1024), 16,
+                                               whole ? off[j] : MX_OUTSIDE, 0, 0, 0);
     }
   }
 
@@ -176,13 +193,6 @@ struct Stage {
   }
 };
 
-// Which row of which matrix a tile's row is (runs of 8).
-template <typename E>
-struct RowOf {
-  const E* p;
-  int64_t row;
-};
-
 // A tile's place among `tiles_m` x `tiles_n`: workgroups go round the 8 XCDs, so each XCD is
 // given a contiguous run of the order, and the order walks 8 tiles of m for each of n, so
 // that what an XCD works on at once shares its operands in that XCD's L2.
@@ -197,21 +207,37 @@ __device__ __forceinline__ void tile_of(uint32_t bid, uint32_t tiles_m, uint32_t
   tn = in / high;
 }
 
-// The main loop over `steps` staged steps: load(step, buffer) starts the copies of a step,
-// and a step is multiplied while the next one's copies run.  acc[i][j] is the transposed
-// 16 x 16 tile of rows a_row + 16 i of A and b_row + 16 j of B: lane l holds row l % 16 of A and
-// rows (l / 16) * 4 + r of B.
-template <typename E, typename SA, typename SB, int TM, int TN, typename Load>
-__device__ __forceinline__ void product_loop(f32x4 (&acc)[TM][TN], char* lds, int steps, int a_row,
-                                             int b_row, Load&& load) {
+// The steps of a product's loop: k in MX_BK from `from` to `to`, for each of `pairs` pairs of
+// operands in turn.
+struct Steps {
+  int64_t k, from, to;
+  int pair, pairs;
+  __device__ __forceinline__ Steps(int64_t from_, int64_t to_, int pairs_)
+      : k(from_), from(from_), to(to_), pair(from_ < to_ ? 0 : pairs_), pairs(pairs_) {}
+  __device__ __forceinline__ bool more() const { return pair < pairs; }
+  __device__ __forceinline__ void next() {
+    k += MX_BK;
+    if (k >= to) k = from, ++pair;
+  }
+};
+
+// The main loop: copy(step, buffer) starts the copies of a step, and a step is multiplied
+// while the next one's copies run.  acc[i][j] is the transposed 16 x 16 tile of rows
+// a_row + 16 i of A and b_row + 16 j of B: lane l holds row l % 16 of A and rows
+// (l / 16) * 4 + r of B.
+template <typename E, typename SA, typename SB, int TM, int TN, typename Copy>
+__device__ __forceinline__ void product_loop(f32x4 (&acc)[TM][TN], char* lds, Steps s, int a_row,
+                                             int b_row, Copy&& copy) {
   constexpr int BYTES = SA::BYTES + SB::BYTES;
-  load(0, lds);
-#pragma unroll 1
-  for (int s = 0; s < steps; ++s) {
+  int turn = 0;
+  if (s.more()) copy(s, lds);
+  while (s.more()) {
     // everyone's copies of this step are there, and nobody reads the other buffer any more
     __syncthreads();
-    const char* cur = lds + (s & 1) * BYTES;
-    if (s + 1 < steps) load(s + 1, lds + ((s + 1) & 1) * BYTES);
+    const char* cur = lds + turn * BYTES;
+    turn ^= 1;
+    s.next();
+    if (s.more()) copy(s, lds + turn * BYTES);
 #pragma unroll
     for (int kk = 0; kk < 2; ++kk) {
       frag_t<E> a[TM], b[TN];
