@@ -9,14 +9,21 @@
 #include "gated_ffn.cuh"
 
 // ---------------------------------------------------------------------------
-// The hidden products.  A workgroup's tile is 128 rows by 64 hidden columns: its B rows
+// The hidden products.  The B rows of a workgroup's tile
 // are runs of 16 of Wg and of Wu in turn, so that a lane's accumulators hold g and u
 // of the same row and columns and the gate is taken in registers.  The backward adds
 // dh = dy Wd for the same tile before its gate.
 // ---------------------------------------------------------------------------
 
-#define FT_M 128
-#define FT_F 64
+// Tiles: 128 x 128 in four wavefronts, two workgroups a CU; 256 x 256 in eight, one a CU, for
+// products of operands that both run along k, where there are tiles enough for the CUs.
+// A larger tile stages fewer bytes per product and its wavefronts' 128 x 64 read fewer
+// fragments: the hidden products of 8192 x 1024 x 2 4096 take 131 us (1050 TFLOP/s) in the
+// large tiles, 161 in the small. With an operand across k the turning reads, twice as
+// many, leave the large tile's lockstep behind two small ones (dW of that block 175 us
+// against 154), and so does the backward's third accumulator (343 against 305).
+typedef Tile<2, 2, 4, 4> TileSmall;
+typedef Tile<2, 4, 8, 4> TileLarge;
 
 template <typename E>
 struct HiddenArgs {
@@ -31,30 +38,31 @@ struct HiddenArgs {
   int32_t add;    // add to sums
 };
 
-template <typename T, bool BACK>
-__global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename Planes<T>::E> a) {
+template <typename T, bool BACK, typename Z>
+__global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<typename Planes<T>::E> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, PAIRS = PlanePairs<T>::N;
-  using SX = Stage<E, FT_M, ALONG, 256>;
-  using SW = Stage<E, 2 * FT_F, ALONG, 256>;
-  using SD = Stage<E, FT_F, ACROSS, 256>;
+  constexpr int TM = Z::TM, TF = Z::TN / 2, F = Z::N / 2;  // hidden columns of the tile
+  using SX = Stage<E, Z::M, ALONG, Z::THREADS>;
+  using SW = Stage<E, Z::N, ALONG, Z::THREADS>;
+  using SD = Stage<E, F, ACROSS, Z::THREADS>;
   __shared__ __attribute__((aligned(1024))) char lds[2 * (SX::BYTES + SW::BYTES)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
+  const int wm = wave / Z::WN, wn = wave % Z::WN;
   uint32_t tm, tn;
-  tile_of(blockIdx.x, (uint32_t)((a.rows + FT_M - 1) / FT_M), (a.hidden8 + FT_F - 1) / FT_F, tm, tn);
-  const int64_t m0 = (int64_t)tm * FT_M;
-  const int f0 = tn * FT_F;
+  tile_of(blockIdx.x, (uint32_t)((a.rows + Z::M - 1) / Z::M), (a.hidden8 + F - 1) / F, tm, tn);
+  const int64_t m0 = (int64_t)tm * Z::M;
+  const int f0 = tn * F;
 
-  f32x4 gu[4][4] = {};
+  f32x4 gu[TM][2 * TF] = {};
   {
     SX sx;
     SW sw;
     sx.begin(a.x.pitch, m0, a.rows, a.width8);
     sw.begin(a.wg.pitch, f0, a.hidden, a.width8, [](int r) { return (r >> 5) * 16 + (r & 15); });
     const E *x = a.x.p + m0 * a.x.pitch, *wg = a.wg.p + f0 * a.wg.pitch, *wu = a.wu.p + f0 * a.wu.pitch;
-    product_loop<E, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * 64, wn * 64,
+    product_loop<E, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * TM * 16, wn * TF * 32,
                             [&](const Steps& s, char* to) {
                               const int64_t w = PlanePairs<T>::b(s.pair) * a.wg.plane;
                               sx.copy(to, x + PlanePairs<T>::a(s.pair) * a.x.plane, s.k);
@@ -62,14 +70,14 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
                                       [](int r) { return (r & 16) != 0; });
                             });
   }
-  f32x4 dh[4][2] = {};
+  f32x4 dh[TM][TF] = {};
   if constexpr (BACK) {
     SX sy;
     SD sd;
     sy.begin(a.dy.pitch, m0, a.rows, a.out8);
     sd.begin(a.wd.pitch, f0, a.hidden8, a.out);
     const E *dy = a.dy.p + m0 * a.dy.pitch, *wd = a.wd.p + f0;
-    product_loop<E, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * 64, wn * 32,
+    product_loop<E, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * TM * 16, wn * TF * 16,
                             [&](const Steps& s, char* to) {
                               sy.copy(to, dy + PlanePairs<T>::a(s.pair) * a.dy.plane, s.k);
                               sd.copy(to + SX::BYTES, wd + PlanePairs<T>::b(s.pair) * a.wd.plane, s.k);
@@ -77,11 +85,11 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
   }
 
   const int group = lane >> 4;
-  float sg[2][4] = {}, su[2][4] = {};
+  float sg[TF][4] = {}, su[TF][4] = {};
   with_activation(a.act, [&](auto kind) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    const int f = f0 + wn * 32 + j * 16 + group * 4;
+  for (int j = 0; j < TF; ++j) {
+    const int f = f0 + wn * TF * 16 + j * 16 + group * 4;
     float bg[4], bu[4];
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -89,8 +97,8 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
       bu[r] = a.bu && f + r < a.hidden ? to_f32(((const T*)a.bu)[f + r]) : 0.f;
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t m = m0 + wm * 64 + i * 16 + (lane & 15);
+    for (int i = 0; i < TM; ++i) {
+      const int64_t m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
       const bool live = m < a.rows && f < a.hidden8;
       four_t<E> h[P], dg[P], du[P];
 #pragma unroll
@@ -133,9 +141,9 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
   });
   if constexpr (BACK) {
     if (!a.sums) return;
-    float* s = (float*)lds;  // [2 wm][2][64]; the main loop's last barrier freed it
+    float* s = (float*)lds;  // [WM][2][F]; the main loop's last barrier freed it
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < TF; ++j)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -144,16 +152,19 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
           su[j][r] += __shfl_xor(su[j][r], off, 64);
         }
         if ((lane & 15) == 0) {
-          s[wm * 128 + wn * 32 + j * 16 + group * 4 + r] = sg[j][r];
-          s[wm * 128 + 64 + wn * 32 + j * 16 + group * 4 + r] = su[j][r];
+          const int f = wn * TF * 16 + j * 16 + group * 4 + r;
+          s[(wm * 2) * F + f] = sg[j][r];
+          s[(wm * 2 + 1) * F + f] = su[j][r];
         }
       }
     __syncthreads();
-    if (threadIdx.x < 128) {
-      const int f = f0 + (threadIdx.x & 63);
+    if (threadIdx.x < 2 * F) {
+      const int which = threadIdx.x / F, f = f0 + threadIdx.x % F;
       if (f < a.hidden8) {
-        float* out = a.sums + (int64_t)tm * 2 * a.hidden8 + (threadIdx.x >> 6) * a.hidden8 + f;
-        const float v = s[threadIdx.x] + s[128 + threadIdx.x];
+        float* out = a.sums + ((int64_t)tm * 2 + which) * a.hidden8 + f;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < Z::WM; ++w) v += s[w * 2 * F + threadIdx.x];
         *out = a.add ? *out + v : v;
       }
     }
@@ -164,8 +175,6 @@ __global__ void __launch_bounds__(256, 2) ffn_hidden_kernel(HiddenArgs<typename 
 // Plain products: C = A B' (+ bias), 128 x 128 tiles, either rounded to the call's type
 // or, with the sum over k split, as 32-bit partial sums that a second launch joins.
 // ---------------------------------------------------------------------------
-
-#define GT 128
 
 template <typename E>
 struct ProductArgs {
@@ -184,22 +193,24 @@ struct ProductArgs {
   int32_t add;              // add to what `partial` holds
 };
 
-template <typename T, Along KA, Along KB>
-__global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typename Planes<T>::E> g) {
+template <typename T, Along KA, Along KB, typename Z>
+__global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<typename Planes<T>::E> g) {
   using E = typename Planes<T>::E;
   constexpr int PAIRS = PlanePairs<T>::N;
-  using SA = Stage<E, GT, KA, 256>;
-  using SB = Stage<E, GT, KB, 256>;
+  constexpr int TM = Z::TM, TN = Z::TN;
+  using SA = Stage<E, Z::M, KA, Z::THREADS>;
+  using SB = Stage<E, Z::N, KB, Z::THREADS>;
   __shared__ __attribute__((aligned(1024))) char lds[2 * (SA::BYTES + SB::BYTES)];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int wm = wave >> 1, wn = wave & 1;
-  const uint32_t tiles_m = (uint32_t)((g.M + GT - 1) / GT), tiles_n = (g.N + GT - 1) / GT;
+  const int wm = wave / Z::WN, wn = wave % Z::WN;
+  const uint32_t tiles_m = (uint32_t)((g.M + Z::M - 1) / Z::M);
+  const uint32_t tiles_n = (g.N + Z::N - 1) / Z::N;
   uint32_t tm, tn;
   const uint32_t split = blockIdx.x / (tiles_m * tiles_n);
   tile_of(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
-  const int64_t m0 = (int64_t)tm * GT;
-  const int n0 = tn * GT;
+  const int64_t m0 = (int64_t)tm * Z::M;
+  const int n0 = tn * Z::N;
   const int64_t all = (g.K + MX_BK - 1) / MX_BK;
   const int64_t from = all * split / g.splits * MX_BK;
   const int64_t to = min(all * (split + 1) / g.splits * MX_BK, g.K);
@@ -210,8 +221,9 @@ __global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typenam
   sb.begin(g.b.pitch, n0, g.b_limit, g.K);
   const int64_t at_a = KA == ALONG ? m0 * g.a.pitch : m0;
   const int64_t at_b = KB == ALONG ? n0 * g.b.pitch : n0;
-  f32x4 acc[4][4] = {};
-  product_loop<E, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * 64, wn * 64,
+  f32x4 acc[TM][TN] = {};
+  product_loop<E, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * TM * 16,
+                          wn * TN * 16,
                           [&](const Steps& s, char* to_lds) {
                             const bool second = s.pair >= PAIRS;
                             const int pair = second ? s.pair - PAIRS : s.pair;
@@ -221,12 +233,12 @@ __global__ void __launch_bounds__(256, 2) ffn_product_kernel(ProductArgs<typenam
                                                             PlanePairs<T>::b(pair) * g.b.plane, s.k);
                           });
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t m = m0 + wm * 64 + i * 16 + (lane & 15);
+  for (int i = 0; i < TM; ++i) {
+    const int64_t m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
     if (m >= g.M) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int n = n0 + wn * 64 + j * 16 + (lane >> 4) * 4;
+    for (int j = 0; j < TN; ++j) {
+      const int n = n0 + wn * TN * 16 + j * 16 + (lane >> 4) * 4;
       if (g.partial) {
         float* at = g.partial + ((int64_t)split * g.M + m) * g.N + n;
 #pragma unroll
@@ -293,7 +305,7 @@ static int check_sizes(const char* name, uint64_t rows, uint32_t width, uint32_t
 // Rows of one pass: what keeps the hidden tensors of a pass (six bytes a value and plane)
 // within 64M values; the next rows reuse them.
 static int64_t pass_rows(int64_t rows, int64_t hidden) {
-  const int64_t most = std::max<int64_t>((64 << 20) / round8(hidden) / FT_M * FT_M, FT_M);
+  const int64_t most = std::max<int64_t>((64 << 20) / round8(hidden) / 256 * 256, 256);
   return std::min(rows, most);
 }
 
@@ -301,6 +313,13 @@ static int64_t pass_rows(int64_t rows, int64_t hidden) {
 // chip twice, none shorter than four steps.
 static int splits_of(int64_t tiles_, int64_t k) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles_, k / (4 * MX_BK)));
+}
+
+// Whether there are enough tiles Z of an M x N product for the CUs.
+#define FILLING_TILES 224
+template <typename Z>
+static bool fills(int64_t M, int64_t N, int64_t times = 1) {
+  return tiles(M, Z::M) * tiles(N, Z::N) * times >= FILLING_TILES;
 }
 
 #define COLUMN_RUNS 64
@@ -328,10 +347,10 @@ struct Plan {
     if (back) {
       dy = c.take<E>(P * pass * O8);
       dgu = c.take<E>(2 * P * pass * F8);
-      gu_sums = c.take<float>(tiles(pass, FT_M) * 2 * F8);
+      gu_sums = c.take<float>(tiles(pass, TileSmall::M) * 2 * F8);
       dy_sums = c.take<float>(COLUMN_RUNS * O);
-      split_gu = splits_of(tiles(2 * F8, GT) * tiles(D, GT), pass);
-      split_d = splits_of(tiles(O, GT) * tiles(F, GT), pass);
+      split_gu = splits_of(tiles(2 * F8, 128) * tiles(D, 128), pass);
+      split_d = splits_of(tiles(O, 128) * tiles(F, 128), pass);
       // (one sum over all rows is rounded where it is taken)
       dwgu = split_gu > 1 || pass < rows ? c.take<float>(split_gu * 2 * F8 * D) : nullptr;
       dwd = split_d > 1 || pass < rows ? c.take<float>(split_d * O * F) : nullptr;
@@ -343,8 +362,28 @@ struct Plan {
 template <typename T, Along KA, Along KB>
 static void product(hipStream_t s, ProductArgs<typename Planes<T>::E> g) {
   g.wide = g.N % 4 == 0 && aligned16((const T*)g.c, 0) && aligned16((const T*)g.c2, 0);
-  const int64_t n = tiles(g.M, GT) * tiles(g.N, GT) * g.splits;
-  hipLaunchKernelGGL((ffn_product_kernel<T, KA, KB>), dim3((unsigned)n), dim3(256), 0, s, g);
+  const auto launch = [&](auto tile) {
+    using Z = decltype(tile);
+    hipLaunchKernelGGL((ffn_product_kernel<T, KA, KB, Z>),
+                       dim3((unsigned)(tiles(g.M, Z::M) * tiles(g.N, Z::N) * g.splits)),
+                       dim3(Z::THREADS), 0, s, g);
+  };
+  if constexpr (KA == ALONG && KB == ALONG)
+    if (fills<TileLarge>(g.M, g.N, g.splits)) return launch(TileLarge());
+  launch(TileSmall());
+}
+
+template <typename T, bool BACK>
+static void hidden_products(hipStream_t s, const HiddenArgs<typename Planes<T>::E>& a) {
+  const auto launch = [&](auto tile) {
+    using Z = decltype(tile);
+    hipLaunchKernelGGL((ffn_hidden_kernel<T, BACK, Z>),
+                       dim3((unsigned)(tiles(a.rows, Z::M) * tiles(a.hidden8, Z::N / 2))),
+                       dim3(Z::THREADS), 0, s, a);
+  };
+  if constexpr (!BACK)
+    if (fills<TileLarge>(a.rows, 2 * a.hidden8)) return launch(TileLarge());
+  launch(TileSmall());
 }
 
 static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out,
@@ -413,8 +452,7 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
       a.wg = wg, a.wu = wu;
       a.rows = m, a.width8 = p.D8, a.hidden = p.F, a.hidden8 = p.F8, a.act = activation;
       a.bg = b_gate, a.bu = b_up, a.h = p.h, a.plane = m * p.F8;
-      hipLaunchKernelGGL((ffn_hidden_kernel<T, false>),
-                         dim3((unsigned)(tiles(m, FT_M) * tiles(p.F8, FT_F))), dim3(256), 0, stream, a);
+      hidden_products<T, false>(stream, a);
       ProductArgs<E> g{};
       g.a = {p.h, a.plane, p.F8}, g.b = wd;
       g.M = m, g.N = p.O, g.K = p.F8, g.a_limit = m, g.b_limit = p.O, g.splits = 1;
@@ -472,8 +510,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       a.act = activation, a.bg = b_gate, a.bu = b_up;
       a.h = p.h, a.dgu = p.dgu, a.plane = m * p.F8;
       a.sums = hidden_sums ? p.gu_sums : nullptr, a.add = r > 0;
-      hipLaunchKernelGGL((ffn_hidden_kernel<T, true>),
-                         dim3((unsigned)(tiles(m, FT_M) * tiles(p.F8, FT_F))), dim3(256), 0, stream, a);
+      hidden_products<T, true>(stream, a);
       if (dx) {
         ProductArgs<E> g{};
         g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.a2 = {p.dgu + p.F8, 2 * a.plane, 2 * p.F8};
@@ -510,7 +547,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up);
     }
     if (p.dwd || !some) join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down);
-    const int64_t row_tiles = tiles(p.pass, FT_M);
+    const int64_t row_tiles = tiles(p.pass, TileSmall::M);
     join.add(p.gu_sums, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_gate);
     join.add(p.gu_sums + p.F8, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_up);
     join.add(p.dy_sums, p.O, p.O, some * COLUMN_RUNS, 1, p.O, db_down);

@@ -106,6 +106,7 @@ struct Stage {
   static_assert(PASSES * 1024 * WAVES == BYTES, "whole passes");
   static constexpr int CHUNKS = (K_ == ALONG ? MX_BK : ROWS) / 8;  // of an LDS row
   static constexpr int PER = 64 / CHUNKS;                          // LDS rows of one KB
+  static constexpr int READS = K_ == ALONG ? 1 : 2;                // LDS reads of a fragment
 
   // Which unit of 32 bytes an ACROSS row's units are exchanged with: rows that one
   // transposing read touches together (bits 0, 1 and 3) meet different banks.
@@ -221,35 +222,76 @@ struct Steps {
   }
 };
 
-// The main loop: copy(step, buffer) starts the copies of a step, and a step is multiplied
-// while the next one's copies run.  acc[i][j] is the transposed 16 x 16 tile of rows
-// a_row + 16 i of A and b_row + 16 j of B: lane l holds row l % 16 of A and rows
-// (l / 16) * 4 + r of B.
+// A workgroup's tile: WM x WN wavefronts of TM x TN tiles of 16.
+template <int WM_, int WN_, int TM_, int TN_>
+struct Tile {
+  static constexpr int WM = WM_, WN = WN_, TM = TM_, TN = TN_;
+  static constexpr int THREADS = 64 * WM * WN, M = 16 * WM * TM, N = 16 * WN * TN;
+};
+
+// This wavefront's copies have landed and its LDS reads are done, and so are the others'.
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+// The main loop: copy(step, buffer) starts the copies of a step into one of two buffers.
+// acc[i][j] is the transposed 16 x 16 tile of rows a_row + 16 i of A and b_row + 16 j of B:
+// lane l holds row l % 16 of A and rows (l / 16) * 4 + r of B.
+//
+// A step is two halves of k = 32, and the fragments of the half to come are read while a
+// half is multiplied, so the matrix cores have operands in registers across the barrier in
+// the middle of the step: behind it the step's buffer is read out and takes the copies of
+// the step after next, and the next step's copies have landed.
 template <typename E, typename SA, typename SB, int TM, int TN, typename Copy>
-__device__ __forceinline__ void product_loop(f32x4 (&acc)[TM][TN], char* lds, Steps s, int a_row,
+__device__ __forceinline__ void product_loop(f32x4 (&acc)[TM][TN], char* lds, Steps ahead, int a_row,
                                              int b_row, Copy&& copy) {
   constexpr int BYTES = SA::BYTES + SB::BYTES;
-  int turn = 0;
-  if (s.more()) copy(s, lds);
-  while (s.more()) {
-    // everyone's copies of this step are there, and nobody reads the other buffer any more
-    __syncthreads();
-    const char* cur = lds + turn * BYTES;
-    turn ^= 1;
-    s.next();
-    if (s.more()) copy(s, lds + turn * BYTES);
+  if (!ahead.more()) return;
+  frag_t<E> a[2][TM], b[2][TN];
+  const auto read = [&](const char* from, int half) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      frag_t<E> a[TM], b[TN];
+    for (int i = 0; i < TM; ++i) a[half][i] = SA::fragment(from, a_row + i * 16, half);
 #pragma unroll
-      for (int i = 0; i < TM; ++i) a[i] = SA::fragment(cur, a_row + i * 16, kk);
+    for (int j = 0; j < TN; ++j) b[half][j] = SB::fragment(from + SA::BYTES, b_row + j * 16, half);
+  };
+  const auto multiply = [&](int half) {
 #pragma unroll
-      for (int j = 0; j < TN; ++j) b[j] = SB::fragment(cur + SA::BYTES, b_row + j * 16, kk);
+    for (int i = 0; i < TM; ++i)
 #pragma unroll
-      for (int i = 0; i < TM; ++i)
+      for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[half][j], a[half][i], acc[i][j]);
+  };
+  // the reads dealt evenly among the products
+  const auto mix = [] {
+    constexpr int READS = TM * SA::READS + TN * SB::READS, PRODUCTS = TM * TN;
+    constexpr int GROUPS = READS < PRODUCTS ? READS : PRODUCTS;
 #pragma unroll
-        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[j], a[i], acc[i][j]);
+    for (int i = 0; i < GROUPS; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / GROUPS, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, (READS + GROUPS - 1) / GROUPS, 0);
     }
+  };
+  char *cur = lds, *other = lds + BYTES;
+  copy(ahead, cur);
+  ahead.next();
+  stage_barrier();
+  if (ahead.more()) copy(ahead, other);
+  read(cur, 0);
+  while (ahead.more()) {
+    read(cur, 1);
+    multiply(0);
+    mix();
+    stage_barrier();
+    ahead.next();
+    if (ahead.more()) copy(ahead, cur);
+    char* t = cur;
+    cur = other;
+    other = t;
+    read(cur, 0);
+    multiply(1);
+    mix();
   }
-  __syncthreads();
+  read(cur, 1);
+  multiply(0);
+  multiply(1);
+  stage_barrier();
 }
