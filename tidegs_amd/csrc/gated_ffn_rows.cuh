@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(64 * WAVES) ffn_rows_fwd_kernel(ForwardArgs<T>
     }
     f32x4 y[OT][RT] = {};
     for (int c = 0; c < a.chunks; ++c) {
-      __syncthreads();  // the chunk is there, and nobody reads the one before it
+      stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (c & 1) * C::KB * 1024;
       if (c + 1 < a.chunks)
         copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
@@ -252,10 +252,10 @@ __global__ void __launch_bounds__(64 * WAVES) ffn_rows_dx_kernel(BackwardArgs<T>
     f32x4 dx[DT][RT] = {};
     for (int c = 0; c < a.chunks; ++c) {
       if (BUFFERS == 1 && c) {
-        __syncthreads();
+        stage_barrier();
         copy_chunk<C::KB, WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
       }
-      __syncthreads();  // the chunk is there, and nobody reads the one before it
+      stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
       if (BUFFERS == 2 && c + 1 < a.chunks)
         copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
@@ -475,7 +475,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
   if (blockIdx.x < tiles) stage(blockIdx.x, lds);
   int turn = 0;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
-    __syncthreads();  // the tile is there, and nobody reads the one before it
+    stage_barrier();  // the tile is there, and nobody reads the one before it
     const char* xs = lds + turn * BYTES;
     const char* ys = xs + P * XB;
     if (tile + gridDim.x < tiles) stage(tile + gridDim.x, lds + (turn ^ 1) * BYTES);

@@ -229,9 +229,13 @@ struct Tile {
   static constexpr int THREADS = 64 * WM * WN, M = 16 * WM * TM, N = 16 * WN * TN;
 };
 
-// This wavefront's copies have landed and its LDS reads are done, and so are the others'.
+// Behind it every wavefront's copies to LDS have landed and its LDS reads are done.  The wait
+// is spelled out: __syncthreads() orders LDS accesses, and the compiler does not
+// count the copies among them at every barrier.
 __device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // The main loop: copy(step, buffer) starts the copies of a step into one of two buffers.
