@@ -54,10 +54,16 @@ struct RowMap {
   }
 };
 
+// Sum over the LANES lanes of a row, the same in each of them: DPP within 16 lanes (every
+// step adds a group of lanes that all hold one sum to another), shuffles beyond.
 template <int LANES>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-  for (int off = 1; off < LANES; off <<= 1) v += __shfl_xor(v, off, 64);
+  v += tgs_dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += tgs_dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += tgs_dpp<0x141>(v);  // row_half_mirror
+  if constexpr (LANES >= 16) v += tgs_dpp<0x140>(v);  // row_mirror
+  if constexpr (LANES >= 32) v += __shfl_xor(v, 16, 64);
+  if constexpr (LANES >= 64) v += __shfl_xor(v, 32, 64);
   return v;
 }
 
@@ -81,14 +87,33 @@ __device__ __forceinline__ float normalise(float (&x)[E], int lane, uint32_t n, 
 }
 
 // The weight's or bias's values of this lane's columns; `other` where there are none.
-template <typename Map, typename W, int E>
+template <typename Map, bool VEC, typename W, int E>
 __device__ __forceinline__ void load_columns(const W* w, int lane, uint32_t n, float other,
                                              float (&v)[E]) {
+  constexpr int R = VEC ? Vec16<W>::N : 1;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
+  for (int e = 0; e < E; e += R) {
     const uint32_t c = Map::column(lane, e);
-    v[e] = w && c < n ? to_f32(w[c]) : other;
+    if (w && c < n) {
+      if constexpr (VEC) {
+        const Vec16<W> t = *(const Vec16<W>*)(w + c);
+#pragma unroll
+        for (int k = 0; k < R; ++k) v[e + k] = to_f32(t.v[k]);
+      } else {
+        v[e] = to_f32(w[c]);
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < R; ++k) v[e + k] = other;
+    }
   }
+}
+
+// Rows that a lane has in flight at once: what keeps enough bytes on their way (4M rows of
+// 64 bfloat16: forward 197 us with one, 5.2 TB/s; see the launch for both).
+template <int E>
+constexpr int rows_at_once() {
+  return E <= 4 ? 4 : E <= 16 ? 2 : 1;
 }
 
 template <typename T, typename W, int LANES, int E, bool VEC>
@@ -96,21 +121,28 @@ __global__ void __launch_bounds__(256) layer_norm_fwd_kernel(
     uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const W* __restrict__ weight,
     const W* __restrict__ bias, float eps, T* __restrict__ y) {
   using Map = RowMap<T, LANES, E, VEC>;
-  constexpr int PER = 256 / LANES;  // rows of a workgroup at once
+  constexpr int PER = 256 / LANES, U = rows_at_once<E>();  // rows of a workgroup at once
   const int lane = threadIdx.x % LANES;
   float w[E], b[E];
-  load_columns<Map>(weight, lane, n, 1.f, w);
-  load_columns<Map>(bias, lane, n, 0.f, b);
-  // (the shuffles stay inside the lanes of one row, so a wavefront whose last rows
-  // are missing needs no barrier)
-  for (uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES; r < rows;
-       r += (uint64_t)gridDim.x * PER) {
-    float v[E];
-    Map::load(x + (int64_t)r * pitch, lane, n, v);
-    normalise<Map, LANES, E>(v, lane, n, eps);
+  load_columns<Map, VEC>(weight, lane, n, 1.f, w);
+  load_columns<Map, VEC>(bias, lane, n, 0.f, b);
+  // (a row's sums stay inside its own lanes, so lanes without a row need no barrier)
+  for (uint64_t r0 = (uint64_t)blockIdx.x * PER * U + threadIdx.x / LANES; r0 < rows;
+       r0 += (uint64_t)gridDim.x * PER * U) {
+    float v[U][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = fmaf(v[e], w[e], b[e]);
-    Map::store(y + r * n, lane, n, v);
+    for (int k = 0; k < U; ++k) {
+      const uint64_t r = min(r0 + k * PER, rows - 1);  // (the last row again: not stored)
+      Map::load(x + (int64_t)r * pitch, lane, n, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      normalise<Map, LANES, E>(v[k], lane, n, eps);
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[k][e] = fmaf(v[k][e], w[e], b[e]);
+      const uint64_t r = r0 + k * PER;
+      if (r < rows) Map::store(y + r * n, lane, n, v[k]);
+    }
   }
 }
 
@@ -120,32 +152,41 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(
     int64_t dy_pitch, const W* __restrict__ weight, float eps, T* __restrict__ dx,
     float* __restrict__ partial) {
   using Map = RowMap<T, LANES, E, VEC>;
-  constexpr int PER = 256 / LANES;
+  constexpr int PER = 256 / LANES, U = rows_at_once<E>();
   __shared__ float s_part[2][LANES * E];
   const int lane = threadIdx.x % LANES;
   float w[E], dw[E] = {}, db[E] = {};
-  load_columns<Map>(weight, lane, n, 1.f, w);
-  for (uint64_t r = (uint64_t)blockIdx.x * PER + threadIdx.x / LANES; r < rows;
-       r += (uint64_t)gridDim.x * PER) {
-    float v[E], g[E];
-    Map::load(x + (int64_t)r * pitch, lane, n, v);
-    Map::load(dy + (int64_t)r * dy_pitch, lane, n, g);
-    const float rstd = normalise<Map, LANES, E>(v, lane, n, eps);
-    float s = 0.f, q = 0.f;
+  load_columns<Map, VEC>(weight, lane, n, 1.f, w);
+  for (uint64_t r0 = (uint64_t)blockIdx.x * PER * U + threadIdx.x / LANES; r0 < rows;
+       r0 += (uint64_t)gridDim.x * PER * U) {
+    float v[U][E], g[U][E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      dw[e] = fmaf(g[e], v[e], dw[e]);
-      db[e] += g[e];
-      g[e] *= w[e];
-      s += g[e];
-      q = fmaf(g[e], v[e], q);
+    for (int k = 0; k < U; ++k) {
+      const uint64_t r = min(r0 + k * PER, rows - 1);
+      Map::load(x + (int64_t)r * pitch, lane, n, v[k]);
+      Map::load(dy + (int64_t)r * dy_pitch, lane, n, g[k]);
     }
-    if (dx) {
-      s = group_sum<LANES>(s) / (float)n;
-      q = group_sum<LANES>(q) / (float)n;
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = rstd * (g[e] - s - v[e] * q);
-      Map::store(dx + r * n, lane, n, v);
+    for (int k = 0; k < U; ++k) {
+      const uint64_t r = r0 + k * PER;
+      if (r >= rows) break;
+      const float rstd = normalise<Map, LANES, E>(v[k], lane, n, eps);
+      float s = 0.f, q = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        dw[e] = fmaf(g[k][e], v[k][e], dw[e]);
+        db[e] += g[k][e];
+        g[k][e] *= w[e];
+        s += g[k][e];
+        q = fmaf(g[k][e], v[k][e], q);
+      }
+      if (dx) {
+        s = group_sum<LANES>(s) / (float)n;
+        q = group_sum<LANES>(q) / (float)n;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[k][e] = rstd * (g[k][e] - s - v[k][e] * q);
+        Map::store(dx + r * n, lane, n, v[k]);
+      }
     }
   }
   if (!partial) return;
@@ -271,10 +312,12 @@ __global__ void __launch_bounds__(1024) layer_norm_join_kernel(uint32_t parts, u
 
 #define LN_MAX_HELD 4096  // values of a row that 64 lanes hold in registers
 
-// Workgroups of a launch: enough to fill the chip, few enough that a workgroup's rows
-// pay for its loads of the weights.
+// Workgroups of a backward launch: each leaves a partial row of both sums, so none for fewer
+// than 16 rows once the CUs have one each (8191 rows of 1024: 2048 workgroups' partial rows
+// were as many bytes as x).
 static uint32_t norm_groups(uint64_t rows) {
-  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>((rows + 3) / 4, 1), 2048);
+  return (uint32_t)std::min<uint64_t>(std::max<uint64_t>(rows / 16, std::min<uint64_t>(rows, 256)),
+                                      2048);
 }
 
 // Calls f(LANES, E) as constants: the fewest lanes that hold n values.
@@ -290,7 +333,8 @@ static void with_row_map(uint32_t n, F&& f) {
   }
   if constexpr (R < 2) {
     LN_MAP(16, 1);
-    LN_MAP(64, 1);
+    LN_MAP(16, 2);
+    LN_MAP(16, 4);
     LN_MAP(64, 2);
   }
   if constexpr (R < 8) LN_MAP(64, 4);
@@ -320,15 +364,16 @@ extern "C" int tgs_layer_norm_fwd(uint64_t rows, uint32_t width, int32_t dtype, 
       };
       const auto held = [&](auto vec) {
         with_row_map<T, vec.value>(width, [&](auto lanes, auto e) {
-          const uint64_t per = 256 / lanes.value;
+          const uint64_t per = 256 / lanes.value * rows_at_once<e.value>();
           launch(layer_norm_fwd_kernel<T, W, lanes.value, e.value, vec.value>,
-                 std::min<uint64_t>((rows + per - 1) / per, 2048));
+                 std::min<uint64_t>((rows + per - 1) / per, 4096));
         });
       };
       if (width > LN_MAX_HELD)
-        launch(layer_norm_fwd_wide_kernel<T, W>, norm_groups(rows));
+        launch(layer_norm_fwd_wide_kernel<T, W>, std::min<uint64_t>(rows, 4096));
       else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
-               aligned16((const T*)y, width))
+               aligned16((const T*)y, width) && aligned16((const W*)weight, 0) &&
+               aligned16((const W*)bias, 0))
         held(std::true_type());
       else
         held(std::false_type());
@@ -364,7 +409,7 @@ extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, 
       tgs_set_error("tgs_layer_norm_bwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
-    TGS_CHECK_ARG(!sums || workspace, "tgs_layer_norm_bwd: null workspace");
+    TGS_CHECK_ARG(!sums || rows == 0 || workspace, "tgs_layer_norm_bwd: null workspace");
     if (!sums && (!dx || rows == 0)) return TGS_OK;
     float* partial = sums ? (float*)workspace : nullptr;
     const auto typed = [&](auto wtag) {
@@ -376,7 +421,7 @@ extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, 
       uint32_t parts = groups;
       const auto held = [&](auto vec) {
         with_row_map<T, vec.value>(width, [&](auto lanes, auto e) {
-          const uint64_t per = 256 / lanes.value;
+          const uint64_t per = 256 / lanes.value * rows_at_once<e.value>();
           parts = (uint32_t)std::min<uint64_t>((rows + per - 1) / per, groups);
           launch(layer_norm_bwd_kernel<T, W, lanes.value, e.value, vec.value>, parts);
         });
@@ -385,7 +430,8 @@ extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, 
         if (width > LN_MAX_HELD)
           launch(layer_norm_bwd_wide_kernel<T, W>, groups);
         else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
-                 aligned16((const T*)dy, dy_pitch) && (!dx || aligned16((const T*)dx, width)))
+                 aligned16((const T*)dy, dy_pitch) && (!dx || aligned16((const T*)dx, width)) &&
+                 aligned16((const W*)weight, 0))
           held(std::true_type());
         else
           held(std::false_type());
