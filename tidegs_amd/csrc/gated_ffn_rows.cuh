@@ -113,20 +113,20 @@ __device__ __forceinline__ void copy_chunk(char* lds, const char* src) {
                                                (j + wave) * 1024 + (threadIdx.x & 63) * 16, 0, 0, 0);
 }
 
-#define FR_WAVES 8
+#define FR_WAVES 8  // of a workgroup
 
-template <typename T, int DK, int OT, int RT, int ACT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
+template <typename T, int DK, int OT, int RT, int ACT>
+__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N;
   using C = ForwardChunk<T, DK, OT>;
   __shared__ __attribute__((aligned(1024))) char lds[2 * C::KB * 1024];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int TILE = 16 * RT * WAVES;
+  constexpr int TILE = 16 * RT * FR_WAVES;
   {
     const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, WAVES>(lds, a.packed);
+    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
     frag_t<E> x[RT][DK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -141,7 +141,7 @@ __global__ void __launch_bounds__(64 * WAVES) ffn_rows_fwd_kernel(ForwardArgs<T>
       stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (c & 1) * C::KB * 1024;
       if (c + 1 < a.chunks)
-        copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
+        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
                                     a.packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
@@ -224,8 +224,8 @@ struct BackwardArgs {
   int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
 };
 
-template <typename T, int DK, int OK, int RT, int ACT, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) ffn_rows_dx_kernel(BackwardArgs<T> a) {
+template <typename T, int DK, int OK, int RT, int ACT>
+__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK;
   using C = BackwardChunk<T, DK, OK>;
@@ -233,10 +233,10 @@ __global__ void __launch_bounds__(64 * WAVES) ffn_rows_dx_kernel(BackwardArgs<T>
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * C::KB * 1024];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  constexpr int TILE = 16 * RT * WAVES;
+  constexpr int TILE = 16 * RT * FR_WAVES;
   {
     const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, WAVES>(lds, a.packed);
+    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
     frag_t<E> x[RT][DK][P], dy[RT][OK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -253,12 +253,12 @@ __global__ void __launch_bounds__(64 * WAVES) ffn_rows_dx_kernel(BackwardArgs<T>
     for (int c = 0; c < a.chunks; ++c) {
       if (BUFFERS == 1 && c) {
         stage_barrier();
-        copy_chunk<C::KB, WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
+        copy_chunk<C::KB, FR_WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
       }
       stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
       if (BUFFERS == 2 && c + 1 < a.chunks)
-        copy_chunk<C::KB, WAVES>(lds + (~c & 1) * C::KB * 1024,
+        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
                                     a.packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
@@ -412,13 +412,20 @@ struct RowTile {
   }
 };
 
+// Wavefronts of a workgroup at most: two a SIMD, or one with twice the registers where three
+// planes of more than 128 columns of x and dy together need them.
+template <typename T, int DK, int OK>
+constexpr int weight_waves() {
+  return Planes<T>::N == 3 && DK + OK > 4 ? 4 : FR_WAVES;
+}
+
 template <typename T>
 constexpr int weight_rows() {  // of a staged tile
   return Planes<T>::N == 1 ? 64 : 32;
 }
 
 template <typename T, int DK, int OK, int FT, int ACT>
-__global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T> a) {
+__global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_kernel(WeightArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK, OT = 2 * OK, ROWS = weight_rows<T>();
   using X = RowTile<DK>;
@@ -428,7 +435,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int f0 = (blockIdx.y * waves + wave) * 16 * FT;
-  const bool sum_dy = a.dy_sums && blockIdx.y == 0 && wave == 0;
+  const bool sum_dy = a.dy_sums && blockIdx.y == 0;
   const int width8 = (a.width + 7) & ~7, out8 = (a.out + 7) & ~7;
 
   frag_t<E> wg[FT][DK][P], wu[FT][DK][P], wd[FT][OK][P];
@@ -456,11 +463,8 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
         for (int s = 0; s < P; ++s) wd[i][k][s][j] = p[s];
       }
   }
-  frag_t<E> ones;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) ones[j] = (E)1.f;
-
-  f32x4 dwg[FT][DT] = {}, dwu[FT][DT] = {}, dwd[FT][OT] = {}, dys[OT] = {};
+  f32x4 dwg[FT][DT] = {}, dwu[FT][DT] = {}, dwd[FT][OT] = {};
+  float dys[8] = {};  // of eight columns of dy, over every blockDim.x / Y::CHUNKS-th row
   float sg[FT] = {}, su[FT] = {};
   const int64_t tiles = (a.rows + ROWS - 1) / ROWS;
   const auto stage = [&](int64_t tile, char* to) {
@@ -479,6 +483,15 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
     const char* xs = lds + turn * BYTES;
     const char* ys = xs + P * XB;
     if (tile + gridDim.x < tiles) stage(tile + gridDim.x, lds + (turn ^ 1) * BYTES);
+    if (sum_dy)
+      for (int row = threadIdx.x / Y::CHUNKS; row < ROWS; row += blockDim.x / Y::CHUNKS)
+#pragma unroll
+        for (int s = P - 1; s >= 0; --s) {
+          const int c = (threadIdx.x % Y::CHUNKS) ^ Y::turn(row);
+          const frag_t<E> v = *(const frag_t<E>*)(ys + s * YB + row * Y::PITCH + c * 16);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) dys[j] += (float)v[j];
+        }
     if (f0 >= a.hidden) continue;
 #pragma unroll 1
     for (int row = 0; row < ROWS; row += 32) {
@@ -547,9 +560,6 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
         for (int s = 0; s < P; ++s) y[s] = Y::template columns<E>(ys + s * YB, row, o * 16);
 #pragma unroll
         for (int i = 0; i < FT; ++i) dwd[i][o] = mfma_planes<T>(h[i], y, dwd[i][o]);
-        if (sum_dy)
-#pragma unroll
-          for (int s = P - 1; s >= 0; --s) dys[o] = mfma32(y[s], ones, dys[o]);
       }
     }
   }
@@ -589,14 +599,18 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dw_kernel(WeightArgs<T
       }
     }
   }
-  if (sum_dy && (lane & 15) == 0)
+  if (sum_dy) {
+    float* sum = (float*)lds;  // [blockDim.x / Y::CHUNKS][Y::CHUNKS * 8]
+    stage_barrier();
 #pragma unroll
-    for (int o = 0; o < OT; ++o)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int n = o * 16 + (lane >> 4) * 4 + r;
-        if (n < a.out) put(a.dy_sums + (int64_t)blockIdx.x * a.out + n, dys[o][r]);
-      }
+    for (int j = 0; j < 8; ++j) sum[threadIdx.x * 8 + j] = dys[j];
+    __syncthreads();
+    for (int n = threadIdx.x; n < a.out; n += blockDim.x) {
+      float v = 0.f;
+      for (int r = n; r < (int)blockDim.x * 8; r += Y::CHUNKS * 8) v += sum[r];
+      put(a.dy_sums + (int64_t)blockIdx.x * a.out + n, v);
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -655,11 +669,11 @@ struct RowPlan {
     constexpr int P = Planes<T>::N;
     pass = std::min<int64_t>(rows, ROW_PASS);
     const int64_t slices = tiles(hidden, 16 * FT);
-    waves = (int)std::min<int64_t>(slices, FR_WAVES);
+    waves = (int)std::min<int64_t>(slices, weight_waves<T, DK, OK>());
     columns = (int)tiles(slices, waves);
-    // workgroups that the chip holds at once: 256 of eight wavefronts
+    // workgroups that the chip holds at once
     runs = (int)std::max<int64_t>(
-        1, std::min<int64_t>(tiles(pass, weight_rows<T>()), 256 * FR_WAVES / (waves * columns)));
+        1, std::min<int64_t>(tiles(pass, weight_rows<T>()), 256 * weight_waves<T, DK, OK>() / (waves * columns)));
     Carver c{(char*)ws};
     packed = c.take<char>(BackwardChunk<T, DK, OK>::KB * 1024 * tiles(hidden, 32));
     x = c.take<E>(P * pass * round8(width));
@@ -697,13 +711,12 @@ static bool wide_stores(const void* p, int64_t cols) {
   return cols % 4 == 0 && aligned16((const T*)p, 0);
 }
 
-// Rows that fill the chip with wavefronts of 32 rows take them, fewer take 16 (RT as a
-// constant, and the workgroups of WAVES wavefronts).
-template <int WAVES, typename F>
+// Wavefronts take 16 RT rows (a constant) where such fill the chip, 16 where they do not.
+template <int RT, typename F>
 static void with_rows(int64_t rows, F&& f) {
-  const auto launch = [&](auto rt) { f(rt, (unsigned)tiles(rows, 16 * rt.value * WAVES)); };
-  if (rows >= 32 * 8 * 256)
-    launch(std::integral_constant<int, 2>());
+  const auto launch = [&](auto rt) { f(rt, (unsigned)tiles(rows, 16 * rt.value * FR_WAVES)); };
+  if (rows >= 16 * RT * FR_WAVES * 256)
+    launch(std::integral_constant<int, RT>());
   else
     launch(std::integral_constant<int, 1>());
 }
@@ -721,11 +734,14 @@ void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
     const ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
                            c.x_pitch, c.width, c.out, chunks,
                            wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
-    constexpr int WAVES = Planes<T>::N * (DK + OT) <= 8 ? 8 : 4;
-    with_rows<WAVES>(c.rows, [&](auto rt, unsigned groups) {
+    // 32 rows share a fragment's reads, 16 leave room for a second workgroup: 500k rows
+    // bfloat16 of 32-128-16: 27 and 30 us, 64-256-64: 77 and 76, 128-256-128: 191 and 145;
+    // 300k rows float32 of 59-128-3: 114 and 96
+    constexpr int RT = Planes<T>::N == 1 && DK <= 2 ? 2 : 1;
+    with_rows<RT>(c.rows, [&](auto rt, unsigned groups) {
       with_activation(c.act, [&](auto act) {
-        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value, WAVES>),
-                           dim3(groups), dim3(64 * WAVES), 0, stream, a);
+        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value>), dim3(groups),
+                           dim3(64 * FR_WAVES), 0, stream, a);
       });
     });
   });
@@ -747,11 +763,14 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
                               c.dy_pitch, c.width, c.out, chunks,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
                               wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
-      constexpr int WAVES = Planes<T>::N * (2 * DK + OK) <= 6 ? 8 : 4;
-      with_rows<WAVES>(c.rows, [&](auto rt, unsigned groups) {
+      // 16 rows where 32 do not fit the registers (100k rows float32 of 128-256-128: 246 us,
+      // 462 with 32); else 32 (64-256-64: 113 us, 125 with 16; 500k bfloat16 of
+      // 128-256-128: 244 and 281, of 64-256-64: 115 and 108)
+      constexpr int RT = Planes<T>::N == 3 && DK + OK > 4 ? 1 : 2;
+      with_rows<RT>(c.rows, [&](auto rt, unsigned groups) {
         with_activation(c.act, [&](auto act) {
-          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value, WAVES>),
-                             dim3(groups), dim3(64 * WAVES), 0, stream, a);
+          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), dim3(groups),
+                             dim3(64 * FR_WAVES), 0, stream, a);
         });
       });
     }
