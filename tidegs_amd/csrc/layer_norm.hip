@@ -23,18 +23,31 @@ struct RowMap {
   __device__ static __forceinline__ int column(int lane, int e) {
     return (e / R * LANES + lane) * R + e % R;
   }
-  __device__ static __forceinline__ void load(const T* row, int lane, uint32_t n, float (&v)[E]) {
+  // A row as it lies in memory: the loads of several rows are on their way before the first
+  // is converted.  Lanes past the end load the row's first values and keep zeros.
+  struct Raw {
+    Vec16<T> run[VEC ? E / R : 1];
+    T one[VEC ? 1 : E];
+  };
+  __device__ static __forceinline__ void load(const T* row, int lane, uint32_t n, Raw& v) {
 #pragma unroll
     for (int e = 0; e < E; e += R) {
       const uint32_t c = column(lane, e);
-      if constexpr (VEC) {
-        Vec16<T> t = {};
-        if (c < n) t = *(const Vec16<T>*)(row + c);
+      if constexpr (VEC)
+        v.run[e / R] = *(const Vec16<T>*)(row + (c < n ? c : 0));
+      else
+        v.one[e] = row[c < n ? c : 0];
+    }
+  }
+  __device__ static __forceinline__ void convert(const Raw& raw, int lane, uint32_t n,
+                                                 float (&v)[E]) {
 #pragma unroll
-        for (int k = 0; k < R; ++k) v[e + k] = to_f32(t.v[k]);
-      } else {
-        v[e] = c < n ? to_f32(row[c]) : 0.f;
-      }
+    for (int e = 0; e < E; ++e) {
+      const bool in = (uint32_t)column(lane, e / R * R) < n;
+      if constexpr (VEC)
+        v[e] = in ? to_f32(raw.run[e / R].v[e % R]) : 0.f;
+      else
+        v[e] = in ? to_f32(raw.one[e]) : 0.f;
     }
   }
   __device__ static __forceinline__ void store(T* row, int lane, uint32_t n, const float (&v)[E]) {
@@ -67,20 +80,26 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// x becomes xhat; returns rstd.  Lanes past the row's end hold zeros.
+// x becomes xhat; returns rstd.  Lanes past the row's end hold zeros, and keep them: the
+// mean that is taken from them is zero.
 template <typename Map, int LANES, int E>
-__device__ __forceinline__ float normalise(float (&x)[E], int lane, uint32_t n, float eps) {
+__device__ __forceinline__ float normalise(float (&x)[E], int lane, uint32_t n, float inv_n,
+                                           float eps) {
   float s = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) s += x[e];
-  const float mean = group_sum<LANES>(s) / (float)n;
+  const float mean = group_sum<LANES>(s) * inv_n;
   float q = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    x[e] = (uint32_t)Map::column(lane, e) < n ? x[e] - mean : 0.f;
-    q = fmaf(x[e], x[e], q);
+  for (int e = 0; e < E; e += Map::R) {
+    const float m = (uint32_t)Map::column(lane, e) < n ? mean : 0.f;
+#pragma unroll
+    for (int k = 0; k < Map::R; ++k) {
+      x[e + k] -= m;
+      q = fmaf(x[e + k], x[e + k], q);
+    }
   }
-  const float rstd = 1.f / sqrtf(group_sum<LANES>(q) / (float)n + eps);
+  const float rstd = __builtin_amdgcn_rsqf(fmaf(group_sum<LANES>(q), inv_n, eps));
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] *= rstd;
   return rstd;
@@ -109,8 +128,7 @@ __device__ __forceinline__ void load_columns(const W* w, int lane, uint32_t n, f
   }
 }
 
-// Rows that a lane has in flight at once: what keeps enough bytes on their way (4M rows of
-// 64 bfloat16: forward 197 us with one, 5.2 TB/s; see the launch for both).
+// Rows that a lane has in flight at once.
 template <int E>
 constexpr int rows_at_once() {
   return E <= 4 ? 4 : E <= 16 ? 2 : 1;
@@ -123,25 +141,28 @@ __global__ void __launch_bounds__(256) layer_norm_fwd_kernel(
   using Map = RowMap<T, LANES, E, VEC>;
   constexpr int PER = 256 / LANES, U = rows_at_once<E>();  // rows of a workgroup at once
   const int lane = threadIdx.x % LANES;
+  const float inv_n = 1.f / (float)n;
   float w[E], b[E];
   load_columns<Map, VEC>(weight, lane, n, 1.f, w);
   load_columns<Map, VEC>(bias, lane, n, 0.f, b);
   // (a row's sums stay inside its own lanes, so lanes without a row need no barrier)
   for (uint64_t r0 = (uint64_t)blockIdx.x * PER * U + threadIdx.x / LANES; r0 < rows;
        r0 += (uint64_t)gridDim.x * PER * U) {
-    float v[U][E];
+    typename Map::Raw raw[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const uint64_t r = min(r0 + k * PER, rows - 1);  // (the last row again: not stored)
-      Map::load(x + (int64_t)r * pitch, lane, n, v[k]);
+      Map::load(x + (int64_t)r * pitch, lane, n, raw[k]);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
-      normalise<Map, LANES, E>(v[k], lane, n, eps);
+      float v[E];
+      Map::convert(raw[k], lane, n, v);
+      normalise<Map, LANES, E>(v, lane, n, inv_n, eps);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[k][e] = fmaf(v[k][e], w[e], b[e]);
+      for (int e = 0; e < E; ++e) v[e] = fmaf(v[e], w[e], b[e]);
       const uint64_t r = r0 + k * PER;
-      if (r < rows) Map::store(y + r * n, lane, n, v[k]);
+      if (r < rows) Map::store(y + r * n, lane, n, v);
     }
   }
 }
@@ -150,42 +171,46 @@ template <typename T, typename W, int LANES, int E, bool VEC>
 __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(
     uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const T* __restrict__ dy,
     int64_t dy_pitch, const W* __restrict__ weight, float eps, T* __restrict__ dx,
-    float* __restrict__ partial) {
+    float* __restrict__ partial, W* __restrict__ dweight, W* __restrict__ dbias) {
   using Map = RowMap<T, LANES, E, VEC>;
   constexpr int PER = 256 / LANES, U = rows_at_once<E>();
   __shared__ float s_part[2][LANES * E];
   const int lane = threadIdx.x % LANES;
+  const float inv_n = 1.f / (float)n;
   float w[E], dw[E] = {}, db[E] = {};
   load_columns<Map, VEC>(weight, lane, n, 1.f, w);
   for (uint64_t r0 = (uint64_t)blockIdx.x * PER * U + threadIdx.x / LANES; r0 < rows;
        r0 += (uint64_t)gridDim.x * PER * U) {
-    float v[U][E], g[U][E];
+    typename Map::Raw raw_x[U], raw_dy[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const uint64_t r = min(r0 + k * PER, rows - 1);
-      Map::load(x + (int64_t)r * pitch, lane, n, v[k]);
-      Map::load(dy + (int64_t)r * dy_pitch, lane, n, g[k]);
+      Map::load(x + (int64_t)r * pitch, lane, n, raw_x[k]);
+      Map::load(dy + (int64_t)r * dy_pitch, lane, n, raw_dy[k]);
     }
 #pragma unroll
     for (int k = 0; k < U; ++k) {
       const uint64_t r = r0 + k * PER;
       if (r >= rows) break;
-      const float rstd = normalise<Map, LANES, E>(v[k], lane, n, eps);
+      float v[E], g[E];
+      Map::convert(raw_x[k], lane, n, v);
+      Map::convert(raw_dy[k], lane, n, g);
+      const float rstd = normalise<Map, LANES, E>(v, lane, n, inv_n, eps);
       float s = 0.f, q = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        dw[e] = fmaf(g[k][e], v[k][e], dw[e]);
-        db[e] += g[k][e];
-        g[k][e] *= w[e];
-        s += g[k][e];
-        q = fmaf(g[k][e], v[k][e], q);
+        dw[e] = fmaf(g[e], v[e], dw[e]);
+        db[e] += g[e];
+        g[e] *= w[e];
+        s += g[e];
+        q = fmaf(g[e], v[e], q);
       }
       if (dx) {
-        s = group_sum<LANES>(s) / (float)n;
-        q = group_sum<LANES>(q) / (float)n;
+        s = group_sum<LANES>(s) * inv_n;
+        q = group_sum<LANES>(q) * inv_n;
 #pragma unroll
-        for (int e = 0; e < E; ++e) v[k][e] = rstd * (g[k][e] - s - v[k][e] * q);
-        Map::store(dx + r * n, lane, n, v[k]);
+        for (int e = 0; e < E; ++e) v[e] = rstd * (g[e] - s - v[e] * q);
+        Map::store(dx + r * n, lane, n, v);
       }
     }
   }
@@ -208,12 +233,18 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_kernel(
     }
     __syncthreads();
   }
-  for (uint32_t i = threadIdx.x; i < 2 * n; i += 256)
-    partial[(uint64_t)blockIdx.x * 2 * n + i] = i < n ? s_part[0][i] : s_part[1][i - n];
+  for (uint32_t i = threadIdx.x; i < 2 * n; i += 256) {
+    const float v = i < n ? s_part[0][i] : s_part[1][i - n];
+    W* out = i < n ? dweight : dbias;
+    if (gridDim.x > 1)
+      partial[(uint64_t)blockIdx.x * 2 * n + i] = v;
+    else if (out)  // nothing to join
+      out[i < n ? i : i - n] = from_f32<W>(v);
+  }
 }
 
 // A row of any width, one workgroup per row, read again for each of its sums (rows
-// that 64 lanes do not hold in registers: 4096 values).
+// that 64 lanes do not hold in registers).
 __device__ __forceinline__ float block_sum(float v, float* s) {
   v = tgs_wave_sum(v);
   __syncthreads();
@@ -257,7 +288,7 @@ template <typename T, typename W>
 __global__ void __launch_bounds__(256) layer_norm_bwd_wide_kernel(
     uint64_t rows, uint32_t n, const T* __restrict__ x, int64_t pitch, const T* __restrict__ dy,
     int64_t dy_pitch, const W* __restrict__ weight, float eps, T* __restrict__ dx,
-    float* __restrict__ partial) {
+    float* __restrict__ partial, W*, W*) {
   __shared__ float s[4];
   float* dw = partial ? partial + (uint64_t)blockIdx.x * 2 * n : nullptr;
   if (dw)
@@ -287,30 +318,35 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_kernel(
   }
 }
 
-// dw and db: the partial rows' sums, 32 columns by 32 interleaved runs of rows.
+// dw and db: the partial rows' sums, 8 columns by 128 interleaved runs of rows a workgroup
+// (32 by 32 left the few columns of narrow rows to four workgroups: 20 us for 2048 partial
+// rows of 59, now 5).
 template <typename W>
 __global__ void __launch_bounds__(1024) layer_norm_join_kernel(uint32_t parts, uint32_t n,
                                                                const float* __restrict__ partial,
                                                                W* __restrict__ dweight,
                                                                W* __restrict__ dbias) {
-  __shared__ float s[32][33];
-  const uint32_t c = blockIdx.x * 32 + threadIdx.x % 32, k = threadIdx.x / 32;
+  __shared__ float s[1024];
+  const uint32_t c = blockIdx.x * 8 + threadIdx.x % 8, k = threadIdx.x / 8;
   float a = 0.f;
-  if (c < 2 * n)
-    for (uint32_t p = k; p < parts; p += 32) a += partial[(uint64_t)p * 2 * n + c];
-  s[k][threadIdx.x % 32] = a;
-  __syncthreads();
-  for (uint32_t h = 16; h > 0; h >>= 1) {
-    if (k < h) s[k][threadIdx.x % 32] += s[k + h][threadIdx.x % 32];
+  if (c < 2 * n) {
+#pragma unroll 8
+    for (uint32_t p = k; p < parts; p += 128) a += partial[(uint64_t)p * 2 * n + c];
+  }
+  s[threadIdx.x] = a;
+  for (uint32_t h = 64; h > 0; h >>= 1) {
     __syncthreads();
+    if (k < h) s[threadIdx.x] += s[threadIdx.x + 8 * h];
   }
   if (k == 0 && c < 2 * n) {
     W* out = c < n ? dweight : dbias;
-    if (out) out[c < n ? c : c - n] = from_f32<W>(s[0][threadIdx.x % 32]);
+    if (out) out[c < n ? c : c - n] = from_f32<W>(s[threadIdx.x]);
   }
 }
 
-#define LN_MAX_HELD 4096  // values of a row that 64 lanes hold in registers
+// Values of a row that 64 lanes hold in registers; half as many one by one, whose backward
+// would spill.
+static uint32_t most_held(bool vec) { return vec ? 4096 : 2048; }
 
 // Workgroups of a backward launch: each leaves a partial row of both sums, so none for fewer
 // than 16 rows once the CUs have one each (8191 rows of 1024: 2048 workgroups' partial rows
@@ -341,7 +377,7 @@ static void with_row_map(uint32_t n, F&& f) {
   LN_MAP(64, 8);
   LN_MAP(64, 16);
   LN_MAP(64, 32);
-  LN_MAP(64, 64);
+  if constexpr (R > 1) LN_MAP(64, 64);
 #undef LN_MAP
 }
 
@@ -369,11 +405,12 @@ extern "C" int tgs_layer_norm_fwd(uint64_t rows, uint32_t width, int32_t dtype, 
                  std::min<uint64_t>((rows + per - 1) / per, 4096));
         });
       };
-      if (width > LN_MAX_HELD)
+      const bool vec = width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
+                       aligned16((const T*)y, width) && aligned16((const W*)weight, 0) &&
+                       aligned16((const W*)bias, 0);
+      if (width > most_held(vec))
         launch(layer_norm_fwd_wide_kernel<T, W>, std::min<uint64_t>(rows, 4096));
-      else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
-               aligned16((const T*)y, width) && aligned16((const W*)weight, 0) &&
-               aligned16((const W*)bias, 0))
+      else if (vec)
         held(std::true_type());
       else
         held(std::false_type());
@@ -416,8 +453,12 @@ extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, 
       using W = decltype(wtag);
       const auto launch = [&](auto kernel, uint32_t g) {
         hipLaunchKernelGGL(kernel, dim3(g), dim3(256), 0, stream, rows, width, (const T*)x,
-                           x_pitch, (const T*)dy, dy_pitch, (const W*)weight, eps, (T*)dx, partial);
+                           x_pitch, (const T*)dy, dy_pitch, (const W*)weight, eps, (T*)dx, partial,
+                           (W*)dweight, (W*)dbias);
       };
+      const bool vec = width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
+                       aligned16((const T*)dy, dy_pitch) && (!dx || aligned16((const T*)dx, width)) &&
+                       aligned16((const W*)weight, 0);
       uint32_t parts = groups;
       const auto held = [&](auto vec) {
         with_row_map<T, vec.value>(width, [&](auto lanes, auto e) {
@@ -427,17 +468,15 @@ extern "C" int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, 
         });
       };
       if (rows) {
-        if (width > LN_MAX_HELD)
+        if (width > most_held(vec))
           launch(layer_norm_bwd_wide_kernel<T, W>, groups);
-        else if (width % Vec16<T>::N == 0 && aligned16((const T*)x, x_pitch) &&
-                 aligned16((const T*)dy, dy_pitch) && (!dx || aligned16((const T*)dx, width)) &&
-                 aligned16((const W*)weight, 0))
+        else if (vec)
           held(std::true_type());
         else
           held(std::false_type());
       }
-      if (sums)
-        hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((2 * width + 31) / 32), dim3(1024), 0,
+      if (sums && (parts != 1 || width > most_held(vec)))
+        hipLaunchKernelGGL(layer_norm_join_kernel<W>, dim3((2 * width + 7) / 8), dim3(1024), 0,
                            stream, parts, width, partial, (W*)dweight, (W*)dbias);
     };
     if (weight_dtype == dtype)

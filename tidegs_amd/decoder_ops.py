@@ -64,8 +64,16 @@ def _parameter(t: Optional[Tensor], name: str, shape, x: Tensor, also=()) -> Opt
     return t.contiguous()
 
 
-def _workspace(nbytes: int, device) -> Optional[Tensor]:
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+def _once(backward):
+    """``backward`` as an autograd Function's: not differentiable again, which only a
+    backward that records its own graph has to be told (the wrapper that tells it
+    costs as much as a launch)."""
+    recorded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, dy):
+        return recorded(ctx, dy) if torch.is_grad_enabled() else backward(ctx, dy)
+
+    return staticmethod(run)
 
 
 # ---------------------------------------------------------------------------
@@ -74,42 +82,47 @@ def _workspace(nbytes: int, device) -> Optional[Tensor]:
 
 
 def _layer_norm_fwd(x, weight, bias, eps):
+    """(x as it is read, y, the arguments that the backward's call shares)."""
     x, rows, pitch = _rows(x)
     width = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
+    code = _DTYPES[x.dtype]
     w = weight if weight is not None else bias
-    N.call("tgs_layer_norm_fwd", rows, width, _DTYPES[x.dtype], x.data_ptr(), pitch,
-           N.ptr(weight), N.ptr(bias), _DTYPES[x.dtype if w is None else w.dtype], eps,
-           y.data_ptr(), N.stream_handle(x.device))
-    return x, y
+    w_code = code if w is None or w.dtype == x.dtype else _DTYPES[w.dtype]
+    N.call("tgs_layer_norm_fwd", rows, width, code, x.data_ptr(), pitch, N.ptr(weight),
+           N.ptr(bias), w_code, eps, y.data_ptr(), N.stream_handle(x.device))
+    return x, y, (rows, width, code, pitch, w_code, eps)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        x, y = _layer_norm_fwd(x, weight, bias, eps)
+        x, y, ctx.call = _layer_norm_fwd(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, bias)
-        ctx.eps = eps
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, weight, bias = ctx.saved_tensors
-        x, rows, pitch = _rows(x)
-        dy, _, dy_pitch = _rows(dy)
-        width, dev = x.shape[-1], x.device
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
-        dw = torch.empty_like(weight) if need_w else None
-        db = torch.empty_like(bias) if need_b else None
-        w = weight if weight is not None else bias
-        ws = _workspace(N.load().tgs_layer_norm_bwd_workspace_size(rows, width), dev) \
-            if need_w or need_b else None
-        N.call("tgs_layer_norm_bwd", rows, width, _DTYPES[x.dtype], x.data_ptr(), pitch,
-               dy.data_ptr(), dy_pitch, N.ptr(weight),
-               _DTYPES[x.dtype if w is None else w.dtype], ctx.eps, N.ptr(dx), N.ptr(dw),
-               N.ptr(db), N.ptr(ws), 0 if ws is None else ws.numel(), N.stream_handle(dev))
+        rows, width, code, pitch, w_code, eps = ctx.call
+        dy_pitch = width
+        if not dy.is_contiguous():
+            dy, _, dy_pitch = _rows(dy)
+        need_x, need_w, need_b, _ = ctx.needs_input_grad
+        dx = dw = db = ws = None
+        ws_bytes = 0
+        if need_x:
+            dx = x.new_empty(x.shape)
+        if need_w:
+            dw = weight.new_empty(width)
+        if need_b:
+            db = bias.new_empty(width)
+        if need_w or need_b:
+            ws_bytes = N.load().tgs_layer_norm_bwd_workspace_size(rows, width)
+            ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
+        N.call("tgs_layer_norm_bwd", rows, width, code, x.data_ptr(), pitch, dy.data_ptr(),
+               dy_pitch, N.ptr(weight), w_code, eps, N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(ws),
+               ws_bytes, N.stream_handle(x.device))
         return dx, dw, db, None
 
 
@@ -155,8 +168,7 @@ class _Dropout(torch.autograd.Function):
         ctx.draws = threshold, seed, offset
         return _dropout(x, residual, threshold, seed, offset)
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         dx = _dropout(dy.contiguous(), None, *ctx.draws) if ctx.needs_input_grad[0] else None
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None
@@ -198,43 +210,42 @@ def dropout(x: Tensor, p: float, seed: int, offset: int = 0,
 
 
 def _gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
+    """(x as it is read, y, the arguments that the backward's call shares)."""
     x, rows, pitch = _rows(x)
     (hidden, width), out = w_gate.shape, w_down.shape[0]
-    y = torch.empty((*x.shape[:-1], out), dtype=x.dtype, device=x.device)
+    y = x.new_empty((*x.shape[:-1], out))
     code = _DTYPES[x.dtype]
-    ws = _workspace(N.load().tgs_gated_ffn_fwd_workspace_size(rows, width, hidden, out, code),
-                    x.device)
+    nbytes = N.load().tgs_gated_ffn_fwd_workspace_size(rows, width, hidden, out, code)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     N.call("tgs_gated_ffn_fwd", rows, width, hidden, out, code, act, x.data_ptr(), pitch,
            w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), N.ptr(b_gate), N.ptr(b_up),
-           N.ptr(b_down), y.data_ptr(), N.ptr(ws), 0 if ws is None else ws.numel(),
-           N.stream_handle(x.device))
-    return x, y
+           N.ptr(b_down), y.data_ptr(), ws.data_ptr(), nbytes, N.stream_handle(x.device))
+    return x, y, (rows, width, hidden, out, code, act, pitch)
 
 
 class _GatedFfn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
-        x, y = _gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
+        x, y, ctx.call = _gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act)
         ctx.save_for_backward(x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-        ctx.act = act
         return y
 
-    @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
-        x, w_gate, w_up, w_down, b_gate, b_up, b_down = saved = ctx.saved_tensors
-        x, rows, pitch = _rows(x)
-        dy, _, dy_pitch = _rows(dy)
-        (hidden, width), out = w_gate.shape, w_down.shape[0]
-        code, dev = _DTYPES[x.dtype], x.device
-        grads = [torch.empty(t.shape, dtype=t.dtype, device=dev) if need else None
+        saved = ctx.saved_tensors
+        x, w_gate, w_up, w_down, b_gate, b_up, _ = saved
+        rows, width, hidden, out, code, act, pitch = ctx.call
+        dy_pitch = out
+        if not dy.is_contiguous():
+            dy, _, dy_pitch = _rows(dy)
+        grads = [t.new_empty(t.shape) if need else None
                  for t, need in zip(saved, ctx.needs_input_grad)]
-        ws = _workspace(N.load().tgs_gated_ffn_bwd_workspace_size(rows, width, hidden, out, code),
-                        dev)
-        N.call("tgs_gated_ffn_bwd", rows, width, hidden, out, code, ctx.act, x.data_ptr(), pitch,
+        nbytes = N.load().tgs_gated_ffn_bwd_workspace_size(rows, width, hidden, out, code)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("tgs_gated_ffn_bwd", rows, width, hidden, out, code, act, x.data_ptr(), pitch,
                w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), N.ptr(b_gate), N.ptr(b_up),
-               dy.data_ptr(), dy_pitch, *(N.ptr(t) for t in grads), N.ptr(ws),
-               0 if ws is None else ws.numel(), N.stream_handle(dev))
+               dy.data_ptr(), dy_pitch, *map(N.ptr, grads), ws.data_ptr(), nbytes,
+               N.stream_handle(x.device))
         return *grads, None
 
 
