@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
     sx.begin(a.x.pitch, m0, a.rows, a.width8);
     sw.begin(a.wg.pitch, f0, a.hidden, a.width8, [](int r) { return (r >> 5) * 16 + (r & 15); });
     const E *x = a.x.p + m0 * a.x.pitch, *wg = a.wg.p + f0 * a.wg.pitch, *wu = a.wu.p + f0 * a.wu.pitch;
-    product_loop<E, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * TM * 16, wn * TF * 32,
+    product_loop<E, false, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * TM * 16, wn * TF * 32,
                             [&](const Steps& s, char* to) {
                               const int64_t w = PlanePairs<T>::b(s.pair) * a.wg.plane;
                               sx.copy(to, x + PlanePairs<T>::a(s.pair) * a.x.plane, s.k);
@@ -77,7 +77,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
     sy.begin(a.dy.pitch, m0, a.rows, a.out8);
     sd.begin(a.wd.pitch, f0, a.hidden8, a.out);
     const E *dy = a.dy.p + m0 * a.dy.pitch, *wd = a.wd.p + f0;
-    product_loop<E, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * TM * 16, wn * TF * 16,
+    product_loop<E, P == 3, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * TM * 16, wn * TF * 16,
                             [&](const Steps& s, char* to) {
                               sy.copy(to, dy + PlanePairs<T>::a(s.pair) * a.dy.plane, s.k);
                               sd.copy(to + SX::BYTES, wd + PlanePairs<T>::b(s.pair) * a.wd.plane, s.k);
@@ -110,7 +110,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
 #pragma unroll
         for (int q = 0; q < P; ++q) h[q][r] = p[q];
         if constexpr (BACK) {
-          const float d = dh[i][j][r];
+          const float d = P == 3 && i % 2 ? -dh[i][j][r] : dh[i][j][r];
           // (behind the last hidden column zeros, whatever x holds)
           const float vg = f + r < a.hidden ? d * u * act.y : 0.f;
           const float vu = f + r < a.hidden ? d * act.x : 0.f;
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<
   const int64_t at_a = KA == ALONG ? m0 * g.a.pitch : m0;
   const int64_t at_b = KB == ALONG ? n0 * g.b.pitch : n0;
   f32x4 acc[TM][TN] = {};
-  product_loop<E, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * TM * 16,
+  product_loop<E, false, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * TM * 16,
                           wn * TN * 16,
                           [&](const Steps& s, char* to_lds) {
                             const bool second = s.pair >= PAIRS;

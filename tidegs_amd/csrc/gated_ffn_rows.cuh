@@ -518,7 +518,10 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
         for (int k = 0; k < OK; ++k) {
           frag_t<E> y[P];
 #pragma unroll
-          for (int s = 0; s < P; ++s) y[s] = Y::template rows<E>(ys + s * YB, row, t, k);
+          for (int s = 0; s < P; ++s) {
+            y[s] = Y::template rows<E>(ys + s * YB, row, t, k);
+            if (P == 3 && t) y[s] = negated<E>(y[s]);
+          }
 #pragma unroll
           for (int i = 0; i < FT; ++i) dh[i] = mfma_planes<T>(y, wd[i][k], dh[i]);
         }
@@ -527,7 +530,8 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
               const float2 v = activation<T, ACT>(g[i][r]);
-              const float vg = dh[i][r] * u[i][r] * v.y, vu = dh[i][r] * v.x;
+              const float d = P == 3 && t ? -dh[i][r] : dh[i][r];
+              const float vg = d * u[i][r] * v.y, vu = d * v.x;
               sg[i] += vg;
               su[i] += vu;
               E p[P];
