@@ -8,10 +8,10 @@ enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
 
 // act(g) and its derivative.  Exponentials are 2^(g log2 e) on the hardware unit: a relative
 // error of |g| 2^-24, which the factor s (1 - s) |g| <= 0.28 |g| of silu and the decay of
-// the others keep under 2^-23 of |g| in the result.  gelu of 16-bit tensors takes
-// erfc from Abramowitz and Stegun 7.1.26 (off by 1.5e-7 at most, a 2^-13th of a
-// bfloat16's spacing at 1), which shares its exponential with the derivative.
-template <typename T, int ACT>
+// the others keep under 2^-23 of |g| in the result.  gelu takes erfc from Abramowitz and
+// Stegun 7.1.26, whose error in erf (1.5e-7 at most) is that of a 32-bit 1 + erf, and
+// which shares its exponential with the derivative.
+template <int ACT>
 __device__ __forceinline__ float2 activation(float g) {
   if constexpr (ACT == ACT_RELU) {
     return g > 0.f ? make_float2(g, 1.f) : make_float2(0.f * g, 0.f);
@@ -21,18 +21,13 @@ __device__ __forceinline__ float2 activation(float g) {
     return make_float2(a, fmaf(a, 1.f - s, s));
   } else {
     const float e = __builtin_amdgcn_exp2f(g * g * -0.72134752f);  // exp(-g^2 / 2)
-    float phi;
-    if constexpr (sizeof(T) == 4) {
-      phi = 0.5f * (1.f + erff(g * 0.70710678f));
-    } else {
-      const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
-      float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-      q = fmaf(t, q, 0.5f * 1.421413741f);
-      q = fmaf(t, q, 0.5f * -0.284496736f);
-      q = fmaf(t, q, 0.5f * 0.254829592f);
-      q = q * t * e;
-      phi = g >= 0.f ? 1.f - q : q;
-    }
+    const float t = __builtin_amdgcn_rcpf(fmaf(fabsf(g), 0.3275911f * 0.70710678f, 1.f));
+    float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    q = fmaf(t, q, 0.5f * 1.421413741f);
+    q = fmaf(t, q, 0.5f * -0.284496736f);
+    q = fmaf(t, q, 0.5f * 0.254829592f);
+    q = q * t * e;
+    const float phi = g >= 0.f ? 1.f - q : q;
     return make_float2(g * phi, fmaf(g * 0.39894228f, e, phi));
   }
 }

@@ -100,31 +100,29 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
     for (int i = 0; i < TM; ++i) {
       const int64_t m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
       const bool live = m < a.rows && f < a.hidden8;
-      four_t<E> h[P], dg[P], du[P];
+      float vh[4], vg[4], vu[4];
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
+        // (behind the last hidden column zeros, whatever x holds)
+        const bool in = f + r < a.hidden;
         const float g = gu[i][2 * j][r] + bg[r], u = gu[i][2 * j + 1][r] + bu[r];
-        const float2 act = activation<T, kind.value>(g);
-        E p[P];
-        split<T>(f + r < a.hidden ? act.x * u : 0.f, p);
-#pragma unroll
-        for (int q = 0; q < P; ++q) h[q][r] = p[q];
+        const float2 act = activation<kind.value>(g);
+        vh[r] = in ? act.x * u : 0.f;
         if constexpr (BACK) {
           const float d = P == 3 && i % 2 ? -dh[i][j][r] : dh[i][j][r];
-          // (behind the last hidden column zeros, whatever x holds)
-          const float vg = f + r < a.hidden ? d * u * act.y : 0.f;
-          const float vu = f + r < a.hidden ? d * act.x : 0.f;
+          vg[r] = in ? d * u * act.y : 0.f;
+          vu[r] = in ? d * act.x : 0.f;
           if (m < a.rows) {
-            sg[j][r] += vg;
-            su[j][r] += vu;
+            sg[j][r] += vg[r];
+            su[j][r] += vu[r];
           }
-          split<T>(vg, p);
-#pragma unroll
-          for (int q = 0; q < P; ++q) dg[q][r] = p[q];
-          split<T>(vu, p);
-#pragma unroll
-          for (int q = 0; q < P; ++q) du[q][r] = p[q];
         }
+      }
+      four_t<E> h[P], dg[P], du[P];
+      split4<T>(vh, h);
+      if constexpr (BACK) {
+        split4<T>(vg, dg);
+        split4<T>(vu, du);
       }
       if (!live) continue;
 #pragma unroll

@@ -91,17 +91,16 @@ __global__ void __launch_bounds__(64 * FEW_HIDDEN_WAVES) ffn_few_hidden_kernel(F
 #pragma unroll
   for (int w = 1; w < W; ++w) gs += s[w][wave][0][lane], us += s[w][wave][1][lane];
   if (m >= a.rows || f >= a.hidden8) return;
-  four_t<E> h[P];
+  float v[4];
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const bool in = f + r < a.hidden;
     const float gv = gs[r] + (a.bg && in ? to_f32(a.bg[f + r]) : 0.f);
     const float uv = us[r] + (a.bu && in ? to_f32(a.bu[f + r]) : 0.f);
-    E p[P];
-    split<T>(in ? activation<T, ACT>(gv).x * uv : 0.f, p);
-#pragma unroll
-    for (int q = 0; q < P; ++q) h[q][r] = p[q];
+    v[r] = in ? activation<ACT>(gv).x * uv : 0.f;
   }
+  four_t<E> h[P];
+  split4<T>(v, h);
 #pragma unroll
   for (int q = 0; q < P; ++q)
     *(four_t<E>*)(a.h + ((int64_t)q * a.rows + m) * a.hidden8 + f) = h[q];

@@ -166,14 +166,14 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
           for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
         }
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i) {
+          float v[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              E p[P];
-              split<T>(activation<T, ACT>(g[i][r]).x * u[i][r], p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) h[i][s][t * 4 + r] = p[s];
-            }
+          for (int r = 0; r < 4; ++r) v[r] = activation<ACT>(g[i][r]).x * u[i][r];
+          four_t<E> p[P];
+          split4<T>(v, p);
+          set_half<E, P>(h[i], t, p);
+        }
       }
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
@@ -289,18 +289,20 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
           for (int i = 0; i < RT; ++i) dh[i] = mfma_planes<T>(w, dy[i][k], dh[i]);
         }
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i) {
+          float vg[4], vu[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float2 v = activation<T, ACT>(g[i][r]);
-              E p[P];
-              split<T>(dh[i][r] * u[i][r] * v.y, p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) dg[i][s][t * 4 + r] = p[s];
-              split<T>(dh[i][r] * v.x, p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) du[i][s][t * 4 + r] = p[s];
-            }
+          for (int r = 0; r < 4; ++r) {
+            const float2 v = activation<ACT>(g[i][r]);
+            vg[r] = dh[i][r] * u[i][r] * v.y;
+            vu[r] = dh[i][r] * v.x;
+          }
+          four_t<E> p[P];
+          split4<T>(vg, p);
+          set_half<E, P>(dg[i], t, p);
+          split4<T>(vu, p);
+          set_half<E, P>(du[i], t, p);
+        }
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
@@ -526,25 +528,26 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
           for (int i = 0; i < FT; ++i) dh[i] = mfma_planes<T>(y, wd[i][k], dh[i]);
         }
 #pragma unroll
-          for (int i = 0; i < FT; ++i)
+        for (int i = 0; i < FT; ++i) {
+          float vg[4], vu[4], vh[4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-              const float2 v = activation<T, ACT>(g[i][r]);
-              const float d = P == 3 && t ? -dh[i][r] : dh[i][r];
-              const float vg = d * u[i][r] * v.y, vu = d * v.x;
-              sg[i] += vg;
-              su[i] += vu;
-              E p[P];
-              split<T>(vg, p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) dg[i][s][t * 4 + r] = p[s];
-              split<T>(vu, p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) du[i][s][t * 4 + r] = p[s];
-              split<T>(v.x * u[i][r], p);
-#pragma unroll
-              for (int s = 0; s < P; ++s) h[i][s][t * 4 + r] = p[s];
-            }
+          for (int r = 0; r < 4; ++r) {
+            const float2 v = activation<ACT>(g[i][r]);
+            const float d = P == 3 && t ? -dh[i][r] : dh[i][r];
+            vg[r] = d * u[i][r] * v.y;
+            vu[r] = d * v.x;
+            vh[r] = v.x * u[i][r];
+            sg[i] += vg[r];
+            su[i] += vu[r];
+          }
+          four_t<E> p[P];
+          split4<T>(vg, p);
+          set_half<E, P>(dg[i], t, p);
+          split4<T>(vu, p);
+          set_half<E, P>(du[i], t, p);
+          split4<T>(vh, p);
+          set_half<E, P>(h[i], t, p);
+        }
       }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {

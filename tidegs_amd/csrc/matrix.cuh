@@ -76,6 +76,46 @@ __device__ __forceinline__ void split(float v, typename Planes<T>::E (&p)[Planes
   }
 }
 
+// Four values at once, as kernels split what they compute: a 32-bit value's planes are its
+// bits in three runs of 8 (each cut off, not rounded: exact, and the products left out
+// then come to 2^-26 of the whole), two values a word, six operations a value instead of
+// nine.  A value that is not finite comes out as NaN.
+template <typename T>
+__device__ __forceinline__ void split4(const float (&v)[4],
+                                       four_t<typename Planes<T>::E> (&out)[Planes<T>::N]) {
+  if constexpr (Planes<T>::N == 1) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) out[0][r] = (typename Planes<T>::E)v[r];
+  } else {
+    union {
+      uint32_t w[2];
+      four_t<bf16_t> f;
+    } u;
+    float rest[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int q = 0; q < 3; ++q) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+        u.w[k] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * k + 1]),
+                                       __float_as_uint(rest[2 * k]), 0x07060302);
+      out[q] = u.f;
+      if (q < 2)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          rest[r] -= __uint_as_float(__float_as_uint(rest[r]) & 0xFFFF0000u);
+    }
+  }
+}
+
+// The halves of fragments.
+template <typename E, int P>
+__device__ __forceinline__ void set_half(frag_t<E> (&f)[P], int half, const four_t<E> (&v)[P]) {
+#pragma unroll
+  for (int q = 0; q < P; ++q)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) f[q][half * 4 + r] = v[q][r];
+}
+
 // The pairs of planes that a product multiplies, the smallest first.
 template <typename T>
 struct PlanePairs {
