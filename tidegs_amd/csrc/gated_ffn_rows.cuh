@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK;
   using C = BackwardChunk<T, DK, OK>;
-  constexpr int BUFFERS = C::KB <= 80 ? 2 : 1;
+  constexpr int BUFFERS = P == 3 ? 1 : 2;  // one, so that two workgroups share a CU
   __shared__ __attribute__((aligned(1024))) char lds[BUFFERS * C::KB * 1024];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -770,10 +770,10 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
                               c.dy_pitch, c.width, c.out, chunks,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
                               wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
-      // 16 rows where 32 do not fit the registers (100k rows float32 of 128-256-128: 246 us,
-      // 462 with 32); else 32 (64-256-64: 113 us, 125 with 16; 500k bfloat16 of
-      // 128-256-128: 244 and 281, of 64-256-64: 115 and 108)
-      constexpr int RT = Planes<T>::N == 3 && DK + OK > 4 ? 1 : 2;
+      // 500k rows bfloat16, 32 and 16 rows a wavefront: 128-256-128 244 and 281 us, 64-256-64
+      // 115 and 108; float32 with 16 rows and one chunk buffer, where two workgroups share
+      // a CU, against 32 and two: 300k of 59-128-3 147 and 175 us
+      constexpr int RT = Planes<T>::N == 3 ? 1 : 2;
       with_rows<RT>(c.rows, [&](auto rt, unsigned groups) {
         with_activation(c.act, [&](auto act) {
           hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), dim3(groups),
