@@ -307,10 +307,11 @@ static int64_t pass_rows(int64_t rows, int64_t hidden) {
   return std::min(rows, most);
 }
 
-// Parts that a product's sum over `k` values is split into so that its workgroups fill the
-// chip twice, none shorter than four steps.
-static int splits_of(int64_t tiles_, int64_t k) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(512 / tiles_, k / (4 * MX_BK)));
+static int splits_of(int64_t tiles_, int64_t k) { return split_parts(tiles_, k / MX_BK); }
+
+// Values that the partial sums of a rows x N product over k may take, whatever its splits.
+static int64_t partial_values(int64_t rows, int64_t N, int64_t k) {
+  return std::min(rows * N * std::max<int64_t>(1, k / MX_BK / 4), (int64_t)SPLIT_TILES * 128 * 128);
 }
 
 // Whether there are enough tiles Z of an M x N product for the CUs.
@@ -329,7 +330,7 @@ struct Plan {
   static constexpr int P = Planes<T>::N;
   int64_t rows, D, F, O, D8, F8, O8, pass;
   E *x, *wg, *wu, *wd, *dy, *h, *dgu;
-  float *gu_sums, *dy_sums, *dwgu, *dwd;
+  float *parts, *gu_sums, *dy_sums, *dwgu, *dwd;  // parts: of y or dx
   int split_gu = 1, split_d = 1;
   uint64_t bytes;
 
@@ -342,6 +343,7 @@ struct Plan {
     wu = c.take<E>(P * F * D8);
     wd = c.take<E>(P * O * F8);
     h = c.take<E>(P * pass * F8);
+    parts = c.take<float>(back ? partial_values(pass, D, F) : partial_values(pass, O, F8));
     if (back) {
       dy = c.take<E>(P * pass * O8);
       dgu = c.take<E>(2 * P * pass * F8);
@@ -369,6 +371,18 @@ static void product(hipStream_t s, ProductArgs<typename Planes<T>::E> g) {
   if constexpr (KA == ALONG && KB == ALONG)
     if (fills<TileLarge>(g.M, g.N, g.splits)) return launch(TileLarge());
   launch(TileSmall());
+}
+
+// A product of rows, its sum over k split where its tiles are few.
+template <typename T, Along KA, Along KB>
+static void row_product(hipStream_t s, ProductArgs<typename Planes<T>::E> g, float* parts) {
+  g.splits = splits_of(tiles(g.M, TileSmall::M) * tiles(g.N, TileSmall::N), g.K);
+  if (g.splits == 1) return product<T, KA, KB>(s, g);
+  g.partial = parts;
+  product<T, KA, KB>(s, g);
+  Joiner<T> join;
+  join.add(parts, g.M * g.N, g.N, g.splits, g.M, g.N, g.c, g.bias);
+  join.launch(s);
 }
 
 template <typename T, bool BACK>
@@ -453,9 +467,9 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
       hidden_products<T, false>(stream, a);
       ProductArgs<E> g{};
       g.a = {p.h, a.plane, p.F8}, g.b = wd;
-      g.M = m, g.N = p.O, g.K = p.F8, g.a_limit = m, g.b_limit = p.O, g.splits = 1;
+      g.M = m, g.N = p.O, g.K = p.F8, g.a_limit = m, g.b_limit = p.O;
       g.bias = b_down, g.c = (T*)y + r * p.O;
-      product<T, ALONG, ALONG>(stream, g);
+      row_product<T, ALONG, ALONG>(stream, g, p.parts);
     }
     TGS_RETURN_LAUNCH("tgs_gated_ffn_fwd");
   });
@@ -514,9 +528,9 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
         g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.a2 = {p.dgu + p.F8, 2 * a.plane, 2 * p.F8};
         g.b = wg, g.b2 = wu;
         // (k runs to the weights' last row; behind it dg and du are zero)
-        g.M = m, g.N = p.D, g.K = p.F, g.a_limit = m, g.b_limit = p.D8, g.splits = 1;
+        g.M = m, g.N = p.D, g.K = p.F, g.a_limit = m, g.b_limit = p.D8;
         g.c = (T*)dx + r * p.D;
-        product<T, ALONG, ACROSS>(stream, g);
+        row_product<T, ALONG, ACROSS>(stream, g, p.parts);
       }
       if (dw_gate || dw_up) {
         ProductArgs<E> g{};

@@ -97,6 +97,7 @@ struct ForwardArgs {
   const T* bd;
   int64_t rows, x_pitch;
   int32_t width, out, chunks;
+  float* parts;      // not null: [gridDim.y, rows, out], chunks dealt over gridDim.y
   int32_t wide;      // x is read 16 bytes at a time
   int32_t wide_out;  // y is written four values at a time
 };
@@ -115,6 +116,13 @@ __device__ __forceinline__ void copy_chunk(char* lds, const char* src) {
 
 #define FR_WAVES 8  // of a workgroup
 
+// Up to four values of a partial row.
+__device__ __forceinline__ void put_part(float* at, f32x4 v, int left) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (r < left) at[r] = v[r];
+}
+
 template <typename T, int DK, int OT, int RT, int ACT>
 __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
   using E = typename Planes<T>::E;
@@ -126,7 +134,11 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
   constexpr int TILE = 16 * RT * FR_WAVES;
   {
     const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
+    // this workgroup's chunks
+    const int first = a.chunks * blockIdx.y / gridDim.y;
+    const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
+    const char* packed = a.packed + (int64_t)first * C::KB * 1024;
+    copy_chunk<C::KB, FR_WAVES>(lds, packed);
     frag_t<E> x[RT][DK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -137,12 +149,12 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
                          x[i][k]);
     }
     f32x4 y[OT][RT] = {};
-    for (int c = 0; c < a.chunks; ++c) {
+    for (int c = 0; c < chunks; ++c) {
       stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (c & 1) * C::KB * 1024;
-      if (c + 1 < a.chunks)
+      if (c + 1 < chunks)
         copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
-                                    a.packed + (int64_t)(c + 1) * C::KB * 1024);
+                                    packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
         for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
@@ -193,6 +205,10 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
       for (int i = 0; i < RT; ++i) {
         const int64_t m = m0 + i * 16;
         if (m >= a.rows || n >= a.out) continue;
+        if (a.parts) {
+          put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.out + n, y[o][i], a.out - n);
+          continue;
+        }
         T* at = a.y + m * a.out + n;
         if (a.wide_out) {
           four_t<T> v;
@@ -221,6 +237,7 @@ struct BackwardArgs {
   const char* packed;
   int64_t rows, x_pitch, dy_pitch;
   int32_t width, out, chunks;
+  float* parts;                    // not null: [gridDim.y, rows, width], as the forward's
   int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
 };
 
@@ -236,7 +253,11 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
   constexpr int TILE = 16 * RT * FR_WAVES;
   {
     const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    copy_chunk<C::KB, FR_WAVES>(lds, a.packed);
+    // this workgroup's chunks
+    const int first = a.chunks * blockIdx.y / gridDim.y;
+    const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
+    const char* packed = a.packed + (int64_t)first * C::KB * 1024;
+    copy_chunk<C::KB, FR_WAVES>(lds, packed);
     frag_t<E> x[RT][DK][P], dy[RT][OK][P];
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
@@ -250,16 +271,16 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
         load_fragment<T>(a.dy + m * a.dy_pitch, k * 32 + c, a.out, m < a.rows, a.wide_dy, dy[i][k]);
     }
     f32x4 dx[DT][RT] = {};
-    for (int c = 0; c < a.chunks; ++c) {
+    for (int c = 0; c < chunks; ++c) {
       if (BUFFERS == 1 && c) {
         stage_barrier();
-        copy_chunk<C::KB, FR_WAVES>(lds, a.packed + (int64_t)c * C::KB * 1024);
+        copy_chunk<C::KB, FR_WAVES>(lds, packed + (int64_t)c * C::KB * 1024);
       }
       stage_barrier();  // the chunk is there, and nobody reads the one before it
       const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
-      if (BUFFERS == 2 && c + 1 < a.chunks)
+      if (BUFFERS == 2 && c + 1 < chunks)
         copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
-                                    a.packed + (int64_t)(c + 1) * C::KB * 1024);
+                                    packed + (int64_t)(c + 1) * C::KB * 1024);
       const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
 #pragma unroll
         for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
@@ -322,6 +343,10 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
       for (int i = 0; i < RT; ++i) {
         const int64_t m = m0 + i * 16;
         if (m >= a.rows || n >= a.width) continue;
+        if (a.parts) {
+          put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.width + n, dx[d][i], a.width - n);
+          continue;
+        }
         T* at = a.dx + m * a.width + n;
         if (a.wide_dx) {
           four_t<T> v;
@@ -659,6 +684,12 @@ static void with_narrow_back(int width, int out, F&& f) {
   return by_out(std::integral_constant<int, 4>());
 }
 
+// Values that the partial sums of rows of `cols` may take, however the chunks are dealt.
+static int64_t partial_values(int64_t rows, int64_t cols, int64_t hidden) {
+  return std::min(rows * std::max<int64_t>(1, tiles(hidden, 32) / 4),
+                  (int64_t)SPLIT_TILES * 16 * FR_WAVES) * cols;
+}
+
 #define ROW_PASS (1 << 20)  // rows whose x and dy are laid out at a time
 
 // The backward's workspace.
@@ -670,7 +701,7 @@ struct RowPlan {
   int waves, columns, runs;  // of a workgroup; workgroups along hidden and along rows
   char* packed;
   E *x, *dy;
-  float *dwgu, *dwd, *sums, *dy_sums;
+  float *parts, *dwgu, *dwd, *sums, *dy_sums;  // parts: of dx
   uint64_t bytes;
   RowPlan(void* ws, int64_t rows, int64_t width, int64_t hidden, int64_t out) {
     constexpr int P = Planes<T>::N;
@@ -685,6 +716,7 @@ struct RowPlan {
     packed = c.take<char>(BackwardChunk<T, DK, OK>::KB * 1024 * tiles(hidden, 32));
     x = c.take<E>(P * pass * round8(width));
     dy = c.take<E>(P * pass * round8(out));
+    parts = c.take<float>(partial_values(rows, width, hidden));
     dwgu = c.take<float>(runs * 2 * hidden * width);
     dwd = c.take<float>(runs * hidden * out);
     sums = c.take<float>(runs * 2 * hidden);
@@ -703,7 +735,8 @@ uint64_t RowKernels<T>::workspace(int64_t rows, int32_t width, int32_t hidden, i
     });
   else
     with_narrow(width, out, [&](auto dk, auto ot) {
-      bytes = ForwardChunk<T, dk.value, ot.value>::KB * 1024 * tiles(hidden, 32);
+      bytes = ForwardChunk<T, dk.value, ot.value>::KB * 1024 * tiles(hidden, 32) +
+              partial_values(rows, out, hidden) * sizeof(float);
     });
   return bytes;
 }
@@ -719,9 +752,15 @@ static bool wide_stores(const void* p, int64_t cols) {
 }
 
 // Wavefronts take 16 RT rows (a constant) where such fill the chip, 16 where they do not.
+// Where even those leave CUs idle, the chunks of the hidden columns are dealt over
+// several workgroups, whose partial sums a further launch joins (1000 rows of 64-4096-64:
+// one workgroup walks 128 chunks in 65 us).
 template <int RT, typename F>
-static void with_rows(int64_t rows, F&& f) {
-  const auto launch = [&](auto rt) { f(rt, (unsigned)tiles(rows, 16 * rt.value * FR_WAVES)); };
+static void with_rows(int64_t rows, int chunks, F&& f) {
+  const auto launch = [&](auto rt) {
+    const int64_t groups = tiles(rows, 16 * rt.value * FR_WAVES);
+    f(rt, dim3((unsigned)groups, rt.value == RT && RT > 1 ? 1 : split_parts(groups, chunks)));
+  };
   if (rows >= 16 * RT * FR_WAVES * 256)
     launch(std::integral_constant<int, RT>());
   else
@@ -738,18 +777,25 @@ void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
                         DK, OT, 0, C::KB};
     hipLaunchKernelGGL((ffn_pack_kernel<T, false>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                        stream, pack);
-    const ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
-                           c.x_pitch, c.width, c.out, chunks,
+    float* parts = (float*)((char*)workspace + C::KB * 1024 * chunks);
+    ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
+                           c.x_pitch, c.width, c.out, chunks, nullptr,
                            wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
     // 32 rows share a fragment's reads, 16 leave room for a second workgroup: 500k rows
     // bfloat16 of 32-128-16: 27 and 30 us, 64-256-64: 77 and 76, 128-256-128: 191 and 145;
     // 300k rows float32 of 59-128-3: 114 and 96
     constexpr int RT = Planes<T>::N == 1 && DK <= 2 ? 2 : 1;
-    with_rows<RT>(c.rows, [&](auto rt, unsigned groups) {
+    with_rows<RT>(c.rows, chunks, [&](auto rt, dim3 grid) {
+      if (grid.y > 1) a.parts = parts;
       with_activation(c.act, [&](auto act) {
-        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value>), dim3(groups),
+        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value>), grid,
                            dim3(64 * FR_WAVES), 0, stream, a);
       });
+      if (grid.y > 1) {
+        Joiner<T> join;
+        join.add(parts, c.rows * c.out, c.out, grid.y, c.rows, c.out, c.y, c.bd);
+        join.launch(stream);
+      }
     });
   });
 }
@@ -766,19 +812,25 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
                           DK, 0, OK, C::KB};
       hipLaunchKernelGGL((ffn_pack_kernel<T, true>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                          stream, pack);
-      const BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
-                              c.dy_pitch, c.width, c.out, chunks,
+      BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
+                              c.dy_pitch, c.width, c.out, chunks, nullptr,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
                               wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
       // 500k rows bfloat16, 32 and 16 rows a wavefront: 128-256-128 244 and 281 us, 64-256-64
       // 115 and 108; float32 with 16 rows and one chunk buffer, where two workgroups share
       // a CU, against 32 and two: 300k of 59-128-3 147 and 175 us
       constexpr int RT = Planes<T>::N == 3 ? 1 : 2;
-      with_rows<RT>(c.rows, [&](auto rt, unsigned groups) {
+      with_rows<RT>(c.rows, chunks, [&](auto rt, dim3 grid) {
+        if (grid.y > 1) a.parts = p.parts;
         with_activation(c.act, [&](auto act) {
-          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), dim3(groups),
+          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), grid,
                              dim3(64 * FR_WAVES), 0, stream, a);
         });
+        if (grid.y > 1) {
+          Joiner<T> join;
+          join.add(p.parts, c.rows * c.width, c.width, grid.y, c.rows, c.width, c.dx);
+          join.launch(stream);
+        }
       });
     }
     if (!(c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd)) return;
