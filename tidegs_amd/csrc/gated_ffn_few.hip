@@ -42,10 +42,11 @@ struct FewArgs {
   T* y;
   int64_t x_pitch;
   int32_t rows, width, hidden, hidden8, out;
+  int32_t each;  // outputs of a workgroup: 16, or 8 where 16 would leave half the CUs idle
   int32_t wide_x, wide_w, wide_d;  // rows of x, of Wg and Wu, of Wd are read 16 bytes at a time
 };
 
-#define FEW_HIDDEN_WAVES 4
+#define FEW_HIDDEN_WAVES 8
 #define FEW_OUT_WAVES 16
 
 template <typename T, int RT, int ACT>
@@ -114,8 +115,8 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
   __shared__ f32x4 s[W][RT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int o0 = blockIdx.x * 16, row = lane & 15, col = (lane >> 4) * 8;
-  const int live = min(16, a.out - o0);
+  const int o0 = blockIdx.x * a.each, row = lane & 15, col = (lane >> 4) * 8;
+  const int live = min(a.each, a.out - o0);
   const int64_t from = (int64_t)o0 * a.hidden;
   const rsrc_t rd = buffer_of(a.wd + from, (uint32_t)(live * a.hidden * sizeof(T)));
   const rsrc_t rh = buffer_of(a.h, (uint32_t)(P * a.rows * a.hidden8 * 2));
@@ -157,7 +158,7 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
   if (m >= a.rows) return;
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    if (o + r < a.out)
+    if (o + r < o0 + live)
       a.y[(int64_t)m * a.out + o + r] = from_f32<T>(v[r] + (a.bd ? to_f32(a.bd[o + r]) : 0.f));
 }
 
@@ -175,6 +176,7 @@ void FewKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
   const FewArgs<T> a{(const T*)c.x, (const T*)c.wg, (const T*)c.wu, (const T*)c.wd,
                      (const T*)c.bg, (const T*)c.bu, (const T*)c.bd, (E*)workspace, (T*)c.y,
                      c.x_pitch, (int32_t)c.rows, c.width, c.hidden, (int32_t)round8(c.hidden), c.out,
+                     c.out < 16 * 128 ? 8 : 16,
                      wide(c.x, c.width, c.x_pitch),
                      wide(c.wg, c.width, c.width) && wide(c.wu, c.width, c.width),
                      wide(c.wd, c.hidden, c.hidden)};
@@ -183,7 +185,7 @@ void FewKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
       hipLaunchKernelGGL((ffn_few_hidden_kernel<T, rt.value, act.value>),
                          dim3((unsigned)tiles(c.hidden, 16)), dim3(64 * FEW_HIDDEN_WAVES), 0, stream, a);
     });
-    hipLaunchKernelGGL((ffn_few_out_kernel<T, rt.value>), dim3((unsigned)tiles(c.out, 16)),
+    hipLaunchKernelGGL((ffn_few_out_kernel<T, rt.value>), dim3((unsigned)tiles(c.out, a.each)),
                        dim3(64 * FEW_OUT_WAVES), 0, stream, a);
   };
   if (c.rows <= 16)

@@ -13,6 +13,7 @@ same bits for the same inputs.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import Optional
 
@@ -55,13 +56,26 @@ def _parameter(t: Optional[Tensor], name: str, shape, x: Tensor, also=()) -> Opt
     """A weight or bias: its shape, type and device checked, dense."""
     if t is None:
         return None
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
     if t.dtype != x.dtype and t.dtype not in also:
         raise TypeError(f"{name} must be {x.dtype} like x, got {t.dtype}")
     if t.device != x.device:
         raise ValueError(f"{name} is on {t.device}, x on {x.device}")
-    return t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(query: str, *sizes: int) -> int:
+    return getattr(N.load(), query)(*sizes)
+
+
+def _any_grad(*tensors: Optional[Tensor]) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _once(backward):
@@ -118,7 +132,7 @@ class _LayerNorm(torch.autograd.Function):
         if need_b:
             db = bias.new_empty(width)
         if need_w or need_b:
-            ws_bytes = N.load().tgs_layer_norm_bwd_workspace_size(rows, width)
+            ws_bytes = _workspace_size("tgs_layer_norm_bwd_workspace_size", rows, width)
             ws = torch.empty(ws_bytes, dtype=torch.uint8, device=x.device)
         N.call("tgs_layer_norm_bwd", rows, width, code, x.data_ptr(), pitch, dy.data_ptr(),
                dy_pitch, N.ptr(weight), w_code, eps, N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(ws),
@@ -144,8 +158,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     bias = _parameter(bias, "bias", shape, x, (torch.float32,))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}: one type is needed")
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (x, weight, bias)):
+    if _any_grad(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm_fwd(x, weight, bias, float(eps))[1]
 
@@ -198,8 +211,7 @@ def dropout(x: Tensor, p: float, seed: int, offset: int = 0,
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
     threshold = int(math.floor(p * 65536 + 0.5))
-    if torch.is_grad_enabled() and (x.requires_grad or
-                                    (residual is not None and residual.requires_grad)):
+    if _any_grad(x, residual):
         return _Dropout.apply(x, residual, threshold, int(seed), int(offset))
     return _dropout(x, residual, threshold, int(seed), int(offset))
 
@@ -215,7 +227,7 @@ def _gated_ffn_fwd(x, w_gate, w_up, w_down, b_gate, b_up, b_down, act):
     (hidden, width), out = w_gate.shape, w_down.shape[0]
     y = x.new_empty((*x.shape[:-1], out))
     code = _DTYPES[x.dtype]
-    nbytes = N.load().tgs_gated_ffn_fwd_workspace_size(rows, width, hidden, out, code)
+    nbytes = _workspace_size("tgs_gated_ffn_fwd_workspace_size", rows, width, hidden, out, code)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
     N.call("tgs_gated_ffn_fwd", rows, width, hidden, out, code, act, x.data_ptr(), pitch,
            w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), N.ptr(b_gate), N.ptr(b_up),
@@ -240,7 +252,8 @@ class _GatedFfn(torch.autograd.Function):
             dy, _, dy_pitch = _rows(dy)
         grads = [t.new_empty(t.shape) if need else None
                  for t, need in zip(saved, ctx.needs_input_grad)]
-        nbytes = N.load().tgs_gated_ffn_bwd_workspace_size(rows, width, hidden, out, code)
+        nbytes = _workspace_size("tgs_gated_ffn_bwd_workspace_size", rows, width, hidden, out,
+                                 code)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
         N.call("tgs_gated_ffn_bwd", rows, width, hidden, out, code, act, x.data_ptr(), pitch,
                w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr(), N.ptr(b_gate), N.ptr(b_up),
@@ -280,6 +293,6 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     b_up = _parameter(b_up, "b_up", (hidden,), x)
     b_down = _parameter(b_down, "b_down", (out,), x)
     args = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+    if _any_grad(*args):
         return _GatedFfn.apply(*args, act)
     return _gated_ffn_fwd(*args, act)[1]
