@@ -41,12 +41,12 @@ struct HiddenArgs {
 template <typename T, bool BACK, typename Z>
 __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<typename Planes<T>::E> a) {
   using E = typename Planes<T>::E;
-  constexpr int P = Planes<T>::N, PAIRS = PlanePairs<T>::N;
+  constexpr int P = Planes<T>::N, BK = stage_k<T>();
   constexpr int TM = Z::TM, TF = Z::TN / 2, F = Z::N / 2;  // hidden columns of the tile
-  using SX = Stage<E, Z::M, ALONG, Z::THREADS>;
-  using SW = Stage<E, Z::N, ALONG, Z::THREADS>;
-  using SD = Stage<E, F, ACROSS, Z::THREADS>;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (SX::BYTES + SW::BYTES)];
+  using SX = Stage<E, Z::M, ALONG, Z::THREADS, BK>;
+  using SW = Stage<E, Z::N, ALONG, Z::THREADS, BK>;
+  using SD = Stage<E, F, ACROSS, Z::THREADS, BK>;
+  __shared__ __attribute__((aligned(1024))) char lds[Loop<E, P>::template bytes<SX, SW>()];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / Z::WN, wn = wave % Z::WN;
@@ -62,13 +62,13 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
     sx.begin(a.x.pitch, m0, a.rows, a.width8);
     sw.begin(a.wg.pitch, f0, a.hidden, a.width8, [](int r) { return (r >> 5) * 16 + (r & 15); });
     const E *x = a.x.p + m0 * a.x.pitch, *wg = a.wg.p + f0 * a.wg.pitch, *wu = a.wu.p + f0 * a.wu.pitch;
-    product_loop<E, false, SX, SW>(gu, lds, Steps(0, a.width8, PAIRS), wm * TM * 16, wn * TF * 32,
-                            [&](const Steps& s, char* to) {
-                              const int64_t w = PlanePairs<T>::b(s.pair) * a.wg.plane;
-                              sx.copy(to, x + PlanePairs<T>::a(s.pair) * a.x.plane, s.k);
-                              sw.copy(to + SX::BYTES, wg + w, wu + w, s.k,
-                                      [](int r) { return (r & 16) != 0; });
-                            });
+    Loop<E, P>::template run<false, SX, SW>(
+        gu, lds, Steps(BK, 0, a.width8, 1), wm * TM * 16, wn * TF * 32,
+        [&](const Steps& s, int q, char* to_x, char* to_w) {
+          sx.copy(to_x, x + q * a.x.plane, s.k);
+          sw.copy(to_w, wg + q * a.wg.plane, wu + q * a.wu.plane, s.k,
+                  [](int r) { return (r & 16) != 0; });
+        });
   }
   f32x4 dh[TM][TF] = {};
   if constexpr (BACK) {
@@ -77,11 +77,12 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
     sy.begin(a.dy.pitch, m0, a.rows, a.out8);
     sd.begin(a.wd.pitch, f0, a.hidden8, a.out);
     const E *dy = a.dy.p + m0 * a.dy.pitch, *wd = a.wd.p + f0;
-    product_loop<E, P == 3, SX, SD>(dh, lds, Steps(0, a.out, PAIRS), wm * TM * 16, wn * TF * 16,
-                            [&](const Steps& s, char* to) {
-                              sy.copy(to, dy + PlanePairs<T>::a(s.pair) * a.dy.plane, s.k);
-                              sd.copy(to + SX::BYTES, wd + PlanePairs<T>::b(s.pair) * a.wd.plane, s.k);
-                            });
+    Loop<E, P>::template run<P == 3, SX, SD>(
+        dh, lds, Steps(BK, 0, a.out, 1), wm * TM * 16, wn * TF * 16,
+        [&](const Steps& s, int q, char* to_y, char* to_w) {
+          sy.copy(to_y, dy + q * a.dy.plane, s.k);
+          sd.copy(to_w, wd + q * a.wd.plane, s.k);
+        });
   }
 
   const int group = lane >> 4;
@@ -194,11 +195,11 @@ struct ProductArgs {
 template <typename T, Along KA, Along KB, typename Z>
 __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<typename Planes<T>::E> g) {
   using E = typename Planes<T>::E;
-  constexpr int PAIRS = PlanePairs<T>::N;
+  constexpr int P = Planes<T>::N, BK = stage_k<T>();
   constexpr int TM = Z::TM, TN = Z::TN;
-  using SA = Stage<E, Z::M, KA, Z::THREADS>;
-  using SB = Stage<E, Z::N, KB, Z::THREADS>;
-  __shared__ __attribute__((aligned(1024))) char lds[2 * (SA::BYTES + SB::BYTES)];
+  using SA = Stage<E, Z::M, KA, Z::THREADS, BK>;
+  using SB = Stage<E, Z::N, KB, Z::THREADS, BK>;
+  __shared__ __attribute__((aligned(1024))) char lds[Loop<E, P>::template bytes<SA, SB>()];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int wm = wave / Z::WN, wn = wave % Z::WN;
@@ -209,9 +210,9 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<
   tile_of(blockIdx.x % (tiles_m * tiles_n), tiles_m, tiles_n, tm, tn);
   const int64_t m0 = (int64_t)tm * Z::M;
   const int n0 = tn * Z::N;
-  const int64_t all = (g.K + MX_BK - 1) / MX_BK;
-  const int64_t from = all * split / g.splits * MX_BK;
-  const int64_t to = min(all * (split + 1) / g.splits * MX_BK, g.K);
+  const int64_t all = (g.K + BK - 1) / BK;
+  const int64_t from = all * split / g.splits * BK;
+  const int64_t to = min(all * (split + 1) / g.splits * BK, g.K);
 
   SA sa;
   SB sb;
@@ -220,16 +221,12 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<
   const int64_t at_a = KA == ALONG ? m0 * g.a.pitch : m0;
   const int64_t at_b = KB == ALONG ? n0 * g.b.pitch : n0;
   f32x4 acc[TM][TN] = {};
-  product_loop<E, false, SA, SB>(acc, lds, Steps(from, to, PAIRS * (g.a2.p ? 2 : 1)), wm * TM * 16,
-                          wn * TN * 16,
-                          [&](const Steps& s, char* to_lds) {
-                            const bool second = s.pair >= PAIRS;
-                            const int pair = second ? s.pair - PAIRS : s.pair;
-                            sa.copy(to_lds, (second ? g.a2.p : g.a.p) + at_a +
-                                                PlanePairs<T>::a(pair) * g.a.plane, s.k);
-                            sb.copy(to_lds + SA::BYTES, (second ? g.b2.p : g.b.p) + at_b +
-                                                            PlanePairs<T>::b(pair) * g.b.plane, s.k);
-                          });
+  Loop<E, P>::template run<false, SA, SB>(
+      acc, lds, Steps(BK, from, to, g.a2.p ? 2 : 1), wm * TM * 16, wn * TN * 16,
+      [&](const Steps& s, int q, char* to_a, char* to_b) {
+        sa.copy(to_a, (s.pair ? g.a2.p : g.a.p) + at_a + q * g.a.plane, s.k);
+        sb.copy(to_b, (s.pair ? g.b2.p : g.b.p) + at_b + q * g.b.plane, s.k);
+      });
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int64_t m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
@@ -307,11 +304,15 @@ static int64_t pass_rows(int64_t rows, int64_t hidden) {
   return std::min(rows, most);
 }
 
-static int splits_of(int64_t tiles_, int64_t k) { return split_parts(tiles_, k / MX_BK); }
+template <typename T>
+static int splits_of(int64_t tiles_, int64_t k) {
+  return split_parts(tiles_, k / stage_k<T>());
+}
 
 // Values that the partial sums of a rows x N product over k may take, whatever its splits.
+template <typename T>
 static int64_t partial_values(int64_t rows, int64_t N, int64_t k) {
-  return std::min(rows * N * std::max<int64_t>(1, k / MX_BK / 4), (int64_t)SPLIT_TILES * 128 * 128);
+  return std::min(rows * N * std::max<int64_t>(1, k / stage_k<T>() / 4), (int64_t)SPLIT_TILES * 128 * 128);
 }
 
 // Whether there are enough tiles Z of an M x N product for the CUs.
@@ -343,14 +344,14 @@ struct Plan {
     wu = c.take<E>(P * F * D8);
     wd = c.take<E>(P * O * F8);
     h = c.take<E>(P * pass * F8);
-    parts = c.take<float>(back ? partial_values(pass, D, F) : partial_values(pass, O, F8));
+    parts = c.take<float>(back ? partial_values<T>(pass, D, F) : partial_values<T>(pass, O, F8));
     if (back) {
       dy = c.take<E>(P * pass * O8);
       dgu = c.take<E>(2 * P * pass * F8);
       gu_sums = c.take<float>(tiles(pass, TileSmall::M) * 2 * F8);
       dy_sums = c.take<float>(COLUMN_RUNS * O);
-      split_gu = splits_of(tiles(2 * F8, 128) * tiles(D, 128), pass);
-      split_d = splits_of(tiles(O, 128) * tiles(F, 128), pass);
+      split_gu = splits_of<T>(tiles(2 * F8, 128) * tiles(D, 128), pass);
+      split_d = splits_of<T>(tiles(O, 128) * tiles(F, 128), pass);
       // (one sum over all rows is rounded where it is taken)
       dwgu = split_gu > 1 || pass < rows ? c.take<float>(split_gu * 2 * F8 * D) : nullptr;
       dwd = split_d > 1 || pass < rows ? c.take<float>(split_d * O * F) : nullptr;
@@ -368,7 +369,7 @@ static void product(hipStream_t s, ProductArgs<typename Planes<T>::E> g) {
                        dim3((unsigned)(tiles(g.M, Z::M) * tiles(g.N, Z::N) * g.splits)),
                        dim3(Z::THREADS), 0, s, g);
   };
-  if constexpr (KA == ALONG && KB == ALONG)
+  if constexpr (Planes<T>::N == 1 && KA == ALONG && KB == ALONG)
     if (fills<TileLarge>(g.M, g.N, g.splits)) return launch(TileLarge());
   launch(TileSmall());
 }
@@ -376,7 +377,7 @@ static void product(hipStream_t s, ProductArgs<typename Planes<T>::E> g) {
 // A product of rows, its sum over k split where its tiles are few.
 template <typename T, Along KA, Along KB>
 static void row_product(hipStream_t s, ProductArgs<typename Planes<T>::E> g, float* parts) {
-  g.splits = splits_of(tiles(g.M, TileSmall::M) * tiles(g.N, TileSmall::N), g.K);
+  g.splits = splits_of<T>(tiles(g.M, TileSmall::M) * tiles(g.N, TileSmall::N), g.K);
   if (g.splits == 1) return product<T, KA, KB>(s, g);
   g.partial = parts;
   product<T, KA, KB>(s, g);
@@ -393,7 +394,7 @@ static void hidden_products(hipStream_t s, const HiddenArgs<typename Planes<T>::
                        dim3((unsigned)(tiles(a.rows, Z::M) * tiles(a.hidden8, Z::N / 2))),
                        dim3(Z::THREADS), 0, s, a);
   };
-  if constexpr (!BACK)
+  if constexpr (Planes<T>::N == 1 && !BACK)
     if (fills<TileLarge>(a.rows, 2 * a.hidden8)) return launch(TileLarge());
   launch(TileSmall());
 }

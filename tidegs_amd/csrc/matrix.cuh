@@ -116,23 +116,14 @@ __device__ __forceinline__ void set_half(frag_t<E> (&f)[P], int half, const four
     for (int r = 0; r < 4; ++r) f[q][half * 4 + r] = v[q][r];
 }
 
-// The pairs of planes that a product multiplies, the smallest first.
-template <typename T>
-struct PlanePairs {
-  static constexpr int N = 1;
-  __device__ static __forceinline__ int a(int) { return 0; }
-  __device__ static __forceinline__ int b(int) { return 0; }
-};
-template <>
-struct PlanePairs<float> {
-  static constexpr int N = 6;
-  __device__ static __forceinline__ int a(int i) { return (0x201100 >> (4 * (5 - i))) & 3; }
-  __device__ static __forceinline__ int b(int i) { return (0x021010 >> (4 * (5 - i))) & 3; }
-};
-
 enum Along { ALONG, ACROSS };
 
-#define MX_BK 64  // k of one staged step
+// k of one staged step: of one plane, or of all three, which are multiplied in one step (each
+// plane staged once for the six products that it takes part in).
+template <typename T>
+constexpr int stage_k() {
+  return Planes<T>::N == 1 ? 64 : 32;
+}
 
 // A matrix operand: planes `plane` values apart, rows `pitch` values apart.
 template <typename E>
@@ -152,21 +143,23 @@ __device__ __forceinline__ rsrc_t buffer_of(const void* p, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), 0, (int)bytes, 0x00027000);
 }
 
-// ROWS of an operand by MX_BK of its k, staged by the THREADS of a workgroup.  Where each
+// ROWS of an operand by BK of its k, staged by the THREADS of a workgroup.  Where each
 // lane reads is worked out once; a step moves the buffer's base.
-template <typename E, int ROWS, Along K_, int THREADS>
+template <typename E, int ROWS, Along K_, int THREADS, int BK>
 struct Stage {
-  static constexpr int BYTES = ROWS * MX_BK * 2;
+  static constexpr int BYTES = ROWS * BK * 2;
   static constexpr int WAVES = THREADS / 64;
   static constexpr int PASSES = BYTES / (1024 * WAVES);
   static_assert(PASSES * 1024 * WAVES == BYTES, "whole passes");
-  static constexpr int CHUNKS = (K_ == ALONG ? MX_BK : ROWS) / 8;  // of an LDS row
+  static constexpr int CHUNKS = (K_ == ALONG ? BK : ROWS) / 8;  // of an LDS row
   static constexpr int PER = 64 / CHUNKS;                          // LDS rows of one KB
   static constexpr int READS = K_ == ALONG ? 1 : 2;                // LDS reads of a fragment
 
-  // Which unit of 32 bytes an ACROSS row's units are exchanged with: rows that one
-  // transposing read touches together (bits 0, 1 and 3) meet different banks.
+  // What a row's chunks (ALONG) or units of 32 bytes (ACROSS) are exchanged with, so that the
+  // rows that one read touches together meet different banks: 16 in a row, or those that
+  // differ in bits 0, 1 and 3.
   __device__ static __forceinline__ int turn(int row) {
+    if constexpr (K_ == ALONG) return BK == 64 ? row & 7 : (row >> 2) & 3;
     if constexpr (ROWS >= 128) return (row & 3) | ((row >> 1) & 4);
     return ((row >> 1) & 1) | ((row >> 2) & 2);
   }
@@ -189,7 +182,7 @@ struct Stage {
     for (int j = 0; j < PASSES; ++j) {
       const int row = (j * WAVES + wave) * PER + lane / CHUNKS, pos = lane % CHUNKS;
       if constexpr (K_ == ALONG) {
-        chunk = pos ^ (row & 7);
+        chunk = pos ^ turn(row);
         const int r = of(row);
         off[j] = r < left ? (uint32_t)(r * pitch + chunk * 8) * 2 : MX_OUTSIDE;
       } else {
@@ -203,7 +196,7 @@ struct Stage {
     begin(pitch_, row0, rows, K_end, [](int r) { return r; });
   }
 
-  // Starts the copies of k0 .. k0 + MX_BK - 1; `p` is the tile's first row's or column's
+  // Starts the copies of k0 .. k0 + BK - 1; `p` is the tile's first row's or column's
   // place in the plane, p2 that of the rows that `other` says come from another matrix.
   __device__ __forceinline__ void copy(char* lds, const E* p, int64_t k0) const {
     copy(lds, p, p, k0, [](int) { return false; });
@@ -212,7 +205,7 @@ struct Stage {
   __device__ __forceinline__ void copy(char* lds, const E* p, const E* p2, int64_t k0,
                                        Other&& other) const {
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int left = (int)min((int64_t)MX_BK, K - k0);
+    const int left = (int)min((int64_t)BK, K - k0);
     const int64_t at = K_ == ALONG ? k0 : k0 * pitch;
     // ALONG: chunks that start before K are there whole (operands end on chunks)
     const uint32_t bytes = K_ == ALONG ? last + ((left + 7) & ~7) * 2 : (uint32_t)(left * pitch) * 2;
@@ -231,8 +224,8 @@ struct Stage {
   __device__ static __forceinline__ frag_t<E> fragment(const char* lds, int row, int kk) {
     const int lane = threadIdx.x & 63;
     if constexpr (K_ == ALONG) {
-      const int r = row + (lane & 15), c = (kk * 4 + (lane >> 4)) ^ (lane & 7);
-      return *(const frag_t<E>*)(lds + r * 128 + c * 16);
+      const int r = row + (lane & 15), c = (kk * 4 + (lane >> 4)) ^ turn(lane & 15);
+      return *(const frag_t<E>*)(lds + r * BK * 2 + c * 16);
     } else {
       const int k = kk * 32 + (lane >> 4) * 8 + ((lane >> 2) & 3);
       const int unit = (row >> 4) ^ turn(k);
@@ -264,16 +257,16 @@ __device__ __forceinline__ void tile_of(uint32_t bid, uint32_t tiles_m, uint32_t
   tn = in / high;
 }
 
-// The steps of a product's loop: k in MX_BK from `from` to `to`, for each of `pairs` pairs of
+// The steps of a product's loop: k in BK from `from` to `to`, for each of `pairs` pairs of
 // operands in turn.
 struct Steps {
   int64_t k, from, to;
-  int pair, pairs;
-  __device__ __forceinline__ Steps(int64_t from_, int64_t to_, int pairs_)
-      : k(from_), from(from_), to(to_), pair(from_ < to_ ? 0 : pairs_), pairs(pairs_) {}
+  int pair, pairs, BK;
+  __device__ __forceinline__ Steps(int BK_, int64_t from_, int64_t to_, int pairs_)
+      : k(from_), from(from_), to(to_), pair(from_ < to_ ? 0 : pairs_), pairs(pairs_), BK(BK_) {}
   __device__ __forceinline__ bool more() const { return pair < pairs; }
   __device__ __forceinline__ void next() {
-    k += MX_BK;
+    k += BK;
     if (k >= to) k = from, ++pair;
   }
 };
@@ -294,68 +287,123 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// The main loop: copy(step, buffer) starts the copies of a step into one of two buffers.
-// acc[i][j] is the transposed 16 x 16 tile of rows a_row + 16 i of A and b_row + 16 j of B:
-// lane l holds row l % 16 of A and rows (l / 16) * 4 + r of B.
-//
-// A step is two halves of k = 32, and the fragments of the half to come are read while a
-// half is multiplied, so the matrix cores have operands in registers across the barrier in
-// the middle of the step: behind it the step's buffer is read out and takes the copies of
-// the step after next, and the next step's copies have landed.
+// The main loop: copy(step, plane, a, b) starts the copies of a step's planes of the operands
+// to a and b in LDS.  acc[i][j] is the transposed 16 x 16 tile of rows a_row + 16 i of A and
+// b_row + 16 j of B: lane l holds row l % 16 of A and rows (l / 16) * 4 + r of B.
 // FLIP: the products of every other of A's tiles come out negated.
-template <typename E, bool FLIP, typename SA, typename SB, int TM, int TN, typename Copy>
-__device__ __forceinline__ void product_loop(f32x4 (&acc)[TM][TN], char* lds, Steps ahead, int a_row,
+//
+// One plane: two buffers.  A step is two halves of k = 32, and the fragments of the half to
+// come are read while a half is multiplied, so the matrix cores have operands in registers
+// across the barrier in the middle of the step: behind it the step's buffer is read out and
+// takes the copies of the step after next, and the next step's copies have landed.
+//
+// Three planes: one buffer and two workgroups a CU, one copying while the other multiplies;
+// a step's 96 products a wavefront outlast its copies.  Pair after pair of planes, each in
+// steps of its own, staged every plane twice as often and took 219 us for the forward
+// of 1000 rows 1024-4096-1024.
+template <typename E, int P>
+struct Loop;
+
+template <typename E>
+struct Loop<E, 1> {
+  template <typename SA, typename SB>
+  static constexpr int bytes() {
+    return 2 * (SA::BYTES + SB::BYTES);
+  }
+  template <bool FLIP, typename SA, typename SB, int TM, int TN, typename Copy>
+  __device__ static __forceinline__ void run(f32x4 (&acc)[TM][TN], char* lds, Steps ahead, int a_row,
                                              int b_row, Copy&& copy) {
-  constexpr int BYTES = SA::BYTES + SB::BYTES;
-  if (!ahead.more()) return;
-  frag_t<E> a[2][TM], b[2][TN];
-  const auto read = [&](const char* from, int half) {
+    constexpr int BYTES = SA::BYTES + SB::BYTES;
+    static_assert(!FLIP, "of three planes' loop");
+    if (!ahead.more()) return;
+    frag_t<E> a[2][TM], b[2][TN];
+    const auto read = [&](const char* from, int half) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
-      a[half][i] = SA::fragment(from, a_row + i * 16, half);
-      if (FLIP && i % 2) a[half][i] = negated<E>(a[half][i]);
+      for (int i = 0; i < TM; ++i) a[half][i] = SA::fragment(from, a_row + i * 16, half);
+#pragma unroll
+      for (int j = 0; j < TN; ++j) b[half][j] = SB::fragment(from + SA::BYTES, b_row + j * 16, half);
+    };
+    const auto multiply = [&](int half) {
+#pragma unroll
+      for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[half][j], a[half][i], acc[i][j]);
+    };
+    // the reads dealt evenly among the products
+    const auto mix = [] {
+      constexpr int READS = TM * SA::READS + TN * SB::READS, PRODUCTS = TM * TN;
+      constexpr int GROUPS = READS < PRODUCTS ? READS : PRODUCTS;
+#pragma unroll
+      for (int i = 0; i < GROUPS; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / GROUPS, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, (READS + GROUPS - 1) / GROUPS, 0);
+      }
+    };
+    char *cur = lds, *other = lds + BYTES;
+    copy(ahead, 0, cur, cur + SA::BYTES);
+    ahead.next();
+    stage_barrier();
+    if (ahead.more()) copy(ahead, 0, other, other + SA::BYTES);
+    read(cur, 0);
+    while (ahead.more()) {
+      read(cur, 1);
+      multiply(0);
+      mix();
+      stage_barrier();
+      ahead.next();
+      if (ahead.more()) copy(ahead, 0, cur, cur + SA::BYTES);
+      char* t = cur;
+      cur = other;
+      other = t;
+      read(cur, 0);
+      multiply(1);
+      mix();
     }
-#pragma unroll
-    for (int j = 0; j < TN; ++j) b[half][j] = SB::fragment(from + SA::BYTES, b_row + j * 16, half);
-  };
-  const auto multiply = [&](int half) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[half][j], a[half][i], acc[i][j]);
-  };
-  // the reads dealt evenly among the products
-  const auto mix = [] {
-    constexpr int READS = TM * SA::READS + TN * SB::READS, PRODUCTS = TM * TN;
-    constexpr int GROUPS = READS < PRODUCTS ? READS : PRODUCTS;
-#pragma unroll
-    for (int i = 0; i < GROUPS; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, PRODUCTS / GROUPS, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, (READS + GROUPS - 1) / GROUPS, 0);
-    }
-  };
-  char *cur = lds, *other = lds + BYTES;
-  copy(ahead, cur);
-  ahead.next();
-  stage_barrier();
-  if (ahead.more()) copy(ahead, other);
-  read(cur, 0);
-  while (ahead.more()) {
     read(cur, 1);
     multiply(0);
-    mix();
-    stage_barrier();
-    ahead.next();
-    if (ahead.more()) copy(ahead, cur);
-    char* t = cur;
-    cur = other;
-    other = t;
-    read(cur, 0);
     multiply(1);
-    mix();
+    stage_barrier();
   }
-  read(cur, 1);
-  multiply(0);
-  multiply(1);
-  stage_barrier();
-}
+};
+
+template <typename E>
+struct Loop<E, 3> {
+  template <typename SA, typename SB>
+  static constexpr int bytes() {
+    return 3 * (SA::BYTES + SB::BYTES);
+  }
+  template <bool FLIP, typename SA, typename SB, int TM, int TN, typename Copy>
+  __device__ static __forceinline__ void run(f32x4 (&acc)[TM][TN], char* lds, Steps s, int a_row,
+                                             int b_row, Copy&& copy) {
+    char* to_b = lds + 3 * SA::BYTES;
+    for (; s.more(); s.next()) {
+#pragma unroll
+      for (int q = 0; q < 3; ++q) copy(s, q, lds + q * SA::BYTES, to_b + q * SB::BYTES);
+      stage_barrier();
+      frag_t<E> a[3][TM], b[3][TN];
+#pragma unroll
+      for (int q = 2; q >= 0; --q) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+          a[q][i] = SA::fragment(lds + q * SA::BYTES, a_row + i * 16, 0);
+          if (FLIP && i % 2) a[q][i] = negated<E>(a[q][i]);
+        }
+#pragma unroll
+        for (int j = 0; j < TN; ++j) b[q][j] = SB::fragment(to_b + q * SB::BYTES, b_row + j * 16, 0);
+      }
+      const auto multiply = [&](int pa, int pb) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+          for (int j = 0; j < TN; ++j) acc[i][j] = mfma32(b[pb][j], a[pa][i], acc[i][j]);
+      };
+      multiply(2, 0);  // the smallest first
+      multiply(0, 2);
+      multiply(1, 1);
+      multiply(1, 0);
+      multiply(0, 1);
+      multiply(0, 0);
+      stage_barrier();
+    }
+  }
+};
