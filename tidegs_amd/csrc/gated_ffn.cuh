@@ -162,7 +162,7 @@ struct JoinJobs {
 
 // A job's workgroup takes 256 / groups values, each summed by `groups` threads over parts g,
 // g + groups, ... and then over the threads: one thread per value took 62 us for 256 parts of
-// 49k values, a load after another, 32 take 12.
+// 49k values, a load after another; eight take 10.
 template <typename T>
 __global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
   __shared__ float s[256];
@@ -260,7 +260,8 @@ struct Joiner {
   void add(const float* partial, int64_t part, int64_t pitch, int64_t parts, int64_t rows,
            int64_t cols, void* to, const void* bias = nullptr) {
     if (!to) return;
-    const int groups = parts > 4 ? 8 : 1;
+    // (many values in few parts keep the chip busy with a thread each)
+    const int groups = parts > (rows * cols < 65536 ? 4 : 32) ? 8 : 1;
     blocks += (uint32_t)tiles(rows * cols, 256 / groups);
     jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, groups, rows, to,
                             bias, blocks};

@@ -272,6 +272,7 @@ __global__ void __launch_bounds__(256) ffn_column_sum_kernel(int64_t rows, int32
   const int64_t from = rows * blockIdx.y / gridDim.y, to = rows * (blockIdx.y + 1) / gridDim.y;
   float acc = 0.f;
   if (c < cols)
+#pragma unroll 8
     for (int64_t r = from + k; r < to; r += 4) acc += to_f32(p[r * pitch + c]);
   s[k][threadIdx.x & 63] = acc;
   __syncthreads();
@@ -322,7 +323,7 @@ static bool fills(int64_t M, int64_t N, int64_t times = 1) {
   return tiles(M, Z::M) * tiles(N, Z::N) * times >= FILLING_TILES;
 }
 
-#define COLUMN_RUNS 64
+#define COLUMN_RUNS 128
 
 // Everything a call keeps in its workspace.
 template <typename T>
