@@ -137,6 +137,8 @@ def test_entry_points_check_their_arguments():
     if lib.tgs_gated_ffn_fwd_workspace_size(4, 8, 16, 3, 0):
         refused(ffn(ws=0), "workspace too small")
     assert ffn(rows=0) == 0
+    refused(lib.tgs_gated_ffn_fwd(4, 8, 16, 3, 0, 0, fake, 8, fake, fake, fake, None, None, None,
+                                  fake, ctypes.c_void_p(0x1008), 1 << 30, None), "16 bytes")
 
 
 def test_workspace_sizes_never_shrink_with_the_rows():

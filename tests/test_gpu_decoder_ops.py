@@ -384,6 +384,21 @@ def test_gated_ffn(gpu, rows, D, F, O, dtype):
     _check_ffn(args, dy, act, f"{rows} x {D}-{F}-{O}")
 
 
+# sums over k split over workgroups (few tiles), 256 x 256 tiles, wavefronts of 32 rows, rows
+# that take several passes (hidden values and copies of unaligned rows in parts)
+FFN_LARGE = [(70, 264, 4096, 200), (300, 64, 4096, 64), (140, 128, 2048, 100), (33, 1000, 520, 1000),
+             (4200, 136, 2048, 136), (15000, 136, 64, 1024), (70001, 64, 40, 48),
+             (16500, 136, 4096, 136), ((1 << 20) + 300, 20, 32, 5)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D,F,O", FFN_LARGE)
+def test_gated_ffn_large(gpu, rows, D, F, O, dtype):
+    announce(f"gated ffn {rows} x {D}-{F}-{O} {dtype}")
+    args, dy = _ffn_inputs(rows, D, F, O, dtype, True, rows + D + F + O)
+    _check_ffn(args, dy, "silu", f"{rows} x {D}-{F}-{O}")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("pitch", [1, 8, 5])

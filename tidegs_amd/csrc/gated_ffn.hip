@@ -298,11 +298,11 @@ static int check_sizes(const char* name, uint64_t rows, uint32_t width, uint32_t
   return TGS_OK;
 }
 
-// Rows of one pass: what keeps the hidden tensors of a pass (six bytes a value and plane)
-// within 64M values; the next rows reuse them.
-static int64_t pass_rows(int64_t rows, int64_t hidden) {
-  const int64_t most = std::max<int64_t>((64 << 20) / round8(hidden) / 256 * 256, 256);
-  return std::min(rows, most);
+// Rows of one pass: what keeps the hidden tensors of a pass (six bytes a value and plane) and
+// the copies of its x and dy within 64M values each; the next rows reuse them.
+static int64_t pass_rows(int64_t rows, int64_t width, int64_t hidden, int64_t out) {
+  const int64_t cols = round8(std::max(hidden, std::max(width, out)));
+  return std::min(rows, std::max<int64_t>((64 << 20) / cols / 256 * 256, 256));
 }
 
 template <typename T>
@@ -339,7 +339,7 @@ struct Plan {
   Plan(void* ws, int64_t rows_, int64_t D_, int64_t F_, int64_t O_, bool back)
       : rows(rows_), D(D_), F(F_), O(O_), D8(round8(D_)), F8(round8(F_)), O8(round8(O_)) {
     Carver c{(char*)ws};
-    pass = pass_rows(rows, F);
+    pass = pass_rows(rows, D, F, O);
     x = c.take<E>(P * pass * D8);
     wg = c.take<E>(P * F * D8);
     wu = c.take<E>(P * F * D8);
@@ -441,6 +441,8 @@ extern "C" int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_fwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
+    TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0,
+                  "tgs_gated_ffn_fwd: the workspace starts on 16 bytes");
     FfnCall c{};
     c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
     c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
@@ -497,6 +499,8 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       tgs_set_error("tgs_gated_ffn_bwd: workspace too small");
       return TGS_ERR_WORKSPACE;
     }
+    TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0,
+                  "tgs_gated_ffn_bwd: the workspace starts on 16 bytes");
     if (rows && RowKernels<T>::takes(width, out)) {
       FfnCall c{};
       c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
