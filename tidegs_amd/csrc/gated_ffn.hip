@@ -9,17 +9,23 @@
 #include "gated_ffn.cuh"
 
 // ---------------------------------------------------------------------------
-// The hidden products.  The B rows of a workgroup's tile
-// are runs of 16 of Wg and of Wu in turn, so that a lane's accumulators hold g and u
-// of the same row and columns and the gate is taken in registers.  The backward adds
-// dh = dy Wd for the same tile before its gate.
+// The hidden products.  The B rows of a workgroup's tile are runs of 16 of Wg and of Wu in
+// turn, so that a lane's accumulators hold g and u of the same row and columns and the gate
+// is taken in registers.  The backward adds dh = dy Wd for the same tile before its gate.
+//
+// Bound by the matrix cores and what feeds them: at 8192 rows of 1024-4096-1024 bfloat16 the
+// forward's hidden products take 139 us (990 TFLOP/s), y 81 (850), the backward's three
+// hidden products 300 (690, with 200 MB of h, dg and du written), dX and dW 160 each (860);
+// a library product of 8192^3 reaches 1307.  g and u are computed again in the backward
+// rather than kept: kept in 32 bits they are 268 MB to write and to read, about 120 us,
+// for the 137 GFLOP (140 us) that they save.
 // ---------------------------------------------------------------------------
 
 // Tiles: 128 x 128 in four wavefronts, two workgroups a CU; 256 x 256 in eight, one a CU, for
 // products of operands that both run along k, where there are tiles enough for the CUs.
 // A larger tile stages fewer bytes per product and its wavefronts' 128 x 64 read fewer
-// fragments: the hidden products of 8192 x 1024 x 2 4096 take 131 us (1050 TFLOP/s) in the
-// large tiles, 161 in the small. With an operand across k the turning reads, twice as
+// fragments: the hidden products of 8192 x 1024 x 2 4096 take 139 us in the large tiles, 161
+// in the small. With an operand across k the turning reads, twice as
 // many, leave the large tile's lockstep behind two small ones (dW of that block 175 us
 // against 154), and so does the backward's third accumulator (343 against 305).
 typedef Tile<2, 2, 4, 4> TileSmall;
