@@ -716,9 +716,10 @@ struct RowPlan {
     const int64_t slices = tiles(hidden, 16 * FT);
     waves = (int)std::min<int64_t>(slices, weight_waves<T, DK, OK>());
     columns = (int)tiles(slices, waves);
-    // workgroups that the chip holds at once
+    // workgroups that the chip holds at once, whole ones a CU (500k rows of 64-224-64: 7
+    // wavefronts each, 256 workgroups; 292 of them left a second round to 36)
     runs = (int)std::max<int64_t>(
-        1, std::min<int64_t>(tiles(pass, weight_rows<T>()), 256 * weight_waves<T, DK, OK>() / (waves * columns)));
+        1, std::min<int64_t>(tiles(pass, weight_rows<T>()), 256 * (weight_waves<T, DK, OK>() / waves) / columns));
     Carver c{(char*)ws};
     packed = c.take<char>(BackwardChunk<T, DK, OK>::KB * 1024 * tiles(hidden, 32));
     x = c.take<E>(P * pass * round8(width));
