@@ -399,6 +399,21 @@ def test_gated_ffn_large(gpu, rows, D, F, O, dtype):
     _check_ffn(args, dy, "silu", f"{rows} x {D}-{F}-{O}")
 
 
+# narrow rows whose hidden columns one workgroup holds (65 to 256 of them), every width of its
+# exchange, hidden columns that end inside a wavefront's, rows inside a tile
+FFN_ALONGSIDE = [(35, 64, 65, 64), (64, 64, 128, 33), (1, 32, 96, 3), (1000, 59, 129, 3), (97, 64, 160, 64),
+                 (4099, 64, 256, 64), (333, 20, 250, 48), (20001, 32, 256, 32), (66, 33, 224, 64)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("rows,D,F,O", FFN_ALONGSIDE)
+def test_gated_ffn_one_workgroup_of_hidden_columns(gpu, rows, D, F, O, act, dtype):
+    announce(f"gated ffn {rows} x {D}-{F}-{O} {act} {dtype}")
+    args, dy = _ffn_inputs(rows, D, F, O, dtype, F % 2 == 0, rows + D + F + O)
+    _check_ffn(args, dy, act, f"{rows} x {D}-{F}-{O}")
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
 @pytest.mark.parametrize("pitch", [1, 8, 5])

@@ -130,6 +130,21 @@ __device__ __forceinline__ void put_part(float* at, f32x4 v, int left) {
     if (r < left) at[r] = v[r];
 }
 
+// Up to four values of a result's row, in one store where its rows allow that.
+template <typename T>
+__device__ __forceinline__ void put_four(T* at, f32x4 v, int left, bool whole) {
+  if (whole) {
+    four_t<T> t;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) t[r] = from_f32<T>(v[r]);
+    *(four_t<T>*)at = t;
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (r < left) at[r] = from_f32<T>(v[r]);
+  }
+}
+
 template <typename T, int DK, int OT, int RT, int ACT>
 __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs<T> a) {
   using E = typename Planes<T>::E;
@@ -354,17 +369,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
           put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.width + n, dx[d][i], a.width - n);
           continue;
         }
-        T* at = a.dx + m * a.width + n;
-        if (a.wide_dx) {
-          four_t<T> v;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = from_f32<T>(dx[d][i][r]);
-          *(four_t<T>*)at = v;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.width) at[r] = from_f32<T>(dx[d][i][r]);
-        }
+        put_four(a.dx + m * a.width + n, dx[d][i], a.width - n, a.wide_dx);
       }
     }
   }
@@ -389,6 +394,9 @@ struct WeightArgs {
   float *dwgu, *dwd, *sums, *dy_sums;  // [gridDim.x, ...]; dy_sums nullable
   int64_t rows;
   int32_t width, hidden, out, add;
+  T* dx;  // where dx is taken along; its packed weights, their chunks, four values at a time
+  const char* packed;
+  int32_t chunks, wide_dx;
 };
 
 // Rows of a tile in LDS, of STEPS k steps of 32 (64 bytes each), and what its 16-byte
@@ -458,14 +466,28 @@ constexpr int weight_rows() {  // of a staged tile
   return Planes<T>::N == 1 ? 64 : 32;
 }
 
-template <typename T, int DK, int OK, int FT, int ACT>
-__global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_kernel(WeightArgs<T> a) {
+// DX: the wavefronts of a workgroup that takes dx along (0: it does not).  It holds every
+// hidden column, so dg and du of 32 rows, exchanged through LDS, are all that dx of these
+// rows wants: tiles of 16 rows and columns, dealt over the wavefronts.  Wg' and Wu' stay in
+// LDS.  Of 1M rows of 64-256-64 bfloat16 that saves the hidden products, the gate and the
+// reads of x and dy that a kernel of its own for dx repeats.
+template <typename T, int DK, int OK, int FT, int ACT, int DX>
+__global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), (DX ? 2 : 1))
+    ffn_rows_dw_kernel(WeightArgs<T> a) {
   using E = typename Planes<T>::E;
   constexpr int P = Planes<T>::N, DT = 2 * DK, OT = 2 * OK, ROWS = weight_rows<T>();
   using X = RowTile<DK>;
   using Y = RowTile<OK>;
   constexpr int XB = ROWS * X::PITCH, YB = ROWS * Y::PITCH, BYTES = P * (XB + YB);
-  __shared__ __attribute__((aligned(1024))) char lds[2 * BYTES];
+  using C = BackwardChunk<T, DK, OK>;
+  // dg, then du, by hidden columns: of a tile's rows, or of half of them where that lets two
+  // workgroups share a CU
+  constexpr int EXCHANGED = DX == 8 ? 64 : 32;
+  using G = RowTile<EXCHANGED / 32>;
+  constexpr int COLUMNS = DX * 16 * FT, WB = 2 * DT * 1024;  // WB: Wg' and Wu' of 32 columns
+  static_assert(!DX || (P == 1 && FT == 2), "a wavefront's hidden columns are a chunk");
+  __shared__ __attribute__((aligned(1024))) char
+      lds[2 * BYTES + DX * WB + (DX ? 2 * COLUMNS * G::PITCH : 0)];
   const int lane = threadIdx.x & 63, waves = blockDim.x >> 6;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int f0 = (blockIdx.y * waves + wave) * 16 * FT;
@@ -511,6 +533,37 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
     }
   };
   if (blockIdx.x < tiles) stage(blockIdx.x, lds);
+  char* const wx = lds + 2 * BYTES;
+  char* const exchange = wx + DX * WB;
+  if (DX && blockIdx.x < tiles)
+    for (int c = 0; c < a.chunks; ++c)
+      copy_chunk<WB / 1024, DX ? DX : 1>(wx + c * WB, a.packed + ((int64_t)c * C::KB + 4 * DK + 2 * OK) * 1024);
+  if constexpr (DX > 0)  // (behind the last chunk dg and du are zero: so are the weights)
+    for (int i = a.chunks * WB / 16 + threadIdx.x; i < DX * WB / 16; i += 64 * DX)
+      ((i32x4*)wx)[i] = i32x4{};
+  // dx of the exchanged rows, from m0 on: a wavefront takes 16 of them by 32 columns.
+  const auto take_dx = [&](int64_t m0) {
+    for (int q = wave; q < DK * EXCHANGED / 16; q += DX) {
+      const int m16 = q % (EXCHANGED / 16) * 16, d = q / (EXCHANGED / 16) * 2;
+      f32x4 v[2] = {};  // (in the order of the kernel that takes dx alone)
+#pragma unroll 4
+      for (int c = 0; c < DX; ++c) {
+        const frag_t<E>* w = (const frag_t<E>*)(wx + c * WB + d * 1024) + lane;
+        const frag_t<E> g = G::template columns<E>(exchange, c * 32, m16);
+        const frag_t<E> u = G::template columns<E>(exchange, COLUMNS + c * 32, m16);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[i * 64], g, v[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[(DT + i) * 64], u, v[i]);
+      }
+      const int64_t m = m0 + m16 + (lane & 15);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = (d + i) * 16 + (lane >> 4) * 4;
+        if (m < a.rows && n < a.width) put_four(a.dx + m * a.width + n, v[i], a.width - n, a.wide_dx);
+      }
+    }
+  };
   int turn = 0;
   for (int64_t tile = blockIdx.x; tile < tiles; tile += gridDim.x, turn ^= 1) {
     stage_barrier();  // the tile is there, and nobody reads the one before it
@@ -526,7 +579,7 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
 #pragma unroll
           for (int j = 0; j < 8; ++j) dys[j] += (float)v[j];
         }
-    if (f0 >= a.hidden) continue;
+    if (!DX && f0 >= a.hidden) continue;
 #pragma unroll 1
     for (int row = 0; row < ROWS; row += 32) {
       frag_t<E> dg[FT][P], du[FT][P], h[FT][P];
@@ -581,6 +634,17 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
           set_half<E, P>(h[i], t, p);
         }
       }
+      if constexpr (DX > 0) {
+        if (row && EXCHANGED < ROWS) lds_barrier();  // nobody reads those of the rows before
+#pragma unroll
+        for (int i = 0; i < FT; ++i) {
+          const int f = wave * 16 * FT + i * 16 + (lane & 15);
+          char* at = exchange + f * G::PITCH +
+                     (((EXCHANGED == 64 ? row / 8 : 0) + (lane >> 4)) ^ G::turn(f)) * 16;
+          *(frag_t<E>*)at = dg[i][0];
+          *(frag_t<E>*)(at + COLUMNS * G::PITCH) = du[i][0];
+        }
+      }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         frag_t<E> x[P];
@@ -600,6 +664,14 @@ __global__ void __launch_bounds__((64 * weight_waves<T, DK, OK>())) ffn_rows_dw_
 #pragma unroll
         for (int i = 0; i < FT; ++i) dwd[i][o] = mfma_planes<T>(h[i], y, dwd[i][o]);
       }
+      if constexpr (DX && EXCHANGED < ROWS) {
+        lds_barrier();  // dg and du are there
+        take_dx(tile * ROWS + row);
+      }
+    }
+    if constexpr (DX && EXCHANGED == ROWS) {
+      lds_barrier();
+      take_dx(tile * ROWS);
     }
   }
 
@@ -815,11 +887,20 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
     using C = BackwardChunk<T, DK, OK>;
     const RowPlan<T, DK, OK> p(workspace, c.rows, c.width, c.hidden, c.out);
     const int chunks = (int)tiles(c.hidden, 32);
+    const bool weights = c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd;
+    // dx with the weights' gradients where a workgroup of four or eight wavefronts has all hidden
+    // columns (with one or two, most of its wavefronts would have none).  bfloat16, against two
+    // kernels: 1M rows of 64-256-64 455 and 555 us, 64-128-64 280 and 315; 500k of 32-256-32
+    // 157 and 195, 64-192-64 239 and 253, 64-160-64 232 and 235
+    constexpr bool ALONGSIDE = RowPlan<T, DK, OK>::FT == 2;
+    const bool alongside = ALONGSIDE && c.dx && weights && p.columns == 1 && p.waves > 2;
     if (c.dx) {
       const PackArgs pack{c.wg, c.wu, c.wd, c.bg, c.bu, p.packed, c.width, c.hidden, c.out,
                           DK, 0, OK, C::KB};
       hipLaunchKernelGGL((ffn_pack_kernel<T, true>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                          stream, pack);
+    }
+    if (c.dx && !alongside) {
       BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
                               c.dy_pitch, c.width, c.out, chunks, nullptr,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
@@ -841,7 +922,7 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
         }
       });
     }
-    if (!(c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd)) return;
+    if (!weights) return;
     Layer<T> lay;
     for (int64_t r = 0; r < c.rows; r += p.pass) {
       const int64_t m = std::min(p.pass, c.rows - r);
@@ -853,10 +934,25 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       a.bg = (const T*)c.bg, a.bu = (const T*)c.bu;
       a.dwgu = p.dwgu, a.dwd = p.dwd, a.sums = p.sums, a.dy_sums = c.dbd ? p.dy_sums : nullptr;
       a.rows = m, a.width = c.width, a.hidden = c.hidden, a.out = c.out, a.add = r > 0;
-      with_activation(c.act, [&](auto act) {
-        hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value>),
-                           dim3(p.runs, p.columns), dim3(64 * p.waves), 0, stream, a);
-      });
+      a.dx = c.dx ? (T*)c.dx + r * c.width : nullptr;
+      a.packed = p.packed, a.chunks = chunks, a.wide_dx = wide_stores<T>(c.dx, c.width);
+      const auto launch = [&](auto dx, int waves) {
+        with_activation(c.act, [&](auto act) {
+          hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value, dx.value>),
+                             dim3(p.runs, p.columns), dim3(64 * waves), 0, stream, a);
+        });
+      };
+      if constexpr (ALONGSIDE) {
+        if (alongside && p.waves <= 4) {
+          launch(std::integral_constant<int, 4>(), 4);
+          continue;
+        }
+        if (alongside) {
+          launch(std::integral_constant<int, 8>(), 8);
+          continue;
+        }
+      }
+      launch(std::integral_constant<int, 0>(), p.waves);
     }
     const int64_t F = c.hidden, D = c.width, O = c.out;
     Joiner<T> join;

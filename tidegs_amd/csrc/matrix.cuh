@@ -287,6 +287,13 @@ __device__ __forceinline__ void stage_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// Behind it every wavefront's LDS accesses are done; copies to LDS may still be on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
 // The main loop: copy(step, plane, a, b) starts the copies of a step's planes of the operands
 // to a and b in LDS.  acc[i][j] is the transposed 16 x 16 tile of rows a_row + 16 i of A and
 // b_row + 16 j of B: lane l holds row l % 16 of A and rows (l / 16) * 4 + r of B.
