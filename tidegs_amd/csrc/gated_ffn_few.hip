@@ -6,7 +6,9 @@
 // operand of its products, 16 a tile: the same four matrix instructions a weight whether one
 // row or sixteen are there, and the loads are what counts.  Two launches, the hidden
 // values of a call (32 rows of 4096: 256 KB) between them in L2.  One row of 1024-4096-1024
-// bfloat16 takes 5.4 + 5.7 us: 3.1 and 1.5 TB/s of weights.
+// bfloat16 takes 5.5 + 6 us: 3.0 and 1.4 TB/s of weights.  The matrix cores idle meanwhile,
+// so a hidden value of 16 bits is multiplied with what its rounding left as a second plane:
+// y is off by its own rounding alone.
 #include "gated_ffn.cuh"
 
 // Sixteen bytes at a byte offset of a buffer; zeros past its end.
@@ -34,11 +36,15 @@ __device__ __forceinline__ void load_planes(rsrc_t r, uint32_t at, bool live,
   }
 }
 
+// Planes of a hidden value.
+template <typename T>
+constexpr int HIDDEN_PLANES = Planes<T>::N == 1 ? 2 : 3;
+
 template <typename T>
 struct FewArgs {
   using E = typename Planes<T>::E;
   const T *x, *wg, *wu, *wd, *bg, *bu, *bd;
-  E* h;  // [planes, rows, hidden8]
+  E* h;  // [HIDDEN_PLANES, rows, hidden8]
   T* y;
   int64_t x_pitch;
   int32_t rows, width, hidden, hidden8, out;
@@ -101,17 +107,27 @@ __global__ void __launch_bounds__(64 * FEW_HIDDEN_WAVES) ffn_few_hidden_kernel(F
     const float uv = us[r] + (a.bu && in ? to_f32(a.bu[f + r]) : 0.f);
     v[r] = in ? activation<ACT>(gv).x * uv : 0.f;
   }
-  four_t<E> h[P];
-  split4<T>(v, h);
+  constexpr int HP = HIDDEN_PLANES<T>;
+  four_t<E> h[HP];
+  if constexpr (P == 1) {
 #pragma unroll
-  for (int q = 0; q < P; ++q)
+    for (int r = 0; r < 4; ++r) {
+      h[0][r] = (E)v[r];
+      const float rest = v[r] - (float)h[0][r];  // not finite: nothing
+      h[1][r] = (E)(__builtin_fabsf(rest) < __builtin_inff() ? rest : 0.f);
+    }
+  } else {
+    split4<T>(v, h);
+  }
+#pragma unroll
+  for (int q = 0; q < HP; ++q)
     *(four_t<E>*)(a.h + ((int64_t)q * a.rows + m) * a.hidden8 + f) = h[q];
 }
 
 template <typename T, int RT>
 __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs<T> a) {
   using E = typename Planes<T>::E;
-  constexpr int P = Planes<T>::N, W = FEW_OUT_WAVES;
+  constexpr int P = Planes<T>::N, HP = HIDDEN_PLANES<T>, W = FEW_OUT_WAVES;
   __shared__ f32x4 s[W][RT][64];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -119,7 +135,7 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
   const int live = min(a.each, a.out - o0);
   const int64_t from = (int64_t)o0 * a.hidden;
   const rsrc_t rd = buffer_of(a.wd + from, (uint32_t)(live * a.hidden * sizeof(T)));
-  const rsrc_t rh = buffer_of(a.h, (uint32_t)(P * a.rows * a.hidden8 * 2));
+  const rsrc_t rh = buffer_of(a.h, (uint32_t)(HP * a.rows * a.hidden8 * 2));
   f32x4 y[RT] = {};
   const int steps = (a.hidden + 31) / 32;
 #pragma unroll 4
@@ -133,9 +149,9 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int m = i * 16 + row;
-      frag_t<E> h[P];
+      frag_t<E> h[HP];
 #pragma unroll
-      for (int q = 0; q < P; ++q) {
+      for (int q = 0; q < HP; ++q) {
         union {
           i32x4 w;
           frag_t<E> f;
@@ -144,7 +160,10 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
                              ? (uint32_t)((q * a.rows + m) * a.hidden8 + c) * 2 : MX_OUTSIDE);
         h[q] = v.f;
       }
-      y[i] = mfma_planes<T>(w, h, y[i]);
+      if constexpr (P == 1)
+        y[i] = mfma32(w[0], h[0], mfma32(w[0], h[1], y[i]));
+      else
+        y[i] = mfma_planes<T>(w, h, y[i]);
     }
   }
 #pragma unroll
@@ -164,7 +183,7 @@ __global__ void __launch_bounds__(64 * FEW_OUT_WAVES) ffn_few_out_kernel(FewArgs
 
 template <typename T>
 uint64_t FewKernels<T>::workspace(int64_t rows, int32_t hidden) {
-  return Planes<T>::N * rows * round8(hidden) * 2;
+  return HIDDEN_PLANES<T> * rows * round8(hidden) * 2;
 }
 
 template <typename T>

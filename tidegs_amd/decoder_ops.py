@@ -273,7 +273,7 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     Differentiable in every tensor; the backward computes the hidden values
     again.  The hidden product and its gradients are rounded to the tensors'
     type between the matrix products, as a stored hidden tensor would be
-    (float32 tensors are not).
+    (float32 tensors are not, nor is the hidden product of up to 32 rows).
     """
     _dtype(x, "x")
     act = _ACTIVATIONS.get(activation)
