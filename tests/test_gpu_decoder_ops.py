@@ -400,9 +400,10 @@ def test_gated_ffn_large(gpu, rows, D, F, O, dtype):
 
 
 # narrow rows whose hidden columns one workgroup holds (65 to 256 of them), every width of its
-# exchange, hidden columns that end inside a wavefront's, rows inside a tile
+# exchange, hidden columns that end inside a wavefront's, rows inside a tile, a second pass of rows
 FFN_ALONGSIDE = [(35, 64, 65, 64), (64, 64, 128, 33), (1, 32, 96, 3), (1000, 59, 129, 3), (97, 64, 160, 64),
-                 (4099, 64, 256, 64), (333, 20, 250, 48), (20001, 32, 256, 32), (66, 33, 224, 64)]
+                 (4099, 64, 256, 64), (333, 20, 250, 48), (20001, 32, 256, 32), (66, 33, 224, 64),
+                 ((1 << 20) + 300, 12, 100, 7)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)

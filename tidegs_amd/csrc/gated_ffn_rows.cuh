@@ -15,8 +15,8 @@
 // Bound by the gate's arithmetic: 1M rows of 64-256-64 bfloat16 issue vector instructions in
 // 61% of the SIMDs' cycles, among them an exponential and a reciprocal a hidden value at a
 // quarter of the rate, beside matrix instructions in 34%, with no LDS bank conflicts.
-//   1M rows bfloat16 of 64-256-48, forward: 132 us, 680 TFLOP/s; of 64-256-64: forward 162,
-//     dx 240, weights' gradients 349 us (605, 680 and 560 TFLOP/s, hidden products included)
+//   1M rows bfloat16 of 64-256-48, forward: 132 us, 680 TFLOP/s; of 64-256-64: forward 156
+//     (630), backward in one kernel 480 (550, the hidden products included)
 //   300k rows float32 of 59-128-3 (six products a product): 89, 170 and 163 us
 #pragma once
 
