@@ -14,7 +14,7 @@ enum { ACT_SILU = 0, ACT_GELU = 1, ACT_RELU = 2 };
 template <int ACT>
 __device__ __forceinline__ float2 activation(float g) {
   if constexpr (ACT == ACT_RELU) {
-    return g > 0.f ? make_float2(g, 1.f) : make_float2(0.f * g, 0.f);
+    return make_float2(g < 0.f ? 0.f : g, g > 0.f ? 1.f : 0.f);  // (NaN stays, -inf gives 0)
   } else if constexpr (ACT == ACT_SILU) {
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f));
     const float a = g * s;
