@@ -6,7 +6,7 @@ import torch
 
 import tidegs_amd as tg
 from tests.gpu_util import announce
-from tests.test_gpu_decoder_ops import DTYPES, _ffn_inputs
+from tests.test_gpu_decoder_ops import DTYPES, _ffn_inputs, _gen, _norm64, _rand, _within
 
 pytestmark = pytest.mark.gpu
 
@@ -38,3 +38,24 @@ def test_relu_closes_at_minus_infinity(gpu, rows, D, F, O, dtype):
     for a, b, name in zip(_forward_backward(shut, dy, "relu"), _forward_backward(zero, dy, "relu"),
                           ("y", *NAMES)):
         assert bool(torch.isfinite(a).all()) and torch.equal(a, b), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [59, 64, 1000, 4500])
+def test_layer_norm_of_tiny_rows_without_eps(gpu, width, dtype):
+    """Rows whose variance, or whose squares, lie below the 32-bit range, beside ordinary ones."""
+    announce(f"layer norm without eps, rows from 1 to 2^-100 {width} {dtype}")
+    g = _gen(width)
+    x = _rand(g, 24, width)
+    scale = 2.0 ** -torch.tensor([0, 40, 60, 62, 63, 64, 66, 70, 74, 80, 90, 100], device=gpu)
+    x = (x * scale.repeat(2)[:, None]).to(dtype)
+    w, b = _rand(g, width, dtype=dtype), _rand(g, width, dtype=dtype)
+    dy = _rand(g, 24, width, dtype=dtype)
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = tg.layer_norm(*leaves, 0.0)
+    got = [y, *torch.autograd.grad(y, leaves, dy)]
+    for t, (v, e), name in zip(got, _norm64(x, w, b, 0.0, dy), ("y", "dx", "dw", "db")):
+        _within(t, v, e, name)
+    # an eps below the squares' range counts as well
+    x = _rand(g, 6, width) * 2.0 ** -66
+    _within(tg.layer_norm(x, eps=2.0 ** -130), *_norm64(x, None, None, 2.0 ** -130)[0], "with eps")

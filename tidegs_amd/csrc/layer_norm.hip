@@ -84,6 +84,16 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// Below this variance (which eps has to be below, too) squares of 32 bits start to fall out of
+// the range and the hardware's reciprocal root takes its argument for zero: the differences are
+// squared again TINY_SCALE times as large, the variance comes out TINY_SCALE^2 as large.
+#define TINY_VARIANCE 0x1p-100f
+#define TINY_SCALE 0x1p100f
+
+__device__ __forceinline__ float tiny_variance(float squares_over_n, float eps) {
+  return squares_over_n + eps * TINY_SCALE * TINY_SCALE;
+}
+
 // x becomes xhat; returns rstd.  Lanes past the row's end hold zeros, and keep them: the
 // mean that is taken from them is zero.
 template <typename Map, int LANES, int E>
@@ -103,10 +113,21 @@ __device__ __forceinline__ float normalise(float (&x)[E], int lane, uint32_t n, 
       q = fmaf(x[e + k], x[e + k], q);
     }
   }
-  const float rstd = __builtin_amdgcn_rsqf(fmaf(group_sum<LANES>(q), inv_n, eps));
+  float var = fmaf(group_sum<LANES>(q), inv_n, eps), scale = 1.f;
+  if (var < TINY_VARIANCE) {  // (the same for all lanes of a row)
+    scale = TINY_SCALE;
+    q = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      x[e] *= scale;
+      q = fmaf(x[e], x[e], q);
+    }
+    var = tiny_variance(group_sum<LANES>(q) * inv_n, eps);
+  }
+  const float rstd = __builtin_amdgcn_rsqf(var);
 #pragma unroll
   for (int e = 0; e < E; ++e) x[e] *= rstd;
-  return rstd;
+  return rstd * scale;
 }
 
 // The weight's or bias's values of this lane's columns; `other` where there are none.
@@ -257,18 +278,29 @@ __device__ __forceinline__ float block_sum(float v, float* s) {
   return (s[0] + s[1]) + (s[2] + s[3]);
 }
 
+// xhat is (x - mean) scale root, dx has the factor scale root as well.
+struct RowStats {
+  float mean, scale, root;
+  __device__ __forceinline__ float xhat(float x) const { return (x - mean) * scale * root; }
+};
+
 template <typename T>
-__device__ __forceinline__ void row_stats(const T* x, uint32_t n, float eps, float* s, float& mean,
-                                          float& rstd) {
+__device__ __forceinline__ RowStats row_stats(const T* x, uint32_t n, float eps, float* s) {
   float a = 0.f;
   for (uint32_t c = threadIdx.x; c < n; c += 256) a += to_f32(x[c]);
-  mean = block_sum(a, s) / (float)n;
-  a = 0.f;
-  for (uint32_t c = threadIdx.x; c < n; c += 256) {
-    const float d = to_f32(x[c]) - mean;
-    a = fmaf(d, d, a);
-  }
-  rstd = 1.f / sqrtf(block_sum(a, s) / (float)n + eps);
+  const float mean = block_sum(a, s) / (float)n;
+  const auto squares = [&](float scale) {
+    float q = 0.f;
+    for (uint32_t c = threadIdx.x; c < n; c += 256) {
+      const float d = (to_f32(x[c]) - mean) * scale;
+      q = fmaf(d, d, q);
+    }
+    return block_sum(q, s) / (float)n;
+  };
+  const float var = squares(1.f) + eps;
+  if (var < TINY_VARIANCE)  // (the same for all threads)
+    return {mean, TINY_SCALE, 1.f / sqrtf(tiny_variance(squares(TINY_SCALE), eps))};
+  return {mean, 1.f, 1.f / sqrtf(var)};
 }
 
 template <typename T, typename W>
@@ -278,10 +310,9 @@ __global__ void __launch_bounds__(256) layer_norm_fwd_wide_kernel(
   __shared__ float s[4];
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + (int64_t)r * pitch;
-    float mean, rstd;
-    row_stats(row, n, eps, s, mean, rstd);
+    const RowStats stats = row_stats(row, n, eps, s);
     for (uint32_t c = threadIdx.x; c < n; c += 256)
-      y[r * n + c] = from_f32<T>(fmaf((to_f32(row[c]) - mean) * rstd,
+      y[r * n + c] = from_f32<T>(fmaf(stats.xhat(to_f32(row[c])),
                                       weight ? to_f32(weight[c]) : 1.f,
                                       bias ? to_f32(bias[c]) : 0.f));
   }
@@ -300,10 +331,10 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_kernel(
   for (uint64_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T* row = x + (int64_t)r * pitch;
     const T* grad = dy + (int64_t)r * dy_pitch;
-    float mean, rstd, a = 0.f, q = 0.f;
-    row_stats(row, n, eps, s, mean, rstd);
+    const RowStats stats = row_stats(row, n, eps, s);
+    float a = 0.f, q = 0.f;
     for (uint32_t c = threadIdx.x; c < n; c += 256) {
-      const float d = to_f32(grad[c]), xh = (to_f32(row[c]) - mean) * rstd;
+      const float d = to_f32(grad[c]), xh = stats.xhat(to_f32(row[c]));
       if (dw) {
         dw[c] = fmaf(d, xh, dw[c]);
         dw[n + c] += d;
@@ -317,7 +348,8 @@ __global__ void __launch_bounds__(256) layer_norm_bwd_wide_kernel(
     if (!dx) continue;
     for (uint32_t c = threadIdx.x; c < n; c += 256) {
       const float g = to_f32(grad[c]) * (weight ? to_f32(weight[c]) : 1.f);
-      dx[r * n + c] = from_f32<T>(rstd * (g - a - (to_f32(row[c]) - mean) * rstd * q));
+      dx[r * n + c] =
+          from_f32<T>(stats.root * stats.scale * (g - a - stats.xhat(to_f32(row[c])) * q));
     }
   }
 }
