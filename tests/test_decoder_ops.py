@@ -153,3 +153,34 @@ def test_workspace_sizes_never_shrink_with_the_rows():
                           lib.tgs_gated_ffn_bwd_workspace_size):
                 got = [query(r, *sizes, dtype) for r in rows]
                 assert got == sorted(got), (sizes, dtype)
+
+
+def test_tangents_are_refused_not_lost(monkeypatch):
+    """Forward-mode differentiation raises, whichever input carries the tangent and whether
+    or not a gradient is asked for as well; calls without tangents pass inside a level.  The
+    launches are left out."""
+    from torch.autograd import forward_ad
+
+    from tidegs_amd import decoder_ops
+
+    monkeypatch.setattr(decoder_ops, "_on_gpu", lambda *a: None)
+    monkeypatch.setattr(N, "call", lambda *a: 0)
+    monkeypatch.setattr(N, "stream_handle", lambda *a: 0)
+    x, w, b = torch.randn(4, 8), torch.ones(8), torch.zeros(8)
+    ffn = list(_ffn().values()) + [torch.zeros(n) for n in (16, 16, 3)]
+    calls = [(tg.layer_norm, [x, w, b]),
+             (lambda x, r: tg.dropout(x, 0.1, 1, residual=r), [x, torch.randn(4, 8)]),
+             (tg.gated_ffn, ffn)]
+    for op, tensors in calls:
+        for i, t in enumerate(tensors):
+            for mode in (torch.enable_grad, torch.no_grad):
+                for needs in (False, True):
+                    with mode(), forward_ad.dual_level():
+                        op(*tensors)
+                        moved = list(tensors)
+                        moved[i] = forward_ad.make_dual(t.clone().requires_grad_(needs),
+                                                        torch.ones_like(t))
+                        with pytest.raises(NotImplementedError, match="jvp"):
+                            op(*moved)
+        with torch.no_grad():
+            assert not op(*tensors).requires_grad

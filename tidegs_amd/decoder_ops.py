@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _native as N
 
@@ -70,11 +71,17 @@ def _workspace_size(query: str, *sizes: int) -> int:
     return getattr(N.load(), query)(*sizes)
 
 
-def _any_grad(*tensors: Optional[Tensor]) -> bool:
+def _recorded(*tensors: Optional[Tensor]) -> bool:
+    """Whether a call goes through its autograd Function: a gradient is asked for, or a tensor
+    carries a tangent, which the Function refuses (the operators have no forward mode) and
+    the bare call would lose."""
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
                 return True
+    if forward_ad._current_level >= 0:  # (asked first: unpacking costs a quarter us a tensor)
+        return any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                   for t in tensors)
     return False
 
 
@@ -158,7 +165,7 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     bias = _parameter(bias, "bias", shape, x, (torch.float32,))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}: one type is needed")
-    if _any_grad(x, weight, bias):
+    if _recorded(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm_fwd(x, weight, bias, float(eps))[1]
 
@@ -211,7 +218,7 @@ def dropout(x: Tensor, p: float, seed: int, offset: int = 0,
     x = x.contiguous()
     residual = residual.contiguous() if residual is not None else None
     threshold = int(math.floor(p * 65536 + 0.5))
-    if _any_grad(x, residual):
+    if _recorded(x, residual):
         return _Dropout.apply(x, residual, threshold, int(seed), int(offset))
     return _dropout(x, residual, threshold, int(seed), int(offset))
 
@@ -293,6 +300,6 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     b_up = _parameter(b_up, "b_up", (hidden,), x)
     b_down = _parameter(b_down, "b_down", (out,), x)
     args = (x, w_gate, w_up, w_down, b_gate, b_up, b_down)
-    if _any_grad(*args):
+    if _recorded(*args):
         return _GatedFfn.apply(*args, act)
     return _gated_ffn_fwd(*args, act)[1]
