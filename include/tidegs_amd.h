@@ -832,7 +832,7 @@ int tgs_dropout(uint64_t n, int32_t dtype, const void* x, const void* residual, 
  * x [rows, width], w_gate and w_up [hidden, width], w_down [out, hidden], biases
  * (each nullable) [hidden], [hidden], [out], y [rows, out] dense, all of `dtype`.
  * activation: 0 silu, 1 gelu (with the error function), 2 relu.  The workspace starts on
- * 16 bytes. */
+ * 16 bytes; its size is 0 for sizes or types that the call refuses. */
 uint64_t tgs_gated_ffn_fwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
                                           uint32_t out, int32_t dtype);
 int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out, int32_t dtype,

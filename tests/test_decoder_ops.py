@@ -184,3 +184,17 @@ def test_tangents_are_refused_not_lost(monkeypatch):
                             op(*moved)
         with torch.no_grad():
             assert not op(*tensors).requires_grad
+
+
+def test_workspace_sizes_of_refused_sizes():
+    """Nothing for what the calls refuse, with the reason (a hidden size of 0 ended the process)."""
+    lib = N.load()
+    for query in (lib.tgs_gated_ffn_fwd_workspace_size, lib.tgs_gated_ffn_bwd_workspace_size):
+        for rows, width, hidden, out, dtype, text in (
+                (4, 64, 0, 64, 1, "positive"), (4, 0, 0, 0, 0, "positive"), (4, 200, 16, 0, 0, "positive"),
+                (4, 65537, 16, 3, 0, "65536"), (4, 1 << 31, 1 << 31, 1 << 31, 2, "65536"),
+                (1 << 31, 64, 64, 64, 0, "rows"), (1 << 63, 64, 64, 64, 0, "rows"),
+                (4, 64, 64, 64, 7, "dtype")):
+            assert query(rows, width, hidden, out, dtype) == 0 and text in N.last_error()
+        for dtype in (0, 1, 2):
+            assert query(0, 64, 64, 64, dtype) > 0 and query(4, 65536, 65536, 65536, dtype) > 0

@@ -409,6 +409,7 @@ static void hidden_products(hipStream_t s, const HiddenArgs<typename Planes<T>::
 static uint64_t workspace_size(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out,
                                int32_t dtype, bool back) {
   uint64_t bytes = 0;
+  if (check_sizes("tgs_gated_ffn workspace", rows, width, hidden, out, ACT_SILU)) return 0;
   with_dtype(dtype, "tgs_gated_ffn workspace", [&](auto tag) -> int {
     using T = decltype(tag);
     bytes = Plan<T>(nullptr, rows, width, hidden, out, back).bytes;
