@@ -6,7 +6,8 @@ import torch
 
 import tidegs_amd as tg
 from tests.gpu_util import announce
-from tests.test_gpu_decoder_ops import DTYPES, _ffn_inputs, _gen, _norm64, _rand, _within
+from tests.test_gpu_decoder_ops import (DTYPES, _ffn64, _ffn_inputs, _gen, _norm64, _rand,
+                                        _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -59,3 +60,52 @@ def test_layer_norm_of_tiny_rows_without_eps(gpu, width, dtype):
     # an eps below the squares' range counts as well
     x = _rand(g, 6, width) * 2.0 ** -66
     _within(tg.layer_norm(x, eps=2.0 ** -130), *_norm64(x, None, None, 2.0 ** -130)[0], "with eps")
+
+
+@pytest.mark.parametrize("scale", [1.0, 1e-2, 1e-6, 3e-7])
+@pytest.mark.parametrize("rows,D,F,O", [(20000, 64, 256, 48), (20000, 128, 80, 100),
+                                        (20000, 20, 600, 3), (9000, 200, 300, 40)])
+def test_half_gradients_of_small_dy(gpu, rows, D, F, O, scale):
+    """The weights' gradients of a mean loss: every row's term lies at or below half's smallest
+    values, their sums do not.  Each term is rounded to 11 bits twice at most, independently
+    of the others, and the sum once: 2^-10 of itself in the norm, and the spacing of half's
+    smallest values where the sum is stored."""
+    announce(f"half gradients of dy of {scale} {rows} x {D}-{F}-{O}")
+    args, dy = _ffn_inputs(rows, D, F, O, torch.float16, True, rows + D)
+    dy = (dy.float() * scale).half()
+    got = _forward_backward(args, dy)
+    for t, (v, _), name in zip(got, _ffn64("silu", *args, dy=dy), ("y", *NAMES)):
+        far = (t.double() - v).norm()
+        assert float(far) <= 2.0 ** -10 * float(v.norm()) + 2.0 ** -25 * math.sqrt(v.numel()), \
+            (name, float(far / v.norm()))
+
+
+@pytest.mark.parametrize("rows,D,F,O", [(20000, 64, 256, 48), (20000, 128, 80, 100), (9000, 200, 300, 40)])
+def test_half_gradients_of_small_hidden_values(gpu, rows, D, F, O):
+    """dWd = dy' h of hidden values at half's smallest, and gradients of dy far from it on
+    either side: the same bounds."""
+    announce(f"half gradients of small hidden values {rows} x {D}-{F}-{O}")
+    args, dy = _ffn_inputs(rows, D, F, O, torch.float16, False, rows + D)
+    for x_scale, dy_scale in ((1e-3, 1.0), (1e-3, 1e-4), (30.0, 1e-6), (1.0, 100.0)):
+        some = [args[0] * x_scale, *args[1:4]]
+        leaves = [t.detach().requires_grad_() for t in some]
+        d = dy * dy_scale
+        grads = torch.autograd.grad(tg.gated_ffn(*leaves), leaves, d)
+        for t, (v, _), name in zip(grads, _ffn64("silu", *some, dy=d)[1:], NAMES):
+            far = (t.double() - v).norm()
+            assert float(far) <= 2.0 ** -10 * float(v.norm()) + 2.0 ** -25 * math.sqrt(v.numel()), \
+                (name, x_scale, dy_scale, float(far / v.norm()))
+
+
+def test_half_gradients_beside_large_rows(gpu):
+    """Rows whose x or dy is far larger than the others' leave these as they are without them."""
+    announce("half gradients beside large rows")
+    for rows, D, F, O in ((300, 64, 256, 48), (300, 128, 80, 100), (300, 200, 300, 40)):
+        args, dy = _ffn_inputs(rows, D, F, O, torch.float16, True, 77)
+        for k, big in ((0, 3e3), (1, 3e4)):
+            x, d = args[0].clone(), dy.clone()
+            (x if k == 0 else d)[5] *= big / 4
+            got = _forward_backward([x, *args[1:]], d)[1]
+            rest = [i for i in range(rows) if i != 5]
+            v, e = _ffn64("silu", x[rest], *args[1:], dy=d[rest])[1]
+            _within(got[rest], v, e, f"dx beside a row of {big}")

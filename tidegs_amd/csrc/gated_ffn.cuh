@@ -99,6 +99,26 @@ struct FfnCall {
 };
 
 // ---------------------------------------------------------------------------
+// Half precision's backward.  h, dg and du are rounded to the tensors' type for the products
+// that sum them over rows; half keeps nothing below 2^-25, where the gradients of a mean over
+// an image's pixels lie, though their sums do not (200k rows with dy of 3e-7: dWg 29% off).  They
+// are multiplied by powers of two before they are rounded and the 32-bit sums divided again,
+// both exact.  The powers are the largest that cannot overflow, by bounds from the tensors'
+// largest magnitudes: half's 40 binary places leave 2^-40 of the bound, some 2^-25 of the values
+// themselves.  Never below 1, so a row far beyond the others takes nothing from them.
+// ---------------------------------------------------------------------------
+
+template <typename T>
+constexpr bool LIFTED = std::is_same<T, f16_t>::value;
+
+struct Lift {
+  float h, back_h, d, back_d;  // of h; of dg and du
+};
+#define LIFT_BLOCKS 512                // of a tensor at most
+#define LIFT_PEAKS (7 * LIFT_BLOCKS)   // floats of workspace
+void ffn_lift(const FfnCall& c, Lift* lift, float* peaks, hipStream_t stream);
+
+// ---------------------------------------------------------------------------
 // Operands that the products cannot read where they lie (32-bit values, rows that do
 // not start on 16 bytes, widths that are no multiple of 8) are laid out as planes
 // with rows of a whole number of chunks, zeros behind the last value.
@@ -153,6 +173,7 @@ struct JoinJob {
   int64_t rows;
   void* out;          // [rows, cols]
   const void* bias;   // [cols], added to the sums; nullable
+  const float* factor;  // of the sums, half's; nullable
   uint32_t blocks;    // of the launch, up to and with this job's
 };
 #define JOIN_JOBS 6
@@ -184,9 +205,11 @@ __global__ void __launch_bounds__(256) ffn_join_kernel(JoinJobs jobs) {
     __syncthreads();
     if (g < h) s[threadIdx.x] += s[threadIdx.x + h * each];
   }
-  if (live && g == 0)
-    ((T*)job.out)[i] =
-        from_f32<T>(s[threadIdx.x] + (job.bias ? to_f32(((const T*)job.bias)[i % job.cols]) : 0.f));
+  if (live && g == 0) {
+    float v = s[threadIdx.x];
+    if (LIFTED<T> && job.factor) v *= *job.factor;
+    ((T*)job.out)[i] = from_f32<T>(v + (job.bias ? to_f32(((const T*)job.bias)[i % job.cols]) : 0.f));
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -258,13 +281,13 @@ struct Joiner {
   int n = 0;
   uint32_t blocks = 0;
   void add(const float* partial, int64_t part, int64_t pitch, int64_t parts, int64_t rows,
-           int64_t cols, void* to, const void* bias = nullptr) {
+           int64_t cols, void* to, const void* bias = nullptr, const float* factor = nullptr) {
     if (!to) return;
     // (many values in few parts keep the chip busy with a thread each)
     const int groups = parts > (rows * cols < 65536 ? 4 : 32) ? 8 : 1;
     blocks += (uint32_t)tiles(rows * cols, 256 / groups);
     jobs.job[n++] = JoinJob{partial, part, pitch, (int32_t)parts, (int32_t)cols, groups, rows, to,
-                            bias, blocks};
+                            bias, factor, blocks};
   }
   void launch(hipStream_t s) {
     if (n) hipLaunchKernelGGL(ffn_join_kernel<T>, dim3(blocks), dim3(256), 0, s, jobs);

@@ -42,6 +42,7 @@ struct HiddenArgs {
   float* sums;  // of dg and du over a tile's rows: [tiles_m, 2 hidden8], nullable
   int64_t plane;  // values between planes of h; dgu's are 2 * plane
   int32_t add;    // add to sums
+  const Lift* lift;  // half's, backward
 };
 
 template <typename T, bool BACK, typename Z>
@@ -93,6 +94,8 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
 
   const int group = lane >> 4;
   float sg[TF][4] = {}, su[TF][4] = {};
+  Lift lift;
+  if constexpr (BACK && LIFTED<T>) lift = *a.lift;
   with_activation(a.act, [&](auto kind) {
 #pragma unroll
   for (int j = 0; j < TF; ++j) {
@@ -116,7 +119,11 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
         const float2 act = activation<kind.value>(g);
         vh[r] = in ? act.x * u : 0.f;
         if constexpr (BACK) {
-          const float d = P == 3 && i % 2 ? -dh[i][j][r] : dh[i][j][r];
+          float d = P == 3 && i % 2 ? -dh[i][j][r] : dh[i][j][r];
+          if constexpr (LIFTED<T>) {
+            d *= lift.d;
+            vh[r] *= lift.h;
+          }
           vg[r] = in ? d * u * act.y : 0.f;
           vu[r] = in ? d * act.x : 0.f;
           if (m < a.rows) {
@@ -196,6 +203,7 @@ struct ProductArgs {
   int32_t wide;             // c is written four values at a time
   float* partial;           // or [splits, M, N]
   int32_t add;              // add to what `partial` holds
+  const float* factor;      // of c, half's; nullable
 };
 
 template <typename T, Along KA, Along KB, typename Z>
@@ -233,6 +241,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<
         sa.copy(to_a, (s.pair ? g.a2.p : g.a.p) + at_a + q * g.a.plane, s.k);
         sb.copy(to_b, (s.pair ? g.b2.p : g.b.p) + at_b + q * g.b.plane, s.k);
       });
+  const float factor = LIFTED<T> && g.factor ? *g.factor : 1.f;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
     const int64_t m = m0 + wm * TM * 16 + i * 16 + (lane & 15);
@@ -254,7 +263,8 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_product_kernel(ProductArgs<
         four_t<T> v;
 #pragma unroll
         for (int r = 0; r < 4; ++r)
-          v[r] = from_f32<T>(acc[i][j][r] + (g.bias && n + r < g.N ? to_f32(((const T*)g.bias)[n + r]) : 0.f));
+          v[r] = from_f32<T>((LIFTED<T> ? acc[i][j][r] * factor : acc[i][j][r]) +
+                             (g.bias && n + r < g.N ? to_f32(((const T*)g.bias)[n + r]) : 0.f));
         if (g.wide) {
           if (n < g.N) *(four_t<T>*)at = v;
         } else {
@@ -339,6 +349,8 @@ struct Plan {
   int64_t rows, D, F, O, D8, F8, O8, pass;
   E *x, *wg, *wu, *wd, *dy, *h, *dgu;
   float *parts, *gu_sums, *dy_sums, *dwgu, *dwd;  // parts: of y or dx
+  Lift* lift = nullptr;  // half's
+  float* peaks = nullptr;
   int split_gu = 1, split_d = 1;
   uint64_t bytes;
 
@@ -362,6 +374,10 @@ struct Plan {
       // (one sum over all rows is rounded where it is taken)
       dwgu = split_gu > 1 || pass < rows ? c.take<float>(split_gu * 2 * F8 * D) : nullptr;
       dwd = split_d > 1 || pass < rows ? c.take<float>(split_d * O * F) : nullptr;
+      if (LIFTED<T>) {
+        lift = c.take<Lift>(1);
+        peaks = c.take<float>(LIFT_PEAKS);
+      }
     }
     bytes = c.used;
   }
@@ -389,7 +405,7 @@ static void row_product(hipStream_t s, ProductArgs<typename Planes<T>::E> g, flo
   g.partial = parts;
   product<T, KA, KB>(s, g);
   Joiner<T> join;
-  join.add(parts, g.M * g.N, g.N, g.splits, g.M, g.N, g.c, g.bias);
+  join.add(parts, g.M * g.N, g.N, g.splits, g.M, g.N, g.c, g.bias, g.factor);
   join.launch(s);
 }
 
@@ -508,13 +524,13 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
     }
     TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 16 == 0,
                   "tgs_gated_ffn_bwd: the workspace starts on 16 bytes");
+    FfnCall c{};
+    c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
+    c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
+    c.bg = b_gate, c.bu = b_up, c.dy = dy, c.dy_pitch = dy_pitch;
+    c.dx = dx, c.dwg = dw_gate, c.dwu = dw_up, c.dwd = dw_down;
+    c.dbg = db_gate, c.dbu = db_up, c.dbd = db_down;
     if (rows && RowKernels<T>::takes(width, out)) {
-      FfnCall c{};
-      c.rows = rows, c.width = width, c.hidden = hidden, c.out = out, c.act = activation;
-      c.x = x, c.x_pitch = x_pitch, c.wg = w_gate, c.wu = w_up, c.wd = w_down;
-      c.bg = b_gate, c.bu = b_up, c.dy = dy, c.dy_pitch = dy_pitch;
-      c.dx = dx, c.dwg = dw_gate, c.dwu = dw_up, c.dwd = dw_down;
-      c.dbg = db_gate, c.dbu = db_up, c.dbd = db_down;
       RowKernels<T>::backward(c, workspace, stream);
       TGS_RETURN_LAUNCH("tgs_gated_ffn_bwd");
     }
@@ -524,6 +540,9 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
     const Operand<E> wu = lay.operand(w_up, p.F, p.D, p.D, p.wu);
     const Operand<E> wd = lay.operand(w_down, p.O, p.F, p.F, p.wd);
     const bool hidden_sums = db_gate || db_up;
+    if (LIFTED<T> && rows) ffn_lift(c, p.lift, p.peaks, stream);
+    const float* const back_d = LIFTED<T> && rows ? &p.lift->back_d : nullptr;
+    const float* const back_h = LIFTED<T> && rows ? &p.lift->back_h : nullptr;
     for (int64_t r = 0; r < p.rows; r += p.pass) {
       const int64_t m = std::min(p.pass, p.rows - r);
       HiddenArgs<E> a{};
@@ -534,7 +553,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
       a.rows = m, a.width8 = p.D8, a.hidden = p.F, a.hidden8 = p.F8, a.out = p.O, a.out8 = p.O8;
       a.act = activation, a.bg = b_gate, a.bu = b_up;
       a.h = p.h, a.dgu = p.dgu, a.plane = m * p.F8;
-      a.sums = hidden_sums ? p.gu_sums : nullptr, a.add = r > 0;
+      a.sums = hidden_sums ? p.gu_sums : nullptr, a.add = r > 0, a.lift = p.lift;
       hidden_products<T, true>(stream, a);
       if (dx) {
         ProductArgs<E> g{};
@@ -542,7 +561,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
         g.b = wg, g.b2 = wu;
         // (k runs to the weights' last row; behind it dg and du are zero)
         g.M = m, g.N = p.D, g.K = p.F, g.a_limit = m, g.b_limit = p.D8;
-        g.c = (T*)dx + r * p.D;
+        g.c = (T*)dx + r * p.D, g.factor = back_d;
         row_product<T, ALONG, ACROSS>(stream, g, p.parts);
       }
       if (dw_gate || dw_up) {
@@ -550,7 +569,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
         g.a = {p.dgu, 2 * a.plane, 2 * p.F8}, g.b = a.x;
         g.M = 2 * p.F8, g.N = p.D, g.K = m, g.a_limit = 2 * p.F8, g.b_limit = p.D8;
         g.splits = p.split_gu, g.partial = p.dwgu, g.add = r > 0;
-        g.c = dw_gate, g.c2 = dw_up, g.each = p.F;
+        g.c = dw_gate, g.c2 = dw_up, g.each = p.F, g.factor = back_d;
         product<T, ACROSS, ACROSS>(stream, g);
       }
       if (dw_down) {
@@ -558,6 +577,7 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
         g.a = a.dy, g.b = {p.h, a.plane, p.F8};
         g.M = p.O, g.N = p.F, g.K = m, g.a_limit = p.O8, g.b_limit = p.F8;
         g.splits = p.split_d, g.partial = p.dwd, g.add = r > 0, g.c = dw_down;
+        g.factor = back_h;
         product<T, ACROSS, ACROSS>(stream, g);
       }
       if (db_down)
@@ -568,13 +588,19 @@ extern "C" int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden,
     Joiner<T> join;
     const int64_t some = p.rows > 0;  // no rows: sums of nothing
     if (p.dwgu || !some) {
-      join.add(p.dwgu, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_gate);
-      join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up);
+      join.add(p.dwgu, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_gate,
+               nullptr, back_d);
+      join.add(p.dwgu + p.F8 * p.D, 2 * p.F8 * p.D, p.D, some * p.split_gu, p.F, p.D, dw_up, nullptr,
+               back_d);
     }
-    if (p.dwd || !some) join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down);
+    if (p.dwd || !some)
+      join.add(p.dwd, p.O * p.F, p.F, some * p.split_d, p.O, p.F, dw_down, nullptr,
+               back_h);
     const int64_t row_tiles = tiles(p.pass, TileSmall::M);
-    join.add(p.gu_sums, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_gate);
-    join.add(p.gu_sums + p.F8, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_up);
+    join.add(p.gu_sums, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_gate, nullptr,
+             back_d);
+    join.add(p.gu_sums + p.F8, 2 * p.F8, p.F8, some * row_tiles, 1, p.F, db_up, nullptr,
+             back_d);
     join.add(p.dy_sums, p.O, p.O, some * COLUMN_RUNS, 1, p.O, db_down);
     join.launch(stream);
     TGS_RETURN_LAUNCH("tgs_gated_ffn_bwd");

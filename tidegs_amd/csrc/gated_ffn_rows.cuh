@@ -261,6 +261,7 @@ struct BackwardArgs {
   int32_t width, out, chunks;
   float* parts;                    // not null: [gridDim.y, rows, width], as the forward's
   int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
+  const Lift* lift;                // half's
 };
 
 template <typename T, int DK, int OK, int RT, int ACT>
@@ -293,6 +294,8 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
         load_fragment<T>(a.dy + m * a.dy_pitch, k * 32 + c, a.out, m < a.rows, a.wide_dy, dy[i][k]);
     }
     f32x4 dx[DT][RT] = {};
+    Lift lift;
+    if constexpr (LIFTED<T>) lift = *a.lift;
     for (int c = 0; c < chunks; ++c) {
       if (BUFFERS == 1 && c) {
         stage_barrier();
@@ -337,8 +340,10 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float2 v = activation<ACT>(g[i][r]);
-            vg[r] = dh[i][r] * u[i][r] * v.y;
-            vu[r] = dh[i][r] * v.x;
+            float d = dh[i][r];
+            if constexpr (LIFTED<T>) d *= lift.d;
+            vg[r] = d * u[i][r] * v.y;
+            vu[r] = d * v.x;
           }
           four_t<E> p[P];
           split4<T>(vg, p);
@@ -365,6 +370,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
       for (int i = 0; i < RT; ++i) {
         const int64_t m = m0 + i * 16;
         if (m >= a.rows || n >= a.width) continue;
+        if constexpr (LIFTED<T>) dx[d][i] *= lift.back_d;
         if (a.parts) {
           put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.width + n, dx[d][i], a.width - n);
           continue;
@@ -397,6 +403,7 @@ struct WeightArgs {
   T* dx;  // where dx is taken along; its packed weights, their chunks, four values at a time
   const char* packed;
   int32_t chunks, wide_dx;
+  const Lift* lift;  // half's
 };
 
 // Rows of a tile in LDS, of STEPS k steps of 32 (64 bytes each), and what its 16-byte
@@ -522,6 +529,8 @@ __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), 
   f32x4 dwg[FT][DT] = {}, dwu[FT][DT] = {}, dwd[FT][OT] = {};
   float dys[8] = {};  // of eight columns of dy, over every blockDim.x / Y::CHUNKS-th row
   float sg[FT] = {}, su[FT] = {};
+  Lift lift;
+  if constexpr (LIFTED<T>) lift = *a.lift;
   const int64_t tiles = (a.rows + ROWS - 1) / ROWS;
   const auto stage = [&](int64_t tile, char* to) {
 #pragma unroll
@@ -560,6 +569,7 @@ __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), 
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const int n = (d + i) * 16 + (lane >> 4) * 4;
+        if constexpr (LIFTED<T>) v[i] *= lift.back_d;
         if (m < a.rows && n < a.width) put_four(a.dx + m * a.width + n, v[i], a.width - n, a.wide_dx);
       }
     }
@@ -618,10 +628,12 @@ __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), 
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
             const float2 v = activation<ACT>(g[i][r]);
-            const float d = P == 3 && t ? -dh[i][r] : dh[i][r];
+            float d = P == 3 && t ? -dh[i][r] : dh[i][r];
+            if constexpr (LIFTED<T>) d *= lift.d;
             vg[r] = d * u[i][r] * v.y;
             vu[r] = d * v.x;
             vh[r] = v.x * u[i][r];
+            if constexpr (LIFTED<T>) vh[r] *= lift.h;
             sg[i] += vg[r];
             su[i] += vu[r];
           }
@@ -781,6 +793,8 @@ struct RowPlan {
   char* packed;
   E *x, *dy;
   float *parts, *dwgu, *dwd, *sums, *dy_sums;  // parts: of dx
+  Lift* lift = nullptr;  // half's
+  float* peaks = nullptr;
   uint64_t bytes;
   RowPlan(void* ws, int64_t rows, int64_t width, int64_t hidden, int64_t out) {
     constexpr int P = Planes<T>::N;
@@ -801,6 +815,10 @@ struct RowPlan {
     dwd = c.take<float>(runs * hidden * out);
     sums = c.take<float>(runs * 2 * hidden);
     dy_sums = c.take<float>(runs * out);
+    if (LIFTED<T>) {
+      lift = c.take<Lift>(1);
+      peaks = c.take<float>(LIFT_PEAKS);
+    }
     bytes = c.used;
   }
 };
@@ -888,6 +906,8 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
     const RowPlan<T, DK, OK> p(workspace, c.rows, c.width, c.hidden, c.out);
     const int chunks = (int)tiles(c.hidden, 32);
     const bool weights = c.dwg || c.dwu || c.dwd || c.dbg || c.dbu || c.dbd;
+    if (!c.dx && !weights) return;
+    if (LIFTED<T>) ffn_lift(c, p.lift, p.peaks, stream);
     // dx with the weights' gradients where a workgroup of four or eight wavefronts has all hidden
     // columns (with one or two, most of its wavefronts would have none).  bfloat16, against two
     // kernels: 1M rows of 64-256-64 455 and 555 us, 64-128-64 280 and 315; 500k of 32-256-32
@@ -904,7 +924,7 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
                               c.dy_pitch, c.width, c.out, chunks, nullptr,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
-                              wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width)};
+                              wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width), p.lift};
       // 500k rows bfloat16, 32 and 16 rows a wavefront: 128-256-128 244 and 281 us, 64-256-64
       // 115 and 108; float32 with 16 rows and one chunk buffer, where two workgroups share
       // a CU, against 32 and two: 300k of 59-128-3 147 and 175 us
@@ -936,6 +956,7 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       a.rows = m, a.width = c.width, a.hidden = c.hidden, a.out = c.out, a.add = r > 0;
       a.dx = c.dx ? (T*)c.dx + r * c.width : nullptr;
       a.packed = p.packed, a.chunks = chunks, a.wide_dx = wide_stores<T>(c.dx, c.width);
+      a.lift = p.lift;
       const auto launch = [&](auto dx, int waves) {
         with_activation(c.act, [&](auto act) {
           hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value, dx.value>),
@@ -955,12 +976,14 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       launch(std::integral_constant<int, 0>(), p.waves);
     }
     const int64_t F = c.hidden, D = c.width, O = c.out;
+    const float* const back_d = LIFTED<T> ? &p.lift->back_d : nullptr;
+    const float* const back_h = LIFTED<T> ? &p.lift->back_h : nullptr;
     Joiner<T> join;
-    join.add(p.dwgu, 2 * F * D, D, p.runs, F, D, c.dwg);
-    join.add(p.dwgu + F * D, 2 * F * D, D, p.runs, F, D, c.dwu);
-    join.add(p.dwd, O * F, F, p.runs, O, F, c.dwd);
-    join.add(p.sums, 2 * F, F, p.runs, 1, F, c.dbg);
-    join.add(p.sums + F, 2 * F, F, p.runs, 1, F, c.dbu);
+    join.add(p.dwgu, 2 * F * D, D, p.runs, F, D, c.dwg, nullptr, back_d);
+    join.add(p.dwgu + F * D, 2 * F * D, D, p.runs, F, D, c.dwu, nullptr, back_d);
+    join.add(p.dwd, O * F, F, p.runs, O, F, c.dwd, nullptr, back_h);
+    join.add(p.sums, 2 * F, F, p.runs, 1, F, c.dbg, nullptr, back_d);
+    join.add(p.sums + F, 2 * F, F, p.runs, 1, F, c.dbu, nullptr, back_d);
     join.add(p.dy_sums, O, O, p.runs, 1, O, c.dbd);
     join.launch(stream);
   });

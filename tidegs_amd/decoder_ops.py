@@ -280,7 +280,10 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     Differentiable in every tensor; the backward computes the hidden values
     again.  The hidden product and its gradients are rounded to the tensors'
     type between the matrix products, as a stored hidden tensor would be
-    (float32 tensors are not, nor is the hidden product of up to 32 rows).
+    (float32 tensors are not, nor is the hidden product of up to 32 rows).  Half
+    precision's backward scales them to the type's range first, by powers of two, so
+    that sums over rows of gradients below its smallest values come out; a hidden
+    product past 65504, or a gradient of one, is infinite there.
     """
     _dtype(x, "x")
     act = _ACTIVATIONS.get(activation)
