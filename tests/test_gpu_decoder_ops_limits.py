@@ -6,8 +6,8 @@ import torch
 
 import tidegs_amd as tg
 from tests.gpu_util import announce
-from tests.test_gpu_decoder_ops import (DTYPES, _ffn64, _ffn_inputs, _gen, _norm64, _rand,
-                                        _within)
+from tests.test_gpu_decoder_ops import (DTYPES, _act64, _ffn64, _ffn_inputs, _gen, _norm64,
+                                        _rand, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -109,3 +109,40 @@ def test_half_gradients_beside_large_rows(gpu):
             rest = [i for i in range(rows) if i != 5]
             v, e = _ffn64("silu", x[rest], *args[1:], dy=d[rest])[1]
             _within(got[rest], v, e, f"dx beside a row of {big}")
+
+
+def test_gelu_is_as_near_as_its_formula_in_32_bits(gpu):
+    """g Phi(g) and its derivative through a block that passes its gate on, against
+    0.5 g (1 + erf(g / sqrt 2)) in 32 bits: no further from 64 bits than 1.5 times that (the
+    derivative 2 times: the exponential takes its argument in 32 bits)."""
+    announce("gelu against its formula in 32 bits")
+    one, zero = torch.ones(1, 1, device=gpu), torch.zeros(1, device=gpu)
+    for scale in (0.3, 1.0, 3.0):
+        x = _rand(_gen(9), 200000, 1, scale=scale).requires_grad_()
+        y = tg.gated_ffn(x, one, one * 0, one, zero, zero + 1, zero, activation="gelu")
+        (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+        g = x.detach()
+        phi = 0.5 * (1 + torch.erf(g * math.sqrt(0.5)))
+        slope = phi + g * torch.exp(-0.5 * g * g) / math.sqrt(2 * math.pi)
+        for got, plain, want, times in zip((y, dx), (g * phi, slope), _act64("gelu", g.double()),
+                                           (1.5, 2.0)):
+            far, plain_far = (float((t.double() - want).norm()) for t in (got, plain))
+            assert far <= times * plain_far, (scale, far, plain_far)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_open_and_large_gates(gpu, act, dtype):
+    """A gate of +inf gives an infinity, large ones their own value or 0."""
+    announce(f"gated ffn: gates of +inf and large ones {act} {dtype}")
+    for rows in (5, 50):
+        for D in (8, 200):
+            x = torch.zeros(rows, D, dtype=dtype, device=gpu)
+            w = torch.zeros(3, D, dtype=dtype, device=gpu)
+            one = torch.ones(3, dtype=dtype, device=gpu)
+            for gate, want in ((math.inf, math.inf), (30000.0, 30000.0), (200.0, 200.0), (-200.0, 0.0),
+                               (-30000.0, 0.0)):
+                wd = torch.tensor([[1.0, 0.0, 0.0]], dtype=dtype, device=gpu)
+                bg = torch.tensor([gate, 0, 0], dtype=dtype, device=gpu)
+                y = tg.gated_ffn(x, w, w, wd, bg, one, None, activation=act)
+                assert torch.equal(y, torch.full_like(y, want)), (rows, D, gate, y.flatten()[0])

@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(Z::THREADS, 2) ffn_hidden_kernel(HiddenArgs<ty
         // (behind the last hidden column zeros, whatever x holds)
         const bool in = f + r < a.hidden;
         const float g = gu[i][2 * j][r] + bg[r], u = gu[i][2 * j + 1][r] + bu[r];
-        const float2 act = activation<kind.value>(g);
+        const float2 act = activation<kind.value, T>(g);
         vh[r] = in ? act.x * u : 0.f;
         if constexpr (BACK) {
           float d = P == 3 && i % 2 ? -dh[i][j][r] : dh[i][j][r];

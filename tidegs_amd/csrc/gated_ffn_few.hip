@@ -105,7 +105,7 @@ __global__ void __launch_bounds__(64 * FEW_HIDDEN_WAVES) ffn_few_hidden_kernel(F
     const bool in = f + r < a.hidden;
     const float gv = gs[r] + (a.bg && in ? to_f32(a.bg[f + r]) : 0.f);
     const float uv = us[r] + (a.bu && in ? to_f32(a.bu[f + r]) : 0.f);
-    v[r] = in ? activation<ACT>(gv).x * uv : 0.f;
+    v[r] = in ? activation<ACT, T>(gv).x * uv : 0.f;
   }
   constexpr int HP = HIDDEN_PLANES<T>;
   four_t<E> h[HP];

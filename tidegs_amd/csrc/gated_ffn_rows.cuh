@@ -203,7 +203,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
         for (int i = 0; i < RT; ++i) {
           float v[4];
 #pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = activation<ACT>(g[i][r]).x * u[i][r];
+          for (int r = 0; r < 4; ++r) v[r] = activation<ACT, T>(g[i][r]).x * u[i][r];
           four_t<E> p[P];
           split4<T>(v, p);
           set_half<E, P>(h[i], t, p);
@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
           float vg[4], vu[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float2 v = activation<ACT>(g[i][r]);
+            const float2 v = activation<ACT, T>(g[i][r]);
             float d = dh[i][r];
             if constexpr (LIFTED<T>) d *= lift.d;
             vg[r] = d * u[i][r] * v.y;
@@ -627,7 +627,7 @@ __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), 
           float vg[4], vu[4], vh[4];
 #pragma unroll
           for (int r = 0; r < 4; ++r) {
-            const float2 v = activation<ACT>(g[i][r]);
+            const float2 v = activation<ACT, T>(g[i][r]);
             float d = P == 3 && t ? -dh[i][r] : dh[i][r];
             if constexpr (LIFTED<T>) d *= lift.d;
             vg[r] = d * u[i][r] * v.y;
