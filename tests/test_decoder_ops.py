@@ -198,3 +198,23 @@ def test_workspace_sizes_of_refused_sizes():
             assert query(rows, width, hidden, out, dtype) == 0 and text in N.last_error()
         for dtype in (0, 1, 2):
             assert query(0, 64, 64, 64, dtype) > 0 and query(4, 65536, 65536, 65536, dtype) > 0
+
+
+def test_six_products_of_planes_keep_24_bits():
+    """The arithmetic of float32 products, on the host: three bfloat16 planes, each what the
+    ones before leave, rounded, are the value; the products left out come to 2^-24 at most."""
+    g = torch.Generator().manual_seed(1)
+    for spread in (2.0 ** -8, 2.0 ** -7, 1.0):  # the worst lie just below 1 + 2^-8
+        planes = []
+        for _ in range(2):
+            v = 1 + spread * torch.rand(1 << 20, generator=g)
+            rest, parts = v.clone(), []
+            for _ in range(3):
+                parts.append(rest.to(torch.bfloat16).float())
+                rest = rest - parts[-1]
+            assert not bool(rest.any())
+            planes.append([p.double() for p in parts])
+        a, b = planes
+        kept = a[0] * b[2] + a[2] * b[0] + a[1] * b[1] + a[1] * b[0] + a[0] * b[1] + a[0] * b[0]
+        want = sum(a) * sum(b)
+        assert float(((kept - want) / want).abs().max()) <= 2.0 ** -24

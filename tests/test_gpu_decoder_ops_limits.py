@@ -146,3 +146,17 @@ def test_open_and_large_gates(gpu, act, dtype):
                 bg = torch.tensor([gate, 0, 0], dtype=dtype, device=gpu)
                 y = tg.gated_ffn(x, w, w, wd, bg, one, None, activation=act)
                 assert torch.equal(y, torch.full_like(y, want)), (rows, D, gate, y.flatten()[0])
+
+
+@pytest.mark.parametrize("rows,O", [(32, 128), (1000, 128), (500, 300)])
+def test_float32_products_of_computed_values(gpu, rows, O):
+    """A hidden value times a weight, one product, where the parts that its six products of
+    bfloat16 planes leave out are largest: 2^-24 of it at most, and a last bit of the sum."""
+    announce(f"float32 products of hidden values {rows} x {O}")
+    g = _gen(rows)
+    x = 1 + 2.0 ** -7 * torch.rand(rows, 1, generator=g, device=gpu)
+    wd = 1 + 2.0 ** -7 * torch.rand(O, 1, generator=g, device=gpu)
+    one, zero = torch.ones(1, 1, device=gpu), torch.zeros(1, device=gpu)
+    y = tg.gated_ffn(x, one, 0 * one, wd, zero, zero + 1, None, activation="relu")
+    want = x.double() * wd.double().t()
+    assert float(((y.double() - want) / want).abs().max()) <= 2.0 ** -24 + 2.0 ** -23

@@ -7,9 +7,10 @@
 // side); both are staged as they lie, and an ACROSS operand is turned while it is read
 // from LDS (the transposing 64-bit LDS read), so no product needs a transposed copy.
 //
-// 32-bit operands come as three bfloat16 planes hi + mid + lo = the value (8 bits each,
-// split exactly up to 2^-27 of it) and are multiplied as the six products of planes
-// whose sum is off by less than 2^-25: hi lo, lo hi, mid mid, mid hi, hi mid, hi hi.
+// 32-bit operands come as three bfloat16 planes hi + mid + lo = the value (each what the ones
+// before it leave, rounded: exact) and are multiplied as six products of planes: hi lo,
+// lo hi, mid mid, mid hi, hi mid, hi hi.  The three left out come to 2^-24 of the product at most
+// (mid is below 2^-8 of the value and lo below 2^-17), to 2^-27 of it on the average.
 // Six bfloat16 products run at 1/6 of that type's rate, 2.7 times the 32-bit matrix
 // instructions' (an 8192^3 product of the vendor's: 1307 and 132 TFLOP/s).
 //
@@ -76,10 +77,8 @@ __device__ __forceinline__ void split(float v, typename Planes<T>::E (&p)[Planes
   }
 }
 
-// Four values at once, as kernels split what they compute: a 32-bit value's planes are its
-// bits in three runs of 8 (each cut off, not rounded: exact, and the products left out
-// then come to 2^-26 of the whole), two values a word, six operations a value instead of
-// nine.  A value that is not finite comes out as NaN.
+// Four values at once, as kernels split what they compute, two values a word.  A 32-bit value that
+// is not finite, or within 2^-9 of the largest, comes out as NaN.
 template <typename T>
 __device__ __forceinline__ void split4(const float (&v)[4],
                                        four_t<typename Planes<T>::E> (&out)[Planes<T>::N]) {
@@ -87,8 +86,11 @@ __device__ __forceinline__ void split4(const float (&v)[4],
 #pragma unroll
     for (int r = 0; r < 4; ++r) out[0][r] = (typename Planes<T>::E)v[r];
   } else {
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef bf16_t bf16x2 __attribute__((ext_vector_type(2)));
     union {
       uint32_t w[2];
+      bf16x2 p[2];
       four_t<bf16_t> f;
     } u;
     float rest[4] = {v[0], v[1], v[2], v[3]};
@@ -96,13 +98,14 @@ __device__ __forceinline__ void split4(const float (&v)[4],
     for (int q = 0; q < 3; ++q) {
 #pragma unroll
       for (int k = 0; k < 2; ++k)
-        u.w[k] = __builtin_amdgcn_perm(__float_as_uint(rest[2 * k + 1]),
-                                       __float_as_uint(rest[2 * k]), 0x07060302);
+        u.p[k] = __builtin_convertvector((f32x2{rest[2 * k], rest[2 * k + 1]}), bf16x2);
       out[q] = u.f;
       if (q < 2)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-          rest[r] -= __uint_as_float(__float_as_uint(rest[r]) & 0xFFFF0000u);
+        for (int k = 0; k < 2; ++k) {
+          rest[2 * k] -= __uint_as_float(u.w[k] << 16);
+          rest[2 * k + 1] -= __uint_as_float(u.w[k] & 0xFFFF0000u);
+        }
     }
   }
 }
