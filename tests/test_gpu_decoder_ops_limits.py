@@ -160,3 +160,28 @@ def test_float32_products_of_computed_values(gpu, rows, O):
     y = tg.gated_ffn(x, one, 0 * one, wd, zero, zero + 1, None, activation="relu")
     want = x.double() * wd.double().t()
     assert float(((y.double() - want) / want).abs().max()) <= 2.0 ** -24 + 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,D,F,O", [(5, 8, 3, 4), (50, 8, 3, 4), (66000, 8, 40, 4), (50, 100, 70, 20),
+                                        (300, 64, 100, 33), (300, 33, 130, 64), (50, 64, 2100, 7),
+                                        (50, 200, 70, 20)])
+def test_infinite_rows_come_out_infinite(gpu, rows, D, F, O, dtype):
+    """Weights and rows are positive, so a row with an infinity has infinite outputs, whatever
+    the hidden columns are padded to; so has a row's dx where dy has one."""
+    announce(f"gated ffn: infinite rows {rows} x {D}-{F}-{O} {dtype}")
+    g = _gen(F)
+    args = [torch.rand(s, generator=g, device=gpu).add(0.5).to(dtype)
+            for s in ((rows, D), (F, D), (F, D), (O, F), (F,), (F,), (O,))]
+    args[1:4] = [w / w.shape[1] for w in args[1:4]]
+    dy = torch.rand(rows, O, generator=g, device=gpu).to(dtype)
+    clean = _forward_backward(args, dy)[:2]
+    bad, dbad = args[0].clone(), dy.clone()
+    bad[3, D - 1], dbad[4, 0] = math.inf, math.inf
+    with torch.no_grad():
+        y = tg.gated_ffn(bad, *args[1:])
+    dx = _forward_backward(args, dbad)[1]
+    for t, row, c in ((y, 3, clean[0]), (dx, 4, clean[1])):
+        assert bool((t[row] == math.inf).all()), t[row]
+        rest = torch.arange(rows, device=gpu) != row
+        assert torch.equal(t[rest], c[rest])

@@ -35,6 +35,17 @@ struct BackwardChunk {  // Wg, Wu: two tiles by DK; Wd': two tiles by OK; Wg', W
   static constexpr int KB = FRAGMENTS * Planes<T>::N + 1;
 };
 
+// The columns of a chunk's fragment behind the last hidden one become zeros: there g and u are
+// products with zeros, NaN where x is infinite, and would reach the row's other outputs.
+// (Three planes make an infinity NaN by themselves.)
+template <typename E, int P>
+__device__ __forceinline__ void keep_hidden(frag_t<E> (&f)[P], int left) {
+  if constexpr (P == 1) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[0][e] = (int)(threadIdx.x & 63) / 16 * 8 + e < left ? f[0][e] : (E)0.f;
+  }
+}
+
 struct PackArgs {
   const void *wg, *wu, *wd, *bg, *bu;
   char* out;
@@ -103,7 +114,7 @@ struct ForwardArgs {
   const char* packed;
   const T* bd;
   int64_t rows, x_pitch;
-  int32_t width, out, chunks;
+  int32_t width, out, chunks, hidden;
   float* parts;      // not null: [gridDim.y, rows, out], chunks dealt over gridDim.y
   int32_t wide;      // x is read 16 bytes at a time
   int32_t wide_out;  // y is written four values at a time
@@ -209,6 +220,9 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
           set_half<E, P>(h[i], t, p);
         }
       }
+      if (P == 1 && (first + c + 1) * 32 > a.hidden)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) keep_hidden<E, P>(h[i], a.hidden - (first + c) * 32);
 #pragma unroll
       for (int o = 0; o < OT; ++o) {
         frag_t<E> w[P];
@@ -258,7 +272,7 @@ struct BackwardArgs {
   T* dx;
   const char* packed;
   int64_t rows, x_pitch, dy_pitch;
-  int32_t width, out, chunks;
+  int32_t width, out, chunks, hidden;
   float* parts;                    // not null: [gridDim.y, rows, width], as the forward's
   int32_t wide, wide_dy, wide_dx;  // 16 bytes at a time; dx: four values
   const Lift* lift;                // half's
@@ -352,6 +366,12 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
           set_half<E, P>(du[i], t, p);
         }
       }
+      if (P == 1 && (first + c + 1) * 32 > a.hidden)
+#pragma unroll
+        for (int i = 0; i < RT; ++i) {
+          keep_hidden<E, P>(dg[i], a.hidden - (first + c) * 32);
+          keep_hidden<E, P>(du[i], a.hidden - (first + c) * 32);
+        }
 #pragma unroll
       for (int d = 0; d < DT; ++d) {
         frag_t<E> w[P];
@@ -477,8 +497,10 @@ constexpr int weight_rows() {  // of a staged tile
 // hidden column, so dg and du of 32 rows, exchanged through LDS, are all that dx of these
 // rows wants: tiles of 16 rows and columns, dealt over the wavefronts.  Wg' and Wu' stay in
 // LDS.  Of 1M rows of 64-256-64 bfloat16 that saves the hidden products, the gate and the
-// reads of x and dy that a kernel of its own for dx repeats.
-template <typename T, int DK, int OK, int FT, int ACT, int DX>
+// reads of x and dy that a kernel of its own for dx repeats.  FULL: they have a hidden column
+// each (32 DX of them); a loop of known length over these spills less (1M rows of 64-256-64:
+// 545 us against 566, both directions).
+template <typename T, int DK, int OK, int FT, int ACT, int DX, bool FULL>
 __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), (DX ? 2 : 1))
     ffn_rows_dw_kernel(WeightArgs<T> a) {
   using E = typename Planes<T>::E;
@@ -547,24 +569,29 @@ __global__ void __launch_bounds__((64 * (DX ? DX : weight_waves<T, DK, OK>())), 
   if (DX && blockIdx.x < tiles)
     for (int c = 0; c < a.chunks; ++c)
       copy_chunk<WB / 1024, DX ? DX : 1>(wx + c * WB, a.packed + ((int64_t)c * C::KB + 4 * DK + 2 * OK) * 1024);
-  if constexpr (DX > 0)  // (behind the last chunk dg and du are zero: so are the weights)
-    for (int i = a.chunks * WB / 16 + threadIdx.x; i < DX * WB / 16; i += 64 * DX)
-      ((i32x4*)wx)[i] = i32x4{};
   // dx of the exchanged rows, from m0 on: a wavefront takes 16 of them by 32 columns.
   const auto take_dx = [&](int64_t m0) {
     for (int q = wave; q < DK * EXCHANGED / 16; q += DX) {
       const int m16 = q % (EXCHANGED / 16) * 16, d = q / (EXCHANGED / 16) * 2;
       f32x4 v[2] = {};  // (in the order of the kernel that takes dx alone)
-#pragma unroll 4
-      for (int c = 0; c < DX; ++c) {
+      const auto add = [&](int c, auto whole) {
         const frag_t<E>* w = (const frag_t<E>*)(wx + c * WB + d * 1024) + lane;
-        const frag_t<E> g = G::template columns<E>(exchange, c * 32, m16);
-        const frag_t<E> u = G::template columns<E>(exchange, COLUMNS + c * 32, m16);
+        frag_t<E> g[P], u[P];
+        g[0] = G::template columns<E>(exchange, c * 32, m16);
+        u[0] = G::template columns<E>(exchange, COLUMNS + c * 32, m16);
+        if constexpr (!whole.value) {
+          keep_hidden<E, P>(g, a.hidden - c * 32);
+          keep_hidden<E, P>(u, a.hidden - c * 32);
+        }
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[i * 64], g, v[i]);
+        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[i * 64], g[0], v[i]);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[(DT + i) * 64], u, v[i]);
-      }
+        for (int i = 0; i < 2; ++i) v[i] = mfma32(w[(DT + i) * 64], u[0], v[i]);
+      };
+      const int whole = FULL ? DX : a.hidden / 32;
+#pragma unroll 4
+      for (int c = 0; c < whole; ++c) add(c, std::true_type());
+      if (!FULL && whole < a.chunks) add(whole, std::false_type());
       const int64_t m = m0 + m16 + (lane & 15);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
@@ -877,7 +904,7 @@ void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
                        stream, pack);
     float* parts = (float*)((char*)workspace + C::KB * 1024 * chunks);
     ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
-                           c.x_pitch, c.width, c.out, chunks, nullptr,
+                           c.x_pitch, c.width, c.out, chunks, c.hidden, nullptr,
                            wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
     // 32 rows share a fragment's reads, 16 leave room for a second workgroup: 500k rows
     // bfloat16 of 32-128-16: 27 and 30 us, 64-256-64: 77 and 76, 128-256-128: 191 and 145;
@@ -922,7 +949,7 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
     }
     if (c.dx && !alongside) {
       BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
-                              c.dy_pitch, c.width, c.out, chunks, nullptr,
+                              c.dy_pitch, c.width, c.out, chunks, c.hidden, nullptr,
                               wide_rows<T>(c.x, c.width, c.x_pitch),
                               wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width), p.lift};
       // 500k rows bfloat16, 32 and 16 rows a wavefront: 128-256-128 244 and 281 us, 64-256-64
@@ -957,23 +984,29 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
       a.dx = c.dx ? (T*)c.dx + r * c.width : nullptr;
       a.packed = p.packed, a.chunks = chunks, a.wide_dx = wide_stores<T>(c.dx, c.width);
       a.lift = p.lift;
-      const auto launch = [&](auto dx, int waves) {
+      const auto launch = [&](auto dx, auto full, int waves) {
         with_activation(c.act, [&](auto act) {
-          hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value, dx.value>),
+          hipLaunchKernelGGL((ffn_rows_dw_kernel<T, DK, OK, RowPlan<T, DK, OK>::FT, act.value, dx.value,
+                                                 full.value>),
                              dim3(p.runs, p.columns), dim3(64 * waves), 0, stream, a);
         });
       };
       if constexpr (ALONGSIDE) {
-        if (alongside && p.waves <= 4) {
-          launch(std::integral_constant<int, 4>(), 4);
-          continue;
-        }
         if (alongside) {
-          launch(std::integral_constant<int, 8>(), 8);
+          const auto with = [&](auto dx) {
+            if (c.hidden == 32 * dx.value)
+              launch(dx, std::true_type(), dx.value);
+            else
+              launch(dx, std::false_type(), dx.value);
+          };
+          if (p.waves <= 4)
+            with(std::integral_constant<int, 4>());
+          else
+            with(std::integral_constant<int, 8>());
           continue;
         }
       }
-      launch(std::integral_constant<int, 0>(), p.waves);
+      launch(std::integral_constant<int, 0>(), std::false_type(), p.waves);
     }
     const int64_t F = c.hidden, D = c.width, O = c.out;
     const float* const back_d = LIFTED<T> ? &p.lift->back_d : nullptr;

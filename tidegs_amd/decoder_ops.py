@@ -283,7 +283,8 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     (float32 tensors are not, nor is the hidden product of up to 32 rows).  Half
     precision's backward scales them to the type's range first, by powers of two, so
     that sums over rows of gradients below its smallest values come out; a hidden
-    product past 65504, or a gradient of one, is infinite there.
+    product past 65504, or a gradient of one, is infinite there.  A row's infinities
+    and NaN stay in that row's y and dx; in float32 an infinity comes out as NaN.
     """
     _dtype(x, "x")
     act = _ACTIVATIONS.get(activation)
