@@ -1,4 +1,11 @@
-"""The decoder operators at the ends of their types' ranges."""
+"""The decoder operators at the ends of their types' ranges, in sums over many rows and
+in the kernels that only some sizes reach.
+
+Bounds element by element are those of ``test_gpu_decoder_ops``.  Where a bound over many
+rows would admit zeros (it grows with the rows, the sum with their square root), the inputs
+leave few terms or the error is taken in the norm, and the test asserts that a sum that
+lacks them would not pass.
+"""
 import math
 
 import pytest
@@ -6,7 +13,7 @@ import torch
 
 import tidegs_amd as tg
 from tests.gpu_util import announce
-from tests.test_gpu_decoder_ops import (DTYPES, _act64, _ffn64, _ffn_inputs, _gen, _norm64,
+from tests.test_gpu_decoder_ops import (DTYPES, UNIT, _act64, _ffn64, _ffn_inputs, _gen, _norm64,
                                         _rand, _within)
 
 pytestmark = pytest.mark.gpu
@@ -185,3 +192,56 @@ def test_infinite_rows_come_out_infinite(gpu, rows, D, F, O, dtype):
         assert bool((t[row] == math.inf).all()), t[row]
         rest = torch.arange(rows, device=gpu) != row
         assert torch.equal(t[rest], c[rest])
+
+
+# rows in several passes: narrow rows with dx beside the weights' gradients and without, wide
+# rows; the first and the last pass's rows
+FFN_PASSES = [((1 << 20) + 300, 20, 32, 5, 1 << 20), ((1 << 20) + 300, 12, 100, 7, 1 << 20),
+              (16500, 136, 4096, 136, 16384)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D,F,O,one_pass", FFN_PASSES)
+def test_every_pass_reaches_the_sums_over_rows(gpu, rows, D, F, O, one_pass, dtype):
+    """dy is zero but in some rows of one pass: the sums are those rows', which a bound over
+    them alone checks.  Zeros, all that is left without that pass, lie outside it."""
+    announce(f"gated ffn: passes of {rows} x {D}-{F}-{O} {dtype}")
+    args, dy = _ffn_inputs(rows, D, F, O, dtype, True, rows + F)
+    for first, last in ((0, 100), (one_pass - 100, one_pass), (one_pass, one_pass + 100),
+                        (rows - 100, rows)):
+        some = torch.zeros_like(dy)
+        some[first:last] = dy[first:last]
+        got = _forward_backward(args, some)
+        want = _ffn64("silu", args[0][first:last].contiguous(), *args[1:], dy=dy[first:last])
+        for k, name in enumerate(NAMES):
+            v, e = want[1 + k]
+            t = got[1 + k]
+            if name == "dx":
+                assert not bool(t[:first].any()) and not bool(t[last:].any())
+                t = t[first:last]
+            else:
+                assert float((v.abs() > e).double().mean()) > 0.7, f"{name}: zeros would pass"
+            _within(t, v, e, f"{name} of rows {first}:{last}")
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D,F,O", [(70001, 64, 40, 48), ((1 << 20) + 30000, 20, 32, 5),
+                                        ((1 << 20) + 30000, 12, 100, 7), (40001, 100, 64, 90),
+                                        (18000, 136, 4096, 136)])
+def test_sums_over_many_rows(gpu, rows, D, F, O, dtype):
+    """The parameters' gradients in the norm.  A row's terms carry two independent roundings of
+    the tensors' type and the sum one: 3 u of the whole; of float32, whose terms carry some tens
+    of 2^-24 and whose partial sums are of up to 2^17 rows, 2^-17.  A pass that is left out
+    or zeros are further off."""
+    announce(f"gated ffn: sums over {rows} rows {D}-{F}-{O} {dtype}")
+    args, dy = _ffn_inputs(rows, D, F, O, dtype, True, rows + F + 1)
+    got = _forward_backward(args, dy)
+    want = _ffn64("silu", *args, dy=dy)
+    part = (1 << 20) if rows > 1 << 20 else 16384
+    lost = _ffn64("silu", args[0][:part].contiguous(), *args[1:], dy=dy[:part]) if part < rows else None
+    limit = 2.0 ** -17 if dtype == torch.float32 else 3 * UNIT[dtype]
+    for k in range(2, 8):
+        v = want[k][0]
+        assert float((got[k].double() - v).norm() / v.norm()) <= limit, NAMES[k - 1]
+        if lost is not None:
+            assert float((lost[k][0] - v).norm() / v.norm()) > 2 * limit, NAMES[k - 1]
