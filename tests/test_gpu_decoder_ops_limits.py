@@ -13,8 +13,8 @@ import torch
 
 import tidegs_amd as tg
 from tests.gpu_util import announce
-from tests.test_gpu_decoder_ops import (DTYPES, UNIT, _act64, _ffn64, _ffn_inputs, _gen, _norm64,
-                                        _rand, _within)
+from tests.test_gpu_decoder_ops import (DTYPES, UNIT, _act64, _check_ffn, _ffn64, _ffn_inputs, _gen,
+                                        _norm64, _rand, _within)
 
 pytestmark = pytest.mark.gpu
 
@@ -245,3 +245,18 @@ def test_sums_over_many_rows(gpu, rows, D, F, O, dtype):
         assert float((got[k].double() - v).norm() / v.norm()) <= limit, NAMES[k - 1]
         if lost is not None:
             assert float((lost[k][0] - v).norm() / v.norm()) > 2 * limit, NAMES[k - 1]
+
+
+# up to 32 rows with 16 outputs a workgroup (from 2048 outputs on); 16-bit rows 32 a wavefront
+# (from 65536 rows on) in the widest dx kernels and in the forward's, by their outputs
+FFN_BRANCHES = [(1, 64, 64, 2048), (32, 64, 64, 2051), (32, 64, 64, 2048), (1, 70, 33, 2051),
+                (66000, 128, 48, 128), (66000, 100, 40, 20), (66000, 64, 48, 32), (66000, 64, 48, 64),
+                (66000, 40, 48, 100)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,D,F,O", FFN_BRANCHES)
+def test_kernels_of_some_sizes(gpu, rows, D, F, O, dtype):
+    announce(f"gated ffn {rows} x {D}-{F}-{O} {dtype}")
+    args, dy = _ffn_inputs(rows, D, F, O, dtype, True, rows + D + F + O)
+    _check_ffn(args, dy, "silu", f"{rows} x {D}-{F}-{O}")
