@@ -260,3 +260,36 @@ def test_kernels_of_some_sizes(gpu, rows, D, F, O, dtype):
     announce(f"gated ffn {rows} x {D}-{F}-{O} {dtype}")
     args, dy = _ffn_inputs(rows, D, F, O, dtype, True, rows + D + F + O)
     _check_ffn(args, dy, "silu", f"{rows} x {D}-{F}-{O}")
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows", [1, 16, 17, 32])
+@pytest.mark.parametrize("D,F,O", [(64, 256, 48), (100, 1000, 30), (256, 1024, 2051)])
+def test_few_rows_keep_their_hidden_values(gpu, rows, D, F, O, dtype):
+    """Up to 32 rows multiply a hidden value with what its rounding left.  What is lost then, u^2
+    of a hidden value and the sums' 2^-24 sqrt(F), is a hundredth of the results' spacing at most,
+    so y is the 64-bit result rounded but for one value in fifty (and two); hidden values rounded
+    once move one in ten at least."""
+    announce(f"gated ffn: hidden values of {rows} rows {D}-{F}-{O} {dtype}")
+    args, _ = _ffn_inputs(rows, D, F, O, dtype, True, rows + F)
+    x, wg, wu, wd, bg, bu, bd = (t.double() for t in args)
+    h = _act64("silu", x @ wg.t() + bg)[0] * (x @ wu.t() + bu)
+    want = (h @ wd.t() + bd).to(dtype)
+    once = (h.to(dtype).double() @ wd.t() + bd).to(dtype)
+    n = want.numel()
+    assert int((once != want).sum()) > 2 + n / 10, "a hidden value rounded once would pass"
+    assert int((tg.gated_ffn(*args) != want).sum()) <= 2 + n / 50
+
+
+def test_half_hidden_values_up_to_the_largest(gpu):
+    """A hidden value of 65472 is half's own; its product with a small weight is right."""
+    announce("gated ffn: half hidden values near the largest")
+    for rows, D, F, O in ((5, 64, 64, 8), (150, 64, 64, 48), (150, 200, 300, 40)):
+        one = torch.zeros(F, D, dtype=torch.float16, device=gpu)
+        one[:, 0] = 1
+        x = torch.zeros(rows, D, dtype=torch.float16, device=gpu)
+        x[:, 0] = 255.875  # squared 65472.0156: rounds to 65472
+        wd = torch.zeros(O, F, dtype=torch.float16, device=gpu)
+        wd[:, 1] = 2.0 ** -6
+        y = tg.gated_ffn(x, one, one, wd, activation="relu")
+        assert torch.equal(y, torch.full_like(y, 1023.0)), y.flatten()[0]
