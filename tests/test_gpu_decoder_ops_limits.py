@@ -293,3 +293,20 @@ def test_half_hidden_values_up_to_the_largest(gpu):
         wd[:, 1] = 2.0 ** -6
         y = tg.gated_ffn(x, one, one, wd, activation="relu")
         assert torch.equal(y, torch.full_like(y, 1023.0)), y.flatten()[0]
+
+
+def test_more_than_a_billion_rows(gpu):
+    """2^30 + 100 rows of one value: four threads a row pass what one launch may have."""
+    rows, part = (1 << 30) + 100, 1000
+    announce(f"gated ffn: {rows} rows of one value")
+    g = _gen(30)
+    x = torch.empty(rows, 1, device=gpu).uniform_(-2, 2, generator=g).requires_grad_()
+    args = [torch.tensor(v, device=gpu).view(s) for v, s in ((0.75, (1, 1)), (-0.5, (1, 1)), (2.0, (1, 1)),
+                                                             (0.25, (1,)), (0.5, (1,)), (-1.0, (1,)))]
+    y = tg.gated_ffn(x, *args)
+    dy = torch.empty(rows, 1, device=gpu).uniform_(-1, 1, generator=g)
+    (dx,) = torch.autograd.grad(y, x, dy)
+    for first in (0, (1 << 29) - 500, (1 << 30) - 500, rows - part):
+        some = slice(first, first + part)
+        for t, (v, e) in zip((y, dx), _ffn64("silu", x.detach()[some], *args, dy=dy[some])):
+            _within(t[some], v, e, f"rows from {first}")

@@ -809,6 +809,9 @@ static int64_t partial_values(int64_t rows, int64_t cols, int64_t hidden) {
 }
 
 #define ROW_PASS (1 << 20)  // rows whose x and dy are laid out at a time
+// Rows of one launch of the kernels that take tiles of 128 rows on: a launch has less than 2^32
+// threads, four a row.
+#define ROW_LAUNCH (1 << 29)
 
 // The backward's workspace.
 template <typename T, int DK, int OK>
@@ -903,25 +906,29 @@ void RowKernels<T>::forward(const FfnCall& c, void* workspace, hipStream_t strea
     hipLaunchKernelGGL((ffn_pack_kernel<T, false>), dim3(chunks * (C::FRAGMENTS + 1)), dim3(64), 0,
                        stream, pack);
     float* parts = (float*)((char*)workspace + C::KB * 1024 * chunks);
-    ForwardArgs<T> a{(const T*)c.x, (T*)c.y, (const char*)workspace, (const T*)c.bd, c.rows,
-                           c.x_pitch, c.width, c.out, chunks, c.hidden, nullptr,
-                           wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
     // 32 rows share a fragment's reads, 16 leave room for a second workgroup: 500k rows
     // bfloat16 of 32-128-16: 27 and 30 us, 64-256-64: 77 and 76, 128-256-128: 191 and 145;
     // 300k rows float32 of 59-128-3: 114 and 96
     constexpr int RT = Planes<T>::N == 1 && DK <= 2 ? 2 : 1;
-    with_rows<RT>(c.rows, chunks, [&](auto rt, dim3 grid) {
-      if (grid.y > 1) a.parts = parts;
-      with_activation(c.act, [&](auto act) {
-        hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value>), grid,
-                           dim3(64 * FR_WAVES), 0, stream, a);
+    for (int64_t r = 0; r < c.rows; r += ROW_LAUNCH) {
+      const int64_t m = std::min<int64_t>(ROW_LAUNCH, c.rows - r);
+      T* const y = (T*)c.y + r * c.out;
+      ForwardArgs<T> a{(const T*)row_at<T>(c.x, r, c.x_pitch), y, (const char*)workspace,
+                       (const T*)c.bd, m, c.x_pitch, c.width, c.out, chunks, c.hidden, nullptr,
+                       wide_rows<T>(c.x, c.width, c.x_pitch), wide_stores<T>(c.y, c.out)};
+      with_rows<RT>(m, chunks, [&](auto rt, dim3 grid) {
+        if (grid.y > 1) a.parts = parts;
+        with_activation(c.act, [&](auto act) {
+          hipLaunchKernelGGL((ffn_rows_fwd_kernel<T, DK, OT, rt.value, act.value>), grid,
+                             dim3(64 * FR_WAVES), 0, stream, a);
+        });
+        if (grid.y > 1) {
+          Joiner<T> join;
+          join.add(parts, m * c.out, c.out, grid.y, m, c.out, y, c.bd);
+          join.launch(stream);
+        }
       });
-      if (grid.y > 1) {
-        Joiner<T> join;
-        join.add(parts, c.rows * c.out, c.out, grid.y, c.rows, c.out, c.y, c.bd);
-        join.launch(stream);
-      }
-    });
+    }
   });
 }
 
@@ -948,26 +955,30 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
                          stream, pack);
     }
     if (c.dx && !alongside) {
-      BackwardArgs<T> a{(const T*)c.x, (const T*)c.dy, (T*)c.dx, p.packed, c.rows, c.x_pitch,
-                              c.dy_pitch, c.width, c.out, chunks, c.hidden, nullptr,
-                              wide_rows<T>(c.x, c.width, c.x_pitch),
-                              wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width), p.lift};
       // 500k rows bfloat16, 32 and 16 rows a wavefront: 128-256-128 244 and 281 us, 64-256-64
       // 115 and 108; float32 with 16 rows and one chunk buffer, where two workgroups share
       // a CU, against 32 and two: 300k of 59-128-3 147 and 175 us
       constexpr int RT = Planes<T>::N == 3 ? 1 : 2;
-      with_rows<RT>(c.rows, chunks, [&](auto rt, dim3 grid) {
-        if (grid.y > 1) a.parts = p.parts;
-        with_activation(c.act, [&](auto act) {
-          hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), grid,
-                             dim3(64 * FR_WAVES), 0, stream, a);
+      for (int64_t r = 0; r < c.rows; r += ROW_LAUNCH) {
+        const int64_t m = std::min<int64_t>(ROW_LAUNCH, c.rows - r);
+        T* const dx = (T*)c.dx + r * c.width;
+        BackwardArgs<T> a{(const T*)row_at<T>(c.x, r, c.x_pitch), (const T*)row_at<T>(c.dy, r, c.dy_pitch),
+                          dx, p.packed, m, c.x_pitch, c.dy_pitch, c.width, c.out, chunks, c.hidden,
+                          nullptr, wide_rows<T>(c.x, c.width, c.x_pitch),
+                          wide_rows<T>(c.dy, c.out, c.dy_pitch), wide_stores<T>(c.dx, c.width), p.lift};
+        with_rows<RT>(m, chunks, [&](auto rt, dim3 grid) {
+          if (grid.y > 1) a.parts = p.parts;
+          with_activation(c.act, [&](auto act) {
+            hipLaunchKernelGGL((ffn_rows_dx_kernel<T, DK, OK, rt.value, act.value>), grid,
+                               dim3(64 * FR_WAVES), 0, stream, a);
+          });
+          if (grid.y > 1) {
+            Joiner<T> join;
+            join.add(p.parts, m * c.width, c.width, grid.y, m, c.width, dx);
+            join.launch(stream);
+          }
         });
-        if (grid.y > 1) {
-          Joiner<T> join;
-          join.add(p.parts, c.rows * c.width, c.width, grid.y, c.rows, c.width, c.dx);
-          join.launch(stream);
-        }
-      });
+      }
     }
     if (!weights) return;
     Layer<T> lay;
