@@ -45,7 +45,8 @@ class AppearanceDecoder(nn.Module):
 
     ``dtype`` is the element type of the decoder's products; its parameters stay
     float32.  In training the residual branch drops a share ``p`` of its values: the
-    mask follows from ``seed`` and the ``step`` of the call.
+    mask follows from ``seed`` and the ``step`` of the call alone, so calls that are to
+    differ (two images of one optimizer step) have steps of their own.
     """
 
     def __init__(self, images: int, width: int = 64, hidden: int = 256, embedding: int = 32,

@@ -15,7 +15,7 @@
 // Memory bound: x is read and y written once, 16 bytes a lane where the pointers allow,
 // and a thread's eight values are one block of the generator, so no draw is thrown away
 // and the generator's arithmetic runs under the loads.  4M rows of 64 bfloat16 with a
-// residual (1.54 GB) take 258 us, 6.0 TB/s; 300k of 59 float32 (142 MB) 25 us, 5.6 TB/s.
+// residual (1.54 GB) take 264 us, 5.8 TB/s; 300k of 59 float32 (142 MB) 26 us, 5.5 TB/s.
 #include "decoder_common.cuh"
 
 __device__ __forceinline__ void philox4x32_10(uint32_t c[4], uint32_t k0, uint32_t k1) {

@@ -13,10 +13,16 @@
 // turn, so that a lane's accumulators hold g and u of the same row and columns and the gate
 // is taken in registers.  The backward adds dh = dy Wd for the same tile before its gate.
 //
+// h, dg and du of 16-bit tensors are rounded to their type where they are written: they are
+// what is stored between the products (200 MB at 8192 rows of 4096), and the matrix cores'
+// operands have that type.  y is 0.0023 of itself off in bfloat16 then, 0.0017 from its own
+// rounding.
+//
 // Bound by the matrix cores and what feeds them: at 8192 rows of 1024-4096-1024 bfloat16 the
-// forward's hidden products take 139 us (990 TFLOP/s), y 81 (850), the backward's three
-// hidden products 300 (690, with 200 MB of h, dg and du written), dX and dW 160 each (860);
-// a library product of 8192^3 reaches 1307.  g and u are computed again in the backward
+// forward's hidden products take 124 us (1110 TFLOP/s), y 76 (900), the backward's three
+// hidden products 264 (780, with 200 MB of h, dg and du written), dx 143 (960), dWg and dWu 137
+// (1000), dWd 145 (470: 256 tiles, one workgroup a CU where two have room); a library product
+// of 8192^3 reaches 1307.  g and u are computed again in the backward
 // rather than kept: kept in 32 bits they are 268 MB to write and to read, about 120 us,
 // for the 137 GFLOP (140 us) that they save.
 // ---------------------------------------------------------------------------
@@ -27,7 +33,8 @@
 // fragments: the hidden products of 8192 x 1024 x 2 4096 take 139 us in the large tiles, 161
 // in the small. With an operand across k the turning reads, twice as
 // many, leave the large tile's lockstep behind two small ones (dW of that block 175 us
-// against 154), and so does the backward's third accumulator (343 against 305).
+// against 154), and so does the backward's third accumulator (343 against 305).  (Pairs of
+// variants, here and below, are from runs of a few passes, at lower clocks than the times above.)
 typedef Tile<2, 2, 4, 4> TileSmall;
 typedef Tile<2, 4, 8, 4> TileLarge;
 

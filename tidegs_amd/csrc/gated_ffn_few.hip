@@ -6,7 +6,8 @@
 // operand of its products, 16 a tile: the same four matrix instructions a weight whether one
 // row or sixteen are there, and the loads are what counts.  Two launches, the hidden
 // values of a call (32 rows of 4096: 256 KB) between them in L2.  One row of 1024-4096-1024
-// bfloat16 takes 5.5 + 6 us: 3.0 and 1.4 TB/s of weights.  The matrix cores idle meanwhile,
+// bfloat16 takes 6.0 + 6.9 us: 2.8 and 1.2 TB/s of weights, of float32 11.3 + 9.8 (3.0 and
+// 1.7), 20 of bfloat16 8.9 + 16.  The matrix cores idle meanwhile,
 // so a hidden value of 16 bits is multiplied with what its rounding left as a second plane:
 // y is off by its own rounding alone.
 #include "gated_ffn.cuh"

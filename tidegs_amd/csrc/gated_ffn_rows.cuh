@@ -8,16 +8,22 @@
 // those 32 columns (the tiles' rows are dealt so that the lane's eight are neighbours).
 // The gate and the rounding happen in place and no value crosses a lane.
 //
+// h, dg and du of 16-bit tensors are rounded to their type there, once, as a stored hidden
+// tensor is: y, dx and the weights' gradients come out 0.0023 of themselves off in bfloat16,
+// where rounding the results alone takes 0.0017.  A second plane of them, as the kernels for few
+// rows keep, would be as many products with them again.
+//
 // The weights are laid out once per call, fragment by fragment as a lane reads them, chunk
 // after chunk; the wavefronts of a workgroup share the chunk in LDS, copied there without
 // registers while the chunk before it is multiplied.
 //
 // Bound by the gate's arithmetic: 1M rows of 64-256-64 bfloat16 issue vector instructions in
-// 61% of the SIMDs' cycles, among them an exponential and a reciprocal a hidden value at a
-// quarter of the rate, beside matrix instructions in 34%, with no LDS bank conflicts.
-//   1M rows bfloat16 of 64-256-48, forward: 132 us, 680 TFLOP/s; of 64-256-64: forward 156
-//     (630), backward in one kernel 480 (550, the hidden products included)
-//   300k rows float32 of 59-128-3 (six products a product): 89, 170 and 163 us
+// 60% of the SIMDs' cycles, among them an exponential and a reciprocal a hidden value at a
+// quarter of the rate, beside matrix instructions in 34%, with no LDS bank conflicts; the
+// backward in one kernel in 41% beside 28%, waiting for LDS and its barriers.
+//   1M rows bfloat16 of 64-256-48, forward: 115 us, 780 TFLOP/s; of 64-256-64: forward 135
+//     (730), backward in one kernel 387 (680, the hidden products included)
+//   300k rows float32 of 59-128-3 (six products a product): 78, 143 and 138 us
 #pragma once
 
 #include "gated_ffn.cuh"
@@ -165,98 +171,85 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_fwd_kernel(ForwardArgs
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int TILE = 16 * RT * FR_WAVES;
-  {
-    const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    // this workgroup's chunks
-    const int first = a.chunks * blockIdx.y / gridDim.y;
-    const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
-    const char* packed = a.packed + (int64_t)first * C::KB * 1024;
-    copy_chunk<C::KB, FR_WAVES>(lds, packed);
-    frag_t<E> x[RT][DK][P];
+  const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
+  // this workgroup's chunks
+  const int first = a.chunks * blockIdx.y / gridDim.y;
+  const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
+  const char* packed = a.packed + (int64_t)first * C::KB * 1024;
+  copy_chunk<C::KB, FR_WAVES>(lds, packed);
+  frag_t<E> x[RT][DK][P];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int64_t m = m0 + i * 16;
+#pragma unroll
+    for (int k = 0; k < DK; ++k)
+      load_fragment<T>(a.x + m * a.x_pitch, k * 32 + (lane >> 4) * 8, a.width, m < a.rows, a.wide,
+                       x[i][k]);
+  }
+  f32x4 y[OT][RT] = {};
+  for (int c = 0; c < chunks; ++c) {
+    stage_barrier();  // the chunk is there, and nobody reads the one before it
+    const char* cur = lds + (c & 1) * C::KB * 1024;
+    if (c + 1 < chunks)
+      copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
+                                  packed + (int64_t)(c + 1) * C::KB * 1024);
+    const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
+#pragma unroll
+      for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
+    };
+    const float* bias = (const float*)(cur + (C::KB - 1) * 1024) + (lane >> 4) * 8;
+    frag_t<E> h[RT][P];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 g[RT], u[RT];
+      const f32x4 bg = *(const f32x4*)(bias + t * 4), bu = *(const f32x4*)(bias + 32 + t * 4);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) g[i] = bg, u[i] = bu;
+#pragma unroll
+      for (int k = 0; k < DK; ++k) {
+        frag_t<E> w[P];
+        fragment(t * DK + k, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) g[i] = mfma_planes<T>(w, x[i][k], g[i]);
+        fragment((2 + t) * DK + k, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float v[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) v[r] = activation<ACT, T>(g[i][r]).x * u[i][r];
+        four_t<E> p[P];
+        split4<T>(v, p);
+        set_half<E, P>(h[i], t, p);
+      }
+    }
+    if (P == 1 && (first + c + 1) * 32 > a.hidden)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) keep_hidden<E, P>(h[i], a.hidden - (first + c) * 32);
+#pragma unroll
+    for (int o = 0; o < OT; ++o) {
+      frag_t<E> w[P];
+      fragment(4 * DK + o, w);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) y[o][i] = mfma_planes<T>(w, h[i], y[o][i]);
+    }
+  }
+#pragma unroll
+  for (int o = 0; o < OT; ++o) {
+    const int n = o * 16 + (lane >> 4) * 4;
+    f32x4 bd;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) bd[r] = a.bd && n + r < a.out ? to_f32(a.bd[n + r]) : 0.f;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int64_t m = m0 + i * 16;
-#pragma unroll
-      for (int k = 0; k < DK; ++k)
-        load_fragment<T>(a.x + m * a.x_pitch, k * 32 + (lane >> 4) * 8, a.width, m < a.rows, a.wide,
-                         x[i][k]);
-    }
-    f32x4 y[OT][RT] = {};
-    for (int c = 0; c < chunks; ++c) {
-      stage_barrier();  // the chunk is there, and nobody reads the one before it
-      const char* cur = lds + (c & 1) * C::KB * 1024;
-      if (c + 1 < chunks)
-        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
-                                    packed + (int64_t)(c + 1) * C::KB * 1024);
-      const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
-#pragma unroll
-        for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
-      };
-      const float* bias = (const float*)(cur + (C::KB - 1) * 1024) + (lane >> 4) * 8;
-      frag_t<E> h[RT][P];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x4 g[RT], u[RT];
-        const f32x4 bg = *(const f32x4*)(bias + t * 4), bu = *(const f32x4*)(bias + 32 + t * 4);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) g[i] = bg, u[i] = bu;
-#pragma unroll
-        for (int k = 0; k < DK; ++k) {
-          frag_t<E> w[P];
-          fragment(t * DK + k, w);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) g[i] = mfma_planes<T>(w, x[i][k], g[i]);
-          fragment((2 + t) * DK + k, w);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          float v[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = activation<ACT, T>(g[i][r]).x * u[i][r];
-          four_t<E> p[P];
-          split4<T>(v, p);
-          set_half<E, P>(h[i], t, p);
-        }
-      }
-      if (P == 1 && (first + c + 1) * 32 > a.hidden)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) keep_hidden<E, P>(h[i], a.hidden - (first + c) * 32);
-#pragma unroll
-      for (int o = 0; o < OT; ++o) {
-        frag_t<E> w[P];
-        fragment(4 * DK + o, w);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) y[o][i] = mfma_planes<T>(w, h[i], y[o][i]);
-      }
-    }
-#pragma unroll
-    for (int o = 0; o < OT; ++o) {
-      const int n = o * 16 + (lane >> 4) * 4;
-      float bd[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) bd[r] = a.bd && n + r < a.out ? to_f32(a.bd[n + r]) : 0.f;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const int64_t m = m0 + i * 16;
-        if (m >= a.rows || n >= a.out) continue;
-        if (a.parts) {
-          put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.out + n, y[o][i], a.out - n);
-          continue;
-        }
-        T* at = a.y + m * a.out + n;
-        if (a.wide_out) {
-          four_t<T> v;
-#pragma unroll
-          for (int r = 0; r < 4; ++r) v[r] = from_f32<T>(y[o][i][r] + bd[r]);
-          *(four_t<T>*)at = v;
-        } else {
-#pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (n + r < a.out) at[r] = from_f32<T>(y[o][i][r] + bd[r]);
-        }
-      }
+      if (m >= a.rows || n >= a.out) continue;
+      if (a.parts)
+        put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.out + n, y[o][i], a.out - n);
+      else
+        put_four(a.y + m * a.out + n, y[o][i] + bd, a.out - n, a.wide_out);
     }
   }
 }
@@ -288,115 +281,113 @@ __global__ void __launch_bounds__(64 * FR_WAVES) ffn_rows_dx_kernel(BackwardArgs
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   constexpr int TILE = 16 * RT * FR_WAVES;
-  {
-    const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
-    // this workgroup's chunks
-    const int first = a.chunks * blockIdx.y / gridDim.y;
-    const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
-    const char* packed = a.packed + (int64_t)first * C::KB * 1024;
-    copy_chunk<C::KB, FR_WAVES>(lds, packed);
-    frag_t<E> x[RT][DK][P], dy[RT][OK][P];
+  const int64_t m0 = (int64_t)blockIdx.x * TILE + wave * 16 * RT + (lane & 15);
+  // this workgroup's chunks
+  const int first = a.chunks * blockIdx.y / gridDim.y;
+  const int chunks = a.chunks * (blockIdx.y + 1) / gridDim.y - first;
+  const char* packed = a.packed + (int64_t)first * C::KB * 1024;
+  copy_chunk<C::KB, FR_WAVES>(lds, packed);
+  frag_t<E> x[RT][DK][P], dy[RT][OK][P];
+#pragma unroll
+  for (int i = 0; i < RT; ++i) {
+    const int64_t m = m0 + i * 16;
+    const int c = (lane >> 4) * 8;
+#pragma unroll
+    for (int k = 0; k < DK; ++k)
+      load_fragment<T>(a.x + m * a.x_pitch, k * 32 + c, a.width, m < a.rows, a.wide, x[i][k]);
+#pragma unroll
+    for (int k = 0; k < OK; ++k)
+      load_fragment<T>(a.dy + m * a.dy_pitch, k * 32 + c, a.out, m < a.rows, a.wide_dy, dy[i][k]);
+  }
+  f32x4 dx[DT][RT] = {};
+  Lift lift;
+  if constexpr (LIFTED<T>) lift = *a.lift;
+  for (int c = 0; c < chunks; ++c) {
+    if (BUFFERS == 1 && c) {
+      stage_barrier();
+      copy_chunk<C::KB, FR_WAVES>(lds, packed + (int64_t)c * C::KB * 1024);
+    }
+    stage_barrier();  // the chunk is there, and nobody reads the one before it
+    const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
+    if (BUFFERS == 2 && c + 1 < chunks)
+      copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
+                                  packed + (int64_t)(c + 1) * C::KB * 1024);
+    const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
+#pragma unroll
+      for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
+    };
+    const float* bias = (const float*)(cur + (C::KB - 1) * 1024) + (lane >> 4) * 8;
+    frag_t<E> dg[RT][P], du[RT][P];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      f32x4 g[RT], u[RT], dh[RT] = {};
+      const f32x4 bg = *(const f32x4*)(bias + t * 4), bu = *(const f32x4*)(bias + 32 + t * 4);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) g[i] = bg, u[i] = bu;
+      frag_t<E> w[P];
+#pragma unroll
+      for (int k = 0; k < DK; ++k) {
+        fragment(t * DK + k, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) g[i] = mfma_planes<T>(w, x[i][k], g[i]);
+        fragment((2 + t) * DK + k, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
+      }
+#pragma unroll
+      for (int k = 0; k < OK; ++k) {
+        fragment(4 * DK + t * OK + k, w);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) dh[i] = mfma_planes<T>(w, dy[i][k], dh[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float vg[4], vu[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float2 v = activation<ACT, T>(g[i][r]);
+          float d = dh[i][r];
+          if constexpr (LIFTED<T>) d *= lift.d;
+          vg[r] = d * u[i][r] * v.y;
+          vu[r] = d * v.x;
+        }
+        four_t<E> p[P];
+        split4<T>(vg, p);
+        set_half<E, P>(dg[i], t, p);
+        split4<T>(vu, p);
+        set_half<E, P>(du[i], t, p);
+      }
+    }
+    if (P == 1 && (first + c + 1) * 32 > a.hidden)
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        keep_hidden<E, P>(dg[i], a.hidden - (first + c) * 32);
+        keep_hidden<E, P>(du[i], a.hidden - (first + c) * 32);
+      }
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      frag_t<E> w[P];
+      fragment(4 * DK + 2 * OK + d, w);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, dg[i], dx[d][i]);
+      fragment(4 * DK + 2 * OK + DT + d, w);
+#pragma unroll
+      for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, du[i], dx[d][i]);
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < DT; ++d) {
+    const int n = d * 16 + (lane >> 4) * 4;
 #pragma unroll
     for (int i = 0; i < RT; ++i) {
       const int64_t m = m0 + i * 16;
-      const int c = (lane >> 4) * 8;
-#pragma unroll
-      for (int k = 0; k < DK; ++k)
-        load_fragment<T>(a.x + m * a.x_pitch, k * 32 + c, a.width, m < a.rows, a.wide, x[i][k]);
-#pragma unroll
-      for (int k = 0; k < OK; ++k)
-        load_fragment<T>(a.dy + m * a.dy_pitch, k * 32 + c, a.out, m < a.rows, a.wide_dy, dy[i][k]);
-    }
-    f32x4 dx[DT][RT] = {};
-    Lift lift;
-    if constexpr (LIFTED<T>) lift = *a.lift;
-    for (int c = 0; c < chunks; ++c) {
-      if (BUFFERS == 1 && c) {
-        stage_barrier();
-        copy_chunk<C::KB, FR_WAVES>(lds, packed + (int64_t)c * C::KB * 1024);
+      if (m >= a.rows || n >= a.width) continue;
+      if constexpr (LIFTED<T>) dx[d][i] *= lift.back_d;
+      if (a.parts) {
+        put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.width + n, dx[d][i], a.width - n);
+        continue;
       }
-      stage_barrier();  // the chunk is there, and nobody reads the one before it
-      const char* cur = lds + (BUFFERS == 2 ? (c & 1) * C::KB * 1024 : 0);
-      if (BUFFERS == 2 && c + 1 < chunks)
-        copy_chunk<C::KB, FR_WAVES>(lds + (~c & 1) * C::KB * 1024,
-                                    packed + (int64_t)(c + 1) * C::KB * 1024);
-      const auto fragment = [&](int q, frag_t<E>(&f)[P]) {
-#pragma unroll
-        for (int s = 0; s < P; ++s) f[s] = ((const frag_t<E>*)(cur + (q * P + s) * 1024))[lane];
-      };
-      const float* bias = (const float*)(cur + (C::KB - 1) * 1024) + (lane >> 4) * 8;
-      frag_t<E> dg[RT][P], du[RT][P];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        f32x4 g[RT], u[RT], dh[RT] = {};
-        const f32x4 bg = *(const f32x4*)(bias + t * 4), bu = *(const f32x4*)(bias + 32 + t * 4);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) g[i] = bg, u[i] = bu;
-        frag_t<E> w[P];
-#pragma unroll
-        for (int k = 0; k < DK; ++k) {
-          fragment(t * DK + k, w);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) g[i] = mfma_planes<T>(w, x[i][k], g[i]);
-          fragment((2 + t) * DK + k, w);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) u[i] = mfma_planes<T>(w, x[i][k], u[i]);
-        }
-#pragma unroll
-        for (int k = 0; k < OK; ++k) {
-          fragment(4 * DK + t * OK + k, w);
-#pragma unroll
-          for (int i = 0; i < RT; ++i) dh[i] = mfma_planes<T>(w, dy[i][k], dh[i]);
-        }
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          float vg[4], vu[4];
-#pragma unroll
-          for (int r = 0; r < 4; ++r) {
-            const float2 v = activation<ACT, T>(g[i][r]);
-            float d = dh[i][r];
-            if constexpr (LIFTED<T>) d *= lift.d;
-            vg[r] = d * u[i][r] * v.y;
-            vu[r] = d * v.x;
-          }
-          four_t<E> p[P];
-          split4<T>(vg, p);
-          set_half<E, P>(dg[i], t, p);
-          split4<T>(vu, p);
-          set_half<E, P>(du[i], t, p);
-        }
-      }
-      if (P == 1 && (first + c + 1) * 32 > a.hidden)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) {
-          keep_hidden<E, P>(dg[i], a.hidden - (first + c) * 32);
-          keep_hidden<E, P>(du[i], a.hidden - (first + c) * 32);
-        }
-#pragma unroll
-      for (int d = 0; d < DT; ++d) {
-        frag_t<E> w[P];
-        fragment(4 * DK + 2 * OK + d, w);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, dg[i], dx[d][i]);
-        fragment(4 * DK + 2 * OK + DT + d, w);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) dx[d][i] = mfma_planes<T>(w, du[i], dx[d][i]);
-      }
-    }
-#pragma unroll
-    for (int d = 0; d < DT; ++d) {
-      const int n = d * 16 + (lane >> 4) * 4;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        const int64_t m = m0 + i * 16;
-        if (m >= a.rows || n >= a.width) continue;
-        if constexpr (LIFTED<T>) dx[d][i] *= lift.back_d;
-        if (a.parts) {
-          put_part(a.parts + ((int64_t)blockIdx.y * a.rows + m) * a.width + n, dx[d][i], a.width - n);
-          continue;
-        }
-        put_four(a.dx + m * a.width + n, dx[d][i], a.width - n, a.wide_dx);
-      }
+      put_four(a.dx + m * a.width + n, dx[d][i], a.width - n, a.wide_dx);
     }
   }
 }
@@ -944,8 +935,9 @@ void RowKernels<T>::backward(const FfnCall& c, void* workspace, hipStream_t stre
     if (LIFTED<T>) ffn_lift(c, p.lift, p.peaks, stream);
     // dx with the weights' gradients where a workgroup of four or eight wavefronts has all hidden
     // columns (with one or two, most of its wavefronts would have none).  bfloat16, against two
-    // kernels: 1M rows of 64-256-64 455 and 555 us, 64-128-64 280 and 315; 500k of 32-256-32
-    // 157 and 195, 64-192-64 239 and 253, 64-160-64 232 and 235
+    // kernels, with the weights' layout and the joins: 1M rows of 64-256-64 407 and 503 us,
+    // 64-128-64 264 and 300; 500k of 32-256-32 147 and 178, 64-192-64 227 and 240, 64-160-64 218
+    // and 218, 64-100-64 152 and 160
     constexpr bool ALONGSIDE = RowPlan<T, DK, OK>::FT == 2;
     const bool alongside = ALONGSIDE && c.dx && weights && p.columns == 1 && p.waves > 2;
     if (c.dx) {

@@ -12,9 +12,11 @@
 // rows of its wavefront, the workgroup joins its wavefronts through LDS into one
 // partial row, and a second launch adds the partial rows, all in a fixed order.
 //
-// 4M rows of 64 bfloat16: forward 177 us (5.8 TB/s), backward 311 (4.9 TB/s) and 8 for the
-// join; 300k rows of 59 float32 at a pitch of 64, read value by value: 24, 45 and 5 us (6.0
-// and 4.7 TB/s); 8191 rows of 1024 halves: 9, 14 and 4 us.
+// 4M rows of 64 bfloat16: forward 179 us (5.7 TB/s), backward 309 (5.0 TB/s) and 7 for the
+// join; 300k rows of 59 float32 at a pitch of 64, read value by value: 24, 44 and 5 us (6.0
+// and 4.8 TB/s); 8191 rows of 1024 halves: 9, 14 and 4 us.  Rows that a workgroup reads again for
+// each sum: 4000 of 5000 bfloat16 52, 432 and 9 us (its partial row is read and written for
+// every row), 4000 of 2501 float32 26, 195 and 6.
 #include "decoder_common.cuh"
 
 // How LANES lanes hold a row of up to LANES * E values.  VEC: lane l has runs of 16

@@ -5,11 +5,12 @@ TideGS itself stores SH coefficients with every Gaussian; these are what a small
 network needs that computes colours (or corrections of them) from features
 stored there and from an embedding of the image.  Inputs are float32, bfloat16 or
 float16 GPU tensors of ``[..., width]``; sums are taken in 32 bits or more and a
-result is rounded once, to its tensor's type.  A tensor whose last dimension is dense and
-whose rows lie at one pitch (columns of a resident table) is read in place by
-``layer_norm`` and ``gated_ffn``; any other is copied first.  Every call runs on
-the current stream, takes its workspaces from torch's allocator and gives the
-same bits for the same inputs.
+result is rounded once, to its tensor's type.  A dense tensor, or a matrix of dense
+rows at one pitch (columns of a resident table), is read in place by ``layer_norm``
+and ``gated_ffn``, a dense one by ``dropout``; any other is copied first.  Every call
+runs on the current stream, takes its workspaces from torch's allocator and gives the
+same bits for the same inputs.  Gradients are taken in reverse mode, once: a tangent of
+forward mode or a second derivative raises.
 """
 from __future__ import annotations
 
@@ -280,7 +281,8 @@ def gated_ffn(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor,
     Differentiable in every tensor; the backward computes the hidden values
     again.  The hidden product and its gradients are rounded to the tensors'
     type between the matrix products, as a stored hidden tensor would be
-    (float32 tensors are not, nor is the hidden product of up to 32 rows).  Half
+    (float32 tensors are not, nor is the hidden product of up to 32 rows: a row's last
+    bits depend on which side of 32 its call is).  Half
     precision's backward scales them to the type's range first, by powers of two, so
     that sums over rows of gradients below its smallest values come out; a hidden
     product past 65504, or a gradient of one, is infinite there.  A row's infinities
