@@ -841,7 +841,9 @@ int tgs_gated_ffn_fwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t o
                       const void* b_down, void* y, void* workspace, uint64_t workspace_bytes,
                       tgs_stream_t stream);
 /* Its gradients, each nullable, of the shapes of what they are gradients of (dx
- * dense).  g = x Wg' + bg and u = x Wu' + bu are computed again. */
+ * dense).  g = x Wg' + bg and u = x Wu' + bu are computed again.  TGS_F16: what is
+ * summed over rows is scaled by powers of two before it is rounded to half, by the
+ * largest magnitudes of the tensors, so sums of terms below 2^-25 come out. */
 uint64_t tgs_gated_ffn_bwd_workspace_size(uint64_t rows, uint32_t width, uint32_t hidden,
                                           uint32_t out, int32_t dtype);
 int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t out, int32_t dtype,
