@@ -853,6 +853,56 @@ int tgs_gated_ffn_bwd(uint64_t rows, uint32_t width, uint32_t hidden, uint32_t o
                       void* dw_down, void* db_gate, void* db_up, void* db_down, void* workspace,
                       uint64_t workspace_bytes, tgs_stream_t stream);
 
+/* ---- steps over many tensors --------------------------------------------- */
+/* AdamW over any number of tensors, 56 of one type a launch:
+ *   g = grad * min(1, max_norm / (*grad_norm + 1e-6))    (grad_norm nullable)
+ *   m = beta1 m + (1 - beta1) g,  v = beta2 v + (1 - beta2) g^2
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * with t the group's step, counted from 1.  state_bits 32:
+ * exp_avg (m) and exp_avg_sq (v) are floats and the scales unused.  8: m is e4m3 to nearest
+ * and v e5m2, rounded stochastically, times a power of two for each 128 values (the scales, [ceil(n /
+ * 128)] floats; a scale brings its block's largest value below 448 or 57344).  Parameters of
+ * 16 bits are rounded stochastically, too: 16 bits of Philox4x32-10 with key `seed` and counter
+ * (i >> 3, step, number), word (i & 7) >> 1, low half first, serve value i of a tensor.
+ * The arrays of tensors and groups are HOST memory, read before the call returns; no two
+ * tensors may overlap.  Pointers need their elements' alignment only. */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;
+  float* exp_avg_sq_scale;
+  uint64_t n;
+  uint32_t number; /* of its stream of draws */
+  uint32_t group;  /* whose hyperparameters it takes */
+  int32_t dtype;   /* the parameter's and the gradient's */
+} tgs_adamw_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+  uint64_t step;          /* 1 .. 2^32 - 1; ignored where step_device is given */
+  const float* lr_device; /* nullable: taken in place of lr (with step_device only) */
+  int64_t* step_device;   /* nullable: advanced by one before it is used, so that a
+                           * captured call counts its replays; every group its own */
+} tgs_adamw_group;
+/* The workspace (16-byte aligned) is needed where steps are counted on the device. */
+uint64_t tgs_adamw_workspace_size(uint32_t n_groups);
+int tgs_adamw(uint32_t n_tensors, const tgs_adamw_tensor* tensors, uint32_t n_groups,
+              const tgs_adamw_group* groups, int32_t state_bits, uint64_t seed,
+              const float* grad_norm, float max_norm, void* workspace, uint64_t workspace_bytes,
+              tgs_stream_t stream);
+
+/* *norm = sqrt of the sum of the squares of all values of all tensors, summed in 64 bits in
+ * a fixed order.  The array of tensors is HOST memory; the workspace starts on 8 bytes. */
+typedef struct {
+  const void* data;
+  uint64_t n;
+  int32_t dtype;
+} tgs_span;
+uint64_t tgs_grad_norm_workspace_size(uint32_t n_tensors);
+int tgs_grad_norm(uint32_t n_tensors, const tgs_span* tensors, float* norm, void* workspace,
+                  uint64_t workspace_bytes, tgs_stream_t stream);
+
 /* ---- on-disk block store (host code, no GPU) ------------------------------ */
 /* Parallel reads of n blocks of the base/patch files (replaces the per-block
  * f.seek + f.read + torch.cat of storage/log_storage_manager.py:208-291 and

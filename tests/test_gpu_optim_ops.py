@@ -1,0 +1,601 @@
+"""AdamW steps over many tensors and the common norm, against their definitions in 64 bits on the
+CPU.
+
+Bounds.  u = 2^-24 is half a step of float32 relative to the value.  m = b1 m + (1 - b1) g: b1 and
+1 - b1 are rounded (u each), so are both products and the sum, and a clipped g carries the clip's u
+and its own: |err m| <= 5 u (|b1 m| + |(1 - b1) g|).  v the same with g twice: 8 u v.  The step
+s m / (sqrt(v) r + eps) has s and r rounded, the root, its product, the sum, the quotient and the
+product: half of v's error, m's, and 8 u of itself; p (1 - lr wd) has the factor's rounding, the
+product's and the difference's: 3 u |p|.  Where a result is then rounded to fewer bits, by a rule
+that is monotonic, it lies between the rule's results for the ends of that interval."""
+import copy
+
+import numpy as np
+import pytest
+import torch
+
+import tidegs_amd as tg
+from tests.gpu_util import announce
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+BLOCK = 128
+F8 = torch.float8_e4m3fn, torch.float8_e5m2
+SIZES = [1, 7, 8, 9, 127, 128, 129, 511, 512, 513, 2047, 2048, 2049, 100_003]
+HYPER = dict(lr=3e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.02)
+
+
+# ---------------------------------------------------------------------------
+# the definition, on the CPU in float64
+# ---------------------------------------------------------------------------
+
+
+def _draws(n, seed, step, number):
+    """16 bits for each value, by Philox4x32-10 in numpy."""
+    low = np.uint64(0xFFFFFFFF)
+    i = np.arange((n + 7) // 8, dtype=np.uint64)
+    c = [i & low, i >> np.uint64(32), np.full_like(i, step), np.full_like(i, number)]
+    k = [np.uint64(seed % (1 << 32)), np.uint64(seed >> 32)]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> np.uint64(32)) ^ c[1] ^ k[0], b & low, (a >> np.uint64(32)) ^ c[3] ^ k[1],
+             a & low]
+        k = [(k[0] + np.uint64(0x9E3779B9)) & low, (k[1] + np.uint64(0xBB67AE85)) & low]
+    words = np.stack(c, 1)
+    halves = np.stack([words & np.uint64(0xFFFF), words >> np.uint64(16)], 2).reshape(-1)[:n]
+    return torch.from_numpy(halves.astype(np.float64))
+
+
+def _spacing(x, lowest, bits):
+    _, e = torch.frexp(x.abs())
+    e = torch.where(x == 0, torch.full_like(e, lowest), e - 1).clamp(min=lowest)
+    return torch.ldexp(torch.ones_like(x), e - bits)
+
+
+def _nearest_e4m3(x):
+    s = _spacing(x, -6, 3)
+    return torch.round(x / s) * s  # (half to even)
+
+
+def _up_e5m2(x, draw):
+    s = _spacing(x, -14, 2)
+    y = torch.floor(x / s + (draw + 0.5) / 65536) * s
+    return torch.where(x > 0, y.clamp(min=2.0 ** -16), torch.zeros_like(y))
+
+
+def _up_16(x, draw, dtype):
+    """Away from zero where the part below the last bit and the draw reach one."""
+    if dtype == torch.bfloat16:
+        s, share = _spacing(x, -126, 7), draw / 65536
+    else:
+        s, share = _spacing(x, -14, 10), torch.floor(draw / 8) / 8192
+    y = torch.sign(x) * torch.floor(x.abs() / s + share) * s
+    return y.to(dtype).double()
+
+
+def _scales(x, top):
+    """By block, of float64 values."""
+    rows = torch.nn.functional.pad(x, (0, -len(x) % BLOCK)).view(-1, BLOCK)
+    most = torch.where(rows.isfinite(), rows.abs(), torch.zeros_like(rows)).amax(1)
+    part, e = torch.frexp(most)
+    e = e - 1 + (part >= 1.7320508 / 2).int()
+    e = torch.where(most > 0, e - top, torch.full_like(e, -120)).clamp(-120, 120)
+    return torch.ldexp(torch.ones_like(most), e)
+
+
+def _by_value(scales, n):
+    return scales.double().repeat_interleave(BLOCK)[:n]
+
+
+class Tensors:
+    """Tensors of the given sizes cut out of flat buffers, ``gap`` values apart (so that they lie on
+    no more than their elements' alignment), with a copy of everything on the CPU."""
+
+    def __init__(self, sizes, dtype, bits, seed=0, gap=1, size=1e-2):
+        g = torch.Generator().manual_seed(seed)
+        self.sizes, self.dtype, self.bits = sizes, dtype, bits
+        total = sum(sizes) + gap * len(sizes) + 1
+
+        def buffers(make, dtype):
+            flat = make(total).to(dtype).cuda()
+            views, at = [], gap
+            for n in sizes:
+                views.append(flat[at:at + n])
+                at += n + gap
+            return flat, views
+
+        def normal(scale):
+            return lambda n: torch.randn(n, generator=g) * scale
+
+        self.flat = {}
+        self.flat["p"], self.p = buffers(normal(0.1), dtype)
+        self.flat["g"], self.g = buffers(normal(size), dtype)
+        m, v = (torch.float32,) * 2 if bits == 32 else F8
+        top = 1.0 if bits == 32 else 100.0
+        self.flat["m"], self.m = buffers(normal(0.3 * (size if bits == 32 else top)), m)
+        self.flat["v"], self.v = buffers(
+            lambda n: (normal(1.0)(n) ** 2 + 1e-3) * (size ** 2 if bits == 32 else top), v)
+        self.ms = self.vs = None
+        if bits == 8:
+            blocks = [-(-n // BLOCK) for n in sizes]
+            self.ms = [torch.exp2(torch.randint(-14, -10, (b,), generator=g).float()).cuda()
+                       for b in blocks]
+            self.vs = [torch.exp2(torch.randint(-24, -18, (b,), generator=g).float()).cuda()
+                       for b in blocks]
+        self.before = {k: t.cpu() for k, t in self.flat.items()}
+        self.start = copy.deepcopy([[t.cpu() for t in x] for x in self._lists()])
+
+    def _lists(self):
+        return [self.p, self.g, self.m, self.v] + ([self.ms, self.vs] if self.bits == 8 else [])
+
+    def step(self, step, seed=0, **other):
+        scales = dict(exp_avg_scales=self.ms, exp_avg_sq_scales=self.vs) if self.bits == 8 else {}
+        tg.adamw_step(self.p, self.g, self.m, self.v, step, **HYPER, seed=seed, **scales, **other)
+
+    def check(self, step, seed=0, clip=1.0, hyper=HYPER, numbers=None):
+        """That the tensors are what one step makes of their start."""
+        (b1, b2), lr, eps = hyper["betas"], hyper["lr"], hyper["eps"]
+        for k, n in enumerate(self.sizes):
+            p, g, m, v = (x[k].double() for x in self.start[:4])
+            if self.bits == 8:
+                m = m * _by_value(self.start[4][k], n)
+                v = v * _by_value(self.start[5][k], n)
+            g = g * clip
+            dm = 5 * U * ((b1 * m).abs() + ((1 - b1) * g).abs()) + 1e-44
+            m = b1 * m + (1 - b1) * g
+            v = b2 * v + (1 - b2) * g * g
+            dv = 8 * U * v + 1e-44
+            s, r = lr / (1 - b1 ** step), 1 / (1 - b2 ** step) ** 0.5
+            denom = v.sqrt() * r + eps
+            move = s * m / denom
+            dp = 3 * U * p.abs() + 12 * U * move.abs() + s * dm / denom
+            p = p * (1 - lr * hyper["weight_decay"]) - move
+            draw = _draws(n, seed, step, k if numbers is None else numbers[k])
+            got = [x[k].cpu().double() for x in (self.p, self.m, self.v)]
+            if self.dtype == torch.float32:
+                _within(got[0], p - dp, p + dp)
+            else:
+                _within(got[0], _up_16(p - dp, draw, self.dtype), _up_16(p + dp, draw, self.dtype))
+            if self.bits == 32:
+                _within(got[1], m - dm, m + dm)
+                _within(got[2], v - dv, v + dv)
+                continue
+            ms, vs = self.ms[k].cpu().double(), self.vs[k].cpu().double()
+            _within(ms, *(_scales(m.abs() + d, 8) for d in (-dm, dm)))
+            _within(vs, *(_scales(v + d, 15) for d in (-dv, dv)))
+            ms, vs = _by_value(ms, n), _by_value(vs, n)
+            _within(got[1], _nearest_e4m3((m - dm) / ms), _nearest_e4m3((m + dm) / ms))
+            _within(got[2], _up_e5m2((v - dv).clamp(min=0) / vs, draw),
+                    _up_e5m2((v + dv) / vs, draw))
+        self.check_gaps()
+
+    def check_gaps(self):
+        """What lies between the tensors is as it was."""
+        for name, views in (("p", self.p), ("m", self.m), ("v", self.v), ("g", [])):
+            mask = torch.ones(self.flat[name].numel(), dtype=torch.bool)
+            for t in views:
+                at = t.storage_offset()
+                mask[at:at + t.numel()] = False
+            now, was = (x.view(torch.uint8).view(len(mask), -1)[mask]
+                        for x in (self.flat[name].cpu(), self.before[name]))
+            assert torch.equal(now, was), name
+
+
+def _within(got, low, high):
+    bad = ~((got >= low) & (got <= high))
+    assert not bad.any(), (int(bad.sum()), got[bad][:4], low[bad][:4], high[bad][:4])
+
+
+# ---------------------------------------------------------------------------
+# adamw_step and grad_norm
+# ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("gap", [1, 8])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_step(gpu, dtype, bits, gap):
+    announce(f"adamw_step {dtype} {bits} gap {gap}")
+    t = Tensors(SIZES, dtype, bits, gap=gap)
+    t.step(17, seed=(5 << 32) + 9)
+    t.check(17, seed=(5 << 32) + 9)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("step", [1, 2, (1 << 32) - 1])
+def test_first_and_last_steps(gpu, step, bits):
+    announce(f"adamw_step number {step}, {bits}")
+    t = Tensors([300, 64], torch.float32, bits, seed=3)
+    t.step(step)
+    t.check(step)
+
+
+def test_from_zero_states(gpu):
+    """Zeros are a start for states and scales of 8 bits."""
+    announce("adamw_step from zeros")
+    t = Tensors([1000, 0, 130], torch.float32, 8, seed=4)
+    for x in t.m + t.v + t.ms + t.vs:
+        x.copy_(torch.zeros_like(x))
+    t.start = [[x.cpu() for x in y] for y in t._lists()]
+    t.before = {k: x.cpu() for k, x in t.flat.items()}
+    t.step(1)
+    t.check(1)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_many_tensors(gpu, bits):
+    """More than a launch takes, empty ones among them."""
+    announce(f"adamw_step of 130 tensors, {bits}")
+    sizes = [(37 * k * k) % 700 for k in range(130)]
+    t = Tensors(sizes, torch.bfloat16, bits, seed=5)
+    t.step(3, seed=1)
+    t.check(3, seed=1)
+
+
+@pytest.mark.parametrize("max_norm", [0.05, 1e3])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipped(gpu, bits, max_norm):
+    announce(f"adamw_step clipped to {max_norm}, {bits}")
+    t = Tensors(SIZES, torch.float32, bits, seed=6)
+    norm = tg.grad_norm(t.g)
+    exact = float(torch.cat([x.cpu().double() for x in t.g]).norm())
+    # its rounding to float32, and sums of at most 4096 terms and joins, in 64 bits
+    assert norm.shape == () and abs(float(norm) - exact) <= exact * (U + 1e-12)
+    t.step(4, grad_norm=norm, max_norm=max_norm)
+    t.check(4, clip=min(1.0, max_norm / (exact + 1e-6)))
+
+
+def test_norm_of_everything(gpu):
+    """Mixed types, empty tensors, 200 of them, other orders and strides, ranges that squares leave."""
+    announce("grad_norm")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    types = [torch.float32, torch.bfloat16, torch.float16]
+    many = [torch.randn((k * k) % 997, generator=g, device=gpu).to(types[k % 3])
+            for k in range(200)]
+    for tensors in (many, many[:1], many[1:2], [torch.randn(3_000_001, generator=g, device=gpu)],
+                    [torch.randn(40, 30, generator=g, device=gpu).t()],
+                    [torch.randn(40, 30, generator=g, device=gpu)[:, ::2]],
+                    [torch.full((5000,), 1e30, device=gpu)],
+                    [torch.full((5000,), 1e-30, device=gpu)], [torch.zeros(0, device=gpu)]):
+        announce(f"grad_norm of {len(tensors)}, first {tuple(tensors[0].shape)}")
+        exact = float(torch.cat([t.cpu().double().reshape(-1) for t in tensors]).norm())
+        got = tg.grad_norm(tensors)
+        assert abs(float(got) - exact) <= exact * (U + 1e-12)
+        assert torch.equal(got, tg.grad_norm(tensors))
+    assert torch.isnan(tg.grad_norm(many + [torch.tensor([float("nan")], device=gpu)]))
+    assert torch.isinf(tg.grad_norm(many + [torch.tensor([-float("inf")], device=gpu)]))
+    assert torch.isinf(tg.grad_norm([torch.full((3,), 3e38, device=gpu)]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_nan_and_infinity_stay_in_their_values(gpu, bits, dtype):
+    announce(f"adamw_step with NaN and infinity, {bits} {dtype}")
+    t = Tensors([400], dtype, bits, seed=7)
+    t.g[0][5], t.g[0][133], t.g[0][399] = float("nan"), float("inf"), -float("inf")
+    bad = torch.zeros(400, dtype=torch.bool)
+    bad[[5, 133, 399]] = True
+    t.step(9)
+    now = [t.p[0].cpu().float(), t.m[0].cpu().float(), t.v[0].cpu().float()]
+    assert torch.isnan(now[0][bad]).all() and not now[1][bad].isfinite().any()
+    assert not now[2][bad].isfinite().any()
+    # the others as if those gradients were zero and their states, which stand in a block, too
+    for x in (now[0], now[1], now[2]):
+        assert x[~bad].isfinite().all()
+    again = Tensors([400], dtype, bits, seed=7)
+    for x, v in ((again.g, 0.0), (again.m, 0.0), (again.v, 0.0)):
+        x[0].copy_(torch.where(bad.cuda(), torch.zeros(400, device=gpu),
+                               x[0].float()).to(x[0].dtype))
+    again.step(9)
+    for a, b in zip((t.p, t.m, t.v), (again.p, again.m, again.v)):
+        assert torch.equal(a[0].float().cpu()[~bad], b[0].float().cpu()[~bad])
+
+
+def test_no_gradients_at_all(gpu):
+    """Zeros stay zeros, a positive second moment never becomes one, scales stay finite."""
+    announce("adamw_step of zeros")
+    t = Tensors([256], torch.float32, 8, seed=8)
+    t.g[0].zero_()
+    first = t.v[0].float().cpu() > 0
+    for k in range(1, 200):
+        t.step(k)
+    assert ((t.v[0].float().cpu() > 0) == first).all()
+    assert torch.isfinite(t.p[0]).all() and torch.isfinite(t.ms[0]).all()
+    for x in (t.m[0], t.v[0]):
+        x.copy_(torch.zeros_like(x))
+    before = t.p[0].clone()
+    t.step(200)
+    assert (t.m[0].float() == 0).all() and (t.v[0].float() == 0).all()
+    want = before.double() * (1 - HYPER["lr"] * HYPER["weight_decay"])
+    assert ((t.p[0].double() - want).abs() <= 3 * U * want.abs()).all()
+
+
+def test_extreme_gradients(gpu):
+    """Blocks of the largest and the smallest values keep finite scales and codes."""
+    announce("adamw_step of extreme gradients")
+    t = Tensors([512], torch.float32, 8, seed=9)
+    for x in t.m + t.v + t.ms + t.vs:
+        x.copy_(torch.zeros_like(x))
+    t.g[0][:128], t.g[0][128:256], t.g[0][256:384] = 1e38, 1e18, 1e-22
+    t.step(1)
+    assert torch.isfinite(t.ms[0]).all() and torch.isfinite(t.vs[0]).all()
+    m = t.m[0].float() * t.ms[0].repeat_interleave(BLOCK)
+    assert torch.isfinite(m).all()
+    assert ((m[:256] / (0.1 * t.g[0][:256]) - 1).abs() <= 2.0 ** -4 * 1.01).all()
+    # (1e38)^2 is past float32: infinite, and the step nothing
+    assert torch.isinf(t.v[0].float()[:128]).all() and torch.isfinite(t.p[0]).all()
+
+
+def test_second_moment_follows_its_average(gpu):
+    """The mean over many values of an 8-bit second moment is that of the exact one: a single value
+    is off by some 25% at random, the mean over 200k of them by 0.06%.  To nearest it would
+    hardly move."""
+    announce("8-bit second moment over 400 steps")
+    n, g = 200_000, torch.Generator(device="cuda").manual_seed(3)
+    p = [torch.zeros(n, device=gpu)]
+    m, v = ([torch.zeros(n, device=gpu).to(d)] for d in F8)
+    ms, vs = ([torch.zeros(-(-n // BLOCK), device=gpu)] for _ in range(2))
+    exact = torch.zeros(n, dtype=torch.float64, device=gpu)
+    for k in range(1, 401):
+        grad = torch.randn(n, generator=g, device=gpu) * (1 if k < 200 else 2)
+        tg.adamw_step(p, [grad], m, v, k, lr=0.0, exp_avg_scales=ms, exp_avg_sq_scales=vs, seed=5)
+        exact = 0.999 * exact + 0.001 * grad.double() ** 2
+    got = v[0].double() * vs[0].double().repeat_interleave(BLOCK)[:n]
+    assert abs(float(got.mean() / exact.mean()) - 1) < 0.005
+    assert float((got / exact - 1).std()) < 0.5
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_16_bit_parameters_move_by_less_than_their_last_bit(gpu, dtype):
+    """100 steps of 1/50 of a last bit move the mean by two of them, as they would in 32 bits: the
+    mean of 100k has a standard deviation below sqrt(100 / 4 / 100k) = 0.016 of a bit."""
+    announce(f"small steps in {dtype}")
+    n, bit = 100_000, torch.finfo(dtype).eps
+    p = [torch.full((n,), 1.5, dtype=dtype, device=gpu)]
+    grad = [torch.ones(n, dtype=dtype, device=gpu)]
+    m, v = ([torch.ones(n, device=gpu)] for _ in range(2))
+    for k in range(1, 101):
+        # (m = v = 1 stay, and their corrections are 1 after so many steps)
+        tg.adamw_step(p, grad, m, v, k + 100_000, lr=bit / 50, eps=0.0, weight_decay=0.0, seed=k)
+    moved = float((1.5 - p[0].double()).mean()) / bit
+    assert abs(moved - 2) < 0.1
+
+
+def test_seeds_steps_and_numbers_draw_apart(gpu):
+    announce("draws of seeds, steps and numbers")
+
+    def result(seed=0, step=5, number=0):
+        g = torch.Generator(device="cuda").manual_seed(1)
+        p, grad = (torch.randn(4096, generator=g, device=gpu).bfloat16() for _ in range(2))
+        p, grad = ([x.clone() for _ in range(number + 1)] for x in (p, grad))
+        m, v = ([torch.zeros(4096, device=gpu) for _ in range(number + 1)] for _ in range(2))
+        tg.adamw_step(p, grad, m, v, step, lr=1e-3, betas=(0.0, 0.0), seed=seed)
+        return p[number]
+
+    base = result()
+    assert torch.equal(base, result())
+    for other in (result(seed=1), result(seed=1 << 32), result(step=6), result(number=1)):
+        assert not torch.equal(base, other)
+
+
+def test_other_orders_and_streams(gpu):
+    """Permuted dense tensors are stepped in place, a gradient of another order is copied; on a
+    stream that is not the default."""
+    announce("adamw_step of permuted tensors on a stream")
+    g = torch.Generator(device="cuda").manual_seed(2)
+    base = [torch.randn(6, 5, 4, generator=g, device=gpu) for _ in range(4)]
+    base[3] = base[3].square()
+    flat = [[x.clone().view(-1)] for x in base]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        p, grad, m, v = (x.clone().permute(2, 0, 1) for x in base)
+        grad = grad.contiguous()  # another order than the parameter's
+        tg.adamw_step([p], [grad], [m], [v], 2, **HYPER)
+    torch.cuda.current_stream().wait_stream(stream)
+    tg.adamw_step(*flat, 2, **HYPER)
+    for a, b in zip((p, m, v), (flat[0], flat[2], flat[3])):
+        assert torch.equal(a.permute(1, 2, 0).reshape(-1), b[0])
+
+
+def test_repeated_tensors_are_refused(gpu):
+    announce("adamw_step: the same tensor twice")
+    p, grad, m, v, w = (torch.zeros(10, device=gpu) for _ in range(5))
+    with pytest.raises(ValueError, match="twice"):
+        tg.adamw_step([p, p], [grad, grad], [m, w], [v, torch.zeros_like(v)], 1, lr=1e-3)
+    with pytest.raises(ValueError, match="twice"):
+        tg.adamw_step([p], [grad], [m], [m], 1, lr=1e-3)
+    with pytest.raises(ValueError, match="grad_norm must"):
+        tg.adamw_step([p], [grad], [m], [v], 1, lr=1e-3, max_norm=1.0,
+                      grad_norm=torch.zeros((), device=gpu, dtype=torch.float64))
+    with pytest.raises(ValueError, match="one device"):
+        tg.adamw_step([p, torch.zeros(3)], [grad, torch.zeros(3)], [m, torch.zeros(3)],
+                      [v, torch.zeros(3)], 1, lr=1e-3)
+
+
+# ---------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------
+
+
+def _network(device, seed=0, dtype=torch.float32):
+    g = torch.Generator().manual_seed(seed)
+    shapes = [(40, 30), (30,), (7,), (3, 5, 2), (1,), (200, 3)]
+    return [(torch.randn(s, generator=g) * 0.3).to(device, dtype).requires_grad_() for s in shapes]
+
+
+def _fill(params, seed, skip=()):
+    g = torch.Generator().manual_seed(seed)
+    for k, p in enumerate(params):
+        grad = torch.randn(p.shape, generator=g)
+        p.grad = None if k in skip else grad.to(p.device, p.dtype)
+
+
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+def test_optimizer_against_torch(gpu, max_norm):
+    """Six steps, two groups, a parameter that is sometimes left out, against torch's AdamW in
+    float64.  By step the moments' errors grow by at most what one step adds: 6 (12 + 5 / (1 - b1))
+    u of a move, and the sum of moves is at most 6 times lr 10; 4 u of the parameter a step."""
+    announce(f"AdamW against torch, max_norm {max_norm}")
+    ours, theirs = _network(gpu), [p.detach().double().requires_grad_() for p in _network("cpu")]
+
+    def groups(p):
+        return [dict(params=p[:3]), dict(params=p[3:], lr=1e-2, betas=(0.8, 0.99),
+                                         weight_decay=0.1)]
+
+    opt, ref = tg.AdamW(groups(ours), lr=2e-3), torch.optim.AdamW(groups(theirs), lr=2e-3)
+    for k in range(6):
+        skip = {1} if k in (0, 3) else {4} if k == 2 else set()
+        _fill(ours, k, skip), _fill(theirs, k, skip)
+        if max_norm:
+            norm = torch.nn.utils.clip_grad_norm_([p for p in theirs if p.grad is not None],
+                                                  max_norm)
+        opt.step(max_norm=max_norm)
+        ref.step()
+        if max_norm:
+            assert abs(float(opt.last_norm) / float(norm) - 1) <= 2 * U + 1e-12
+    for a, b in zip(ours, theirs):
+        far = (a.detach().cpu().double() - b.detach()).abs()
+        assert (far <= 6 * 4 * U * b.abs() + 6 * 62 * U * 1e-2 * 10).all()
+        assert opt.state[a]["step"] == int(ref.state[b]["step"])
+
+
+def test_optimizer_takes_mixed_types_and_many_groups(gpu):
+    """One call for all types and more groups than a launch holds: as each parameter alone."""
+    announce("AdamW of mixed types and seven groups")
+    types = [torch.float32, torch.bfloat16, torch.float16]
+
+    def params():
+        return [p.detach().to(types[k % 3]).requires_grad_()
+                for k, p in enumerate(_network(gpu) + _network(gpu, 1))]
+
+    together = params()
+    opt = tg.AdamW([dict(params=together[2 * k:2 * k + 2], lr=1e-3 * (k + 1)) for k in range(6)])
+    for step in (1, 2):
+        _fill(together, step)
+        opt.step(max_norm=2.0)
+    alone = params()
+    states = [[torch.zeros_like(p, dtype=torch.float32) for _ in range(2)] for p in alone]
+    for step in (1, 2):
+        _fill(alone, step)
+        norm = tg.grad_norm([p.grad for p in alone])
+        for k, (p, s) in enumerate(zip(alone, states)):
+            if p.dtype == torch.float32:
+                tg.adamw_step([p.detach()], [p.grad], [s[0]], [s[1]], step, lr=1e-3 * (k // 2 + 1),
+                              grad_norm=norm, max_norm=2.0)
+    for a, b in zip(together, alone):
+        if a.dtype == torch.float32:
+            assert torch.equal(a, b)
+        else:
+            assert not torch.equal(a.detach(), b.detach())  # (stepped, by draws of its number)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_and_loaded(gpu, dtype, bits):
+    """A loaded optimizer goes on bit by bit, states in their own types."""
+    announce(f"AdamW state dict {dtype} {bits}")
+    a = _network(gpu, dtype=dtype)
+    opt = tg.AdamW(a, state_bits=bits, seed=3)
+    for k in range(3):
+        _fill(a, k)
+        opt.step()
+    saved = copy.deepcopy(opt.state_dict())
+    b = [p.detach().clone().requires_grad_() for p in a]
+    other = tg.AdamW(b, state_bits=bits, seed=3)
+    other.load_state_dict(saved)
+    for o, q in ((opt, a), (other, b)):
+        _fill(q, 9)
+        o.step(max_norm=1.0)
+    for p, q in zip(a, b):
+        assert torch.equal(p, q)
+        for key, t in opt.state[p].items():
+            u = other.state[q][key]
+            same = torch.equal(t.float(), u.float()) and t.dtype == u.dtype \
+                if isinstance(t, torch.Tensor) else t == u
+            assert same, key
+    with pytest.raises(ValueError, match="state_bits"):
+        tg.AdamW(b, state_bits=40 - bits).load_state_dict(saved)
+
+
+def test_stepped_parameters_have_a_new_version(gpu):
+    """A backward through values that a step has replaced is refused."""
+    announce("AdamW: versions")
+    p = torch.ones(4, device=gpu, requires_grad=True)
+    p.grad = torch.ones(4, device=gpu)
+    opt = tg.AdamW([p])
+    loss = (p * p).sum()
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_captured_steps(gpu, bits):
+    """A captured step, clipped, replayed with new gradients and another learning rate: the same
+    bits as the steps one by one, with eager work between the replays."""
+    announce(f"captured AdamW, {bits}")
+
+    def made():
+        params = _network(gpu)
+        lr = torch.tensor(1e-3, device=gpu)
+        groups = [dict(params=params[:2]), dict(params=params[2:], weight_decay=0.1)]
+        opt = tg.AdamW(groups, lr=lr, state_bits=bits, seed=4, capturable=True)
+        return params, lr, opt
+
+    params, lr, opt = made()
+    _fill(params, 0)
+    for p in params:
+        p.grad = p.grad.clone()
+    opt.step(max_norm=0.7)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step(max_norm=0.7)
+    norm = opt.last_norm
+    eager, eager_lr, one = made()
+    _fill(eager, 0)
+    one.step(max_norm=0.7)
+    for k in range(1, 5):
+        lr.fill_(1e-3 / k), eager_lr.fill_(1e-3 / k)
+        _fill(eager, k)
+        for p, q in zip(params, eager):
+            p.grad.copy_(q.grad)
+        one.step(max_norm=0.7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(norm, one.last_norm)
+        for p, q in zip(params, eager):
+            assert torch.equal(p, q), k
+        assert int(opt.state[params[0]]["step"]) == k + 1
+    # the eager form counts on the host: the same steps
+    host = _network(gpu)
+    last = tg.AdamW([dict(params=host[:2]), dict(params=host[2:], weight_decay=0.1)],
+                    state_bits=bits, seed=4)
+    for k in range(5):
+        for group in last.param_groups:
+            group["lr"] = 1e-3 / max(k, 1)
+        _fill(host, k)
+        last.step(max_norm=0.7)
+    # (learning rates in float32 and float64 differ in their last bits)
+    for p, q in zip(params, host):
+        assert float((p - q).detach().abs().max()) <= 1e-6
+    reloaded = tg.AdamW([dict(params=host[:2]), dict(params=host[2:])], state_bits=bits,
+                        capturable=True)
+    reloaded.load_state_dict(last.state_dict())
+    assert int(reloaded.state[host[0]]["step"]) == 5
+    assert reloaded.state[host[0]]["step"] is reloaded.state[host[1]]["step"]
+    assert reloaded.state[host[0]]["step"] is not reloaded.state[host[2]]["step"]
+
+
+def test_captures_that_are_refused(gpu):
+    announce("AdamW: refused captures")
+    params = _network(gpu)
+    _fill(params, 0)
+    for opt, match in ((tg.AdamW(params), "capturable"),
+                       (tg.AdamW(params, capturable=True), "step once")):
+        graph = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match=match):
+            with torch.cuda.graph(graph):
+                opt.step()
+        torch.cuda.synchronize()

@@ -28,6 +28,7 @@ from .gsplat_ops import (
 )
 from .clm_ops import FusedSSIMMap, fused_ssim
 from .decoder_ops import dropout, gated_ffn, layer_norm
+from .optim_ops import AdamW, adamw_step, grad_norm
 from .resident_optim import GPUResidentAdam, GPUResidentSophia
 from .working_set import BlockLayout, ResidentBuffer, ResidentWorkingSet
 
@@ -48,4 +49,7 @@ __all__ = [
     "layer_norm",
     "dropout",
     "gated_ffn",
+    "AdamW",
+    "adamw_step",
+    "grad_norm",
 ]

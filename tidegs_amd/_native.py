@@ -221,6 +221,10 @@ SIGNATURES = {
         ctypes.c_int,
         [U64, U32, U32, U32, I32, I32, P, I64, P, P, P, P, P, P, I64, P, P, P, P, P, P, P, P, U64,
          P]),
+    "tgs_adamw_workspace_size": (U64, [U32]),
+    "tgs_adamw": (ctypes.c_int, [U32, P, U32, P, I32, U64, P, F32, P, U64, P]),
+    "tgs_grad_norm_workspace_size": (U64, [U32]),
+    "tgs_grad_norm": (ctypes.c_int, [U32, P, P, P, U64, P]),
     "tgs_io_read_blocks": (ctypes.c_int, [U32, P, P, P, P, P, U32]),
     "tgs_init_scene_bounds": (ctypes.c_int, [P, U64, P, P, P]),
     "tgs_init_morton_codes": (ctypes.c_int, [P, U64, P, P, P]),

@@ -17,19 +17,7 @@
 // and the generator's arithmetic runs under the loads.  4M rows of 64 bfloat16 with a
 // residual (1.54 GB) take 264 us, 5.8 TB/s; 300k of 59 float32 (142 MB) 26 us, 5.5 TB/s.
 #include "decoder_common.cuh"
-
-__device__ __forceinline__ void philox4x32_10(uint32_t c[4], uint32_t k0, uint32_t k1) {
-#pragma unroll
-  for (int r = 0; r < 10; ++r) {
-    const uint64_t a = (uint64_t)c[0] * 0xD2511F53u, b = (uint64_t)c[2] * 0xCD9E8D57u;
-    c[0] = (uint32_t)(b >> 32) ^ c[1] ^ k0;
-    c[2] = (uint32_t)(a >> 32) ^ c[3] ^ k1;
-    c[1] = (uint32_t)b;
-    c[3] = (uint32_t)a;
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
-  }
-}
+#include "philox.cuh"
 
 // One thread per block of eight values.  VEC: every pointer is 16-byte aligned.
 template <typename T, bool VEC>
@@ -63,7 +51,7 @@ __global__ void __launch_bounds__(256) dropout_kernel(uint64_t n, const T* __res
     T out[8];
 #pragma unroll
     for (int k = 0; k < 8; ++k) {
-      const uint32_t draw = k & 1 ? c[k >> 1] >> 16 : c[k >> 1] & 0xFFFFu;
+      const uint32_t draw = philox_draw16(c, k);
       float v = draw >= threshold ? to_f32(in[k]) * scale : 0.f;
       if (residual) v += to_f32(res[k]);
       out[k] = from_f32<T>(v);
