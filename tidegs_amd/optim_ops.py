@@ -26,7 +26,13 @@ from . import _native as N
 from .decoder_ops import _DTYPES
 
 _BLOCK = 128
+_KEYS = {32: ("exp_avg", "exp_avg_sq"),
+         8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 _STATES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
+
+# (called through map: half the cost of a method of each tensor)
+_data_ptr, _numel, _contiguous = Tensor.data_ptr, Tensor.numel, Tensor.is_contiguous
+_get_device, _same_size = Tensor.get_device, Tensor.is_same_size
 
 
 def _guard(device: torch.device):
@@ -37,14 +43,13 @@ def _guard(device: torch.device):
 
 
 def _on_one_gpu(tensors: Sequence[Tensor], name: str) -> torch.device:
+    indices = set(map(_get_device, tensors))
+    if len(indices) == 1 and indices != {-1}:
+        return tensors[0].device
     devices = {t.device for t in tensors}
     if len(devices) > 1:
         raise ValueError(f"{name} must be on one device, got {sorted(map(str, devices))}")
-    device = devices.pop()
-    if device.type != "cuda":
-        raise RuntimeError(
-            f"{name} must be GPU tensors (the TideGS HIP kernels have no CPU path)")
-    return device
+    raise RuntimeError(f"{name} must be GPU tensors (the TideGS HIP kernels have no CPU path)")
 
 
 # ---------------------------------------------------------------------------
@@ -62,22 +67,23 @@ def grad_norm(tensors: Iterable[Tensor]) -> Tensor:
     tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     if not tensors:
         raise ValueError("grad_norm needs a tensor at least")
-    spans = array.array("Q")
-    kept = []
-    for t in tensors:
-        code = _DTYPES.get(t.dtype)
-        if code is None:
-            raise TypeError(f"tensors must be float32, bfloat16 or float16, got {t.dtype}")
-        if not t.is_contiguous():
-            t = _dense(t)
-            kept.append(t)  # (until the launch)
-        spans.extend((t.data_ptr(), t.numel(), code))
+    n = len(tensors)
+    if not all(map(_contiguous, tensors)):
+        tensors = [t if _is_dense(t) else t.contiguous() for t in tensors]
+    types = [t.dtype for t in tensors]
+    for dtype in set(types):
+        if dtype not in _DTYPES:
+            raise TypeError(f"tensors must be float32, bfloat16 or float16, got {dtype}")
     device = _on_one_gpu(tensors, "tensors")
+    spans = array.array("Q", bytes(24 * n))
+    spans[0::3] = array.array("Q", list(map(_data_ptr, tensors)))
+    spans[1::3] = array.array("Q", list(map(_numel, tensors)))
+    spans[2::3] = array.array("Q", [_DTYPES[dtype] for dtype in types])
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = N.load().tgs_grad_norm_workspace_size(len(tensors))
+    nbytes = N.load().tgs_grad_norm_workspace_size(n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
     with _guard(device):
-        N.call("tgs_grad_norm", len(tensors), spans.buffer_info()[0], norm.data_ptr(),
+        N.call("tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(),
                ws.data_ptr(), nbytes, N.stream_handle(device))
     return norm
 
@@ -92,10 +98,6 @@ def _is_dense(t: Tensor) -> bool:
             return False
         expected *= size
     return True
-
-
-def _dense(t: Tensor) -> Tensor:
-    return t if _is_dense(t) else t.contiguous()
 
 
 # ---------------------------------------------------------------------------
@@ -121,25 +123,23 @@ def _check_seed(seed: int) -> int:
 
 
 class _Call:
-    """The arguments of one ``tgs_adamw``: tensors one by one, checked, and their groups."""
+    """The arguments of one ``tgs_adamw``: tensors, checked, and their groups."""
 
     def __init__(self, bits: int):
         self.bits = bits
-        self.tensors = array.array("Q")
-        self.groups = bytearray()
-        self.count = self.n_groups = 0
-        self.params, self.written, self.kept = [], [], []
+        self.groups = array.array("d")
+        self.n_groups = 0
 
     def group(self, lr, betas, eps, weight_decay, step=0, lr_device=None, step_device=None) -> int:
-        self.groups += array.array("d", (lr, betas[0], betas[1], eps, weight_decay)).tobytes()
-        self.groups += array.array("Q", (step, N.ptr(lr_device) or 0,
-                                         N.ptr(step_device) or 0)).tobytes()
+        self.groups.extend((lr, betas[0], betas[1], eps, weight_decay))
+        words = (step, N.ptr(lr_device) or 0, N.ptr(step_device) or 0)
+        self.groups.frombytes(array.array("Q", words).tobytes())
         self.n_groups += 1
         return self.n_groups - 1
 
-    def add(self, p, g, m, v, m_scale, v_scale, number, group) -> None:
-        code = _DTYPES.get(p.dtype)
-        if code is None:
+    def check(self, p, g, m, v, m_scale, v_scale):
+        """One parameter's tensors; the gradient as it is read."""
+        if p.dtype not in _DTYPES:
             raise TypeError(f"parameters must be float32, bfloat16 or float16, got {p.dtype}")
         shape, device = p.shape, p.device
         if g.layout is not torch.strided:
@@ -153,53 +153,73 @@ class _Call:
             if t.shape != shape or t.dtype != dtype or t.device != device:
                 raise ValueError(f"{name} must have its parameter's shape and device and be {dtype}, "
                                  f"got {tuple(t.shape)}, {t.dtype}, {t.device}")
-        if not (p.is_contiguous() and m.is_contiguous() and v.is_contiguous()):
-            if not (_is_dense(p) and m.stride() == p.stride() and v.stride() == p.stride()):
-                raise ValueError("parameters and states must be dense, in one order of their "
-                                 "values")
-            if g.stride() != p.stride():
-                g = torch.empty_like(p).copy_(g)
-                self.kept.append(g)
-        elif not g.is_contiguous():
-            g = g.contiguous()
-            self.kept.append(g)
-        n = p.numel()
-        scales = 0, 0
         if self.bits == 8:
-            blocks = (n + _BLOCK - 1) // _BLOCK
+            blocks = (p.numel() + _BLOCK - 1) // _BLOCK
             for t, name in ((m_scale, "exp_avg_scale"), (v_scale, "exp_avg_sq_scale")):
                 if t.shape != (blocks,) or t.dtype != torch.float32 or t.device != device \
                         or not t.is_contiguous():
                     raise ValueError(f"{name} must hold {blocks} float32 values on {device}, one "
                                      f"for each {_BLOCK}")
-            scales = m_scale.data_ptr(), v_scale.data_ptr()
-        at = p.data_ptr(), m.data_ptr(), v.data_ptr()
-        if n:
-            self.written.extend(at if self.bits == 32 else at + scales)
-        self.params.append(p)
-        self.tensors.extend((at[0], g.data_ptr(), at[1], at[2], *scales, n, number | group << 32,
-                             code))
-        self.count += 1
+        if p.is_contiguous() and m.is_contiguous() and v.is_contiguous():
+            return g.contiguous()
+        if not (_is_dense(p) and m.stride() == p.stride() and v.stride() == p.stride()):
+            raise ValueError("parameters and states must be dense, in one order of their values")
+        return g if g.stride() == p.stride() else torch.empty_like(p).copy_(g)
 
-    def run(self, seed: int, norm: Optional[Tensor], max_norm: float, live: bool) -> None:
-        if not self.count:
+    def plain(self, params, grads, states) -> bool:
+        """Whether all tensors are what most are: contiguous and of fitting types and sizes,
+        asked for all of them at once (one by one they cost three times as much)."""
+        every = list(itertools.chain(params, grads, *states))
+        indices = set(map(_get_device, every))
+        if len(indices) != 1 or -1 in indices or not all(map(_contiguous, every)):
+            return False
+        types = [p.dtype for p in params]
+        if types != [g.dtype for g in grads] or not _DTYPES.keys() >= set(types):
+            return False
+        for t, dtype in zip(states, _STATES[self.bits] + (torch.float32,) * 2):
+            if {x.dtype for x in t} != {dtype}:
+                return False
+        sizes = list(map(_numel, params))
+        if self.bits == 8:
+            blocks = [(n + _BLOCK - 1) // _BLOCK for n in sizes]
+            if any(list(map(_numel, t)) != blocks or {x.dim() for x in t} != {1}
+                   for t in states[2:]):
+                return False
+        return all(all(map(_same_size, params, t)) for t in (grads, *states[:2]))
+
+    def run(self, params, grads, states, numbers, of, seed, norm, max_norm, live=False) -> None:
+        """``states``: exp_avgs, exp_avg_sqs and, of 8 bits, both lists of scales; ``of``: the
+        group of each parameter."""
+        n = len(params)
+        if not n:
             return
-        device = _on_one_gpu(self.params, "parameters")
-        if len(set(self.written)) != len(self.written):
-            raise ValueError("a parameter or a state is there twice")
+        if not self.plain(params, grads, states):
+            none = (itertools.repeat(None),) * (4 - len(states))
+            grads = [self.check(*t) for t in zip(params, grads, *states, *none)]
+        device = _on_one_gpu(params[:1] if n == 1 else params, "parameters")
         if norm is not None and (norm.numel() != 1 or norm.dtype != torch.float32
                                  or norm.device != device):
             raise ValueError("grad_norm must be one float32 value on the parameters' device")
+        sizes = list(map(_numel, params))
+        columns = [list(map(_data_ptr, t)) for t in (params, grads, *states)]
+        written = [a for k, t in enumerate(columns) if k != 1 for a in t if a]
+        if len(set(written)) != len(written):
+            raise ValueError("a parameter or a state is there twice")
+        tensors = array.array("Q", bytes(72 * n))
+        for k, column in enumerate(columns):
+            tensors[k::9] = array.array("Q", column)
+        tensors[6::9] = array.array("Q", sizes)
+        tensors[7::9] = array.array("Q", [a | b << 32 for a, b in zip(numbers, of)])
+        tensors[8::9] = array.array("Q", [_DTYPES[p.dtype] for p in params])
         ws, nbytes = None, 0
         if live:
             nbytes = N.load().tgs_adamw_workspace_size(self.n_groups)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        groups = array.array("Q", bytes(self.groups))
         with _guard(device):
-            N.call("tgs_adamw", self.count, self.tensors.buffer_info()[0], self.n_groups,
-                   groups.buffer_info()[0], self.bits, seed, N.ptr(norm), max_norm, N.ptr(ws),
-                   nbytes, N.stream_handle(device))
-        increment_version(self.params)
+            N.call("tgs_adamw", n, tensors.buffer_info()[0], self.n_groups,
+                   self.groups.buffer_info()[0], self.bits, seed, N.ptr(norm), max_norm,
+                   N.ptr(ws), nbytes, N.stream_handle(device))
+        increment_version(params)
 
 
 def _check_max_norm(max_norm) -> float:
@@ -244,11 +264,9 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
         raise ValueError("grad_norm and max_norm go together")
     max_norm = 0.0 if max_norm is None else _check_max_norm(max_norm)
     call = _Call(bits)
-    group = call.group(lr, betas, eps, weight_decay, step)
-    none = itertools.repeat(None)
-    for number, tensors in enumerate(zip(*lists, *([none, none] if bits == 32 else []))):
-        call.add(*tensors, number, group)
-    call.run(_check_seed(seed), grad_norm, max_norm, False)
+    call.group(lr, betas, eps, weight_decay, step)
+    n = len(params)
+    call.run(*lists[:2], lists[2:], range(n), [0] * n, _check_seed(seed), grad_norm, max_norm)
 
 
 # ---------------------------------------------------------------------------
@@ -330,7 +348,7 @@ class AdamW(torch.optim.Optimizer):
         if capturing and not self.capturable:
             raise RuntimeError("a captured step needs capturable=True: its count of steps would "
                                "stand still")
-        call, grads, stepped, number = _Call(self.state_bits), [], [], 0
+        call, params, stepped, numbers, groups, number = _Call(self.state_bits), [], [], [], [], 0
         for group in self.param_groups:
             lr, lr_device = self._lr(group)
             of = {}  # the call's group by count of steps
@@ -348,15 +366,17 @@ class AdamW(torch.optim.Optimizer):
                     of[key] = call.group(
                         lr, group["betas"], group["eps"], group["weight_decay"],
                         0 if self.capturable else key + 1, lr_device, count)
-                call.add(p, p.grad, state["exp_avg"], state["exp_avg_sq"],
-                         state.get("exp_avg_scale"), state.get("exp_avg_sq_scale"), number - 1,
-                         of[key])
-                grads.append(p.grad)
+                params.append(p)
                 stepped.append(state)
-        if not stepped:
+                numbers.append(number - 1)
+                groups.append(of[key])
+        if not params:
             return loss
+        grads = [p.grad for p in params]
+        states = [[state[key] for state in stepped] for key in _KEYS[self.state_bits]]
         self.last_norm = grad_norm(grads) if max_norm is not None else None
-        call.run(self.seed, self.last_norm, max_norm or 0.0, self.capturable)
+        call.run(params, grads, states, numbers, groups, self.seed, self.last_norm,
+                 max_norm or 0.0, self.capturable)
         if not self.capturable:
             for state in stepped:
                 state["step"] += 1
