@@ -473,7 +473,8 @@ extern "C" int tgs_adamw(uint32_t n_tensors, const tgs_adamw_tensor* tensors, ui
 
 #define NORM_TENSORS 64
 #define NORM_CHUNK 8192
-#define NORM_PARTS 2048  // workgroups of all launches
+#define NORM_PARTS 2048  // workgroups of a launch
+#define NORM_SINGLE 8    // chunks that one workgroup sums alone
 
 struct NormBatch {
   uint32_t count;
@@ -502,8 +503,10 @@ __device__ __forceinline__ double group_sum64(double v) {
   return sum;
 }
 
+// One workgroup writes the norm itself.
 template <typename T>
-__global__ void __launch_bounds__(256) norm_kernel(NormBatch b, double* __restrict__ parts) {
+__global__ void __launch_bounds__(256) norm_kernel(NormBatch b, double* __restrict__ parts,
+                                                   float* __restrict__ norm) {
   double sum = 0;
   for (uint32_t chunk = blockIdx.x; chunk < b.first[b.count]; chunk += gridDim.x) {
     const uint32_t k = tensor_of(b, chunk);
@@ -528,7 +531,11 @@ __global__ void __launch_bounds__(256) norm_kernel(NormBatch b, double* __restri
       }
   }
   sum = group_sum64<4>(sum);
-  if (threadIdx.x == 0) parts[blockIdx.x] = sum;
+  if (threadIdx.x != 0) return;
+  if (norm)
+    *norm = (float)sqrt(sum);
+  else
+    parts[blockIdx.x] = sum;
 }
 
 __global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t count,
@@ -543,15 +550,15 @@ __global__ void __launch_bounds__(1024) norm_join_kernel(uint32_t count,
 // Launches over the tensors of one type; returns the number of workgroups.
 template <typename T>
 static uint32_t norm_launches(uint32_t n_tensors, const tgs_span* tensors, int32_t dtype,
-                              double* parts, hipStream_t stream) {
+                              double* parts, float* norm, hipStream_t stream) {
   uint32_t groups = 0;
   NormBatch b = {};
   uint64_t chunks = 0;
   const auto flush = [&] {
     if (!b.count) return;
     b.first[b.count] = (uint32_t)chunks;
-    const uint32_t grid = (uint32_t)std::min<uint64_t>(chunks, NORM_PARTS);
-    hipLaunchKernelGGL(norm_kernel<T>, dim3(grid), dim3(256), 0, stream, b, parts + groups);
+    const uint32_t grid = norm ? 1 : (uint32_t)std::min<uint64_t>(chunks, NORM_PARTS);
+    hipLaunchKernelGGL(norm_kernel<T>, dim3(grid), dim3(256), 0, stream, b, parts + groups, norm);
     groups += grid;
     b.count = 0;
     chunks = 0;
@@ -591,12 +598,22 @@ extern "C" int tgs_grad_norm(uint32_t n_tensors, const tgs_span* tensors, float*
   TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 8 == 0,
                 "tgs_grad_norm: the workspace starts on 8 bytes");
   double* parts = (double*)workspace;
+  // A few values of one type: one workgroup, one launch.
+  uint64_t total = 0;
+  bool single = n_tensors > 0 && n_tensors <= NORM_TENSORS;
+  for (uint32_t k = 0; k < n_tensors; ++k) {
+    total += (tensors[k].n + NORM_CHUNK - 1) / NORM_CHUNK;
+    single &= tensors[k].dtype == tensors[0].dtype;
+  }
+  single &= total > 0 && total <= NORM_SINGLE;
   uint32_t count = 0;
   for (int32_t dtype = TGS_F32; dtype <= TGS_F16; ++dtype)
     with_dtype(dtype, "tgs_grad_norm", [&](auto tag) {
-      count += norm_launches<decltype(tag)>(n_tensors, tensors, dtype, parts + count, stream);
+      count += norm_launches<decltype(tag)>(n_tensors, tensors, dtype, parts + count,
+                                            single ? norm : nullptr, stream);
       return TGS_OK;
     });
+  if (single) TGS_RETURN_LAUNCH("tgs_grad_norm");
   hipLaunchKernelGGL(norm_join_kernel, dim3(1), dim3(1024), 0, stream, count, parts, norm);
   TGS_RETURN_LAUNCH("tgs_grad_norm");
 }

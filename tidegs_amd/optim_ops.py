@@ -15,7 +15,7 @@ from __future__ import annotations
 import array
 import itertools
 import math
-from contextlib import nullcontext
+import struct
 from typing import Iterable, Optional, Sequence, Tuple
 
 import torch
@@ -23,7 +23,7 @@ from torch import Tensor
 from torch.autograd.graph import increment_version
 
 from . import _native as N
-from .decoder_ops import _DTYPES
+from .decoder_ops import _DTYPES, _workspace_size
 
 _BLOCK = 128
 _KEYS = {32: ("exp_avg", "exp_avg_sq"),
@@ -35,11 +35,23 @@ _data_ptr, _numel, _contiguous = Tensor.data_ptr, Tensor.numel, Tensor.is_contig
 _get_device, _same_size = Tensor.get_device, Tensor.is_same_size
 
 
-def _guard(device: torch.device):
-    """Makes ``device`` the current one for a launch, where it is not."""
-    if device.index == torch.cuda.current_device():
-        return nullcontext()
-    return torch.cuda.device(device)
+def _launch(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point on ``device``'s current stream, with it as the current device."""
+    if device.index == torch._C._cuda_getDevice():
+        N.call(name, *args, N.stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            N.call(name, *args, N.stream_handle(device))
+
+
+def _rows_of(columns: Sequence[Sequence[int]], n: int) -> array.array:
+    """The columns' values row by row.  Few rows go through a list: 2.3 us in place of 4.7 for one,
+    8 in place of 11 for 17; 74 in place of 46 for 200."""
+    k = len(columns)
+    rows = [0] * (k * n) if n < 32 else array.array("Q", bytes(8 * k * n))
+    for i, column in enumerate(columns):
+        rows[i::k] = column if n < 32 else array.array("Q", column)
+    return array.array("Q", rows) if n < 32 else rows
 
 
 def _on_one_gpu(tensors: Sequence[Tensor], name: str) -> torch.device:
@@ -75,16 +87,13 @@ def grad_norm(tensors: Iterable[Tensor]) -> Tensor:
         if dtype not in _DTYPES:
             raise TypeError(f"tensors must be float32, bfloat16 or float16, got {dtype}")
     device = _on_one_gpu(tensors, "tensors")
-    spans = array.array("Q", bytes(24 * n))
-    spans[0::3] = array.array("Q", list(map(_data_ptr, tensors)))
-    spans[1::3] = array.array("Q", list(map(_numel, tensors)))
-    spans[2::3] = array.array("Q", [_DTYPES[dtype] for dtype in types])
+    spans = _rows_of((list(map(_data_ptr, tensors)), list(map(_numel, tensors)),
+                      [_DTYPES[dtype] for dtype in types]), n)
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = N.load().tgs_grad_norm_workspace_size(n)
+    nbytes = _workspace_size("tgs_grad_norm_workspace_size", n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    with _guard(device):
-        N.call("tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(),
-               ws.data_ptr(), nbytes, N.stream_handle(device))
+    _launch(device, "tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(), ws.data_ptr(),
+            nbytes)
     return norm
 
 
@@ -122,18 +131,20 @@ def _check_seed(seed: int) -> int:
     return int(seed)
 
 
+_GROUP = struct.Struct("5d3Q")  # tgs_adamw_group
+
+
 class _Call:
     """The arguments of one ``tgs_adamw``: tensors, checked, and their groups."""
 
     def __init__(self, bits: int):
         self.bits = bits
-        self.groups = array.array("d")
+        self.groups = b""
         self.n_groups = 0
 
     def group(self, lr, betas, eps, weight_decay, step=0, lr_device=None, step_device=None) -> int:
-        self.groups.extend((lr, betas[0], betas[1], eps, weight_decay))
-        words = (step, N.ptr(lr_device) or 0, N.ptr(step_device) or 0)
-        self.groups.frombytes(array.array("Q", words).tobytes())
+        self.groups += _GROUP.pack(lr, *betas, eps, weight_decay, step, N.ptr(lr_device) or 0,
+                                   N.ptr(step_device) or 0)
         self.n_groups += 1
         return self.n_groups - 1
 
@@ -168,7 +179,7 @@ class _Call:
 
     def plain(self, params, grads, states) -> bool:
         """Whether all tensors are what most are: contiguous and of fitting types and sizes,
-        asked for all of them at once (one by one they cost three times as much)."""
+        asked for all of them at once (one by one they cost twice as much)."""
         every = list(itertools.chain(params, grads, *states))
         indices = set(map(_get_device, every))
         if len(indices) != 1 or -1 in indices or not all(map(_contiguous, every)):
@@ -185,7 +196,8 @@ class _Call:
             if any(list(map(_numel, t)) != blocks or {x.dim() for x in t} != {1}
                    for t in states[2:]):
                 return False
-        return all(all(map(_same_size, params, t)) for t in (grads, *states[:2]))
+        return all(map(_same_size, params, grads)) \
+            and all(list(map(_numel, t)) == sizes for t in states[:2])
 
     def run(self, params, grads, states, numbers, of, seed, norm, max_norm, live=False) -> None:
         """``states``: exp_avgs, exp_avg_sqs and, of 8 bits, both lists of scales; ``of``: the
@@ -205,20 +217,16 @@ class _Call:
         written = [a for k, t in enumerate(columns) if k != 1 for a in t if a]
         if len(set(written)) != len(written):
             raise ValueError("a parameter or a state is there twice")
-        tensors = array.array("Q", bytes(72 * n))
-        for k, column in enumerate(columns):
-            tensors[k::9] = array.array("Q", column)
-        tensors[6::9] = array.array("Q", sizes)
-        tensors[7::9] = array.array("Q", [a | b << 32 for a, b in zip(numbers, of)])
-        tensors[8::9] = array.array("Q", [_DTYPES[p.dtype] for p in params])
+        if self.bits == 32:
+            columns += [[0] * n] * 2
+        tensors = _rows_of((*columns, sizes, [a | b << 32 for a, b in zip(numbers, of)],
+                            [_DTYPES[p.dtype] for p in params]), n)
         ws, nbytes = None, 0
         if live:
-            nbytes = N.load().tgs_adamw_workspace_size(self.n_groups)
+            nbytes = _workspace_size("tgs_adamw_workspace_size", self.n_groups)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        with _guard(device):
-            N.call("tgs_adamw", n, tensors.buffer_info()[0], self.n_groups,
-                   self.groups.buffer_info()[0], self.bits, seed, N.ptr(norm), max_norm,
-                   N.ptr(ws), nbytes, N.stream_handle(device))
+        _launch(device, "tgs_adamw", n, tensors.buffer_info()[0], self.n_groups, self.groups,
+                self.bits, seed, N.ptr(norm), max_norm, N.ptr(ws), nbytes)
         increment_version(params)
 
 
