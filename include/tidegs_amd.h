@@ -821,6 +821,34 @@ int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, const void*
                        int32_t weight_dtype, float eps, void* dx, void* dweight, void* dbias,
                        void* workspace, uint64_t workspace_bytes, tgs_stream_t stream);
 
+/* Group norm over x [samples, pixels, width], the channels last, with an activation: over all
+ * pixels of a sample and width / groups neighbouring channels,
+ * y = act((x - mean) / sqrt(var + eps) * weight + bias), y dense.  activation: 0 silu, 1 gelu
+ * (with the error function), 2 relu, 3 none.  x_sample and x_pitch: the distances of samples
+ * and of pixels in values.  weight and bias [width] are nullable (1 and 0) and of type
+ * weight_dtype: x's or TGS_F32.  eps lies in 2^-80 .. 2^80.
+ * stats: where its size is not 0, what the forward leaves for the backward (mean and 1 /
+ * sqrt(var + eps) of each sample's group); otherwise nullable, computed again. */
+uint64_t tgs_group_norm_stats_size(uint64_t samples, uint64_t pixels, uint32_t width,
+                                   uint32_t groups, int32_t dtype);
+uint64_t tgs_group_norm_fwd_workspace_size(uint64_t samples, uint64_t pixels, uint32_t width,
+                                           uint32_t groups, int32_t dtype);
+int tgs_group_norm_fwd(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
+                       int32_t dtype, int32_t activation, const void* x, int64_t x_sample,
+                       int64_t x_pitch, const void* weight, const void* bias,
+                       int32_t weight_dtype, float eps, void* y, float* stats, void* workspace,
+                       uint64_t workspace_bytes, tgs_stream_t stream);
+/* Its gradients, each nullable: dx dense, dweight and dbias [width] of weight_dtype.  The
+ * workspace starts on 8 bytes, as the forward's and the stats do. */
+uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t pixels, uint32_t width,
+                                           uint32_t groups, int32_t dtype);
+int tgs_group_norm_bwd(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
+                       int32_t dtype, int32_t activation, const void* x, int64_t x_sample,
+                       int64_t x_pitch, const void* dy, int64_t dy_sample, int64_t dy_pitch,
+                       const void* weight, const void* bias, int32_t weight_dtype, float eps,
+                       const float* stats, void* dx, void* dweight, void* dbias, void* workspace,
+                       uint64_t workspace_bytes, tgs_stream_t stream);
+
 /* Dropout: y[i] = (draw[i] >= threshold ? x[i] * 65536 / (65536 - threshold) : 0)
  * + residual[i] (nullable), threshold <= 65536 in 65536ths.  draw[i]: 16 bits of
  * Philox4x32-10 with key `seed` and counter (i >> 3, offset), word (i & 7) >> 1, low

@@ -11,8 +11,10 @@ Drop-in surfaces (same names and call conventions as the reference):
 * ``ResidentWorkingSet``: GPU materialization and writeback of the resident
   block set (the Triton movers of TideGS's double-buffered working set)
 
-Beside them, for decoders over per-Gaussian features: ``layer_norm``, ``dropout``
-and ``gated_ffn`` (``decoder_ops``).
+Beside them, for decoders over per-Gaussian features and over rendered images of
+them: ``layer_norm``, ``group_norm``, ``dropout`` and ``gated_ffn`` (``decoder_ops``),
+and the optimizer of everything that is not a resident block: ``AdamW``,
+``adamw_step`` and ``grad_norm`` (``optim_ops``).
 
 All compute runs in hand-written HIP kernels in ``libtidegs_amd.so`` behind a
 plain C ABI (``include/tidegs_amd.h``); PyTorch only provides device memory and
@@ -27,7 +29,7 @@ from .gsplat_ops import (
     spherical_harmonics,
 )
 from .clm_ops import FusedSSIMMap, fused_ssim
-from .decoder_ops import dropout, gated_ffn, layer_norm
+from .decoder_ops import dropout, gated_ffn, group_norm, layer_norm
 from .optim_ops import AdamW, adamw_step, grad_norm
 from .resident_optim import GPUResidentAdam, GPUResidentSophia
 from .working_set import BlockLayout, ResidentBuffer, ResidentWorkingSet
@@ -47,6 +49,7 @@ __all__ = [
     "ResidentBuffer",
     "BlockLayout",
     "layer_norm",
+    "group_norm",
     "dropout",
     "gated_ffn",
     "AdamW",

@@ -211,6 +211,16 @@ SIGNATURES = {
     "tgs_layer_norm_bwd_workspace_size": (U64, [U64, U32]),
     "tgs_layer_norm_bwd": (
         ctypes.c_int, [U64, U32, I32, P, I64, P, I64, P, I32, F32, P, P, P, P, U64, P]),
+    "tgs_group_norm_stats_size": (U64, [U64, U64, U32, U32, I32]),
+    "tgs_group_norm_fwd_workspace_size": (U64, [U64, U64, U32, U32, I32]),
+    "tgs_group_norm_fwd": (
+        ctypes.c_int,
+        [U64, U64, U32, U32, I32, I32, P, I64, I64, P, P, I32, F32, P, P, P, U64, P]),
+    "tgs_group_norm_bwd_workspace_size": (U64, [U64, U64, U32, U32, I32]),
+    "tgs_group_norm_bwd": (
+        ctypes.c_int,
+        [U64, U64, U32, U32, I32, I32, P, I64, I64, P, I64, I64, P, P, I32, F32, P, P, P, P, P,
+         U64, P]),
     "tgs_dropout": (ctypes.c_int, [U64, I32, P, P, P, U32, U64, U64, P]),
     "tgs_gated_ffn_fwd_workspace_size": (U64, [U64, U32, U32, U32, I32]),
     "tgs_gated_ffn_fwd": (

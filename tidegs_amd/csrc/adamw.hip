@@ -22,6 +22,7 @@
 // serves both its v and its parameter: each is unbiased, and nothing multiplies their errors.
 #include "decoder_common.cuh"
 #include "philox.cuh"
+#include "vector_io.cuh"
 
 #include <math.h>
 
@@ -73,33 +74,21 @@ __device__ __forceinline__ uint32_t tensor_of(const Batch& b, uint32_t chunk) {
   return __builtin_amdgcn_readfirstlane(__popcll(tgs_ballot(at)) - 1);
 }
 
-// Eight consecutive values, on their elements' alignment alone (tensors may be cut out of a flat
-// buffer anywhere): the memory system takes such loads at any address.
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef u32x4 u32x4_at1 __attribute__((aligned(1)));
-typedef u32x2 u32x2_at1 __attribute__((aligned(1)));
-
+// Eight consecutive values (tensors may be cut out of a flat buffer anywhere); past the end of
+// the tensor zeros, and nothing stored.
 template <typename T>
 struct Eight {
-  static constexpr int WORDS = 8 * sizeof(T) / 4;
   union {
-    uint32_t w[WORDS];
+    uint32_t w[8 * sizeof(T) / 4];
     T v[8];
   };
   template <bool FULL>
   __device__ __forceinline__ void load(const T* p, uint64_t i, uint64_t n) {
     if constexpr (FULL) {
-      if constexpr (WORDS == 2) {
-        *(u32x2*)w = *(const u32x2_at1*)(p + i);
-      } else {
-#pragma unroll
-        for (int k = 0; k < WORDS; k += 4)
-          *(u32x4*)(w + k) = *(const u32x4_at1*)((const uint32_t*)(p + i) + k);
-      }
+      load_bytes<8 * sizeof(T)>(w, p + i);
     } else {
 #pragma unroll
-      for (int k = 0; k < WORDS; ++k) w[k] = 0;
+      for (int k = 0; k < (int)(8 * sizeof(T) / 4); ++k) w[k] = 0;
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (i + k < n) v[k] = p[i + k];
@@ -108,13 +97,7 @@ struct Eight {
   template <bool FULL>
   __device__ __forceinline__ void store(T* p, uint64_t i, uint64_t n) const {
     if constexpr (FULL) {
-      if constexpr (WORDS == 2) {
-        *(u32x2_at1*)(p + i) = *(const u32x2*)w;
-      } else {
-#pragma unroll
-        for (int k = 0; k < WORDS; k += 4)
-          *(u32x4_at1*)((uint32_t*)(p + i) + k) = *(const u32x4*)(w + k);
-      }
+      store_bytes<8 * sizeof(T)>(p + i, w);
     } else {
 #pragma unroll
       for (int k = 0; k < 8; ++k)

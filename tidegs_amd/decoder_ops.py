@@ -1,13 +1,14 @@
-"""Operators of a decoder over per-Gaussian features: ``layer_norm``, ``dropout`` and
-``gated_ffn``, forward and backward in the HIP kernels of ``libtidegs_amd.so``.
+"""Operators of a decoder over per-Gaussian features or rendered images of them:
+``layer_norm``, ``group_norm``, ``dropout`` and ``gated_ffn``, forward and backward in the HIP
+kernels of ``libtidegs_amd.so``.
 
 TideGS itself stores SH coefficients with every Gaussian; these are what a small
 network needs that computes colours (or corrections of them) from features
 stored there and from an embedding of the image.  Inputs are float32, bfloat16 or
 float16 GPU tensors of ``[..., width]``; sums are taken in 32 bits or more and a
 result is rounded once, to its tensor's type.  A dense tensor, or a matrix of dense
-rows at one pitch (columns of a resident table), is read in place by ``layer_norm``
-and ``gated_ffn``, a dense one by ``dropout``; any other is copied first.  Every call
+rows at one pitch (columns of a resident table), is read in place by ``layer_norm``,
+``group_norm`` and ``gated_ffn``, a dense one by ``dropout``; any other is copied first.  Every call
 runs on the current stream, takes its workspaces from torch's allocator and gives the
 same bits for the same inputs.  Gradients are taken in reverse mode, once: a tangent of
 forward mode or a second derivative raises.
@@ -169,6 +170,116 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
     if _recorded(x, weight, bias):
         return _LayerNorm.apply(x, weight, bias, float(eps))
     return _layer_norm_fwd(x, weight, bias, float(eps))[1]
+
+
+# ---------------------------------------------------------------------------
+# group_norm
+# ---------------------------------------------------------------------------
+
+_MIN_EPS, _MAX_EPS = 2.0 ** -80, 2.0 ** 80
+
+
+def _pixels(x: Tensor):
+    """``x`` [samples, ..., width] as samples of pixels: (tensor, distance of samples, distance of
+    pixels), in place where its pixels lie at one pitch."""
+    width = x.shape[-1]
+    if not x.is_contiguous():
+        pitch = inner = 0  # of the pixels, and how many there are in the dimensions so far
+        for size, stride in zip(reversed(x.shape[1:-1]), reversed(x.stride()[1:-1])):
+            if size == 1:
+                continue
+            if not inner:
+                pitch, inner = stride, 1
+            if stride != pitch * inner:
+                pitch = -1
+                break
+            inner *= size
+        if (x.stride(-1) == 1 or width == 1) and (pitch >= width or not inner):
+            return x, x.stride(0), max(pitch, width)
+        x = x.contiguous()
+    return x, x.numel() // x.shape[0] if x.shape[0] else 0, width
+
+
+def _group_norm_fwd(x, groups, weight, bias, eps, act):
+    """(x as it is read, y, what is kept for the backward, the arguments that its call shares)."""
+    x, sample, pitch = _pixels(x)
+    samples, width = x.shape[0], x.shape[-1]
+    pixels = math.prod(x.shape[1:-1])
+    y = x.new_empty(x.shape)
+    code = _DTYPES[x.dtype]
+    w = weight if weight is not None else bias
+    w_code = code if w is None or w.dtype == x.dtype else _DTYPES[w.dtype]
+    sizes = samples, pixels, width, groups, code
+    kept = _workspace_size("tgs_group_norm_stats_size", *sizes)
+    nbytes = _workspace_size("tgs_group_norm_fwd_workspace_size", *sizes)
+    stats = torch.empty(kept, dtype=torch.uint8, device=x.device) if kept else None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
+    N.call("tgs_group_norm_fwd", *sizes, act, x.data_ptr(), sample, pitch, N.ptr(weight),
+           N.ptr(bias), w_code, eps, y.data_ptr(), N.ptr(stats), N.ptr(ws), nbytes,
+           N.stream_handle(x.device))
+    return x, y, stats, (sizes, act, sample, pitch, w_code, eps)
+
+
+class _GroupNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups, weight, bias, eps, act):
+        x, y, stats, ctx.call = _group_norm_fwd(x, groups, weight, bias, eps, act)
+        ctx.save_for_backward(x, weight, bias, stats)
+        return y
+
+    @_once
+    def backward(ctx, dy):
+        x, weight, bias, stats = ctx.saved_tensors
+        sizes, act, sample, pitch, w_code, eps = ctx.call
+        dy, dy_sample, dy_pitch = _pixels(dy)
+        need_x, _, need_w, need_b, _, _ = ctx.needs_input_grad
+        dx = x.new_empty(x.shape) if need_x else None
+        dw = weight.new_empty(weight.shape) if need_w else None
+        db = bias.new_empty(bias.shape) if need_b else None
+        nbytes = _workspace_size("tgs_group_norm_bwd_workspace_size", *sizes)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+        N.call("tgs_group_norm_bwd", *sizes, act, x.data_ptr(), sample, pitch, dy.data_ptr(),
+               dy_sample, dy_pitch, N.ptr(weight), N.ptr(bias), w_code, eps, N.ptr(stats),
+               N.ptr(dx), N.ptr(dw), N.ptr(db), ws.data_ptr(), nbytes, N.stream_handle(x.device))
+        return dx, None, dw, db, None, None
+
+
+def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
+               bias: Optional[Tensor] = None, eps: float = 1e-5,
+               activation: Optional[str] = None) -> Tensor:
+    """``act((x - mean) / sqrt(var + eps) * weight + bias)`` with mean and variance over each
+    sample's groups of channels.
+
+    x [samples, ..., width], channels last, as ``rasterize_to_pixels`` leaves images; a group is
+    width / num_groups neighbouring channels of all of a sample's pixels.  weight and bias
+    [width] of x's type, or both float32, or None; ``activation`` None, "silu", "gelu" (with the
+    error function) or "relu".  Differentiable in all three tensors.  Images whose pixels lie at
+    one pitch (columns of wider rows) are read in place.  A NaN or an infinity makes its
+    sample's group NaN and no other, and so do differences past 1e18, whose squares leave
+    float32.
+    """
+    _dtype(x, "x")
+    act = 3 if activation is None else _ACTIVATIONS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be None or one of {sorted(_ACTIVATIONS)}, "
+                         f"got {activation!r}")
+    if x.dim() < 2 or not 0 < x.shape[-1] <= _MAX_WIDTH:
+        raise ValueError(f"x needs samples and 1..{_MAX_WIDTH} channels, got shape "
+                         f"{tuple(x.shape)}")
+    if num_groups < 1 or x.shape[-1] % num_groups:
+        raise ValueError(f"{x.shape[-1]} channels do not make {num_groups} groups")
+    if not _MIN_EPS <= eps <= _MAX_EPS:
+        raise ValueError(f"eps must lie in {_MIN_EPS:.3g}..{_MAX_EPS:.3g} (squares below leave "
+                         f"float32), got {eps}")
+    _on_gpu(x, "x")
+    shape = x.shape[-1:]
+    weight = _parameter(weight, "weight", shape, x, (torch.float32,))
+    bias = _parameter(bias, "bias", shape, x, (torch.float32,))
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}: one type is needed")
+    if _recorded(x, weight, bias):
+        return _GroupNorm.apply(x, int(num_groups), weight, bias, float(eps), act)
+    return _group_norm_fwd(x, int(num_groups), weight, bias, float(eps), act)[1]
 
 
 # ---------------------------------------------------------------------------
