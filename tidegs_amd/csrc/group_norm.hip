@@ -10,13 +10,14 @@
 //
 // Memory bound.  Two ways, by the size of a group:
 //
-// Held (up to 64 lanes by 8 runs of values): a team of lanes keeps a group in registers, so x
-// is read once and a launch does all.  The backward computes mean and rstd again.
+// Held (up to 8 runs of 16 bytes a lane of up to 64, or of a workgroup's 256): a team of lanes
+// keeps a group in registers, so x is read once and one launch does all.  The backward computes
+// mean and rstd again.
 //
 // Streamed: workgroups take runs of pixels by up to 64 vectors of channels and leave each channel's
-// mean and sum of squared differences (of dz and dz xhat in the backward), a second launch
-// joins them by group, a third reads x again and writes.  The forward keeps mean and rstd for
-// the backward.
+// mean and sum of squared differences (of dz and dz xhat in the backward); they are joined by
+// group, by the workgroups that read x again and write where they are few, by a launch of its
+// own otherwise.  The forward keeps mean and rstd for the backward.
 //
 // Sums of squares are of differences from a value near by (a thread's first one, a mean), and
 // partial ones are joined by their means, so no large mean cancels.  All joins are in a fixed
@@ -27,6 +28,10 @@
 #define ACT_NONE 3
 #define HELD_RUNS 8     // runs of a lane at most
 #define TILE_VECTORS 64  // vectors of channels of a streaming workgroup
+#define JOINED_WIDTH 512     // channels, channels of a group and partial values of a sample that
+#define JOINED_EACH 64       // the workgroups that read them join for themselves, and
+#define JOINED_ENTRIES 8192
+#define JOINED_BELOW (1u << 24)  // values of x up to which that is done
 
 struct GnCall {
   uint64_t samples, pixels;
@@ -75,17 +80,28 @@ __device__ __forceinline__ float column(const void* w, int wide, uint32_t c, flo
   return !w ? other : wide ? ((const float*)w)[c] : to_f32(((const T*)w)[c]);
 }
 
-// Sum over the 2^log lanes of a team.
+// Sum over a team: 2^log lanes of a wavefront, or (WIDE) the workgroup.
+template <bool WIDE>
 __device__ __forceinline__ float team_sum(float v, int log) {
-  for (int k = 0; k < log; ++k) v += __shfl_xor(v, 1 << k, 64);
-  return v;
+  if constexpr (WIDE) {
+    __shared__ float s[4];
+    v = tgs_wave_sum(v);
+    __syncthreads();
+    if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
+    __syncthreads();
+    return (s[0] + s[1]) + (s[2] + s[3]);
+  } else {
+    for (int k = 0; k < log; ++k) v += __shfl_xor(v, 1 << k, 64);
+    return v;
+  }
 }
 
 // ---------------------------------------------------------------------------
 // Held groups.  A team has 2^row_log rows of 2^lane_log lanes (as many as hold a pixel's
 // vectors of the group); teams of a workgroup take neighbouring groups.  A team keeps to one
 // group's channels over all its samples, so weights are read once and the weights' gradients
-// stay in registers.
+// stay in registers.  WIDE: the workgroup is one team, and neighbouring groups, which share cache
+// lines, go to one XCD's workgroups (they are dealt out round robin).
 // ---------------------------------------------------------------------------
 
 struct HeldPlan {
@@ -94,17 +110,19 @@ struct HeldPlan {
   uint32_t rows;     // samples that all teams take at once
   uint32_t grid;
   uint32_t partials;  // rows of the weights' gradients
-  int runs;          // of a lane
+  int runs;           // of a lane
+  bool wide;          // a team is a workgroup
 };
 
-template <typename T, int V, int E, bool BACKWARD>
+template <typename T, int V, int E, bool BACKWARD, bool WIDE>
 __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan plan,
                                                               float* __restrict__ partial) {
   const int lane_log = plan.lane_log, team_log = lane_log + plan.row_log;
   const uint32_t lane = threadIdx.x & ((1u << lane_log) - 1);
   const uint32_t row = (threadIdx.x >> lane_log) & ((1u << plan.row_log) - 1);
   const uint32_t team = threadIdx.x >> team_log;
-  const uint64_t id = (uint64_t)blockIdx.x * plan.teams + team;
+  uint64_t id = (uint64_t)blockIdx.x * plan.teams + team;
+  if (WIDE && gridDim.x % 8 == 0) id = (blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
   const bool works = team < plan.teams && id < (uint64_t)plan.rows * k.groups;
   const uint32_t group = (uint32_t)(id % k.groups);
   const bool live = works && lane * V < k.each;
@@ -138,7 +156,7 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
         sum += xh[e][v];
       }
     }
-    const float mean = team_sum(sum, team_log) * inv;
+    const float mean = team_sum<WIDE>(sum, team_log) * inv;
     float squares = 0.f;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
@@ -149,10 +167,9 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
         squares = fmaf(xh[e][v], xh[e][v], squares);
       }
     }
-    const float rstd = __builtin_amdgcn_rsqf(fmaf(team_sum(squares, team_log), inv, k.eps));
+    const float rstd = __builtin_amdgcn_rsqf(fmaf(team_sum<WIDE>(squares, team_log), inv, k.eps));
     T* y = (T*)k.y + (n * k.pixels) * k.width + c0;
     if constexpr (!BACKWARD) {
-      if (k.stats && lane == 0 && row == 0) k.stats[n * k.groups + group] = {mean, rstd};
       with_act(k.act, [&](auto act) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
@@ -186,8 +203,8 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
         }
       });
       if (k.y) {
-        s1 = team_sum(s1, team_log) * inv;
-        s2 = team_sum(s2, team_log) * inv;
+        s1 = team_sum<WIDE>(s1, team_log) * inv;
+        s2 = team_sum<WIDE>(s2, team_log) * inv;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const uint32_t p = row + ((uint32_t)e << plan.row_log);
@@ -203,39 +220,45 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
   }
   if constexpr (BACKWARD) {
     if (!partial) return;
+    if constexpr (!WIDE) {
 #pragma unroll
-    for (int v = 0; v < V; ++v)
-      for (int j = lane_log; j < team_log; ++j) {
-        dw[v] += __shfl_xor(dw[v], 1 << j, 64);
-        db[v] += __shfl_xor(db[v], 1 << j, 64);
+      for (int v = 0; v < V; ++v)
+        for (int j = lane_log; j < team_log; ++j) {
+          dw[v] += __shfl_xor(dw[v], 1 << j, 64);
+          db[v] += __shfl_xor(db[v], 1 << j, 64);
+        }
+      if (plan.teams < k.groups) {  // no two teams of a workgroup have the same channels
+        if (live && row == 0) {
+          float2* out = (float2*)partial + id / k.groups * k.width + c0;
+#pragma unroll
+          for (int v = 0; v < V; ++v) out[v] = {db[v], dw[v]};
+        }
+        return;
       }
-    if (plan.teams < k.groups) {  // no two teams of a workgroup have the same channels
-      if (live && row == 0) {
-        float* out = partial + id / k.groups * 2 * k.width + c0;
-#pragma unroll
-        for (int v = 0; v < V; ++v) out[v] = dw[v], out[k.width + v] = db[v];
-      }
-      return;
     }
-    __shared__ float s[2][256 * V];
+    __shared__ float2 s[256 * V];
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-      s[0][threadIdx.x * V + v] = dw[v];
-      s[1][threadIdx.x * V + v] = db[v];
-    }
+    for (int v = 0; v < V; ++v) s[threadIdx.x * V + v] = {db[v], dw[v]};
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < 2 * k.width; i += 256) {
-      const uint32_t c = i < k.width ? i : i - k.width;
-      const uint32_t at = (((c / k.each) << team_log) * V) + c % k.each;
-      const float* from = s[i < k.width ? 0 : 1] + at;
-      float a = 0.f;
-      for (uint32_t t = 0; t < plan.teams; t += k.groups) a += from[((uint64_t)t << team_log) * V];
-      partial[(uint64_t)blockIdx.x * 2 * k.width + i] = a;
+    // WIDE: the sum over the team's rows; otherwise over the teams of the same group
+    const uint32_t channels = WIDE ? k.each : k.width, count = WIDE ? 1u << plan.row_log : plan.teams;
+    const uint32_t step = WIDE ? 1 : k.groups, stride = (WIDE ? 1u << lane_log : 1u << team_log) * V;
+    float2* out = (float2*)partial + (WIDE ? id / k.groups * k.width + group * k.each
+                                           : (uint64_t)blockIdx.x * k.width);
+    for (uint32_t c = threadIdx.x; c < channels; c += 256) {
+      const float2* from = s + (WIDE ? c : ((c / k.each) << team_log) * V + c % k.each);
+      float2 a = {0.f, 0.f};
+      for (uint32_t t = 0; t < count; t += step) {
+        const float2 p = from[t * stride];
+        a.x += p.x, a.y += p.y;
+      }
+      out[c] = a;
     }
   }
 }
 
-// dw and db: the partial rows' sums, 8 columns by 128 interleaved runs of rows a workgroup.
+// db and dw, which alternate in the partial rows: the rows' sums, 8 values by 128 interleaved
+// runs of rows a workgroup.
 template <typename W>
 __global__ void __launch_bounds__(1024) group_norm_join_kernel(uint32_t parts, uint32_t width,
                                                                const float* __restrict__ partial,
@@ -254,8 +277,8 @@ __global__ void __launch_bounds__(1024) group_norm_join_kernel(uint32_t parts, u
     if (k < h) s[threadIdx.x] += s[threadIdx.x + 8 * h];
   }
   if (k == 0 && c < 2 * width) {
-    W* out = c < width ? dweight : dbias;
-    if (out) out[c < width ? c : c - width] = from_f32<W>(s[threadIdx.x]);
+    W* out = c % 2 ? dweight : dbias;
+    if (out) out[c / 2] = from_f32<W>(s[threadIdx.x]);
   }
 }
 
@@ -269,6 +292,7 @@ struct StreamPlan {
   uint32_t chunks;          // of a sample's pixels
   uint64_t chunk;           // pixels of one
   uint64_t items;           // samples * tiles * chunks
+  bool joined;              // by the workgroups that read the partial values
 };
 
 struct Item {
@@ -299,6 +323,35 @@ __device__ __forceinline__ uint32_t row_count(uint64_t pixels, uint32_t r, uint3
   return pixels > r ? (uint32_t)((pixels - r + rows - 1) / rows) : 0;
 }
 
+// For every `step`th pixel from p on: U loads on their way before the first is used; past the
+// end the last pixel's, unused (so that the rest of a chunk is not loaded one by one).
+template <typename T, int V, int U, typename L, typename F>
+__device__ __forceinline__ void for_pixels(uint64_t p, uint64_t last, uint32_t step, L&& load,
+                                           F&& use) {
+  for (; p < last; p += U * (uint64_t)step) {
+    Run<T, V> run[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(min(p + u * (uint64_t)step, last - 1), run[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * (uint64_t)step < last) use(p + u * (uint64_t)step, run[u]);
+  }
+}
+
+// The same over pairs of runs.
+template <typename T, int V, int U, typename L, typename F>
+__device__ __forceinline__ void for_pixel_pairs(uint64_t p, uint64_t last, uint32_t step, L&& load,
+                                                F&& use) {
+  for (; p < last; p += U * (uint64_t)step) {
+    Run<T, V> a[U], b[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load(min(p + u * (uint64_t)step, last - 1), a[u], b[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (p + u * (uint64_t)step < last) use(p + u * (uint64_t)step, a[u], b[u]);
+  }
+}
+
 // Each channel's mean and sum of squared differences over a chunk of pixels.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) group_norm_stats_kernel(GnCall k, StreamPlan plan,
@@ -314,16 +367,16 @@ __global__ void __launch_bounds__(256) group_norm_stats_kernel(GnCall k, StreamP
       run.load(x + (int64_t)(it.first + it.row) * k.x_pitch);
 #pragma unroll
       for (int v = 0; v < V; ++v) pivot[v] = to_f32(run.v[v]);
-#pragma unroll 4
-      for (uint64_t p = it.first + it.row + rows; p < it.last; p += rows) {
-        run.load(x + (int64_t)p * k.x_pitch);
+      for_pixels<T, V, 8>(it.first + it.row, it.last, rows, [&](uint64_t p, Run<T, V>& r) {
+        r.load(x + (int64_t)p * k.x_pitch);
+      }, [&](uint64_t, const Run<T, V>& r) {
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float d = to_f32(run.v[v]) - pivot[v];
+          const float d = to_f32(r.v[v]) - pivot[v];
           sum[v] += d;
           squares[v] = fmaf(d, d, squares[v]);
         }
-      }
+      });
     }
     const uint32_t count = row_count(it.last - it.first, it.row, rows);
     const float inv = count ? 1.f / (float)count : 0.f;
@@ -354,52 +407,191 @@ __global__ void __launch_bounds__(256) group_norm_stats_kernel(GnCall k, StreamP
   }
 }
 
+// Pixels of a chunk.
+__device__ __forceinline__ float chunk_pixels(const GnCall& k, const StreamPlan& plan, uint32_t q) {
+  const uint64_t first = q * plan.chunk;
+  return (float)(min(first + plan.chunk, k.pixels) - first);
+}
+
+template <int WAVES>
 __device__ __forceinline__ double sum_of_workgroup(double v, double* s) {
 #pragma unroll
   for (int off = 32; off; off >>= 1) v += __shfl_xor(v, off, 64);
   __syncthreads();
   if (threadIdx.x % 64 == 0) s[threadIdx.x / 64] = v;
   __syncthreads();
-  return (s[0] + s[1]) + (s[2] + s[3]);
+  v = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) v += s[w];
+  return v;
+}
+
+// f(chunk, channel) over a group's partial values: as many threads side by side as there are
+// channels, up to 64, the others on further chunks.
+template <typename F>
+__device__ __forceinline__ void for_entries(const StreamPlan& plan, uint32_t each, F&& f) {
+  const uint32_t across = each < 64 ? each : 64, along = blockDim.x / across;
+  const uint32_t c0 = threadIdx.x % across, q0 = threadIdx.x / across;
+  if (q0 >= along) return;
+  for (uint32_t c = c0; c < each; c += across) {
+#pragma unroll 4
+    for (uint32_t q = q0; q < plan.chunks; q += along) f(q, c);
+  }
 }
 
 // Mean and rstd of each sample's group, a workgroup each, in 64 bits.
-__global__ void __launch_bounds__(256) group_norm_finish_kernel(GnCall k, StreamPlan plan,
-                                                                const float2* __restrict__ partial) {
-  __shared__ double s[4];
+__global__ void __launch_bounds__(1024) group_norm_finish_kernel(GnCall k, StreamPlan plan,
+                                                                 const float2* __restrict__ partial) {
+  __shared__ double s[16];
   for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
     const uint64_t n = i / k.groups;
     const float2* from = partial + n * plan.chunks * k.width + i % k.groups * k.each;
-    const uint64_t entries = (uint64_t)plan.chunks * k.each;
-    const auto entry = [&](uint64_t e) { return from[e / k.each * k.width + e % k.each]; };
-    const auto pixels = [&](uint64_t e) {
-      const uint64_t first = e / k.each * plan.chunk;
-      return (double)(min(first + plan.chunk, k.pixels) - first);
-    };
     const double m = (double)k.pixels * k.each;
-    double a = 0;
-    for (uint64_t e = threadIdx.x; e < entries; e += 256) a += entry(e).x * pixels(e);
-    const double mean = sum_of_workgroup(a, s) / m;
-    double q = 0;
-    for (uint64_t e = threadIdx.x; e < entries; e += 256) {
-      const float2 p = entry(e);
+    double a = 0, q = 0;
+    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
+      a += (double)from[(uint64_t)j * k.width + c].x * chunk_pixels(k, plan, j);
+    });
+    const double mean = sum_of_workgroup<16>(a, s) / m;
+    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
+      const float2 p = from[(uint64_t)j * k.width + c];
       const double d = p.x - mean;
-      q += p.y + pixels(e) * d * d;
-    }
-    q = sum_of_workgroup(q, s) / m;
+      q += p.y + chunk_pixels(k, plan, j) * d * d;
+    });
+    q = sum_of_workgroup<16>(q, s) / m;
     if (threadIdx.x == 0) k.stats[i] = {(float)mean, (float)(1.0 / sqrt(q + (double)k.eps))};
   }
 }
 
-// What a thread needs of its channels.
+// sum(g) / m and sum(g xhat) / m of each sample's group, a workgroup each.
+template <typename T>
+__global__ void __launch_bounds__(1024) group_norm_group_sums_kernel(
+    GnCall k, StreamPlan plan, const float2* __restrict__ partial, float2* __restrict__ sums) {
+  __shared__ double s[16];
+  for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
+    const uint64_t n = i / k.groups;
+    const uint32_t c0 = (uint32_t)(i % k.groups) * k.each;
+    const float2* from = partial + n * plan.chunks * k.width + c0;
+    const double m = (double)k.pixels * k.each;
+    double a = 0, b = 0;
+    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
+      const float2 p = from[(uint64_t)j * k.width + c];
+      const float w = column<T>(k.weight, k.wide_weights, c0 + c, 1.f);
+      a += (double)w * p.x;
+      b += (double)w * p.y;
+    });
+    a = sum_of_workgroup<16>(a, s) / m;
+    b = sum_of_workgroup<16>(b, s) / m;
+    if (threadIdx.x == 0) sums[i] = {(float)a, (float)b};
+  }
+}
+
+// The same two joins by a workgroup of 256 for itself, all groups of a sample at once (their
+// channels are one tile): threads by channel over the chunks, then by channel over its group.
+// s: 2 floats for each of 256 threads or of the channels, whichever are more.
+
+// The sums of entry(q, c) over the chunks q, each channel's in s[c].
+template <typename F>
+__device__ __forceinline__ void sum_by_channel(const GnCall& k, const StreamPlan& plan, float2* s,
+                                               F&& entry) {
+  const uint32_t along = k.width < 256 ? 256 / k.width : 1;  // threads of a channel
+  __syncthreads();
+  for (uint32_t t = threadIdx.x; t < along * k.width; t += 256) {
+    const uint32_t c = t % k.width;
+    float2 a = {0.f, 0.f};
+#pragma unroll 8
+    for (uint32_t q = t / k.width; q < plan.chunks; q += along) {
+      const float2 p = entry(q, c);
+      a.x += p.x, a.y += p.y;
+    }
+    s[t] = a;
+  }
+  __syncthreads();
+  if (along > 1) {
+    float2 a = {0.f, 0.f};
+    if (threadIdx.x < k.width)
+      for (uint32_t j = 0; j < along; ++j) {
+        const float2 p = s[j * k.width + threadIdx.x];
+        a.x += p.x, a.y += p.y;
+      }
+    __syncthreads();
+    if (threadIdx.x < k.width) s[threadIdx.x] = a;
+    __syncthreads();
+  }
+}
+
+// s[group] = f(group), for the at most two groups of a thread; f reads s.
+template <typename F>
+__device__ __forceinline__ void replace_by_group(const GnCall& k, float2* s, F&& f) {
+  float2 a[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (threadIdx.x + 256 * j < k.groups) a[j] = f(threadIdx.x + 256 * j);
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+    if (threadIdx.x + 256 * j < k.groups) s[threadIdx.x + 256 * j] = a[j];
+  __syncthreads();
+}
+
+// s[group] = {mean, rstd}
+__device__ __forceinline__ void join_stats(const GnCall& k, const StreamPlan& plan,
+                                           const float2* partial, uint64_t n, float2* s) {
+  const float2* from = partial + n * plan.chunks * k.width;
+  const float pixels = (float)k.pixels, inv = 1.f / pixels;
+  // differences from the first chunk's mean, near to which the others' are
+  sum_by_channel(k, plan, s, [&](uint32_t q, uint32_t c) {
+    const float2 p = from[q * k.width + c];
+    const float d = p.x - from[c].x, nd = chunk_pixels(k, plan, q) * d;
+    return make_float2(nd, fmaf(nd, d, p.y));
+  });
+  for (uint32_t c = threadIdx.x; c < k.width; c += 256) {
+    const float2 a = s[c];
+    s[c] = {fmaf(a.x, inv, from[c].x), fmaxf(fmaf(-a.x * inv, a.x, a.y), 0.f)};
+  }
+  __syncthreads();
+  replace_by_group(k, s, [&](uint32_t g) {
+    const float2* channel = s + g * k.each;
+    float mean = 0.f, m2 = 0.f;
+    for (uint32_t j = 0; j < k.each; ++j) mean += channel[j].x;
+    mean /= (float)k.each;
+    for (uint32_t j = 0; j < k.each; ++j) {
+      const float d = channel[j].x - mean;
+      m2 += fmaf(pixels * d, d, channel[j].y);
+    }
+    return make_float2(mean, 1.f / sqrtf(fmaf(m2, inv / (float)k.each, k.eps)));
+  });
+}
+
+// s[group] = {sum(g) / m, sum(g xhat) / m}
+template <typename T>
+__device__ __forceinline__ void join_sums(const GnCall& k, const StreamPlan& plan,
+                                          const float2* partial, uint64_t n, float2* s) {
+  const float2* from = partial + n * plan.chunks * k.width;
+  const float inv = 1.f / (float)(k.pixels * k.each);
+  sum_by_channel(k, plan, s, [&](uint32_t q, uint32_t c) {
+    const float w = column<T>(k.weight, k.wide_weights, c, 1.f);
+    const float2 p = from[q * k.width + c];
+    return make_float2(w * p.x, w * p.y);
+  });
+  replace_by_group(k, s, [&](uint32_t g) {
+    float2 a = {0.f, 0.f};
+    for (uint32_t j = 0; j < k.each; ++j) {
+      const float2 p = s[g * k.each + j];
+      a.x += p.x, a.y += p.y;
+    }
+    return make_float2(a.x * inv, a.y * inv);
+  });
+}
+
+// What a thread needs of its channels; `stats` of this sample's groups.
 template <typename T, int V>
 struct Columns {
   float mean[V], rstd[V], w[V], b[V];
-  __device__ __forceinline__ void load(const GnCall& k, const Item& it) {
+  __device__ __forceinline__ void load(const GnCall& k, const Item& it, const float2* stats) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t c = it.column + v;
-      const float2 st = k.stats[it.n * k.groups + c / k.each];
+      const float2 st = stats[c / k.each];
       mean[v] = st.x, rstd[v] = st.y;
       w[v] = column<T>(k.weight, k.wide_weights, c, 1.f);
       b[v] = column<T>(k.bias, k.wide_weights, c, 0.f);
@@ -407,27 +599,37 @@ struct Columns {
   }
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamPlan plan) {
+// JOINED: mean and rstd are joined here, and kept by the workgroup of a sample's first chunk.
+template <typename T, int V, bool JOINED>
+__global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamPlan plan,
+                                                               const float2* __restrict__ partial) {
+  __shared__ float2 s[JOINED ? JOINED_WIDTH : 1];
   for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
     const Item it = item_of<V>(k, plan, i);
+    const float2* stats = k.stats + it.n * k.groups;
+    if constexpr (JOINED) {
+      join_stats(k, plan, partial, it.n, s);
+      if (it.chunk == 0)
+        for (uint32_t g = threadIdx.x; g < k.groups; g += 256) k.stats[it.n * k.groups + g] = s[g];
+      stats = s;
+    }
     if (!it.live) continue;
     Columns<T, V> col;
-    col.load(k, it);
+    col.load(k, it, stats);
     const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
     T* y = (T*)k.y + it.n * k.pixels * k.width + it.column;
     with_act(k.act, [&](auto act) {
-#pragma unroll 4
-      for (uint64_t p = it.first + it.row; p < it.last; p += plan.threads_rows) {
-        Run<T, V> run;
-        run.load(x + (int64_t)p * k.x_pitch);
+      for_pixels<T, V, 4>(it.first + it.row, it.last, plan.threads_rows,
+                          [&](uint64_t p, Run<T, V>& r) { r.load(x + (int64_t)p * k.x_pitch); },
+                          [&](uint64_t p, const Run<T, V>& r) {
+        Run<T, V> out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float xh = (to_f32(run.v[v]) - col.mean[v]) * col.rstd[v];
-          run.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh, col.w[v], col.b[v])));
+          const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
+          out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh, col.w[v], col.b[v])));
         }
-        run.store(y + p * k.width);
-      }
+        out.store(y + p * k.width);
+      });
     });
   }
 }
@@ -442,24 +644,24 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
     float db[V] = {}, dw[V] = {};
     if (it.live) {
       Columns<T, V> col;
-      col.load(k, it);
+      col.load(k, it, k.stats + it.n * k.groups);
       const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
       const T* dy = (const T*)k.dy + (int64_t)it.n * k.dy_sample + it.column;
       with_act(k.act, [&](auto act) {
-#pragma unroll 2
-        for (uint64_t p = it.first + it.row; p < it.last; p += plan.threads_rows) {
-          Run<T, V> run, grad;
-          run.load(x + (int64_t)p * k.x_pitch);
-          grad.load(dy + (int64_t)p * k.dy_pitch);
+        for_pixel_pairs<T, V, 4>(it.first + it.row, it.last, plan.threads_rows,
+                                 [&](uint64_t p, Run<T, V>& r, Run<T, V>& g) {
+          r.load(x + (int64_t)p * k.x_pitch);
+          g.load(dy + (int64_t)p * k.dy_pitch);
+        }, [&](uint64_t, const Run<T, V>& r, const Run<T, V>& g) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float xh = (to_f32(run.v[v]) - col.mean[v]) * col.rstd[v];
+            const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
             const float dz =
-                to_f32(grad.v[v]) * act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v]));
+                to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v]));
             db[v] += dz;
             dw[v] = fmaf(dz, xh, dw[v]);
           }
-        }
+        });
       });
     }
     __syncthreads();
@@ -483,83 +685,46 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
   }
 }
 
-// A sample's sums by channel (rows of dw, db for the join) and by group (sum(g) / m and
-// sum(g xhat) / m), a workgroup for each group: 32 runs of chunks by 8 channels.
-template <typename T>
-__global__ void __launch_bounds__(256) group_norm_group_sums_kernel(
-    GnCall k, StreamPlan plan, const float2* __restrict__ partial, float* __restrict__ rows,
-    float2* __restrict__ sums) {
-  __shared__ float s_a[256], s_b[256];
-  for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
-    const uint64_t n = i / k.groups;
-    const uint32_t c0 = (uint32_t)(i % k.groups) * k.each, lane = threadIdx.x % 8;
-    float s1 = 0.f, s2 = 0.f;  // (of the threads below 8)
-    for (uint32_t j = 0; j < k.each; j += 8) {
-      const uint32_t c = c0 + j + lane;
-      const bool ok = j + lane < k.each;
-      float a = 0.f, b = 0.f;
-      if (ok)
-        for (uint32_t q = threadIdx.x / 8; q < plan.chunks; q += 32) {
-          const float2 p = partial[(n * plan.chunks + q) * k.width + c];
-          a += p.x, b += p.y;
-        }
-      s_a[threadIdx.x] = a, s_b[threadIdx.x] = b;
-      for (uint32_t h = 128; h >= 8; h >>= 1) {
-        __syncthreads();
-        if (threadIdx.x < h) {
-          s_a[threadIdx.x] += s_a[threadIdx.x + h];
-          s_b[threadIdx.x] += s_b[threadIdx.x + h];
-        }
-      }
-      if (threadIdx.x < 8 && ok) {
-        a = s_a[lane], b = s_b[lane];
-        const float w = column<T>(k.weight, k.wide_weights, c, 1.f);
-        s1 = fmaf(w, a, s1);
-        s2 = fmaf(w, b, s2);
-        if (rows) rows[n * 2 * k.width + c] = b, rows[(n * 2 + 1) * k.width + c] = a;
-      }
-      __syncthreads();
-    }
-    for (int off = 4; off; off >>= 1) s1 += __shfl_xor(s1, off, 8), s2 += __shfl_xor(s2, off, 8);
-    if (threadIdx.x == 0) {
-      const double m = (double)k.pixels * k.each;
-      sums[i] = {(float)(s1 / m), (float)(s2 / m)};
-    }
-  }
-}
-
-template <typename T, int V>
+// from: the groups' sums, or (JOINED) the partial ones.
+template <typename T, int V, bool JOINED>
 __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan plan,
-                                                            const float2* __restrict__ sums) {
+                                                            const float2* __restrict__ from) {
+  __shared__ float2 s[JOINED ? JOINED_WIDTH : 1];
   for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
     const Item it = item_of<V>(k, plan, i);
+    const float2* sums = from + it.n * k.groups;
+    if constexpr (JOINED) {
+      join_sums<T>(k, plan, from, it.n, s);
+      sums = s;
+    }
     if (!it.live) continue;
     Columns<T, V> col;
-    col.load(k, it);
+    col.load(k, it, k.stats + it.n * k.groups);
     float s1[V], s2[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-      const float2 p = sums[it.n * k.groups + (it.column + v) / k.each];
+      const float2 p = sums[(it.column + v) / k.each];
       s1[v] = p.x, s2[v] = p.y;
     }
     const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
     const T* dy = (const T*)k.dy + (int64_t)it.n * k.dy_sample + it.column;
     T* dx = (T*)k.y + it.n * k.pixels * k.width + it.column;
     with_act(k.act, [&](auto act) {
-#pragma unroll 2
-      for (uint64_t p = it.first + it.row; p < it.last; p += plan.threads_rows) {
-        Run<T, V> run, grad;
-        run.load(x + (int64_t)p * k.x_pitch);
-        grad.load(dy + (int64_t)p * k.dy_pitch);
+      for_pixel_pairs<T, V, 2>(it.first + it.row, it.last, plan.threads_rows,
+                               [&](uint64_t p, Run<T, V>& r, Run<T, V>& g) {
+        r.load(x + (int64_t)p * k.x_pitch);
+        g.load(dy + (int64_t)p * k.dy_pitch);
+      }, [&](uint64_t p, const Run<T, V>& r, const Run<T, V>& g) {
+        Run<T, V> out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float xh = (to_f32(run.v[v]) - col.mean[v]) * col.rstd[v];
-          const float g = to_f32(grad.v[v]) *
+          const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
+          const float d = to_f32(g.v[v]) *
                           act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v])) * col.w[v];
-          run.v[v] = from_f32<T>(col.rstd[v] * (g - s1[v] - xh * s2[v]));
+          out.v[v] = from_f32<T>(col.rstd[v] * (d - s1[v] - xh * s2[v]));
         }
-        run.store(dx + p * k.width);
-      }
+        out.store(dx + p * k.width);
+      });
     });
   }
 }
@@ -587,10 +752,23 @@ static uint32_t vector_of(uint32_t n, int32_t dtype) {
 static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32_t each,
                       uint32_t v, HeldPlan& plan) {
   plan.lane_log = log2_up(each / v);
-  if (plan.lane_log > 6 || pixels > 64 * HELD_RUNS) return false;
-  plan.row_log = std::min(6 - plan.lane_log, log2_up(pixels));
+  plan.wide = false;
+  if (plan.lane_log > 8 || pixels > 256 * HELD_RUNS) return false;
+  const int rows = log2_up(pixels);
+  if (plan.lane_log > 6 || (pixels + (64u >> plan.lane_log) - 1) / (64u >> plan.lane_log) >
+                               HELD_RUNS) {
+    plan.wide = true;  // (the rows fill the workgroup: idle ones cost nothing)
+    plan.row_log = 8 - plan.lane_log;
+    plan.runs = (int)((pixels + (1u << plan.row_log) - 1) >> plan.row_log);
+    if (plan.runs > HELD_RUNS) return false;
+    plan.teams = 1;
+    plan.rows = (uint32_t)std::min<uint64_t>(samples, std::max<uint32_t>(1, 2048 / groups));
+    plan.grid = plan.rows * groups;
+    plan.partials = plan.rows;
+    return true;
+  }
+  plan.row_log = std::min(6 - plan.lane_log, rows);
   plan.runs = (int)((pixels + (1u << plan.row_log) - 1) >> plan.row_log);
-  if (plan.runs > HELD_RUNS) return false;
   const uint32_t teams = 256 >> (plan.lane_log + plan.row_log);
   if (teams >= groups) {
     const uint32_t each_wg = teams / groups;  // samples of a workgroup at once
@@ -608,14 +786,18 @@ static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32
   return true;
 }
 
-static StreamPlan stream_plan(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t v) {
+static StreamPlan stream_plan(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
+                              uint32_t v) {
   StreamPlan plan;
   const uint32_t vectors = width / v;
   plan.tiles = (vectors + TILE_VECTORS - 1) / TILE_VECTORS;
   plan.columns = (vectors + plan.tiles - 1) / plan.tiles;
   plan.threads_rows = 256 / plan.columns;
   // about 2048 workgroups, each with 8 pixels a thread at least
-  const uint64_t wanted = std::max<uint64_t>(1, 2048 / std::max<uint64_t>(1, samples * plan.tiles));
+  uint64_t wanted = std::max<uint64_t>(1, 2048 / std::max<uint64_t>(1, samples * plan.tiles));
+  plan.joined = plan.tiles == 1 && width <= JOINED_WIDTH && width / groups <= JOINED_EACH &&
+                samples * pixels * width < JOINED_BELOW;
+  if (plan.joined) wanted = std::min<uint64_t>(wanted, std::max(1u, JOINED_ENTRIES / width));
   const uint64_t least = 8ull * plan.threads_rows;
   plan.chunk = std::max((pixels + wanted - 1) / wanted, least);
   plan.chunk = (plan.chunk + plan.threads_rows - 1) / plan.threads_rows * plan.threads_rows;
@@ -658,17 +840,23 @@ static void held_launch(const GnCall& k, const HeldPlan& plan, int32_t dtype, fl
                         hipStream_t stream) {
   with_vector(dtype, vector_of(k.each, dtype), [&](auto tag, auto v) {
     using T = decltype(tag);
-    const auto launch = [&](auto kernel) {
-      hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(256), 0, stream, k, plan, partial);
+    const auto launch = [&](auto runs) {
+      const auto start = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(plan.grid), dim3(256), 0, stream, k, plan, partial);
+      };
+      if (plan.wide)
+        start(group_norm_held_kernel<T, v.value, runs.value, BACKWARD, true>);
+      else
+        start(group_norm_held_kernel<T, v.value, runs.value, BACKWARD, false>);
     };
     if (plan.runs == 1)
-      launch(group_norm_held_kernel<T, v.value, 1, BACKWARD>);
+      launch(std::integral_constant<int, 1>());
     else if (plan.runs == 2)
-      launch(group_norm_held_kernel<T, v.value, 2, BACKWARD>);
+      launch(std::integral_constant<int, 2>());
     else if (plan.runs <= 4)
-      launch(group_norm_held_kernel<T, v.value, 4, BACKWARD>);
+      launch(std::integral_constant<int, 4>());
     else
-      launch(group_norm_held_kernel<T, v.value, 8, BACKWARD>);
+      launch(std::integral_constant<int, 8>());
   });
 }
 
@@ -688,7 +876,7 @@ extern "C" uint64_t tgs_group_norm_fwd_workspace_size(uint64_t samples, uint64_t
   if (!gn_sizes_ok(samples, pixels, width, groups, dtype) || samples == 0 || pixels == 0 ||
       gn_held(samples, pixels, width, groups, dtype, held))
     return 0;
-  const StreamPlan plan = stream_plan(samples, pixels, width, vector_of(width, dtype));
+  const StreamPlan plan = stream_plan(samples, pixels, width, groups, vector_of(width, dtype));
   return samples * plan.chunks * width * sizeof(float2);
 }
 
@@ -699,8 +887,8 @@ extern "C" uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t
   if (!gn_sizes_ok(samples, pixels, width, groups, dtype) || samples == 0 || pixels == 0) return 0;
   if (gn_held(samples, pixels, width, groups, dtype, held))
     return (uint64_t)held.partials * 2 * width * sizeof(float);
-  const StreamPlan plan = stream_plan(samples, pixels, width, vector_of(width, dtype));
-  return samples * sizeof(float2) * ((plan.chunks + 1ull) * width + groups);
+  const StreamPlan plan = stream_plan(samples, pixels, width, groups, vector_of(width, dtype));
+  return samples * sizeof(float2) * ((uint64_t)plan.chunks * width + groups);
 }
 
 #define GN_CHECK_CALL(name)                                                                      \
@@ -744,16 +932,22 @@ extern "C" int tgs_group_norm_fwd(uint64_t samples, uint64_t pixels, uint32_t wi
   TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 8 == 0 && (uintptr_t)stats % 8 == 0,
                 "tgs_group_norm_fwd: the workspace and the stats start on 8 bytes");
   const uint32_t v = vector_of(width, dtype);
-  const StreamPlan plan = stream_plan(samples, pixels, width, v);
+  const StreamPlan plan = stream_plan(samples, pixels, width, groups, v);
   const dim3 grid(capped(plan.items)), by_group(capped(samples * groups));
   float2* partial = (float2*)workspace;
   with_vector(dtype, v, [&](auto tag, auto vec) {
     using T = decltype(tag);
     hipLaunchKernelGGL((group_norm_stats_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
                        plan, partial);
-    hipLaunchKernelGGL(group_norm_finish_kernel, by_group, dim3(256), 0, stream, k, plan, partial);
-    hipLaunchKernelGGL((group_norm_apply_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
-                       plan);
+    if (plan.joined) {
+      hipLaunchKernelGGL((group_norm_apply_kernel<T, vec.value, true>), grid, dim3(256), 0, stream,
+                         k, plan, partial);
+      return;
+    }
+    hipLaunchKernelGGL(group_norm_finish_kernel, by_group, dim3(1024), 0, stream, k, plan,
+                       partial);
+    hipLaunchKernelGGL((group_norm_apply_kernel<T, vec.value, false>), grid, dim3(256), 0, stream,
+                       k, plan, nullptr);
   });
   TGS_RETURN_LAUNCH("tgs_group_norm_fwd");
 }
@@ -801,24 +995,29 @@ extern "C" int tgs_group_norm_bwd(uint64_t samples, uint64_t pixels, uint32_t wi
   } else {
     TGS_CHECK_ARG(stats && (uintptr_t)stats % 8 == 0,
                   "tgs_group_norm_bwd: the stats of the forward are needed, on 8 bytes");
-    TGS_CHECK_ARG(!sums || samples < (1ull << 32), "tgs_group_norm_bwd: 2^32 samples and more");
     const uint32_t v = vector_of(width, dtype);
-    const StreamPlan plan = stream_plan(samples, pixels, width, v);
+    const StreamPlan plan = stream_plan(samples, pixels, width, groups, v);
+    TGS_CHECK_ARG(!sums || samples * plan.chunks < (1ull << 32),
+                  "tgs_group_norm_bwd: too many samples for their sums");
     const dim3 grid(capped(plan.items)), by_group(capped(samples * groups));
     float2* partial = (float2*)workspace;
-    float* rows = (float*)(partial + samples * plan.chunks * width);
-    float2* group_sums = (float2*)rows + samples * width;
+    float2* group_sums = partial + samples * plan.chunks * width;
     with_vector(dtype, v, [&](auto tag, auto vec) {
       using T = decltype(tag);
       hipLaunchKernelGGL((group_norm_sums_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
                          plan, partial);
-      hipLaunchKernelGGL(group_norm_group_sums_kernel<T>, by_group, dim3(256), 0, stream, k, plan,
-                         partial, sums ? rows : nullptr, group_sums);
-      if (dx)
-        hipLaunchKernelGGL((group_norm_dx_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
-                           plan, group_sums);
+      if (!dx) return;
+      if (plan.joined) {
+        hipLaunchKernelGGL((group_norm_dx_kernel<T, vec.value, true>), grid, dim3(256), 0, stream,
+                           k, plan, partial);
+        return;
+      }
+      hipLaunchKernelGGL(group_norm_group_sums_kernel<T>, by_group, dim3(1024), 0, stream, k, plan,
+                         partial, group_sums);
+      hipLaunchKernelGGL((group_norm_dx_kernel<T, vec.value, false>), grid, dim3(256), 0, stream,
+                         k, plan, group_sums);
     });
-    join((uint32_t)samples, rows);
+    join((uint32_t)(samples * plan.chunks), (const float*)partial);
   }
   TGS_RETURN_LAUNCH("tgs_group_norm_bwd");
 }
