@@ -289,38 +289,45 @@ __global__ void __launch_bounds__(1024) group_norm_join_kernel(uint32_t parts, u
 struct StreamPlan {
   uint32_t tiles, columns;  // tiles of channels, vectors of a tile
   uint32_t threads_rows;    // pixels that a workgroup takes at once
-  uint32_t chunks;          // of a sample's pixels
-  uint64_t chunk;           // pixels of one
-  uint64_t items;           // samples * tiles * chunks
-  bool joined;              // by the workgroups that read the partial values
+  uint32_t chunks;          // of a sample's pixels: every chunks-th run of threads_rows
+  uint32_t at_once;         // samples of a launch's grid
 };
 
+// The partial values of a sample, as the launch that left them cut its pixels.
+struct Parts {
+  uint32_t chunks, rows;
+  bool joined;  // by the workgroups that read them
+};
+
+// A workgroup's part: a chunk of the pixels (the grid's x) by a tile of channels (its y), of every
+// sample that its z comes to.
 struct Item {
-  uint64_t n, first, last;  // sample, pixels
-  uint32_t chunk, column;   // this thread's first channel
+  uint64_t first;        // this thread's first pixel
+  uint32_t step;         // to its next
+  uint32_t column;       // this thread's first channel
+  uint32_t tile;         // the tile's first channel, and its number of channels
+  uint32_t wide;
   uint32_t row;
   bool live;
 };
 
 template <int V>
-__device__ __forceinline__ Item item_of(const GnCall& k, const StreamPlan& plan, uint64_t i) {
+__device__ __forceinline__ Item item_of(const GnCall& k, const StreamPlan& plan) {
   Item it;
-  it.chunk = (uint32_t)(i % plan.chunks);
-  const uint64_t rest = i / plan.chunks;
-  const uint32_t tile = (uint32_t)(rest % plan.tiles);
-  it.n = rest / plan.tiles;
-  it.first = it.chunk * plan.chunk;
-  it.last = min(it.first + plan.chunk, k.pixels);
   it.row = threadIdx.x / plan.columns;
-  const uint32_t vector = tile * plan.columns + threadIdx.x % plan.columns;
+  it.first = (uint64_t)blockIdx.x * plan.threads_rows + it.row;
+  it.step = plan.chunks * plan.threads_rows;
+  const uint32_t vector = blockIdx.y * plan.columns + threadIdx.x - it.row * plan.columns;
   it.column = vector * V;
+  it.tile = blockIdx.y * plan.columns * V;
+  it.wide = min(plan.columns * V, k.width - it.tile);
   it.live = it.row < plan.threads_rows && vector < k.width / V;
   return it;
 }
 
-// Pixels of [first, last) that row r of a workgroup takes.
-__device__ __forceinline__ uint32_t row_count(uint64_t pixels, uint32_t r, uint32_t rows) {
-  return pixels > r ? (uint32_t)((pixels - r + rows - 1) / rows) : 0;
+// Pixels of `pixels` from `first` on in steps of `step`.
+__device__ __forceinline__ uint32_t count_from(uint64_t first, uint64_t pixels, uint32_t step) {
+  return first < pixels ? (uint32_t)((pixels - first + step - 1) / step) : 0;
 }
 
 // For every `step`th pixel from p on: U loads on their way before the first is used; past the
@@ -352,24 +359,48 @@ __device__ __forceinline__ void for_pixel_pairs(uint64_t p, uint64_t last, uint3
   }
 }
 
+// f(r, c) over the rows of a tile's channels in LDS, c in 0..it.wide - 1: `parts` threads of a
+// channel take a share of the rows each.
+struct TileRows {
+  uint32_t c, part, parts;
+  bool live;
+  __device__ __forceinline__ TileRows(const Item& it, uint32_t rows) {
+    parts = min(max(256u / it.wide, 1u), rows);
+    part = threadIdx.x / it.wide;
+    c = threadIdx.x - part * it.wide;
+    live = part < parts;
+  }
+};
+
 // Each channel's mean and sum of squared differences over a chunk of pixels.
 template <typename T, int V>
 __global__ void __launch_bounds__(256) group_norm_stats_kernel(GnCall k, StreamPlan plan,
                                                                float2* __restrict__ partial) {
-  __shared__ float s_mean[256 * V], s_m2[256 * V];
-  for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
-    const Item it = item_of<V>(k, plan, i);
-    const uint32_t rows = plan.threads_rows;
+  __shared__ float2 s[256 * V];
+  __shared__ float2 s_part[256];
+  const Item it = item_of<V>(k, plan);
+  const uint32_t rows = plan.threads_rows;
+  const uint64_t run = (uint64_t)blockIdx.x * rows;  // the chunk's first pixel
+  // Rows have one pixel more than the last one has, or as many, those with more first.
+  const uint32_t count = count_from(it.first, k.pixels, it.step);
+  const uint32_t least = count_from(run + rows - 1, k.pixels, it.step);
+  const uint32_t longer = count_from(run, k.pixels, it.step) > least
+                              ? (uint32_t)((k.pixels - run) % it.step) : 0;
+  const float inv = count ? 1.f / (float)count : 0.f;
+  const float all = 1.f / (float)((uint64_t)least * rows + longer);
+  for (uint64_t n = blockIdx.z; n < k.samples; n += gridDim.z) {
     float pivot[V] = {}, sum[V] = {}, squares[V] = {};
-    if (it.live && it.first + it.row < it.last) {
-      const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
-      Run<T, V> run;
-      run.load(x + (int64_t)(it.first + it.row) * k.x_pitch);
-#pragma unroll
-      for (int v = 0; v < V; ++v) pivot[v] = to_f32(run.v[v]);
-      for_pixels<T, V, 8>(it.first + it.row, it.last, rows, [&](uint64_t p, Run<T, V>& r) {
+    if (it.live && count) {
+      const T* x = (const T*)k.x + (int64_t)n * k.x_sample + it.column;
+      bool begun = false;
+      for_pixels<T, V, 8>(it.first, k.pixels, it.step, [&](uint64_t p, Run<T, V>& r) {
         r.load(x + (int64_t)p * k.x_pitch);
       }, [&](uint64_t, const Run<T, V>& r) {
+        if (!begun) {
+#pragma unroll
+          for (int v = 0; v < V; ++v) pivot[v] = to_f32(r.v[v]);
+          begun = true;
+        }
 #pragma unroll
         for (int v = 0; v < V; ++v) {
           const float d = to_f32(r.v[v]) - pivot[v];
@@ -378,39 +409,53 @@ __global__ void __launch_bounds__(256) group_norm_stats_kernel(GnCall k, StreamP
         }
       });
     }
-    const uint32_t count = row_count(it.last - it.first, it.row, rows);
-    const float inv = count ? 1.f / (float)count : 0.f;
-    __syncthreads();  // (the last item's values are read)
+    __syncthreads();  // (the last sample's values are read)
     if (it.row < rows) {
-      const uint32_t at = threadIdx.x * V;  // rows of `columns` vectors
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        s_mean[at + v] = fmaf(sum[v], inv, pivot[v]);
-        s_m2[at + v] = fmaxf(fmaf(-sum[v] * inv, sum[v], squares[v]), 0.f);
-      }
+      for (int v = 0; v < V; ++v)
+        s[threadIdx.x * V + v] = {fmaf(sum[v], inv, pivot[v]),
+                                  fmaxf(fmaf(-sum[v] * inv, sum[v], squares[v]), 0.f)};
     }
     __syncthreads();
-    const uint32_t wide = plan.columns * V, tile = it.column / wide * wide;
-    const float all = 1.f / (float)(it.last - it.first);
-    for (uint32_t c = threadIdx.x; c < wide && tile + c < k.width; c += 256) {
-      float mean = 0.f, m2 = 0.f;
-      for (uint32_t r = 0; r < rows; ++r)
-        mean = fmaf(s_mean[r * wide + c],
-                    (float)row_count(it.last - it.first, r, rows) * all, mean);
-      for (uint32_t r = 0; r < rows; ++r) {
-        const float d = s_mean[r * wide + c] - mean;
-        const float n = (float)row_count(it.last - it.first, r, rows);
-        m2 += n > 0.f ? fmaf(n * d, d, s_m2[r * wide + c]) : 0.f;
+    // rows joined from the first row's mean, near to which the others' are
+    const uint32_t pitch = plan.columns * V;
+    for (uint32_t c0 = 0; c0 < it.wide; c0 += 256) {
+      const TileRows t(it, rows);
+      const uint32_t c = it.wide > 256 ? c0 + threadIdx.x : t.c;
+      const bool live = it.wide > 256 ? c < it.wide : t.live;
+      float2 a = {0.f, 0.f};
+      const float near = live ? s[c].x : 0.f;
+      if (live)
+        for (uint32_t r = t.part; r < rows; r += t.parts) {
+          const float m = (float)(least + (r < longer));
+          if (m == 0.f) break;
+          const float2 p = s[r * pitch + c];
+          const float d = p.x - near;
+          a.x = fmaf(m, d, a.x);
+          a.y += fmaf(m * d, d, p.y);
+        }
+      if (t.parts > 1) {
+        s_part[threadIdx.x] = a;
+        __syncthreads();
+        if (threadIdx.x < it.wide)
+          for (uint32_t j = 1; j < t.parts; ++j) {
+            const float2 p = s_part[threadIdx.x + j * it.wide];
+            a.x += p.x, a.y += p.y;
+          }
       }
-      partial[(it.n * plan.chunks + it.chunk) * k.width + tile + c] = {mean, m2};
+      if (live && t.part == 0)
+        partial[(n * plan.chunks + blockIdx.x) * k.width + it.tile + c] = {
+            fmaf(a.x, all, near), fmaxf(fmaf(-a.x * all, a.x, a.y), 0.f)};
     }
   }
 }
 
 // Pixels of a chunk.
-__device__ __forceinline__ float chunk_pixels(const GnCall& k, const StreamPlan& plan, uint32_t q) {
-  const uint64_t first = q * plan.chunk;
-  return (float)(min(first + plan.chunk, k.pixels) - first);
+__device__ __forceinline__ float chunk_pixels(const GnCall& k, const Parts& parts, uint32_t q) {
+  const uint64_t round = (uint64_t)parts.chunks * parts.rows, before = (uint64_t)q * parts.rows;
+  const uint64_t rest = k.pixels % round;
+  const uint64_t more = rest > before ? min(rest - before, (uint64_t)parts.rows) : 0;
+  return (float)(k.pixels / round * parts.rows + more);
 }
 
 template <int WAVES>
@@ -429,33 +474,33 @@ __device__ __forceinline__ double sum_of_workgroup(double v, double* s) {
 // f(chunk, channel) over a group's partial values: as many threads side by side as there are
 // channels, up to 64, the others on further chunks.
 template <typename F>
-__device__ __forceinline__ void for_entries(const StreamPlan& plan, uint32_t each, F&& f) {
+__device__ __forceinline__ void for_entries(const Parts& parts, uint32_t each, F&& f) {
   const uint32_t across = each < 64 ? each : 64, along = blockDim.x / across;
   const uint32_t c0 = threadIdx.x % across, q0 = threadIdx.x / across;
   if (q0 >= along) return;
   for (uint32_t c = c0; c < each; c += across) {
 #pragma unroll 4
-    for (uint32_t q = q0; q < plan.chunks; q += along) f(q, c);
+    for (uint32_t q = q0; q < parts.chunks; q += along) f(q, c);
   }
 }
 
 // Mean and rstd of each sample's group, a workgroup each, in 64 bits.
-__global__ void __launch_bounds__(1024) group_norm_finish_kernel(GnCall k, StreamPlan plan,
+__global__ void __launch_bounds__(1024) group_norm_finish_kernel(GnCall k, Parts parts,
                                                                  const float2* __restrict__ partial) {
   __shared__ double s[16];
   for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
     const uint64_t n = i / k.groups;
-    const float2* from = partial + n * plan.chunks * k.width + i % k.groups * k.each;
+    const float2* from = partial + n * parts.chunks * k.width + i % k.groups * k.each;
     const double m = (double)k.pixels * k.each;
     double a = 0, q = 0;
-    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
-      a += (double)from[(uint64_t)j * k.width + c].x * chunk_pixels(k, plan, j);
+    for_entries(parts, k.each, [&](uint32_t j, uint32_t c) {
+      a += (double)from[(uint64_t)j * k.width + c].x * chunk_pixels(k, parts, j);
     });
     const double mean = sum_of_workgroup<16>(a, s) / m;
-    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
+    for_entries(parts, k.each, [&](uint32_t j, uint32_t c) {
       const float2 p = from[(uint64_t)j * k.width + c];
       const double d = p.x - mean;
-      q += p.y + chunk_pixels(k, plan, j) * d * d;
+      q += p.y + chunk_pixels(k, parts, j) * d * d;
     });
     q = sum_of_workgroup<16>(q, s) / m;
     if (threadIdx.x == 0) k.stats[i] = {(float)mean, (float)(1.0 / sqrt(q + (double)k.eps))};
@@ -465,15 +510,15 @@ __global__ void __launch_bounds__(1024) group_norm_finish_kernel(GnCall k, Strea
 // sum(g) / m and sum(g xhat) / m of each sample's group, a workgroup each.
 template <typename T>
 __global__ void __launch_bounds__(1024) group_norm_group_sums_kernel(
-    GnCall k, StreamPlan plan, const float2* __restrict__ partial, float2* __restrict__ sums) {
+    GnCall k, Parts parts, const float2* __restrict__ partial, float2* __restrict__ sums) {
   __shared__ double s[16];
   for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
     const uint64_t n = i / k.groups;
     const uint32_t c0 = (uint32_t)(i % k.groups) * k.each;
-    const float2* from = partial + n * plan.chunks * k.width + c0;
+    const float2* from = partial + n * parts.chunks * k.width + c0;
     const double m = (double)k.pixels * k.each;
     double a = 0, b = 0;
-    for_entries(plan, k.each, [&](uint32_t j, uint32_t c) {
+    for_entries(parts, k.each, [&](uint32_t j, uint32_t c) {
       const float2 p = from[(uint64_t)j * k.width + c];
       const float w = column<T>(k.weight, k.wide_weights, c0 + c, 1.f);
       a += (double)w * p.x;
@@ -491,7 +536,7 @@ __global__ void __launch_bounds__(1024) group_norm_group_sums_kernel(
 
 // The sums of entry(q, c) over the chunks q, each channel's in s[c].
 template <typename F>
-__device__ __forceinline__ void sum_by_channel(const GnCall& k, const StreamPlan& plan, float2* s,
+__device__ __forceinline__ void sum_by_channel(const GnCall& k, const Parts& parts, float2* s,
                                                F&& entry) {
   const uint32_t along = k.width < 256 ? 256 / k.width : 1;  // threads of a channel
   __syncthreads();
@@ -499,7 +544,7 @@ __device__ __forceinline__ void sum_by_channel(const GnCall& k, const StreamPlan
     const uint32_t c = t % k.width;
     float2 a = {0.f, 0.f};
 #pragma unroll 8
-    for (uint32_t q = t / k.width; q < plan.chunks; q += along) {
+    for (uint32_t q = t / k.width; q < parts.chunks; q += along) {
       const float2 p = entry(q, c);
       a.x += p.x, a.y += p.y;
     }
@@ -534,14 +579,14 @@ __device__ __forceinline__ void replace_by_group(const GnCall& k, float2* s, F&&
 }
 
 // s[group] = {mean, rstd}
-__device__ __forceinline__ void join_stats(const GnCall& k, const StreamPlan& plan,
+__device__ __forceinline__ void join_stats(const GnCall& k, const Parts& parts,
                                            const float2* partial, uint64_t n, float2* s) {
-  const float2* from = partial + n * plan.chunks * k.width;
+  const float2* from = partial + n * parts.chunks * k.width;
   const float pixels = (float)k.pixels, inv = 1.f / pixels;
   // differences from the first chunk's mean, near to which the others' are
-  sum_by_channel(k, plan, s, [&](uint32_t q, uint32_t c) {
+  sum_by_channel(k, parts, s, [&](uint32_t q, uint32_t c) {
     const float2 p = from[q * k.width + c];
-    const float d = p.x - from[c].x, nd = chunk_pixels(k, plan, q) * d;
+    const float d = p.x - from[c].x, nd = chunk_pixels(k, parts, q) * d;
     return make_float2(nd, fmaf(nd, d, p.y));
   });
   for (uint32_t c = threadIdx.x; c < k.width; c += 256) {
@@ -564,11 +609,11 @@ __device__ __forceinline__ void join_stats(const GnCall& k, const StreamPlan& pl
 
 // s[group] = {sum(g) / m, sum(g xhat) / m}
 template <typename T>
-__device__ __forceinline__ void join_sums(const GnCall& k, const StreamPlan& plan,
+__device__ __forceinline__ void join_sums(const GnCall& k, const Parts& parts,
                                           const float2* partial, uint64_t n, float2* s) {
-  const float2* from = partial + n * plan.chunks * k.width;
+  const float2* from = partial + n * parts.chunks * k.width;
   const float inv = 1.f / (float)(k.pixels * k.each);
-  sum_by_channel(k, plan, s, [&](uint32_t q, uint32_t c) {
+  sum_by_channel(k, parts, s, [&](uint32_t q, uint32_t c) {
     const float w = column<T>(k.weight, k.wide_weights, c, 1.f);
     const float2 p = from[q * k.width + c];
     return make_float2(w * p.x, w * p.y);
@@ -602,25 +647,28 @@ struct Columns {
 // JOINED: mean and rstd are joined here, and kept by the workgroup of a sample's first chunk.
 template <typename T, int V, bool JOINED>
 __global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamPlan plan,
+                                                               Parts parts,
                                                                const float2* __restrict__ partial) {
   __shared__ float2 s[JOINED ? JOINED_WIDTH : 1];
-  for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
-    const Item it = item_of<V>(k, plan, i);
-    const float2* stats = k.stats + it.n * k.groups;
+  const Item it = item_of<V>(k, plan);
+  for (uint64_t m = blockIdx.z; m < k.samples; m += gridDim.z) {
+    const uint64_t n = k.samples - 1 - m;
+    const float2* stats = k.stats + n * k.groups;
     if constexpr (JOINED) {
-      join_stats(k, plan, partial, it.n, s);
-      if (it.chunk == 0)
-        for (uint32_t g = threadIdx.x; g < k.groups; g += 256) k.stats[it.n * k.groups + g] = s[g];
+      join_stats(k, parts, partial, n, s);
+      if (blockIdx.x == 0)
+        for (uint32_t g = threadIdx.x; g < k.groups; g += 256) k.stats[n * k.groups + g] = s[g];
       stats = s;
     }
     if (!it.live) continue;
     Columns<T, V> col;
     col.load(k, it, stats);
-    const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
-    T* y = (T*)k.y + it.n * k.pixels * k.width + it.column;
+    const int64_t end = (int64_t)k.pixels - 1;
+    const T* x = (const T*)k.x + (int64_t)n * k.x_sample + end * k.x_pitch + it.column;
+    T* y = (T*)k.y + (n * k.pixels + end) * k.width + it.column;
     with_act(k.act, [&](auto act) {
-      for_pixels<T, V, 4>(it.first + it.row, it.last, plan.threads_rows,
-                          [&](uint64_t p, Run<T, V>& r) { r.load(x + (int64_t)p * k.x_pitch); },
+      for_pixels<T, V, 4>(it.first, k.pixels, it.step,
+                          [&](uint64_t p, Run<T, V>& r) { r.load(x - (int64_t)p * k.x_pitch); },
                           [&](uint64_t p, const Run<T, V>& r) {
         Run<T, V> out;
 #pragma unroll
@@ -628,7 +676,7 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamP
           const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
           out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh, col.w[v], col.b[v])));
         }
-        out.store(y + p * k.width);
+        out.store(y - p * k.width);
       });
     });
   }
@@ -638,28 +686,30 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamP
 template <typename T, int V>
 __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPlan plan,
                                                               float2* __restrict__ partial) {
-  __shared__ float s[2][256 * V];
-  for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
-    const Item it = item_of<V>(k, plan, i);
-    float db[V] = {}, dw[V] = {};
+  __shared__ float2 s[256 * V];
+  __shared__ float2 s_part[256];
+  const Item it = item_of<V>(k, plan);
+  for (uint64_t n = blockIdx.z; n < k.samples; n += gridDim.z) {
+    float db[V] = {}, dw[V] = {};  // (dw of x - mean, times rstd at the end)
+    Columns<T, V> col;
     if (it.live) {
-      Columns<T, V> col;
-      col.load(k, it, k.stats + it.n * k.groups);
-      const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
-      const T* dy = (const T*)k.dy + (int64_t)it.n * k.dy_sample + it.column;
+      col.load(k, it, k.stats + n * k.groups);
+#pragma unroll
+      for (int v = 0; v < V; ++v) col.w[v] *= col.rstd[v];
+      const T* x = (const T*)k.x + (int64_t)n * k.x_sample + it.column;
+      const T* dy = (const T*)k.dy + (int64_t)n * k.dy_sample + it.column;
       with_act(k.act, [&](auto act) {
-        for_pixel_pairs<T, V, 4>(it.first + it.row, it.last, plan.threads_rows,
+        for_pixel_pairs<T, V, 2>(it.first, k.pixels, it.step,
                                  [&](uint64_t p, Run<T, V>& r, Run<T, V>& g) {
           r.load(x + (int64_t)p * k.x_pitch);
           g.load(dy + (int64_t)p * k.dy_pitch);
         }, [&](uint64_t, const Run<T, V>& r, const Run<T, V>& g) {
 #pragma unroll
           for (int v = 0; v < V; ++v) {
-            const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
-            const float dz =
-                to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v]));
+            const float d = to_f32(r.v[v]) - col.mean[v];
+            const float dz = to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.w[v], col.b[v]));
             db[v] += dz;
-            dw[v] = fmaf(dz, xh, dw[v]);
+            dw[v] = fmaf(dz, d, dw[v]);
           }
         });
       });
@@ -667,20 +717,32 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
     __syncthreads();
     if (it.row < plan.threads_rows) {
 #pragma unroll
-      for (int v = 0; v < V; ++v) {
-        s[0][threadIdx.x * V + v] = db[v];
-        s[1][threadIdx.x * V + v] = dw[v];
-      }
+      for (int v = 0; v < V; ++v)
+        s[threadIdx.x * V + v] = {db[v], it.live ? dw[v] * col.rstd[v] : 0.f};
     }
     __syncthreads();
-    const uint32_t wide = plan.columns * V, tile = it.column / wide * wide;
-    for (uint32_t c = threadIdx.x; c < wide && tile + c < k.width; c += 256) {
-      float a = 0.f, b = 0.f;
-      for (uint32_t r = 0; r < plan.threads_rows; ++r) {
-        a += s[0][r * wide + c];
-        b += s[1][r * wide + c];
+    const uint32_t pitch = plan.columns * V;
+    for (uint32_t c0 = 0; c0 < it.wide; c0 += 256) {
+      const TileRows t(it, plan.threads_rows);
+      const uint32_t c = it.wide > 256 ? c0 + threadIdx.x : t.c;
+      const bool live = it.wide > 256 ? c < it.wide : t.live;
+      float2 a = {0.f, 0.f};
+      if (live)
+        for (uint32_t r = t.part; r < plan.threads_rows; r += t.parts) {
+          const float2 p = s[r * pitch + c];
+          a.x += p.x, a.y += p.y;
+        }
+      if (t.parts > 1) {
+        s_part[threadIdx.x] = a;
+        __syncthreads();
+        if (threadIdx.x < it.wide)
+          for (uint32_t j = 1; j < t.parts; ++j) {
+            const float2 p = s_part[threadIdx.x + j * it.wide];
+            a.x += p.x, a.y += p.y;
+          }
       }
-      partial[(it.n * plan.chunks + it.chunk) * k.width + tile + c] = {a, b};
+      if (live && t.part == 0)
+        partial[(n * plan.chunks + blockIdx.x) * k.width + it.tile + c] = a;
     }
   }
 }
@@ -688,32 +750,35 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
 // from: the groups' sums, or (JOINED) the partial ones.
 template <typename T, int V, bool JOINED>
 __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan plan,
+                                                            Parts parts,
                                                             const float2* __restrict__ from) {
   __shared__ float2 s[JOINED ? JOINED_WIDTH : 1];
-  for (uint64_t i = blockIdx.x; i < plan.items; i += gridDim.x) {
-    const Item it = item_of<V>(k, plan, i);
-    const float2* sums = from + it.n * k.groups;
+  const Item it = item_of<V>(k, plan);
+  for (uint64_t m = blockIdx.z; m < k.samples; m += gridDim.z) {
+    const uint64_t n = k.samples - 1 - m;
+    const float2* sums = from + n * k.groups;
     if constexpr (JOINED) {
-      join_sums<T>(k, plan, from, it.n, s);
+      join_sums<T>(k, parts, from, n, s);
       sums = s;
     }
     if (!it.live) continue;
     Columns<T, V> col;
-    col.load(k, it, k.stats + it.n * k.groups);
+    col.load(k, it, k.stats + n * k.groups);
     float s1[V], s2[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float2 p = sums[(it.column + v) / k.each];
       s1[v] = p.x, s2[v] = p.y;
     }
-    const T* x = (const T*)k.x + (int64_t)it.n * k.x_sample + it.column;
-    const T* dy = (const T*)k.dy + (int64_t)it.n * k.dy_sample + it.column;
-    T* dx = (T*)k.y + it.n * k.pixels * k.width + it.column;
+    const int64_t end = (int64_t)k.pixels - 1;
+    const T* x = (const T*)k.x + (int64_t)n * k.x_sample + end * k.x_pitch + it.column;
+    const T* dy = (const T*)k.dy + (int64_t)n * k.dy_sample + end * k.dy_pitch + it.column;
+    T* dx = (T*)k.y + (n * k.pixels + end) * k.width + it.column;
     with_act(k.act, [&](auto act) {
-      for_pixel_pairs<T, V, 2>(it.first + it.row, it.last, plan.threads_rows,
+      for_pixel_pairs<T, V, 2>(it.first, k.pixels, it.step,
                                [&](uint64_t p, Run<T, V>& r, Run<T, V>& g) {
-        r.load(x + (int64_t)p * k.x_pitch);
-        g.load(dy + (int64_t)p * k.dy_pitch);
+        r.load(x - (int64_t)p * k.x_pitch);
+        g.load(dy - (int64_t)p * k.dy_pitch);
       }, [&](uint64_t p, const Run<T, V>& r, const Run<T, V>& g) {
         Run<T, V> out;
 #pragma unroll
@@ -723,7 +788,7 @@ __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan
                           act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v])) * col.w[v];
           out.v[v] = from_f32<T>(col.rstd[v] * (d - s1[v] - xh * s2[v]));
         }
-        out.store(dx + p * k.width);
+        out.store(dx - p * k.width);
       });
     });
   }
@@ -786,24 +851,57 @@ static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32
   return true;
 }
 
-static StreamPlan stream_plan(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
-                              uint32_t v) {
+// Whether the partial values are few enough to be joined by each workgroup that reads them.
+static bool gn_joined(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
+                      uint32_t v) {
+  return width / v <= TILE_VECTORS && width <= JOINED_WIDTH && width / groups <= JOINED_EACH &&
+         samples * pixels * width < JOINED_BELOW;
+}
+
+// About `workgroups` of them, each with 8 pixels a thread at least; `most` chunks of a sample.
+static StreamPlan stream_plan(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t v,
+                              uint64_t workgroups, uint64_t most) {
   StreamPlan plan;
   const uint32_t vectors = width / v;
   plan.tiles = (vectors + TILE_VECTORS - 1) / TILE_VECTORS;
   plan.columns = (vectors + plan.tiles - 1) / plan.tiles;
   plan.threads_rows = 256 / plan.columns;
-  // about 2048 workgroups, each with 8 pixels a thread at least
-  uint64_t wanted = std::max<uint64_t>(1, 2048 / std::max<uint64_t>(1, samples * plan.tiles));
-  plan.joined = plan.tiles == 1 && width <= JOINED_WIDTH && width / groups <= JOINED_EACH &&
-                samples * pixels * width < JOINED_BELOW;
-  if (plan.joined) wanted = std::min<uint64_t>(wanted, std::max(1u, JOINED_ENTRIES / width));
-  const uint64_t least = 8ull * plan.threads_rows;
-  plan.chunk = std::max((pixels + wanted - 1) / wanted, least);
-  plan.chunk = (plan.chunk + plan.threads_rows - 1) / plan.threads_rows * plan.threads_rows;
-  plan.chunks = (uint32_t)((pixels + plan.chunk - 1) / plan.chunk);
-  plan.items = samples * plan.tiles * plan.chunks;
+  const uint64_t wanted =
+      std::min(std::max<uint64_t>(1, workgroups / std::max<uint64_t>(1, samples * plan.tiles)), most);
+  plan.chunks = (uint32_t)std::min(wanted, (pixels + 8 * plan.threads_rows - 1) /
+                                               (8 * plan.threads_rows));
+  plan.at_once = (uint32_t)std::min<uint64_t>(
+      samples,
+      std::max<uint64_t>(1, std::min<uint64_t>(65535, (1u << 23) / (plan.tiles * plan.chunks))));
   return plan;
+}
+
+// The plans of the four streaming launches.
+struct StreamPlans {
+  uint32_t v;
+  bool joined;
+  StreamPlan stats, apply, sums, dx;
+  Parts parts_of(const StreamPlan& plan) const { return {plan.chunks, plan.threads_rows, joined}; }
+};
+
+static StreamPlans stream_plans(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
+                                int32_t dtype) {
+  StreamPlans p;
+  p.v = vector_of(width, dtype);
+  p.joined = gn_joined(samples, pixels, width, groups, p.v);
+  const uint64_t most = p.joined ? std::max<uint64_t>(1, JOINED_ENTRIES / width) : 1ull << 30;
+  const auto plan = [&](uint64_t workgroups, uint64_t most) {
+    return stream_plan(samples, pixels, width, p.v, workgroups, most);
+  };
+  p.stats = plan(1024, most);
+  p.apply = plan(2048, 1ull << 30);
+  p.sums = plan(2048, most);
+  p.dx = plan(2048, 1ull << 30);
+  return p;
+}
+
+static dim3 grid_of(const StreamPlan& plan) {
+  return dim3(plan.chunks, plan.tiles, plan.at_once);
 }
 
 static uint32_t capped(uint64_t n) { return (uint32_t)std::min<uint64_t>(n, 1u << 20); }
@@ -876,8 +974,8 @@ extern "C" uint64_t tgs_group_norm_fwd_workspace_size(uint64_t samples, uint64_t
   if (!gn_sizes_ok(samples, pixels, width, groups, dtype) || samples == 0 || pixels == 0 ||
       gn_held(samples, pixels, width, groups, dtype, held))
     return 0;
-  const StreamPlan plan = stream_plan(samples, pixels, width, groups, vector_of(width, dtype));
-  return samples * plan.chunks * width * sizeof(float2);
+  const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
+  return samples * plans.stats.chunks * width * sizeof(float2);
 }
 
 extern "C" uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t pixels,
@@ -887,8 +985,8 @@ extern "C" uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t
   if (!gn_sizes_ok(samples, pixels, width, groups, dtype) || samples == 0 || pixels == 0) return 0;
   if (gn_held(samples, pixels, width, groups, dtype, held))
     return (uint64_t)held.partials * 2 * width * sizeof(float);
-  const StreamPlan plan = stream_plan(samples, pixels, width, groups, vector_of(width, dtype));
-  return samples * sizeof(float2) * ((uint64_t)plan.chunks * width + groups);
+  const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
+  return samples * sizeof(float2) * ((uint64_t)plans.sums.chunks * width + groups);
 }
 
 #define GN_CHECK_CALL(name)                                                                      \
@@ -931,23 +1029,24 @@ extern "C" int tgs_group_norm_fwd(uint64_t samples, uint64_t pixels, uint32_t wi
   }
   TGS_CHECK_ARG(workspace && (uintptr_t)workspace % 8 == 0 && (uintptr_t)stats % 8 == 0,
                 "tgs_group_norm_fwd: the workspace and the stats start on 8 bytes");
-  const uint32_t v = vector_of(width, dtype);
-  const StreamPlan plan = stream_plan(samples, pixels, width, groups, v);
-  const dim3 grid(capped(plan.items)), by_group(capped(samples * groups));
+  const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
+  const Parts parts = plans.parts_of(plans.stats);
   float2* partial = (float2*)workspace;
-  with_vector(dtype, v, [&](auto tag, auto vec) {
+  with_vector(dtype, plans.v, [&](auto tag, auto v) {
     using T = decltype(tag);
-    hipLaunchKernelGGL((group_norm_stats_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
-                       plan, partial);
-    if (plan.joined) {
-      hipLaunchKernelGGL((group_norm_apply_kernel<T, vec.value, true>), grid, dim3(256), 0, stream,
-                         k, plan, partial);
-      return;
-    }
-    hipLaunchKernelGGL(group_norm_finish_kernel, by_group, dim3(1024), 0, stream, k, plan,
-                       partial);
-    hipLaunchKernelGGL((group_norm_apply_kernel<T, vec.value, false>), grid, dim3(256), 0, stream,
-                       k, plan, nullptr);
+    hipLaunchKernelGGL((group_norm_stats_kernel<T, v.value>), grid_of(plans.stats), dim3(256), 0,
+                       stream, k, plans.stats, partial);
+    if (!parts.joined)
+      hipLaunchKernelGGL(group_norm_finish_kernel, dim3(capped(samples * groups)), dim3(1024), 0,
+                         stream, k, parts, partial);
+    const auto apply = [&](auto kernel) {
+      hipLaunchKernelGGL(kernel, grid_of(plans.apply), dim3(256), 0, stream, k, plans.apply, parts,
+                         partial);
+    };
+    if (parts.joined)
+      apply(group_norm_apply_kernel<T, v.value, true>);
+    else
+      apply(group_norm_apply_kernel<T, v.value, false>);
   });
   TGS_RETURN_LAUNCH("tgs_group_norm_fwd");
 }
@@ -995,29 +1094,30 @@ extern "C" int tgs_group_norm_bwd(uint64_t samples, uint64_t pixels, uint32_t wi
   } else {
     TGS_CHECK_ARG(stats && (uintptr_t)stats % 8 == 0,
                   "tgs_group_norm_bwd: the stats of the forward are needed, on 8 bytes");
-    const uint32_t v = vector_of(width, dtype);
-    const StreamPlan plan = stream_plan(samples, pixels, width, groups, v);
-    TGS_CHECK_ARG(!sums || samples * plan.chunks < (1ull << 32),
+    const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
+    const Parts parts = plans.parts_of(plans.sums);
+    TGS_CHECK_ARG(!sums || samples * parts.chunks < (1ull << 32),
                   "tgs_group_norm_bwd: too many samples for their sums");
-    const dim3 grid(capped(plan.items)), by_group(capped(samples * groups));
     float2* partial = (float2*)workspace;
-    float2* group_sums = partial + samples * plan.chunks * width;
-    with_vector(dtype, v, [&](auto tag, auto vec) {
+    float2* group_sums = partial + samples * parts.chunks * width;
+    with_vector(dtype, plans.v, [&](auto tag, auto v) {
       using T = decltype(tag);
-      hipLaunchKernelGGL((group_norm_sums_kernel<T, vec.value>), grid, dim3(256), 0, stream, k,
-                         plan, partial);
+      hipLaunchKernelGGL((group_norm_sums_kernel<T, v.value>), grid_of(plans.sums), dim3(256), 0,
+                         stream, k, plans.sums, partial);
       if (!dx) return;
-      if (plan.joined) {
-        hipLaunchKernelGGL((group_norm_dx_kernel<T, vec.value, true>), grid, dim3(256), 0, stream,
-                           k, plan, partial);
-        return;
-      }
-      hipLaunchKernelGGL(group_norm_group_sums_kernel<T>, by_group, dim3(1024), 0, stream, k, plan,
-                         partial, group_sums);
-      hipLaunchKernelGGL((group_norm_dx_kernel<T, vec.value, false>), grid, dim3(256), 0, stream,
-                         k, plan, group_sums);
+      if (!parts.joined)
+        hipLaunchKernelGGL(group_norm_group_sums_kernel<T>, dim3(capped(samples * groups)),
+                           dim3(1024), 0, stream, k, parts, partial, group_sums);
+      const auto launch = [&](auto kernel, const float2* from) {
+        hipLaunchKernelGGL(kernel, grid_of(plans.dx), dim3(256), 0, stream, k, plans.dx, parts,
+                           from);
+      };
+      if (parts.joined)
+        launch(group_norm_dx_kernel<T, v.value, true>, partial);
+      else
+        launch(group_norm_dx_kernel<T, v.value, false>, group_sums);
     });
-    join((uint32_t)(samples * plan.chunks), (const float*)partial);
+    join((uint32_t)(samples * parts.chunks), (const float*)partial);
   }
   TGS_RETURN_LAUNCH("tgs_group_norm_bwd");
 }
