@@ -10,7 +10,7 @@
 //
 // Memory bound.  Two ways, by the size of a group:
 //
-// Held (up to 8 runs of 16 bytes a lane of up to 64, or of a workgroup's 256): a team of lanes
+// Held (up to 4 runs of 16 bytes a lane of 64, or 8 of a workgroup's 256): a team of lanes
 // keeps a group in registers, so x is read once and one launch does all.  The backward computes
 // mean and rstd again.
 //
@@ -26,11 +26,12 @@
 #include "vector_io.cuh"
 
 #define ACT_NONE 3
-#define HELD_RUNS 8     // runs of a lane at most
+#define HELD_RUNS 8      // runs of a lane at most where the team is a workgroup
+#define HELD_FEW 4       // and in a wavefront (eight took 460 registers in the backward)
 #define TILE_VECTORS 64  // vectors of channels of a streaming workgroup
 #define JOINED_WIDTH 512     // channels, channels of a group and partial values of a sample that
 #define JOINED_EACH 64       // the workgroups that read them join for themselves, and
-#define JOINED_ENTRIES 8192
+#define JOINED_ENTRIES 4096
 #define JOINED_BELOW (1u << 24)  // values of x up to which that is done
 
 struct GnCall {
@@ -47,6 +48,8 @@ struct GnCall {
   float2* stats;  // mean and rstd of each sample's group
 };
 
+// Calls f with the activation as a constant.  The kernels do so around their loops: inside of them
+// the four forms' registers add up (held backward of one run: 121, outside 86).
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F&& f) {
   if (act == ACT_SILU)
@@ -134,6 +137,7 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
     w[v] = live ? column<T>(k.weight, k.wide_weights, c0 + v, 1.f) : 0.f;
     b[v] = live ? column<T>(k.bias, k.wide_weights, c0 + v, 0.f) : 0.f;
   }
+  with_act(k.act, [&](auto act) {
   for (uint64_t n = id / k.groups; works && n < k.samples; n += plan.rows) {
     const T* x = (const T*)k.x + (int64_t)n * k.x_sample + c0;
     Run<T, V> in[E], grad[BACKWARD ? E : 1];
@@ -170,54 +174,71 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
     const float rstd = __builtin_amdgcn_rsqf(fmaf(team_sum<WIDE>(squares, team_log), inv, k.eps));
     T* y = (T*)k.y + (n * k.pixels) * k.width + c0;
     if constexpr (!BACKWARD) {
-      with_act(k.act, [&](auto act) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t p = row + ((uint32_t)e << plan.row_log);
-          if (!live || p >= k.pixels) continue;
-          Run<T, V> out;
+      for (int e = 0; e < E; ++e) {
+        const uint32_t p = row + ((uint32_t)e << plan.row_log);
+        if (!live || p >= k.pixels) continue;
+        Run<T, V> out;
 #pragma unroll
-          for (int v = 0; v < V; ++v)
-            out.v[v] = from_f32<T>(
-                act_value<act.value, T>(fmaf(xh[e][v] * rstd, w[v], b[v])));
-          out.store(y + (uint64_t)p * k.width);
-        }
-      });
+        for (int v = 0; v < V; ++v)
+          out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh[e][v] * rstd, w[v], b[v])));
+        out.store(y + (uint64_t)p * k.width);
+      }
     } else {
-      float dz[E][V], s1 = 0.f, s2 = 0.f;
-      with_act(k.act, [&](auto act) {
+      // Few runs keep xhat and dz w for the second pass over the team's values; many would take
+      // 128 registers for them (and the kernel 36 us in place of LEAN_US, 16 samples of 1020 pixels
+      // and 512 half channels) and compute them again.
+      constexpr bool KEEP = E <= HELD_FEW / 2;
+      float g[KEEP ? E : 1][V], s1 = 0.f, s2 = 0.f;
+      const auto ok = [&](int e) {
+        return live && row + ((uint32_t)e << plan.row_log) < k.pixels;
+      };
+      const auto both = [&](int e, int v, float& xhat, float& dz) {
+        xhat = (to_f32(in[e].v[v]) - mean) * rstd;
+        dz = to_f32(grad[e].v[v]) * act_slope<act.value, T>(fmaf(xhat, w[v], b[v]));
+      };
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const bool ok = live && row + ((uint32_t)e << plan.row_log) < k.pixels;
+      for (int e = 0; e < E; ++e) {
+        if (!ok(e)) continue;
 #pragma unroll
-          for (int v = 0; v < V; ++v) {
-            xh[e][v] *= rstd;
-            const float z = fmaf(xh[e][v], w[v], b[v]);
-            dz[e][v] = ok ? to_f32(grad[e].v[v]) * act_slope<act.value, T>(z) : 0.f;
-            dw[v] = fmaf(dz[e][v], xh[e][v], dw[v]);
-            db[v] += dz[e][v];
-            dz[e][v] *= w[v];
-            s1 += dz[e][v];
-            s2 = fmaf(dz[e][v], xh[e][v], s2);
+        for (int v = 0; v < V; ++v) {
+          float xhat, dz;
+          both(e, v, xhat, dz);
+          dw[v] = fmaf(dz, xhat, dw[v]);
+          db[v] += dz;
+          dz *= w[v];
+          s1 += dz;
+          s2 = fmaf(dz, xhat, s2);
+          if constexpr (KEEP) xh[e][v] = xhat, g[e][v] = dz;
+        }
+      }
+      if (!k.y) continue;
+      s1 = team_sum<WIDE>(s1, team_log) * inv;
+      s2 = team_sum<WIDE>(s2, team_log) * inv;
+      if constexpr (!KEEP) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) in[e].forget(), grad[e].forget();
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (!ok(e)) continue;
+        Run<T, V> out;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+          float xhat, dz;
+          if constexpr (KEEP) {
+            xhat = xh[e][v], dz = g[e][v];
+          } else {
+            both(e, v, xhat, dz);
+            dz *= w[v];
           }
+          out.v[v] = from_f32<T>(rstd * (dz - s1 - xhat * s2));
         }
-      });
-      if (k.y) {
-        s1 = team_sum<WIDE>(s1, team_log) * inv;
-        s2 = team_sum<WIDE>(s2, team_log) * inv;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t p = row + ((uint32_t)e << plan.row_log);
-          if (!live || p >= k.pixels) continue;
-          Run<T, V> out;
-#pragma unroll
-          for (int v = 0; v < V; ++v)
-            out.v[v] = from_f32<T>(rstd * (dz[e][v] - s1 - xh[e][v] * s2));
-          out.store(y + (uint64_t)p * k.width);
-        }
+        out.store(y + (uint64_t)(row + ((uint32_t)e << plan.row_log)) * k.width);
       }
     }
   }
+  });
   if constexpr (BACKWARD) {
     if (!partial) return;
     if constexpr (!WIDE) {
@@ -543,7 +564,7 @@ __device__ __forceinline__ void sum_by_channel(const GnCall& k, const Parts& par
   for (uint32_t t = threadIdx.x; t < along * k.width; t += 256) {
     const uint32_t c = t % k.width;
     float2 a = {0.f, 0.f};
-#pragma unroll 8
+#pragma unroll 16
     for (uint32_t q = t / k.width; q < parts.chunks; q += along) {
       const float2 p = entry(q, c);
       a.x += p.x, a.y += p.y;
@@ -628,17 +649,17 @@ __device__ __forceinline__ void join_sums(const GnCall& k, const Parts& parts,
   });
 }
 
-// What a thread needs of its channels; `stats` of this sample's groups.
+// What a thread needs of its channels, z = (x - mean) w rstd + b; `stats` of this sample's groups.
 template <typename T, int V>
 struct Columns {
-  float mean[V], rstd[V], w[V], b[V];
+  float mean[V], rstd[V], factor[V], b[V];
   __device__ __forceinline__ void load(const GnCall& k, const Item& it, const float2* stats) {
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const uint32_t c = it.column + v;
       const float2 st = stats[c / k.each];
       mean[v] = st.x, rstd[v] = st.y;
-      w[v] = column<T>(k.weight, k.wide_weights, c, 1.f);
+      factor[v] = column<T>(k.weight, k.wide_weights, c, 1.f) * rstd[v];
       b[v] = column<T>(k.bias, k.wide_weights, c, 0.f);
     }
   }
@@ -673,8 +694,8 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamP
         Run<T, V> out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
-          out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh, col.w[v], col.b[v])));
+          const float d = to_f32(r.v[v]) - col.mean[v];
+          out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(d, col.factor[v], col.b[v])));
         }
         out.store(y - p * k.width);
       });
@@ -694,8 +715,6 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
     Columns<T, V> col;
     if (it.live) {
       col.load(k, it, k.stats + n * k.groups);
-#pragma unroll
-      for (int v = 0; v < V; ++v) col.w[v] *= col.rstd[v];
       const T* x = (const T*)k.x + (int64_t)n * k.x_sample + it.column;
       const T* dy = (const T*)k.dy + (int64_t)n * k.dy_sample + it.column;
       with_act(k.act, [&](auto act) {
@@ -707,7 +726,7 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float d = to_f32(r.v[v]) - col.mean[v];
-            const float dz = to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.w[v], col.b[v]));
+            const float dz = to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
             db[v] += dz;
             dw[v] = fmaf(dz, d, dw[v]);
           }
@@ -764,11 +783,12 @@ __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan
     if (!it.live) continue;
     Columns<T, V> col;
     col.load(k, it, k.stats + n * k.groups);
+    // dx = factor dz - s1 - xhat s2 (rstd twice in s2 would leave float32 for large spreads)
     float s1[V], s2[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const float2 p = sums[(it.column + v) / k.each];
-      s1[v] = p.x, s2[v] = p.y;
+      s1[v] = p.x * col.rstd[v], s2[v] = p.y * col.rstd[v];
     }
     const int64_t end = (int64_t)k.pixels - 1;
     const T* x = (const T*)k.x + (int64_t)n * k.x_sample + end * k.x_pitch + it.column;
@@ -783,10 +803,10 @@ __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan
         Run<T, V> out;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          const float xh = (to_f32(r.v[v]) - col.mean[v]) * col.rstd[v];
-          const float d = to_f32(g.v[v]) *
-                          act_slope<act.value, T>(fmaf(xh, col.w[v], col.b[v])) * col.w[v];
-          out.v[v] = from_f32<T>(col.rstd[v] * (d - s1[v] - xh * s2[v]));
+          const float d = to_f32(r.v[v]) - col.mean[v];
+          const float dz =
+              to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
+          out.v[v] = from_f32<T>(fmaf(-d * col.rstd[v], s2[v], fmaf(dz, col.factor[v], -s1[v])));
         }
         out.store(dx - p * k.width);
       });
@@ -820,8 +840,7 @@ static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32
   plan.wide = false;
   if (plan.lane_log > 8 || pixels > 256 * HELD_RUNS) return false;
   const int rows = log2_up(pixels);
-  if (plan.lane_log > 6 || (pixels + (64u >> plan.lane_log) - 1) / (64u >> plan.lane_log) >
-                               HELD_RUNS) {
+  if (plan.lane_log > 6 || pixels > HELD_FEW * (64u >> plan.lane_log)) {
     plan.wide = true;  // (the rows fill the workgroup: idle ones cost nothing)
     plan.row_log = 8 - plan.lane_log;
     plan.runs = (int)((pixels + (1u << plan.row_log) - 1) >> plan.row_log);
@@ -944,7 +963,7 @@ static void held_launch(const GnCall& k, const HeldPlan& plan, int32_t dtype, fl
       };
       if (plan.wide)
         start(group_norm_held_kernel<T, v.value, runs.value, BACKWARD, true>);
-      else
+      else if constexpr (runs.value <= HELD_FEW)
         start(group_norm_held_kernel<T, v.value, runs.value, BACKWARD, false>);
     };
     if (plan.runs == 1)

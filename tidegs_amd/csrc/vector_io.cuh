@@ -45,4 +45,14 @@ struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Run {
   T v[N];
   __device__ __forceinline__ void load(const T* p) { load_bytes<N * sizeof(T)>(v, p); }
   __device__ __forceinline__ void store(T* p) const { store_bytes<N * sizeof(T)>(p, v); }
+  // Makes the compiler take the values for new ones: what was computed from them is computed
+  // again rather than kept in registers.
+  __device__ __forceinline__ void forget() {
+    if constexpr (sizeof(v) % 4 == 0) {
+#pragma unroll
+      for (int k = 0; k < (int)sizeof(v) / 4; ++k) asm volatile("" : "+v"(((uint32_t*)v)[k]));
+    } else {
+      asm volatile("" : "+v"(*(uint16_t*)v));
+    }
+  }
 };
