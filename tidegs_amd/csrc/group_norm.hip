@@ -241,29 +241,35 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
   });
   if constexpr (BACKWARD) {
     if (!partial) return;
-    if constexpr (!WIDE) {
+    // over the rows of a wavefront
+    const int in_wave = min(team_log, 6);
 #pragma unroll
-      for (int v = 0; v < V; ++v)
-        for (int j = lane_log; j < team_log; ++j) {
-          dw[v] += __shfl_xor(dw[v], 1 << j, 64);
-          db[v] += __shfl_xor(db[v], 1 << j, 64);
-        }
-      if (plan.teams < k.groups) {  // no two teams of a workgroup have the same channels
-        if (live && row == 0) {
-          float2* out = (float2*)partial + id / k.groups * k.width + c0;
-#pragma unroll
-          for (int v = 0; v < V; ++v) out[v] = {db[v], dw[v]};
-        }
-        return;
+    for (int v = 0; v < V; ++v)
+      for (int j = lane_log; j < in_wave; ++j) {
+        dw[v] += __shfl_xor(dw[v], 1 << j, 64);
+        db[v] += __shfl_xor(db[v], 1 << j, 64);
       }
-    }
-    __shared__ float2 s[256 * V];
+    if (!WIDE && plan.teams < k.groups) {  // no two teams of a workgroup have the same channels
+      if (live && row == 0) {
+        float2* out = (float2*)partial + id / k.groups * k.width + c0;
 #pragma unroll
-    for (int v = 0; v < V; ++v) s[threadIdx.x * V + v] = {db[v], dw[v]};
+        for (int v = 0; v < V; ++v) out[v] = {db[v], dw[v]};
+      }
+      return;
+    }
+    // WIDE: over the wavefronts (one row of each, all rows where a row is longer than one);
+    // otherwise over the teams of the same group
+    __shared__ float2 s[256 * V];
+    const int rows_log = WIDE ? max(6 - lane_log, 0) : 0;
+    const uint32_t at = WIDE ? ((row >> rows_log) << lane_log) + lane : threadIdx.x;
+    if (!WIDE || (row & ((1u << rows_log) - 1)) == 0) {
+#pragma unroll
+      for (int v = 0; v < V; ++v) s[at * V + v] = {db[v], dw[v]};
+    }
     __syncthreads();
-    // WIDE: the sum over the team's rows; otherwise over the teams of the same group
-    const uint32_t channels = WIDE ? k.each : k.width, count = WIDE ? 1u << plan.row_log : plan.teams;
-    const uint32_t step = WIDE ? 1 : k.groups, stride = (WIDE ? 1u << lane_log : 1u << team_log) * V;
+    const uint32_t channels = WIDE ? k.each : k.width, step = WIDE ? 1 : k.groups;
+    const uint32_t count = WIDE ? 1u << (plan.row_log - rows_log) : plan.teams;
+    const uint32_t stride = (1u << (WIDE ? lane_log : team_log)) * V;
     float2* out = (float2*)partial + (WIDE ? id / k.groups * k.width + group * k.each
                                            : (uint64_t)blockIdx.x * k.width);
     for (uint32_t c = threadIdx.x; c < channels; c += 256) {
@@ -857,7 +863,7 @@ static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32
   if (teams >= groups) {
     const uint32_t each_wg = teams / groups;  // samples of a workgroup at once
     plan.teams = each_wg * groups;
-    plan.grid = (uint32_t)std::min<uint64_t>((samples + each_wg - 1) / each_wg, 2048);
+    plan.grid = (uint32_t)std::min<uint64_t>((samples + each_wg - 1) / each_wg, 1280);
     plan.rows = plan.grid * each_wg;
     plan.partials = plan.grid;
   } else {
