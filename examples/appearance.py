@@ -72,7 +72,7 @@ def train(steps, decoded=True, seed=0, dtype=torch.bfloat16, say=lambda *a: None
         decoder = AppearanceDecoder(len(images), width=32, hidden=64, dtype=dtype).cuda()
         features = (torch.randn(scene.n, 32, device="cuda") * 0.5).requires_grad_()
         groups += [dict(params=decoder.parameters(), lr=5e-3), dict(params=[features], lr=5e-3)]
-    optimizer = torch.optim.Adam(groups)
+    optimizer = tg.AdamW(groups, weight_decay=0.0)
 
     def colors(camera, step=None):
         return decoder(features, camera, step) if decoded else None

@@ -312,6 +312,16 @@ def stream_handle(device=None) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
+def launch(device: torch.device, name: str, *args) -> None:
+    """Calls an entry point, whose last argument is its stream, on ``device``'s current one and
+    with it as the current device."""
+    if device.index == torch._C._cuda_getDevice():
+        call(name, *args, stream_handle(device))
+    else:
+        with torch.cuda.device(device):
+            call(name, *args, stream_handle(device))
+
+
 def require_cuda(*tensors, names=None) -> None:
     for i, t in enumerate(tensors):
         if t is None:

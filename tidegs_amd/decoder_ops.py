@@ -214,9 +214,8 @@ def _group_norm_fwd(x, groups, weight, bias, eps, act):
     nbytes = _workspace_size("tgs_group_norm_fwd_workspace_size", *sizes)
     stats = torch.empty(kept, dtype=torch.uint8, device=x.device) if kept else None
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    N.call("tgs_group_norm_fwd", *sizes, act, x.data_ptr(), sample, pitch, N.ptr(weight),
-           N.ptr(bias), w_code, eps, y.data_ptr(), N.ptr(stats), N.ptr(ws), nbytes,
-           N.stream_handle(x.device))
+    N.launch(x.device, "tgs_group_norm_fwd", *sizes, act, x.data_ptr(), sample, pitch,
+             N.ptr(weight), N.ptr(bias), w_code, eps, y.data_ptr(), N.ptr(stats), N.ptr(ws), nbytes)
     return x, y, stats, (sizes, act, sample, pitch, w_code, eps)
 
 
@@ -238,9 +237,9 @@ class _GroupNorm(torch.autograd.Function):
         db = bias.new_empty(bias.shape) if need_b else None
         nbytes = _workspace_size("tgs_group_norm_bwd_workspace_size", *sizes)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.call("tgs_group_norm_bwd", *sizes, act, x.data_ptr(), sample, pitch, dy.data_ptr(),
-               dy_sample, dy_pitch, N.ptr(weight), N.ptr(bias), w_code, eps, N.ptr(stats),
-               N.ptr(dx), N.ptr(dw), N.ptr(db), ws.data_ptr(), nbytes, N.stream_handle(x.device))
+        N.launch(x.device, "tgs_group_norm_bwd", *sizes, act, x.data_ptr(), sample, pitch,
+                 dy.data_ptr(), dy_sample, dy_pitch, N.ptr(weight), N.ptr(bias), w_code, eps,
+                 N.ptr(stats), N.ptr(dx), N.ptr(dw), N.ptr(db), ws.data_ptr(), nbytes)
         return dx, None, dw, db, None, None
 
 

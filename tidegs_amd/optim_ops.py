@@ -35,15 +35,6 @@ _data_ptr, _numel, _contiguous = Tensor.data_ptr, Tensor.numel, Tensor.is_contig
 _get_device, _same_size = Tensor.get_device, Tensor.is_same_size
 
 
-def _launch(device: torch.device, name: str, *args) -> None:
-    """Calls an entry point on ``device``'s current stream, with it as the current device."""
-    if device.index == torch._C._cuda_getDevice():
-        N.call(name, *args, N.stream_handle(device))
-    else:
-        with torch.cuda.device(device):
-            N.call(name, *args, N.stream_handle(device))
-
-
 def _rows_of(columns: Sequence[Sequence[int]], n: int) -> array.array:
     """The columns' values row by row.  Few rows go through a list: 2.3 us in place of 4.7 for one,
     8 in place of 11 for 17; 74 in place of 46 for 200."""
@@ -92,7 +83,7 @@ def grad_norm(tensors: Iterable[Tensor]) -> Tensor:
     norm = torch.empty((), dtype=torch.float32, device=device)
     nbytes = _workspace_size("tgs_grad_norm_workspace_size", n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    _launch(device, "tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(), ws.data_ptr(),
+    N.launch(device, "tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(), ws.data_ptr(),
             nbytes)
     return norm
 
@@ -225,7 +216,7 @@ class _Call:
         if live:
             nbytes = _workspace_size("tgs_adamw_workspace_size", self.n_groups)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        _launch(device, "tgs_adamw", n, tensors.buffer_info()[0], self.n_groups, self.groups,
+        N.launch(device, "tgs_adamw", n, tensors.buffer_info()[0], self.n_groups, self.groups,
                 self.bits, seed, N.ptr(norm), max_norm, N.ptr(ws), nbytes)
         increment_version(params)
 
