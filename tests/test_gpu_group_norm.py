@@ -23,6 +23,11 @@ HELD = [(1, 1, 1, 1), (1, 1, 8, 1), (2, 1, 8, 4), (3, 1, 64, 4), (1000, 1, 59, 1
         (2, 64, 64, 8), (5, 17, 40, 5), (4, 64, 6, 6), (9, 8, 12, 3), (300, 3, 512, 32),
         (2, 4, 520, 65), (5000, 2, 16, 2), (2, 9, 512, 1), (3, 512, 8, 1), (6, 100, 31, 31),
         (4, 2, 2048, 256)]
+# groups and pixels that are no whole number of vectors: overlapping ones, by teams and streamed
+RAGGED = [(2000, 1, 360, 8), (50, 7, 777, 1), (3, 1, 1036, 1), (3, 1, 4124, 1), (10, 1, 2044, 1),
+          (90, 3, 35, 5), (90, 3, 36, 6), (90, 3, 42, 6), (20, 30, 118, 2), (4, 200, 57, 3),
+          (2, 900, 59, 1), (1, 700, 5, 5), (2, 600, 13, 1), (1, 520, 1003, 17), (1, 600, 1001, 7),
+          (2, 40, 4097, 1), (2, 1100, 6, 1), (3, 2100, 2, 1), (2, 5000, 515, 5)]
 STREAMED = [(4, 1, 1024, 1), (2, 1000, 64, 8), (1, 5000, 3, 1), (3, 777, 48, 6), (1, 20011, 32, 8),
             (2, 33, 1000, 4), (1, 600, 520, 1), (2, 100, 4096, 2), (40, 513, 8, 8),
             (1, 2, 65536, 2), (2, 3000, 20, 5), (1, 513, 7, 7)]
@@ -115,7 +120,7 @@ def _check(x, w, b, dy, groups, act, eps=1e-5):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("shape", HELD + STREAMED)
+@pytest.mark.parametrize("shape", HELD + STREAMED + RAGGED)
 def test_values_and_gradients(gpu, shape, dtype):
     act = ACTS[(sum(shape) + TYPES.index(dtype)) % 4]
     announce(f"group_norm {shape} {dtype} {act}")
@@ -130,7 +135,8 @@ def test_activations(gpu, shape, dtype, act):
     _check(*_inputs(shape, dtype, seed=1), shape[3], act)
 
 
-@pytest.mark.parametrize("shape", [(30, 12, 48, 6), (2, 900, 48, 6), (3, 50, 59, 1)])
+@pytest.mark.parametrize("shape", [(30, 12, 48, 6), (2, 900, 48, 6), (3, 50, 59, 1),
+                                   (2, 1500, 59, 1)])
 def test_layouts(gpu, shape):
     """Columns of wider rows, every second sample, an expanded sample, other orders of x and of dy;
     weights in 32 bits, without weights, without a bias."""
