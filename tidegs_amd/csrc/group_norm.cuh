@@ -34,6 +34,7 @@
 #define JOINED_WIDTH 512     // channels, channels of a group and partial values of a sample that
 #define JOINED_EACH 64       // the workgroups that read them join for themselves, and
 #define JOINED_ENTRIES 4096
+#define JOINED_WORKGROUPS 192  // that leave them
 #define JOINED_BELOW (1u << 24)  // values of x up to which that is done
 
 struct GnCall {
@@ -804,6 +805,11 @@ struct StreamPlans {
   bool joined;
   StreamPlan stats, apply, sums, dx;
   Parts parts_of(const StreamPlan& plan) const { return {plan.chunks, plan.threads_rows, joined}; }
+  // Whether a launch's partial values are joined by channel first: a group has too many of them
+  // for one workgroup.
+  bool by_channel(const StreamPlan& plan, uint32_t each) const {
+    return !joined && (uint64_t)plan.chunks * each > JOINED_ENTRIES;
+  }
 };
 
 static inline dim3 grid_of(const StreamPlan& plan) {
@@ -812,8 +818,17 @@ static inline dim3 grid_of(const StreamPlan& plan) {
 
 static inline uint32_t capped(uint64_t n) { return (uint32_t)std::min<uint64_t>(n, 1u << 20); }
 
-// Mean and rstd of each sample's group from the partial values (group_norm.hip).
+// Mean and rstd of each sample's group from the partial values; partial values joined over the
+// chunks (group_norm.hip).
 void gn_finish(const GnCall& k, const Parts& parts, const float2* partial, hipStream_t stream);
+Parts gn_channels(const GnCall& k, const Parts& parts, bool stats, const float2* partial,
+                  float2* out, hipStream_t stream);
+
+// Rows of db and dw by channel, whose sum is the weights' gradients.
+struct SumRows {
+  const float2* first;
+  uint32_t count;
+};
 
 // By type, in a translation unit each (group_norm_f32.hip and its like).
 template <typename T>
@@ -824,8 +839,8 @@ void gn_streamed_fwd(const GnCall& k, const StreamPlans& plans, float2* partial,
                      hipStream_t stream);
 // (k.y null: no dx)
 template <typename T>
-void gn_streamed_bwd(const GnCall& k, const StreamPlans& plans, float2* partial,
-                     float2* group_sums, hipStream_t stream);
+SumRows gn_streamed_bwd(const GnCall& k, const StreamPlans& plans, float2* workspace,
+                        hipStream_t stream);
 
 #ifdef GN_TYPE
 
@@ -886,7 +901,12 @@ void gn_streamed_fwd(const GnCall& k, const StreamPlans& plans, float2* partial,
   with_run<T>(plans.v, [&](auto v) {
     hipLaunchKernelGGL((group_norm_stats_kernel<T, v.value>), grid_of(plans.stats), dim3(256), 0,
                        stream, k, plans.stats, partial);
-    if (!parts.joined) gn_finish(k, parts, partial, stream);
+    if (plans.by_channel(plans.stats, k.each)) {
+      float2* channels = partial + k.samples * parts.chunks * k.width;
+      gn_finish(k, gn_channels(k, parts, true, partial, channels, stream), channels, stream);
+    } else if (!parts.joined) {
+      gn_finish(k, parts, partial, stream);
+    }
     const auto apply = [&](auto kernel) {
       hipLaunchKernelGGL(kernel, grid_of(plans.apply), dim3(256), 0, stream, k, plans.apply, parts,
                          partial);
@@ -899,13 +919,20 @@ void gn_streamed_fwd(const GnCall& k, const StreamPlans& plans, float2* partial,
 }
 
 template <typename T>
-void gn_streamed_bwd(const GnCall& k, const StreamPlans& plans, float2* partial,
-                     float2* group_sums, hipStream_t stream) {
-  const Parts parts = plans.parts_of(plans.sums);
+SumRows gn_streamed_bwd(const GnCall& k, const StreamPlans& plans, float2* workspace,
+                        hipStream_t stream) {
+  Parts parts = plans.parts_of(plans.sums);
+  float2* partial = workspace;
   with_run<T>(plans.v, [&](auto v) {
     hipLaunchKernelGGL((group_norm_sums_kernel<T, v.value>), grid_of(plans.sums), dim3(256), 0,
                        stream, k, plans.sums, partial);
+    if (plans.by_channel(plans.sums, k.each)) {
+      float2* channels = partial + k.samples * parts.chunks * k.width;
+      parts = gn_channels(k, parts, false, partial, channels, stream);
+      partial = channels;
+    }
     if (!k.y) return;
+    float2* group_sums = partial + k.samples * parts.chunks * k.width;
     if (!parts.joined)
       hipLaunchKernelGGL(group_norm_group_sums_kernel<T>, dim3(capped(k.samples * k.groups)),
                          dim3(1024), 0, stream, k, parts, partial, group_sums);
@@ -918,10 +945,11 @@ void gn_streamed_bwd(const GnCall& k, const StreamPlans& plans, float2* partial,
     else
       launch(group_norm_dx_kernel<T, v.value, false>, group_sums);
   });
+  return {partial, (uint32_t)(k.samples * parts.chunks)};
 }
 
 template void gn_held<GN_TYPE>(const GnCall&, const HeldPlan&, bool, float*, hipStream_t);
 template void gn_streamed_fwd<GN_TYPE>(const GnCall&, const StreamPlans&, float2*, hipStream_t);
-template void gn_streamed_bwd<GN_TYPE>(const GnCall&, const StreamPlans&, float2*, float2*,
-                                       hipStream_t);
+template SumRows gn_streamed_bwd<GN_TYPE>(const GnCall&, const StreamPlans&, float2*,
+                                          hipStream_t);
 #endif

@@ -27,27 +27,86 @@ __global__ void __launch_bounds__(1024) group_norm_join_kernel(uint32_t parts, u
   }
 }
 
-// Mean and rstd of each sample's group, a workgroup each, in 64 bits.
+// Each channel's partial values joined over the chunks, 64 channels by 16 runs of chunks a
+// workgroup: for groups of many channels, whose values one workgroup would read for long (one
+// group of 862 channels of 36471 pixels: 231 us the forward, CHANNELS_US with this launch).
+// STATS: means and sums of squared differences, otherwise sums.
+template <bool STATS>
+__global__ void __launch_bounds__(1024) group_norm_channels_kernel(
+    GnCall k, Parts parts, const float2* __restrict__ partial, float2* __restrict__ out) {
+  __shared__ float2 s[1024];
+  const uint32_t c = blockIdx.x * 64 + threadIdx.x % 64;
+  const bool live = c < k.width;
+  for (uint64_t n = blockIdx.y; n < k.samples; n += gridDim.y) {
+    const float2* from = partial + n * parts.chunks * k.width;
+    float2 a = {0.f, 0.f};
+    const float near = STATS && live ? from[c].x : 0.f;
+    if (live) {
+#pragma unroll 8
+      for (uint32_t q = threadIdx.x / 64; q < parts.chunks; q += 16) {
+        const float2 p = from[(uint64_t)q * k.width + c];
+        if constexpr (STATS) {
+          const float d = p.x - near, nd = chunk_pixels(k, parts, q) * d;
+          a.x += nd, a.y += fmaf(nd, d, p.y);
+        } else {
+          a.x += p.x, a.y += p.y;
+        }
+      }
+    }
+    s[threadIdx.x] = a;
+    for (uint32_t h = 512; h >= 64; h >>= 1) {
+      __syncthreads();
+      if (threadIdx.x < h) {
+        s[threadIdx.x].x += s[threadIdx.x + h].x;
+        s[threadIdx.x].y += s[threadIdx.x + h].y;
+      }
+    }
+    if (threadIdx.x < 64 && live) {
+      a = s[threadIdx.x];
+      if constexpr (STATS) {
+        const float mean = a.x / (float)k.pixels;
+        a = {near + mean, fmaxf(fmaf(-mean, a.x, a.y), 0.f)};
+      }
+      out[n * k.width + c] = a;
+    }
+    __syncthreads();
+  }
+}
+
+// Mean and rstd of each sample's group, a workgroup each: sums of 64 bits of differences from
+// the group's first partial mean.
 __global__ void __launch_bounds__(1024) group_norm_finish_kernel(GnCall k, Parts parts,
                                                                  const float2* __restrict__ partial) {
   __shared__ double s[16];
   for (uint64_t i = blockIdx.x; i < k.samples * k.groups; i += gridDim.x) {
     const uint64_t n = i / k.groups;
     const float2* from = partial + n * parts.chunks * k.width + i % k.groups * k.each;
-    const double m = (double)k.pixels * k.each;
+    const double m = (double)k.pixels * k.each, near = from[0].x;
     double a = 0, q = 0;
     for_entries(parts, k.each, [&](uint32_t j, uint32_t c) {
-      a += (double)from[(uint64_t)j * k.width + c].x * chunk_pixels(k, parts, j);
-    });
-    const double mean = sum_of_workgroup<16>(a, s) / m;
-    for_entries(parts, k.each, [&](uint32_t j, uint32_t c) {
       const float2 p = from[(uint64_t)j * k.width + c];
-      const double d = p.x - mean;
-      q += p.y + chunk_pixels(k, parts, j) * d * d;
+      const double d = p.x - near, nd = chunk_pixels(k, parts, j) * d;
+      a += nd;
+      q += p.y + nd * d;
     });
+    a = sum_of_workgroup<16>(a, s) / m;
     q = sum_of_workgroup<16>(q, s) / m;
-    if (threadIdx.x == 0) k.stats[i] = {(float)mean, (float)(1.0 / sqrt(q + (double)k.eps))};
+    if (threadIdx.x == 0)
+      k.stats[i] = {(float)(near + a),
+                    (float)(1.0 / sqrt(fmax(q - a * a, 0.0) + (double)k.eps))};
   }
+}
+
+Parts gn_channels(const GnCall& k, const Parts& parts, bool stats, const float2* partial,
+                  float2* out, hipStream_t stream) {
+  const dim3 grid((k.width + 63) / 64, (unsigned)std::min<uint64_t>(k.samples, 1024));
+  if (stats)
+    hipLaunchKernelGGL(group_norm_channels_kernel<true>, grid, dim3(1024), 0, stream, k, parts,
+                       partial, out);
+  else
+    hipLaunchKernelGGL(group_norm_channels_kernel<false>, grid, dim3(1024), 0, stream, k, parts,
+                       partial, out);
+  return {1, parts.rows, false};
 }
 
 void gn_finish(const GnCall& k, const Parts& parts, const float2* partial, hipStream_t stream) {
@@ -113,13 +172,6 @@ static bool held_plan(uint64_t samples, uint64_t pixels, uint32_t groups, uint32
   return true;
 }
 
-// Whether the partial values are few enough to be joined by each workgroup that reads them.
-static bool gn_joined(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t groups,
-                      uint32_t v) {
-  return width <= v * TILE_VECTORS && width <= JOINED_WIDTH && width / groups <= JOINED_EACH &&
-         samples * pixels * width < JOINED_BELOW;
-}
-
 // About `workgroups` of them, each with 8 pixels a thread at least; `most` chunks of a sample.
 static StreamPlan stream_plan(uint64_t samples, uint64_t pixels, uint32_t width, uint32_t v,
                               uint64_t workgroups, uint64_t most) {
@@ -142,15 +194,24 @@ static StreamPlans stream_plans(uint64_t samples, uint64_t pixels, uint32_t widt
                                 int32_t dtype) {
   StreamPlans p;
   p.v = vector_of(width, dtype);
-  p.joined = gn_joined(samples, pixels, width, groups, p.v);
-  const uint64_t most = p.joined ? std::max<uint64_t>(1, JOINED_ENTRIES / width) : 1ull << 30;
   const auto plan = [&](uint64_t workgroups, uint64_t most) {
     return stream_plan(samples, pixels, width, p.v, workgroups, most);
   };
-  p.stats = plan(1024, most);
-  p.apply = plan(2048, 1ull << 30);
-  p.sums = plan(2048, most);
-  p.dx = plan(2048, 1ull << 30);
+  constexpr uint64_t ANY = 1ull << 30;
+  p.stats = plan(1024, ANY);
+  p.apply = plan(2048, ANY);
+  p.sums = plan(2048, ANY);
+  p.dx = plan(2048, ANY);
+  // Few partial values are joined by each workgroup that reads them, a launch less, if enough
+  // workgroups are left where chunks are made fewer for it.
+  const uint64_t most = std::max<uint64_t>(1, JOINED_ENTRIES / width);
+  p.joined = width <= p.v * TILE_VECTORS && width <= JOINED_WIDTH &&
+             width / groups <= JOINED_EACH && samples * pixels * width < JOINED_BELOW &&
+             (p.stats.chunks <= most || samples * most >= JOINED_WORKGROUPS);
+  if (p.joined) {
+    p.stats = plan(1024, most);
+    p.sums = plan(2048, most);
+  }
   return p;
 }
 
@@ -185,7 +246,8 @@ extern "C" uint64_t tgs_group_norm_fwd_workspace_size(uint64_t samples, uint64_t
       gn_held(samples, pixels, width, groups, dtype, held))
     return 0;
   const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
-  return samples * plans.stats.chunks * width * sizeof(float2);
+  return samples * ((uint64_t)plans.stats.chunks + (plans.by_channel(plans.stats, width / groups) ? 1 : 0)) *
+         width * sizeof(float2);
 }
 
 extern "C" uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t pixels,
@@ -196,7 +258,9 @@ extern "C" uint64_t tgs_group_norm_bwd_workspace_size(uint64_t samples, uint64_t
   if (gn_held(samples, pixels, width, groups, dtype, held))
     return (uint64_t)held.partials * 2 * width * sizeof(float);
   const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
-  return samples * sizeof(float2) * ((uint64_t)plans.sums.chunks * width + groups);
+  const uint64_t rows =
+      (uint64_t)plans.sums.chunks + (plans.by_channel(plans.sums, width / groups) ? 1 : 0);
+  return samples * sizeof(float2) * (rows * width + groups);
 }
 
 // Calls f with a value of the (checked) type.
@@ -299,15 +363,12 @@ extern "C" int tgs_group_norm_bwd(uint64_t samples, uint64_t pixels, uint32_t wi
     TGS_CHECK_ARG(stats && (uintptr_t)stats % 8 == 0,
                   "tgs_group_norm_bwd: the stats of the forward are needed, on 8 bytes");
     const StreamPlans plans = stream_plans(samples, pixels, width, groups, dtype);
-    const Parts parts = plans.parts_of(plans.sums);
-    TGS_CHECK_ARG(!sums || samples * parts.chunks < (1ull << 32),
+    TGS_CHECK_ARG(!sums || samples * plans.sums.chunks < (1ull << 32),
                   "tgs_group_norm_bwd: too many samples for their sums");
-    float2* partial = (float2*)workspace;
-    float2* group_sums = partial + samples * parts.chunks * width;
     by_type(dtype, [&](auto tag) {
-      gn_streamed_bwd<decltype(tag)>(k, plans, partial, group_sums, stream);
+      const SumRows rows = gn_streamed_bwd<decltype(tag)>(k, plans, (float2*)workspace, stream);
+      join(rows.count, (const float*)rows.first);
     });
-    join((uint32_t)(samples * parts.chunks), (const float*)partial);
   }
   TGS_RETURN_LAUNCH("tgs_group_norm_bwd");
 }
