@@ -119,6 +119,21 @@ def test_optimizer_refusals():
     assert opt.state[p]["step"] == 0  # a refused step does not count
 
 
+def test_optimizer_copies_and_loads():
+    import copy
+    import pickle
+
+    p = torch.zeros(3, requires_grad=True)
+    opt = tg.AdamW([p], state_bits=8, seed=5)
+    for other in (copy.deepcopy(opt), pickle.loads(pickle.dumps(opt))):
+        assert (other.state_bits, other.seed, other.capturable) == (8, 5, False)
+        assert other.step() is None
+    saved = dict(state={0: dict(step=1, exp_avg=torch.zeros(1), exp_avg_sq=torch.zeros(1))},
+                 param_groups=tg.AdamW([p]).state_dict()["param_groups"])
+    with pytest.raises(ValueError, match="shape"):
+        tg.AdamW([p]).load_state_dict(saved)
+
+
 def test_dense_orders():
     from tidegs_amd.optim_ops import _is_dense
 
@@ -128,6 +143,26 @@ def test_dense_orders():
         assert _is_dense(x)
     for x in (t[:, :3], t[..., ::2], torch.zeros(1).expand(4), t[:, 0]):
         assert not _is_dense(x)
+
+
+def test_reader_of_lists():
+    """What it does not read itself: the checks one by one follow."""
+    from tidegs_amd.optim_ops import _lists
+
+    r = _lists()
+    t = [torch.zeros(3)]
+    assert r.spans(t) is None and r.spans([]) is None and r.spans([3]) is None
+    assert r.spans(t[0]) is None  # (rows of a tensor)
+    assert r.adamw(t, t, t, t, None, None, 128, [0], [0]) is None
+    assert r.adamw([], [], [], [], None, None, 128, [], []) is None
+    with pytest.raises(TypeError):
+        r.spans(3)
+    with pytest.raises(TypeError, match="nine"):
+        r.adamw(t, t)
+    with pytest.raises(ValueError, match="one length"):
+        r.adamw(t, t, t, [], None, None, 128, [0], [0])
+    with pytest.raises(TypeError):
+        r.adamw(t, t, t, t, None, None, "128", [0], [0])
 
 
 def test_entry_points_check_their_arguments():

@@ -1,23 +1,28 @@
-"""Build the native library ``libtidegs_amd.so`` from ``csrc/*.hip`` with hipcc.
+"""Build the native library ``libtidegs_amd.so`` from ``csrc/*.hip`` with hipcc, and the
+Python module ``_tensor_lists.so`` from ``csrc/tensor_lists.cpp`` with g++.
 
-Every translation unit is compiled for gfx950 only, in parallel, and linked
-into one shared object that exposes the C ABI declared in
+Every translation unit of the library is compiled for gfx950 only, in parallel, and
+linked into one shared object that exposes the C ABI declared in
 ``include/tidegs_amd.h``.  The library links only the HIP runtime: no torch
-types cross the boundary.
+types cross the boundary.  The module, host code alone, reads lists of torch's tensors
+into the rows of pointers that the library takes.
 """
 from __future__ import annotations
 
 import concurrent.futures as cf
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
 CSRC = PKG_DIR / "csrc"
 OBJ_DIR = PKG_DIR / "_build"
 LIB_PATH = PKG_DIR / "libtidegs_amd.so"
+MODULE_PATH = PKG_DIR / "_tensor_lists.so"
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -48,8 +53,23 @@ def _compile(src: Path, hipcc: str) -> Path:
     return obj
 
 
+def _build_module() -> None:
+    torch_dir = Path(importlib.util.find_spec("torch").origin).parent
+    include, lib = torch_dir / "include", torch_dir / "lib"
+    tmp = MODULE_PATH.with_suffix(".so.tmp")
+    cmd = [shutil.which("g++") or "g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-w",
+           "-I", str(include), "-I", str(include / "torch" / "csrc" / "api" / "include"),
+           "-I", sysconfig.get_paths()["include"], str(CSRC / "tensor_lists.cpp"), "-o", str(tmp),
+           f"-L{lib}", f"-Wl,-rpath,{lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for tensor_lists.cpp:\n{proc.stdout}\n{proc.stderr}")
+    os.replace(tmp, MODULE_PATH)
+
+
 def build(verbose: bool = False, jobs: int | None = None) -> Path:
-    """Compile every HIP source and link ``libtidegs_amd.so``; returns its path."""
+    """Compile every HIP source and link ``libtidegs_amd.so``, and the module; returns the
+    library's path."""
     hipcc = _hipcc()
     OBJ_DIR.mkdir(exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
@@ -57,7 +77,9 @@ def build(verbose: bool = False, jobs: int | None = None) -> Path:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     jobs = jobs or min(len(sources), max(1, min(8, os.cpu_count() or 1)))
     with cf.ThreadPoolExecutor(max_workers=jobs) as ex:
+        module = ex.submit(_build_module)
         objs = list(ex.map(lambda s: _compile(s, hipcc), sources))
+        module.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *map(str, objs), "-o", str(tmp)]
     proc = subprocess.run(cmd, capture_output=True, text=True)

@@ -376,7 +376,7 @@ static void adamw_launches(uint32_t n_tensors, const tgs_adamw_tensor* tensors,
     if (t.n == 0 || t.dtype != dtype) continue;
     uint32_t h = std::find(of, of + used, t.group) - of;
     if (b.count == ADAMW_TENSORS || (h == used && used == ADAMW_GROUPS) ||
-        chunks + chunks_of(t.n) > 0xFFFFFFFFull) {
+        chunks + chunks_of(t.n) > 0x7FFFFFFFull) {
       flush();
       h = 0;
     }
@@ -418,7 +418,7 @@ extern "C" int tgs_adamw(uint32_t n_tensors, const tgs_adamw_tensor* tensors, ui
                   "tgs_adamw: dtype must be 0 (float32), 1 (bfloat16) or 2 (float16), got %d",
                   t.dtype);
     TGS_CHECK_ARG(t.group < n_groups, "tgs_adamw: group %u of %u", t.group, n_groups);
-    TGS_CHECK_ARG(t.n < (1ull << 42), "tgs_adamw: %llu values", (unsigned long long)t.n);
+    TGS_CHECK_ARG(t.n < (1ull << 41), "tgs_adamw: %llu values", (unsigned long long)t.n);
     TGS_CHECK_ARG(t.n == 0 || (t.param && t.grad && t.exp_avg && t.exp_avg_sq &&
                                (state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale))),
                   "tgs_adamw: null pointer in tensor %u", k);

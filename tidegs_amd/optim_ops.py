@@ -30,29 +30,23 @@ _KEYS = {32: ("exp_avg", "exp_avg_sq"),
          8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 _STATES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
 
-# (called through map: half the cost of a method of each tensor)
-_data_ptr, _numel, _contiguous = Tensor.data_ptr, Tensor.numel, Tensor.is_contiguous
-_get_device, _same_size = Tensor.get_device, Tensor.is_same_size
+def _lists():
+    """The module that reads lists of tensors (built with the library)."""
+    N.load()  # (first: its error says how to build both)
+    from . import _tensor_lists
 
-
-def _rows_of(columns: Sequence[Sequence[int]], n: int) -> array.array:
-    """The columns' values row by row.  Few rows go through a list: 2.3 us in place of 4.7 for one,
-    8 in place of 11 for 17; 74 in place of 46 for 200."""
-    k = len(columns)
-    rows = [0] * (k * n) if n < 32 else array.array("Q", bytes(8 * k * n))
-    for i, column in enumerate(columns):
-        rows[i::k] = column if n < 32 else array.array("Q", column)
-    return array.array("Q", rows) if n < 32 else rows
+    return _tensor_lists
 
 
 def _on_one_gpu(tensors: Sequence[Tensor], name: str) -> torch.device:
-    indices = set(map(_get_device, tensors))
-    if len(indices) == 1 and indices != {-1}:
-        return tensors[0].device
     devices = {t.device for t in tensors}
     if len(devices) > 1:
         raise ValueError(f"{name} must be on one device, got {sorted(map(str, devices))}")
-    raise RuntimeError(f"{name} must be GPU tensors (the TideGS HIP kernels have no CPU path)")
+    device = devices.pop()
+    if device.type != "cuda":
+        raise RuntimeError(
+            f"{name} must be GPU tensors (the TideGS HIP kernels have no CPU path)")
+    return device
 
 
 # ---------------------------------------------------------------------------
@@ -70,21 +64,21 @@ def grad_norm(tensors: Iterable[Tensor]) -> Tensor:
     tensors = [tensors] if isinstance(tensors, Tensor) else list(tensors)
     if not tensors:
         raise ValueError("grad_norm needs a tensor at least")
-    n = len(tensors)
-    if not all(map(_contiguous, tensors)):
+    found = _lists().spans(tensors)
+    if found is None:  # not all contiguous, or something is wrong
+        for t in tensors:
+            if t.dtype not in _DTYPES:
+                raise TypeError(f"tensors must be float32, bfloat16 or float16, got {t.dtype}")
+        device = _on_one_gpu(tensors, "tensors")
         tensors = [t if _is_dense(t) else t.contiguous() for t in tensors]
-    types = [t.dtype for t in tensors]
-    for dtype in set(types):
-        if dtype not in _DTYPES:
-            raise TypeError(f"tensors must be float32, bfloat16 or float16, got {dtype}")
-    device = _on_one_gpu(tensors, "tensors")
-    spans = _rows_of((list(map(_data_ptr, tensors)), list(map(_numel, tensors)),
-                      [_DTYPES[dtype] for dtype in types]), n)
+        rows = array.array("Q", itertools.chain.from_iterable(
+            (t.data_ptr(), t.numel(), _DTYPES[t.dtype]) for t in tensors)).tobytes()
+    else:
+        device, rows = tensors[0].device, found[1]
     norm = torch.empty((), dtype=torch.float32, device=device)
-    nbytes = _workspace_size("tgs_grad_norm_workspace_size", n)
+    nbytes = _workspace_size("tgs_grad_norm_workspace_size", len(tensors))
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    N.launch(device, "tgs_grad_norm", n, spans.buffer_info()[0], norm.data_ptr(), ws.data_ptr(),
-            nbytes)
+    N.launch(device, "tgs_grad_norm", len(tensors), rows, norm.data_ptr(), ws.data_ptr(), nbytes)
     return norm
 
 
@@ -168,27 +162,22 @@ class _Call:
             raise ValueError("parameters and states must be dense, in one order of their values")
         return g if g.stride() == p.stride() else torch.empty_like(p).copy_(g)
 
-    def plain(self, params, grads, states) -> bool:
-        """Whether all tensors are what most are: contiguous and of fitting types and sizes,
-        asked for all of them at once (one by one they cost twice as much)."""
-        every = list(itertools.chain(params, grads, *states))
-        indices = set(map(_get_device, every))
-        if len(indices) != 1 or -1 in indices or not all(map(_contiguous, every)):
-            return False
-        types = [p.dtype for p in params]
-        if types != [g.dtype for g in grads] or not _DTYPES.keys() >= set(types):
-            return False
-        for t, dtype in zip(states, _STATES[self.bits] + (torch.float32,) * 2):
-            if {x.dtype for x in t} != {dtype}:
-                return False
-        sizes = list(map(_numel, params))
-        if self.bits == 8:
-            blocks = [(n + _BLOCK - 1) // _BLOCK for n in sizes]
-            if any(list(map(_numel, t)) != blocks or {x.dim() for x in t} != {1}
-                   for t in states[2:]):
-                return False
-        return all(map(_same_size, params, grads)) \
-            and all(list(map(_numel, t)) == sizes for t in states[:2])
+    def checked(self, params, grads, states, numbers, of):
+        """(gradients as they are read, rows of tgs_adamw_tensor) with every tensor checked: what is
+        wrong raises, what is merely not contiguous is taken as ``check`` does."""
+        none = (itertools.repeat(None),) * (4 - len(states))
+        grads = [self.check(*t) for t in zip(params, grads, *states, *none)]
+        _on_one_gpu(params, "parameters")
+        rows, written = array.array("Q"), []
+        for k, p in enumerate(params):
+            at = [t[k].data_ptr() for t in (params, *states)]
+            if p.numel():
+                written += at
+            rows.extend((at[0], grads[k].data_ptr(), *at[1:], *(0,) * (4 - len(states)), p.numel(),
+                         numbers[k] | of[k] << 32, _DTYPES[p.dtype]))
+        if len(set(written)) != len(written):
+            raise ValueError("a parameter or a state is there twice")
+        return grads, rows.tobytes()
 
     def run(self, params, grads, states, numbers, of, seed, norm, max_norm, live=False) -> None:
         """``states``: exp_avgs, exp_avg_sqs and, of 8 bits, both lists of scales; ``of``: the
@@ -196,28 +185,22 @@ class _Call:
         n = len(params)
         if not n:
             return
-        if not self.plain(params, grads, states):
-            none = (itertools.repeat(None),) * (4 - len(states))
-            grads = [self.check(*t) for t in zip(params, grads, *states, *none)]
-        device = _on_one_gpu(params[:1] if n == 1 else params, "parameters")
+        scales = states[2:] or (None, None)
+        found = _lists().adamw(params, grads, *states[:2], *scales, _BLOCK, numbers, of)
+        if found is None:
+            grads, rows = self.checked(params, grads, states, numbers, of)
+        else:
+            rows = found[1]
+        device = params[0].device
         if norm is not None and (norm.numel() != 1 or norm.dtype != torch.float32
                                  or norm.device != device):
             raise ValueError("grad_norm must be one float32 value on the parameters' device")
-        sizes = list(map(_numel, params))
-        columns = [list(map(_data_ptr, t)) for t in (params, grads, *states)]
-        written = [a for k, t in enumerate(columns) if k != 1 for a in t if a]
-        if len(set(written)) != len(written):
-            raise ValueError("a parameter or a state is there twice")
-        if self.bits == 32:
-            columns += [[0] * n] * 2
-        tensors = _rows_of((*columns, sizes, [a | b << 32 for a, b in zip(numbers, of)],
-                            [_DTYPES[p.dtype] for p in params]), n)
         ws, nbytes = None, 0
         if live:
             nbytes = _workspace_size("tgs_adamw_workspace_size", self.n_groups)
             ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        N.launch(device, "tgs_adamw", n, tensors.buffer_info()[0], self.n_groups, self.groups,
-                self.bits, seed, N.ptr(norm), max_norm, N.ptr(ws), nbytes)
+        N.launch(device, "tgs_adamw", n, rows, self.n_groups, self.groups, self.bits, seed,
+                 N.ptr(norm), max_norm, N.ptr(ws), nbytes)
         increment_version(params)
 
 
@@ -301,6 +284,10 @@ class AdamW(torch.optim.Optimizer):
         _check_hyper(0.0, group["betas"], group["eps"], group["weight_decay"])
         super().add_param_group(param_group)
 
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "seed": self.seed,
+                "capturable": self.capturable, "last_norm": None}
+
     def _lr(self, group):
         """(learning rate as a number, as a tensor) of a group, one of them."""
         lr = group["lr"]
@@ -358,6 +345,9 @@ class AdamW(torch.optim.Optimizer):
                     continue
                 if self.capturable and count is None:
                     _on_one_gpu([p], "parameters")
+                    if lr_device is not None and lr_device.device != p.device:
+                        raise ValueError(f"a learning rate is on {lr_device.device}, its "
+                                         f"parameters on {p.device}")
                     count = self._count_of(group, p.device)
                 state = self._state_of(p, count, capturing)
                 key = None if self.capturable else state["step"]
@@ -397,6 +387,9 @@ class AdamW(torch.optim.Optimizer):
                                      f"another state_bits than {self.state_bits}")
                 state = self.state[p]
                 for key in ("exp_avg", "exp_avg_sq"):
+                    if was[key].shape != p.shape:
+                        raise ValueError(f"a saved {key} has shape {tuple(was[key].shape)}, its "
+                                         f"parameter {tuple(p.shape)}")
                     state[key] = torch.empty_like(p, dtype=was[key].dtype,
                                                   memory_format=torch.preserve_format)
                     state[key].copy_(was[key])
