@@ -84,21 +84,23 @@ struct Eight {
   };
   template <bool FULL>
   __device__ __forceinline__ void load(const T* p, uint64_t i, uint64_t n) {
-    if constexpr (FULL) {
+    if (FULL || i + 8 <= n) {
       load_bytes<8 * sizeof(T)>(w, p + i);
     } else {
 #pragma unroll
       for (int k = 0; k < (int)(8 * sizeof(T) / 4); ++k) w[k] = 0;
+      if (i < n) {  // (one lane of a tensor)
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (i + k < n) v[k] = p[i + k];
+        for (int k = 0; k < 8; ++k)
+          if (i + k < n) v[k] = p[i + k];
+      }
     }
   }
   template <bool FULL>
   __device__ __forceinline__ void store(T* p, uint64_t i, uint64_t n) const {
-    if constexpr (FULL) {
+    if (FULL || i + 8 <= n) {
       store_bytes<8 * sizeof(T)>(p + i, w);
-    } else {
+    } else if (i < n) {
 #pragma unroll
       for (int k = 0; k < 8; ++k)
         if (i + k < n) p[i + k] = v[k];
