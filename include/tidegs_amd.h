@@ -828,7 +828,8 @@ int tgs_layer_norm_bwd(uint64_t rows, uint32_t width, int32_t dtype, const void*
  * and of pixels in values.  weight and bias [width] are nullable (1 and 0) and of type
  * weight_dtype: x's or TGS_F32.  eps lies in 2^-80 .. 2^80.
  * stats: where its size is not 0, what the forward leaves for the backward (mean and 1 /
- * sqrt(var + eps) of each sample's group); otherwise nullable, computed again. */
+ * sqrt(var + eps) of each sample's group); otherwise nullable, computed again.
+ * These queries are asked for each size: a larger problem may need less. */
 uint64_t tgs_group_norm_stats_size(uint64_t samples, uint64_t pixels, uint32_t width,
                                    uint32_t groups, int32_t dtype);
 uint64_t tgs_group_norm_fwd_workspace_size(uint64_t samples, uint64_t pixels, uint32_t width,

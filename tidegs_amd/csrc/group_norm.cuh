@@ -19,23 +19,41 @@
 // group, by the workgroups that read x again and write where they are few, by a launch of its
 // own otherwise.  The forward keeps mean and rstd for the backward.
 //
+// Pixels are dealt out to a streaming launch's workgroups a run of rows each in turn, so that all
+// of them read one stretch of memory at a time, and the launch that reads x again begins at its
+// end, which is still cached in part (backward of 4 x 960x540x64 bfloat16: 307 -> 268 us for both).
+// Runs need their elements' alignment only, and where a group or a pixel is no whole number of
+// them the last one overlaps the one before.
+//
 // Sums of squares are of differences from a value near by (a thread's first one, a mean), and
 // partial ones are joined by their means, so no large mean cancels.  All joins are in a fixed
-// order.
+// order.  Sums are taken in 32 bits, those over a whole group's partial values in 64.
+//
+// 1M rows of 64 bfloat16 in 4 groups, held: forward 45 us (5.6 TB/s), backward 77 (5.0 TB/s) and 6
+// for the weights' gradients.  1920x1080x32 bfloat16, silu, streamed: 27 + 7 + 49 us (4.9 and 5.4
+// TB/s, x read twice); 4 x 960x540x64, both directions: 62 + 6 + 91 and 115 + 7 + 139 + 7 us (4.3,
+// 5.8, 4.6 and 5.7 TB/s).  16 x 1020 pixels of 512 halves in 32 groups, held by workgroups: 13
+// and 34 us, of 32-byte pieces of cache lines.
 #pragma once
 
 #include "activation.cuh"
 #include "vector_io.cuh"
 
 #define ACT_NONE 3
-#define HELD_RUNS 8      // runs of a lane at most where the team is a workgroup
-#define HELD_FEW 4       // and in a wavefront (eight took 460 registers in the backward)
+// Groups of up to so many runs a lane are held, of a workgroup's lanes and of a wavefront's (eight
+// took 460 registers in the backward).  16 x 1020 pixels of 512 halves in 32 groups: forward 13 us
+// held and 26 streamed, backward 34 and 32, in one launch less each.
+#define HELD_RUNS 8
+#define HELD_FEW 4
 #define TILE_VECTORS 64  // vectors of channels of a streaming workgroup
-#define JOINED_WIDTH 512     // channels, channels of a group and partial values of a sample that
-#define JOINED_EACH 64       // the workgroups that read them join for themselves, and
+// The workgroups that read partial values join them for themselves up to so many channels,
+// channels of a group, partial values of a sample and values of x, if at least so many workgroups
+// leave them: 3 x 241x137x48 float32, both directions: 120 us a call in five launches, 129 in seven.
+#define JOINED_WIDTH 512
+#define JOINED_EACH 64
 #define JOINED_ENTRIES 4096
-#define JOINED_WORKGROUPS 192  // that leave them
-#define JOINED_BELOW (1u << 24)  // values of x up to which that is done
+#define JOINED_BELOW (1u << 24)
+#define JOINED_WORKGROUPS 192
 
 struct GnCall {
   uint64_t samples, pixels;
@@ -148,106 +166,105 @@ __global__ void __launch_bounds__(256) group_norm_held_kernel(GnCall k, HeldPlan
     b[v] = live ? column<T>(k.bias, k.wide_weights, c0 + v, 0.f) : 0.f;
   }
   with_act(k.act, [&](auto act) {
-  for (uint64_t n = id / k.groups; works && n < k.samples; n += plan.rows) {
-    const T* x = (const T*)k.x + (int64_t)n * k.x_sample + c0;
-    Run<T, V> in[E], grad[BACKWARD ? E : 1];
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const uint32_t p = row + ((uint32_t)e << plan.row_log);
-      const bool ok = live && p < k.pixels;
-      if (ok) in[e].load(x + (int64_t)p * k.x_pitch);
-      if constexpr (BACKWARD)
-        if (ok)
-          grad[e].load((const T*)k.dy + (int64_t)n * k.dy_sample + (int64_t)p * k.dy_pitch + c0);
-    }
-    float xh[E][V], sum = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const bool ok = live && row + ((uint32_t)e << plan.row_log) < k.pixels;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        xh[e][v] = ok ? to_f32(in[e].v[v]) : 0.f;
-        sum += counts(v) ? xh[e][v] : 0.f;
-      }
-    }
-    const float mean = team_sum<WIDE>(sum, team_log) * inv;
-    float squares = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const bool ok = live && row + ((uint32_t)e << plan.row_log) < k.pixels;
-#pragma unroll
-      for (int v = 0; v < V; ++v) {
-        xh[e][v] = ok ? xh[e][v] - mean : 0.f;
-        squares = counts(v) ? fmaf(xh[e][v], xh[e][v], squares) : squares;
-      }
-    }
-    const float rstd = __builtin_amdgcn_rsqf(fmaf(team_sum<WIDE>(squares, team_log), inv, k.eps));
-    T* y = (T*)k.y + (n * k.pixels) * k.width + c0;
-    if constexpr (!BACKWARD) {
+    for (uint64_t n = id / k.groups; works && n < k.samples; n += plan.rows) {
+      const T* x = (const T*)k.x + (int64_t)n * k.x_sample + c0;
+      Run<T, V> in[E], grad[BACKWARD ? E : 1];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const uint32_t p = row + ((uint32_t)e << plan.row_log);
-        if (!live || p >= k.pixels) continue;
-        Run<T, V> out;
-#pragma unroll
-        for (int v = 0; v < V; ++v)
-          out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh[e][v] * rstd, w[v], b[v])));
-        out.store(y + (uint64_t)p * k.width);
+        const bool ok = live && p < k.pixels;
+        if (ok) in[e].load(x + (int64_t)p * k.x_pitch);
+        if constexpr (BACKWARD)
+          if (ok)
+            grad[e].load((const T*)k.dy + (int64_t)n * k.dy_sample + (int64_t)p * k.dy_pitch + c0);
       }
-    } else {
-      // Few runs keep xhat and dz w for the second pass over the team's values; many would take
-      // 128 registers for them (and the kernel 36 us in place of LEAN_US, 16 samples of 1020 pixels
-      // and 512 half channels) and compute them again.
-      constexpr bool KEEP = E <= HELD_FEW / 2;
-      float g[KEEP ? E : 1][V], s1 = 0.f, s2 = 0.f;
-      const auto ok = [&](int e) {
-        return live && row + ((uint32_t)e << plan.row_log) < k.pixels;
-      };
-      const auto both = [&](int e, int v, float& xhat, float& dz) {
-        xhat = (to_f32(in[e].v[v]) - mean) * rstd;
-        dz = to_f32(grad[e].v[v]) * act_slope<act.value, T>(fmaf(xhat, w[v], b[v]));
-      };
+      float xh[E][V], sum = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (!ok(e)) continue;
+        const bool ok = live && row + ((uint32_t)e << plan.row_log) < k.pixels;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          float xhat, dz;
-          both(e, v, xhat, dz);
-          dw[v] = fmaf(dz, xhat, dw[v]);
-          db[v] += dz;
-          dz *= w[v];
-          s1 += counts(v) ? dz : 0.f;
-          s2 = counts(v) ? fmaf(dz, xhat, s2) : s2;
-          if constexpr (KEEP) xh[e][v] = xhat, g[e][v] = dz;
+          xh[e][v] = ok ? to_f32(in[e].v[v]) : 0.f;
+          sum += counts(v) ? xh[e][v] : 0.f;
         }
       }
-      if (!k.y) continue;
-      s1 = team_sum<WIDE>(s1, team_log) * inv;
-      s2 = team_sum<WIDE>(s2, team_log) * inv;
-      if constexpr (!KEEP) {
-#pragma unroll
-        for (int e = 0; e < E; ++e) in[e].forget(), grad[e].forget();
-      }
+      const float mean = team_sum<WIDE>(sum, team_log) * inv;
+      float squares = 0.f;
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (!ok(e)) continue;
-        Run<T, V> out;
+        const bool ok = live && row + ((uint32_t)e << plan.row_log) < k.pixels;
 #pragma unroll
         for (int v = 0; v < V; ++v) {
-          float xhat, dz;
-          if constexpr (KEEP) {
-            xhat = xh[e][v], dz = g[e][v];
-          } else {
+          xh[e][v] = ok ? xh[e][v] - mean : 0.f;
+          squares = counts(v) ? fmaf(xh[e][v], xh[e][v], squares) : squares;
+        }
+      }
+      const float rstd = __builtin_amdgcn_rsqf(fmaf(team_sum<WIDE>(squares, team_log), inv, k.eps));
+      T* y = (T*)k.y + (n * k.pixels) * k.width + c0;
+      if constexpr (!BACKWARD) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const uint32_t p = row + ((uint32_t)e << plan.row_log);
+          if (!live || p >= k.pixels) continue;
+          Run<T, V> out;
+#pragma unroll
+          for (int v = 0; v < V; ++v)
+            out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(xh[e][v] * rstd, w[v], b[v])));
+          out.store(y + (uint64_t)p * k.width);
+        }
+      } else {
+        // Few runs keep xhat and dz w for the second pass over the team's values.  Many compute
+        // them again: kept, the two take 128 registers of eight runs, 460 in all.
+        constexpr bool KEEP = E <= HELD_FEW / 2;
+        float g[KEEP ? E : 1][V], s1 = 0.f, s2 = 0.f;
+        const auto ok = [&](int e) {
+          return live && row + ((uint32_t)e << plan.row_log) < k.pixels;
+        };
+        const auto both = [&](int e, int v, float& xhat, float& dz) {
+          xhat = (to_f32(in[e].v[v]) - mean) * rstd;
+          dz = to_f32(grad[e].v[v]) * act_slope<act.value, T>(fmaf(xhat, w[v], b[v]));
+        };
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (!ok(e)) continue;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float xhat, dz;
             both(e, v, xhat, dz);
+            dw[v] = fmaf(dz, xhat, dw[v]);
+            db[v] += dz;
             dz *= w[v];
+            s1 += counts(v) ? dz : 0.f;
+            s2 = counts(v) ? fmaf(dz, xhat, s2) : s2;
+            if constexpr (KEEP) xh[e][v] = xhat, g[e][v] = dz;
           }
-          out.v[v] = from_f32<T>(rstd * (dz - s1 - xhat * s2));
         }
-        out.store(y + (uint64_t)(row + ((uint32_t)e << plan.row_log)) * k.width);
+        if (!k.y) continue;
+        s1 = team_sum<WIDE>(s1, team_log) * inv;
+        s2 = team_sum<WIDE>(s2, team_log) * inv;
+        if constexpr (!KEEP) {
+#pragma unroll
+          for (int e = 0; e < E; ++e) in[e].forget(), grad[e].forget();
+        }
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          if (!ok(e)) continue;
+          Run<T, V> out;
+#pragma unroll
+          for (int v = 0; v < V; ++v) {
+            float xhat, dz;
+            if constexpr (KEEP) {
+              xhat = xh[e][v], dz = g[e][v];
+            } else {
+              both(e, v, xhat, dz);
+              dz *= w[v];
+            }
+            out.v[v] = from_f32<T>(rstd * (dz - s1 - xhat * s2));
+          }
+          out.store(y + (uint64_t)(row + ((uint32_t)e << plan.row_log)) * k.width);
+        }
       }
     }
-  }
   });
   if constexpr (BACKWARD) {
     if (!partial) return;
@@ -707,7 +724,8 @@ __global__ void __launch_bounds__(256) group_norm_sums_kernel(GnCall k, StreamPl
 #pragma unroll
           for (int v = 0; v < V; ++v) {
             const float d = to_f32(r.v[v]) - col.mean[v];
-            const float dz = to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
+            const float dz =
+                to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
             db[v] += dz;
             dw[v] = fmaf(dz, d, dw[v]);
           }
