@@ -327,6 +327,72 @@ def test_extreme_gradients(gpu):
     assert torch.isinf(t.v[0].float()[:128]).all() and torch.isfinite(t.p[0]).all()
 
 
+@pytest.mark.parametrize("eps", [0.0, 1e-30, 1e-12, 1e-13, 2e-10, 1e-8, 1e20])
+def test_small_and_large_eps(gpu, eps):
+    """Down to gradients whose second moment is no normal float32: there v is off by half its last
+    bit, 2^-150, which is a share r = 2^-150 / v of it, and the move, which goes by 1 / sqrt(v), by up to
+    1 / sqrt(1 - r) - 1 of itself: without bound where r reaches 1, as v is then rounded to 0."""
+    announce(f"adamw_step with eps {eps}")
+    g = torch.Generator().manual_seed(12)
+    grad = torch.randn(3000, generator=g) * 10.0 ** torch.randint(-19, 3, (3000,), generator=g)
+    grad[grad == 0] = 1.0
+    p = torch.randn(3000, generator=g)
+    now, m, v = p.cuda(), torch.zeros(3000, device=gpu), torch.zeros(3000, device=gpu)
+    tg.adamw_step([now], [grad.cuda()], [m], [v], 1, lr=1e-3, eps=eps, weight_decay=0.0)
+    x = grad.double()
+    mm, vv = 0.1 * x, 0.001 * x * x
+    move = 1e-3 / 0.1 * mm / (vv.sqrt() / 0.001 ** 0.5 + eps)
+    # (betas are not exact in float32: each share's rounding, u of 0.9 over 0.1 and of 0.999 over
+    # 0.001, is in both the moments and the corrections that divide by 1 - beta in float64)
+    rest = (1 - 2.0 ** -150 / vv * (1 + 8 * U)).clamp(min=0)
+    far = 3 * U * p.double().abs() + move.abs() * (24 * U + 1 / rest.sqrt() - 1) + 1e-44
+    off = (now.cpu().double() - (p.double() - move)).abs()
+    bad = ~((off <= far) | far.isinf())
+    assert not bad.any(), (off[bad][:4], far[bad][:4])
+    assert far.isfinite().float().mean() > 0.9
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_past_32_bits(gpu, bits):
+    """A tensor of 2^32 values and some: its end as it is in a short one (but for the draws, which go
+    by the index), and the norm of it all."""
+    announce(f"adamw_step of 2^32 values, {bits}")
+    n, k = (1 << 32) + 1000, 1000  # (a whole number of blocks before the end)
+    p = torch.zeros(n, dtype=torch.bfloat16, device=gpu)
+    grad = torch.full((n,), 0.5, dtype=torch.bfloat16, device=gpu)
+    g = torch.Generator(device="cuda").manual_seed(1)
+    p[-k:] = torch.randn(k, generator=g, device=gpu)
+    grad[-k:] = torch.randn(k, generator=g, device=gpu)
+    short = [p[-k:].clone(), grad[-k:].clone()]
+    norm = tg.grad_norm([grad])
+    exact = (0.25 * (n - k) + float(short[1].double().square().sum())) ** 0.5
+    assert abs(float(norm) - exact) <= exact * (U + 1e-12)
+
+    def stepped(p, grad):
+        types = (torch.float32,) * 2 if bits == 32 else F8
+        m, v = (torch.zeros(p.numel(), dtype=t, device=gpu) for t in types)
+        scales = {}
+        if bits == 8:
+            scales = {key: [torch.zeros(-(-p.numel() // BLOCK), device=gpu)]
+                      for key in ("exp_avg_scales", "exp_avg_sq_scales")}
+        tg.adamw_step([p], [grad], [m], [v], 1, lr=1e-2, **scales)
+        return p, m, v, *(t[0] for t in scales.values())
+
+    long, alone = stepped(p, grad), stepped(*short)
+    assert torch.equal(long[1][-k:].float(), alone[1].float())
+    if bits == 32:
+        assert torch.equal(long[2][-k:], alone[2])
+    else:
+        blocks = -(-k // BLOCK)
+        assert torch.equal(long[3][-blocks:], alone[3]) and torch.equal(long[4][-blocks:], alone[4])
+        assert (long[2][-k:].float() - alone[2].float()).abs().le(alone[2].float() / 4).all()
+    off = (long[0][-k:].float() - alone[0].float()).abs()
+    assert (off <= 2.0 ** -7 * alone[0].float().abs() + 1e-6).all()
+    # every other value made the same first step: lr, within a bit of bfloat16
+    for at in (0, (1 << 31) + 5, (1 << 32) - 1):
+        assert abs(float(long[0][at]) + 1e-2) <= 1e-2 * 2.0 ** -7
+
+
 def test_second_moment_follows_its_average(gpu):
     """The mean over many values of an 8-bit second moment is that of the exact one: a single value
     is off by some 25% at random, the mean over 200k of them by 0.06%.  To nearest it would
@@ -586,6 +652,33 @@ def test_captured_steps(gpu, bits):
     assert int(reloaded.state[host[0]]["step"]) == 5
     assert reloaded.state[host[0]]["step"] is reloaded.state[host[1]]["step"]
     assert reloaded.state[host[0]]["step"] is not reloaded.state[host[2]]["step"]
+
+
+def test_two_graphs_and_eager_steps_between(gpu):
+    """Two captured optimizers replayed in turn, with an eager one between them, each as it would be
+    alone."""
+    announce("two captured AdamWs")
+
+    def made(seed):
+        params = _network(gpu, seed)
+        _fill(params, seed)
+        opt = tg.AdamW(params, state_bits=8, seed=seed, capturable=True)
+        opt.step(max_norm=1.0)
+        return params, opt
+
+    captured, alone = [made(k) for k in range(2)], [made(k) for k in range(2)]
+    graphs = []
+    for _, opt in captured:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            opt.step(max_norm=1.0)
+    for order in ((0, 1), (1, 0), (0, 1)):
+        for k in order:
+            graphs[k].replay()
+            alone[1 - k][1].step(max_norm=1.0)  # (eager, between the replays)
+    torch.cuda.synchronize()
+    for (a, _), (b, _) in zip(captured, alone):
+        assert all(torch.equal(p, q) for p, q in zip(a, b))
 
 
 def test_captures_that_are_refused(gpu):

@@ -254,9 +254,9 @@ __device__ __forceinline__ void adamw_eight(const AdamwTensor& t, const AdamwGro
     p[k] = to_f32(p8.v[k]) * decay;
   }
   // The hardware's root and reciprocal are off by one unit, and take what is below 2^-126 for
-  // zero: next to this eps nothing is lost.  (With the exact forms, and conversions and maxima
+  // zero: 2^-63 root at most, 2^-25 of this eps.  (With the exact forms, and conversions and maxima
   // in integer arithmetic, 256M values of bfloat16 with states of 8 bits took 586 us.)
-  if (h.eps >= 0x1p-40f) {
+  if (h.eps >= root * 0x1p-38f) {
 #pragma unroll
     for (int k = 0; k < 8; ++k)
       p[k] -= m[k] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[k]) * root + h.eps) * step_size;

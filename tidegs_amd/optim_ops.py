@@ -30,12 +30,16 @@ _KEYS = {32: ("exp_avg", "exp_avg_sq"),
          8: ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale")}
 _STATES = {32: (torch.float32, torch.float32), 8: (torch.float8_e4m3fn, torch.float8_e5m2)}
 
+_reader = None
+
+
 def _lists():
     """The module that reads lists of tensors (built with the library)."""
-    N.load()  # (first: its error says how to build both)
-    from . import _tensor_lists
-
-    return _tensor_lists
+    global _reader
+    if _reader is None:
+        N.load()  # (first: its error says how to build both)
+        from . import _tensor_lists as _reader
+    return _reader
 
 
 def _on_one_gpu(tensors: Sequence[Tensor], name: str) -> torch.device:
@@ -228,9 +232,11 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     A gradient has its parameter's type.  Without scales the states are float32, of the
     parameters' shapes.  With them (float32, ceil(n / 128) of a parameter of n values, in the
     order of memory) exp_avg is float8_e4m3fn and exp_avg_sq float8_e5m2, to be multiplied by
-    their block's scale; zeros are a start for all four.  Parameters and states are dense
-    and do not overlap; a gradient in another order is copied.  A NaN stays in its value, and an
-    infinity, too: the rest of the block is not touched by it.
+    their block's scale; zeros are a start for all four.  What is rounded stochastically (exp_avg_sq
+    of 8 bits, parameters of 16) draws from ``seed``, the step, a tensor's place in the lists and
+    a value's index.  Parameters and states are dense and do not overlap; a gradient in another
+    order is copied.  A NaN stays in its value, and an infinity, too: the rest of the block is
+    not touched by it.
     """
     bits = 32 if exp_avg_scales is None else 8
     if (exp_avg_scales is None) != (exp_avg_sq_scales is None):
