@@ -202,6 +202,45 @@ def test_gradients_that_are_asked_for(gpu):
             assert torch.equal(torch.autograd.grad(y, one[k], dy)[0], whole[k])
 
 
+def test_once_and_in_reverse_mode(gpu):
+    """A second derivative and a forward tangent raise; a graph kept is used again; a tensor changed in
+    place between is noticed."""
+    announce("group_norm: refused derivatives")
+    x, w, b, dy = _inputs((4, 50, 16, 2), torch.float32, seed=4)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    y = tg.group_norm(leaves[0], 2, leaves[1], leaves[2], activation="silu")
+    first = torch.autograd.grad(y, leaves, dy, retain_graph=True)
+    again = torch.autograd.grad(y, leaves, dy, create_graph=True)
+    assert all(torch.equal(p, q) for p, q in zip(first, again))
+    with pytest.raises(RuntimeError, match="twice"):
+        again[0].sum().backward()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((RuntimeError, NotImplementedError), match="jvp"):
+            tg.group_norm(dual, 2, w, b)
+    y = tg.group_norm(leaves[0], 2, leaves[1], leaves[2])
+    with torch.no_grad():
+        leaves[1].mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(y, leaves, dy)
+
+
+def test_on_another_stream(gpu):
+    """Forward and backward run on the stream that is current in the forward."""
+    announce("group_norm on a stream")
+    x, w, b, dy = _inputs((3, 2000, 32, 4), torch.float32, seed=4)
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(tg.group_norm(leaves[0], 4, leaves[1], leaves[2]), leaves, dy)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        late = leaves[0] * 1.0  # (on this stream: a launch elsewhere would not wait for it)
+        got = torch.autograd.grad(tg.group_norm(late, 4, leaves[1], leaves[2]), leaves, dy)
+    torch.cuda.current_stream().wait_stream(stream)
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+
+
 @pytest.mark.parametrize("shape", [(4, 40, 32, 4), (4, 3000, 32, 4)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_nan_stays_in_its_group(gpu, shape, bad):

@@ -28,8 +28,9 @@ def test_refusals():
 
 def test_pixels_in_place_or_copied():
     """Which layouts are read where they lie, and at what distances."""
-    from tidegs_amd.decoder_ops import _pixels
+    from tidegs_amd.decoder_ops import _group_norm_node
 
+    _pixels = _group_norm_node().pixels
     t = torch.arange(3 * 4 * 5 * 8.0).view(3, 4, 5, 8)
     for x, sample, pitch in (
             (t, 160, 8), (t[..., :6], 160, 8), (t[1:], 160, 8), (t[::2], 320, 8),
@@ -54,6 +55,20 @@ def test_pixels_in_place_or_copied():
               + torch.arange(pixels)[:, None] * p + torch.arange(x.shape[-1]))
         assert torch.equal(flat[at].reshape(x.shape), x)
     assert _pixels(torch.zeros(0, 3, 8))[1:] == (0, 8)
+
+
+def test_node_checks_its_arguments():
+    from tidegs_amd.decoder_ops import _group_norm_node
+
+    node = _group_norm_node()
+    with pytest.raises(TypeError, match="seven"):
+        node.group_norm(torch.zeros(2, 4))
+    with pytest.raises(TypeError, match="a tensor is needed"):
+        node.group_norm(3, None, None, 1, 1e-5, 0, False)
+    with pytest.raises(TypeError):
+        node.group_norm(torch.zeros(2, 4), None, None, "1", 1e-5, 0, False)
+    with pytest.raises(TypeError, match="six"):
+        node.bind(1)
 
 
 def test_entry_points_check_their_arguments():

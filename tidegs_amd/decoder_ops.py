@@ -15,6 +15,7 @@ forward mode or a second derivative raises.
 """
 from __future__ import annotations
 
+import ctypes
 import functools
 import math
 from typing import Optional
@@ -179,68 +180,23 @@ def layer_norm(x: Tensor, weight: Optional[Tensor] = None, bias: Optional[Tensor
 _MIN_EPS, _MAX_EPS = 2.0 ** -80, 2.0 ** 80
 
 
-def _pixels(x: Tensor):
-    """``x`` [samples, ..., width] as samples of pixels: (tensor, distance of samples, distance of
-    pixels), in place where its pixels lie at one pitch."""
-    width = x.shape[-1]
-    if not x.is_contiguous():
-        pitch = inner = 0  # of the pixels, and how many there are in the dimensions so far
-        for size, stride in zip(reversed(x.shape[1:-1]), reversed(x.stride()[1:-1])):
-            if size == 1:
-                continue
-            if not inner:
-                pitch, inner = stride, 1
-            if stride != pitch * inner:
-                pitch = -1
-                break
-            inner *= size
-        if (x.stride(-1) == 1 or width == 1) and (pitch >= width or not inner):
-            return x, x.stride(0), max(pitch, width)
-        x = x.contiguous()
-    return x, x.numel() // x.shape[0] if x.shape[0] else 0, width
+_node = None
 
 
-def _group_norm_fwd(x, groups, weight, bias, eps, act):
-    """(x as it is read, y, what is kept for the backward, the arguments that its call shares)."""
-    x, sample, pitch = _pixels(x)
-    samples, width = x.shape[0], x.shape[-1]
-    pixels = math.prod(x.shape[1:-1])
-    y = x.new_empty(x.shape)
-    code = _DTYPES[x.dtype]
-    w = weight if weight is not None else bias
-    w_code = code if w is None or w.dtype == x.dtype else _DTYPES[w.dtype]
-    sizes = samples, pixels, width, groups, code
-    kept = _workspace_size("tgs_group_norm_stats_size", *sizes)
-    nbytes = _workspace_size("tgs_group_norm_fwd_workspace_size", *sizes)
-    stats = torch.empty(kept, dtype=torch.uint8, device=x.device) if kept else None
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    N.launch(x.device, "tgs_group_norm_fwd", *sizes, act, x.data_ptr(), sample, pitch,
-             N.ptr(weight), N.ptr(bias), w_code, eps, y.data_ptr(), N.ptr(stats), N.ptr(ws), nbytes)
-    return x, y, stats, (sizes, act, sample, pitch, w_code, eps)
+def _group_norm_node():
+    """The module that has group norm's node of the autograd graph (built with the library): both
+    directions of few values take 65 us a call, as a Function in Python they took 107."""
+    global _node
+    if _node is None:
+        lib = N.load()
+        from . import _group_norm_node as node
 
-
-class _GroupNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, groups, weight, bias, eps, act):
-        x, y, stats, ctx.call = _group_norm_fwd(x, groups, weight, bias, eps, act)
-        ctx.save_for_backward(x, weight, bias, stats)
-        return y
-
-    @_once
-    def backward(ctx, dy):
-        x, weight, bias, stats = ctx.saved_tensors
-        sizes, act, sample, pitch, w_code, eps = ctx.call
-        dy, dy_sample, dy_pitch = _pixels(dy)
-        need_x, _, need_w, need_b, _, _ = ctx.needs_input_grad
-        dx = x.new_empty(x.shape) if need_x else None
-        dw = weight.new_empty(weight.shape) if need_w else None
-        db = bias.new_empty(bias.shape) if need_b else None
-        nbytes = _workspace_size("tgs_group_norm_bwd_workspace_size", *sizes)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-        N.launch(x.device, "tgs_group_norm_bwd", *sizes, act, x.data_ptr(), sample, pitch,
-                 dy.data_ptr(), dy_sample, dy_pitch, N.ptr(weight), N.ptr(bias), w_code, eps,
-                 N.ptr(stats), N.ptr(dx), N.ptr(dw), N.ptr(db), ws.data_ptr(), nbytes)
-        return dx, None, dw, db, None, None
+        names = ("last_error", "group_norm_stats_size", "group_norm_fwd_workspace_size",
+                 "group_norm_fwd", "group_norm_bwd_workspace_size", "group_norm_bwd")
+        node.bind(*(ctypes.cast(getattr(lib, "tgs_" + name), ctypes.c_void_p).value
+                    for name in names))
+        _node = node
+    return _node
 
 
 def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
@@ -276,9 +232,8 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
     bias = _parameter(bias, "bias", shape, x, (torch.float32,))
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise TypeError(f"weight is {weight.dtype} and bias {bias.dtype}: one type is needed")
-    if _recorded(x, weight, bias):
-        return _GroupNorm.apply(x, int(num_groups), weight, bias, float(eps), act)
-    return _group_norm_fwd(x, int(num_groups), weight, bias, float(eps), act)[1]
+    return _group_norm_node().group_norm(x, weight, bias, int(num_groups), float(eps), act,
+                                         _recorded(x, weight, bias))
 
 
 # ---------------------------------------------------------------------------
