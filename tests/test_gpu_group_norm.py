@@ -7,6 +7,8 @@ roundings, the activation by at most 1.13 times z's error and 8 u of its value (
 silu's terms), and a result of 16 bits by half its step.  dz takes z's error by the slope's
 slope (at most 0.8), or all of dy where relu's border lies within z's error; the sums over dz take its
 errors' sums and R of their magnitudes."""
+import gc
+
 import pytest
 import torch
 
@@ -329,6 +331,50 @@ def test_captured(gpu, shape):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want)), k
+
+
+def test_captured_beside_a_living_graph(gpu):
+    """Torch would end the process where a captured backward passes a gradient to a leaf of which an
+    eager graph of the default stream lives: the backward raises, the forward does not, and once the
+    graph is gone both are captured."""
+    announce("group_norm: captured beside an eager graph")
+    node = tg.decoder_ops._group_norm_node()
+    x, w, b, dy = _inputs((50, 20, 32, 4), torch.bfloat16, seed=12)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+
+    def call():
+        return tg.group_norm(x, 4, w, b, activation="silu")
+
+    assert not any(map(node.gathered_by_default, leaves))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kept = call()
+    torch.cuda.current_stream().wait_stream(side)
+    assert not any(map(node.gathered_by_default, leaves))
+    del kept
+    kept = call()
+    assert all(map(node.gathered_by_default, leaves))
+    want = [kept.detach(), *torch.autograd.grad(kept, leaves, dy, retain_graph=True)]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="an eager graph of the same tensor lives"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(call(), leaves, dy)
+    forward = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(forward):
+        y = call().detach()
+    del kept
+    gc.collect()  # (the raised error's frames)
+    assert not any(map(node.gathered_by_default, leaves))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+        out = [out.detach(), *torch.autograd.grad(out, leaves, dy)]
+    for k in range(3):
+        forward.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[0]) and all(torch.equal(p, q) for p, q in zip(out, want)), k
 
 
 def test_past_32_bits(gpu):

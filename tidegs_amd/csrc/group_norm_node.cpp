@@ -4,11 +4,13 @@
 // those of the C ABI (include/tidegs_amd.h), whose addresses `bind` is given; arguments have been
 // checked by tidegs_amd.decoder_ops.group_norm.
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 #include "../../include/tidegs_amd.h"
 
@@ -91,6 +93,20 @@ int32_t weight_dtype(const Sizes& sizes, const Tensor& weight, const Tensor& bia
   return w.defined() ? dtype_of(w) : sizes.dtype;
 }
 
+// Whether t is a leaf whose gradients are gathered on the default stream: by the node that an eager
+// graph made there, as long as that graph lives.
+bool gathered_by_default(const Tensor& t) {
+  if (!t.defined() || !t.is_leaf() || !t.requires_grad()) return false;
+  const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
+  const auto stream = node ? node->stream() : std::nullopt;
+  return stream && stream->id() == 0;  // (0: the default stream)
+}
+
+bool capturing(const Tensor& t) {
+  const c10::DeviceGuard guard(t.device());
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+
 // {y, stats or none}
 std::pair<Tensor, Tensor> forward(const Pixels& in, const Tensor& weight, const Tensor& bias,
                                   int64_t groups, double eps, int64_t act) {
@@ -115,7 +131,10 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const Tensor weight = w.value_or(Tensor()), bias = b.value_or(Tensor());
     auto [y, stats] = ::forward(in, weight, bias, groups, eps, act);
     ctx->save_for_backward({in.x, weight, bias, stats});
-    ctx->saved_data["call"] = std::vector<int64_t>{in.sample, in.pitch, groups, act};
+    const bool captured = capturing(x);
+    ctx->saved_data["call"] = std::vector<int64_t>{
+        in.sample, in.pitch, groups, act, captured && gathered_by_default(x),
+        captured && gathered_by_default(weight), captured && gathered_by_default(bias)};
     ctx->saved_data["eps"] = eps;
     return y;
   }
@@ -127,8 +146,13 @@ struct GroupNorm : torch::autograd::Function<GroupNorm> {
     const c10::DeviceGuard guard(x.device());
     const Sizes s(x, call[2]);
     size_t edge = 0;  // (of the tensors that there are)
+    size_t k = 4;
     const auto made = [&](const Tensor& t) {
+      const bool live = call[k++];
       if (!t.defined() || !ctx->needs_input_grad(edge++)) return Tensor();
+      // the default stream cannot wait for a captured one, and torch ends the process over it
+      TORCH_CHECK(!live, "an eager graph of the same tensor lives: release it (and what it computed) "
+                         "before this backward is captured");
       return at::empty(t.sizes(), t.options().memory_format(at::MemoryFormat::Contiguous));
     };
     Tensor dx = made(x), dw = made(weight), db = made(bias);
@@ -206,11 +230,20 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t count) {
   Py_RETURN_NONE;
 }
 
+// gathered_by_default(t) -> bool
+PyObject* gathered(PyObject*, PyObject* arg) {
+  HANDLE_TH_ERRORS
+  return PyBool_FromLong(gathered_by_default(tensor_of(arg)));
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
     {"bind", (PyCFunction)(void (*)(void))bind, METH_FASTCALL, "takes the entry points' addresses"},
     {"group_norm", (PyCFunction)(void (*)(void))group_norm, METH_FASTCALL,
      "group_norm(x, weight, bias, groups, eps, act, recorded) -> y"},
     {"pixels", pixels, METH_O, "(tensor as it is read, distance of samples, of pixels)"},
+    {"gathered_by_default", gathered, METH_O,
+     "whether a leaf's gradients are gathered on the default stream by a graph that lives"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_group_norm_node", nullptr, -1, methods};

@@ -211,7 +211,8 @@ def group_norm(x: Tensor, num_groups: int, weight: Optional[Tensor] = None,
     error function) or "relu".  Differentiable in all three tensors.  Images whose pixels lie at
     one pitch (columns of wider rows) are read in place.  A NaN or an infinity makes its
     sample's group NaN and no other, and so do differences past 1e18, whose squares leave
-    float32.
+    float32.  A backward is captured only while no eager graph of the default stream holds the
+    tensors it gives gradients to: it raises otherwise.
     """
     _dtype(x, "x")
     act = 3 if activation is None else _ACTIVATIONS.get(activation)
