@@ -68,6 +68,7 @@ struct GnCall {
   float eps;
   void* y;   // (dx in the backward)
   float2* stats;  // mean and rstd of each sample's group
+  int32_t once;   // whether y is stored past the caches
 };
 
 // Calls f with the activation as a constant.  The kernels do so around their loops: inside of them
@@ -103,6 +104,20 @@ __device__ __forceinline__ float act_slope(float z) {
 template <typename T>
 __device__ __forceinline__ float column(const void* w, int wide, uint32_t c, float other) {
   return !w ? other : wide ? ((const float*)w)[c] : to_f32(((const T*)w)[c]);
+}
+
+// Stores of a second pass that reads what the first one left in the caches.  Large outputs go past
+// them, measured with y alone and y read by the next kernel (bfloat16, 64 channels, silu, us, plain
+// and past): 64 MB 66, 64 and 85.5, 86; 128 MB 94, 91.5 and 149, 147; 256 MB 187, 155 and 283, 262;
+// 512 MB 355, 325 and 536, 520.  Held groups, read once, lose by it (128 MB: 92, 102 with y read).
+#define ONCE_BYTES (96ull << 20)
+
+template <typename T, int V>
+__device__ __forceinline__ void store(const GnCall& k, const Run<T, V>& run, T* p) {
+  if (k.once)
+    run.store_once(p);
+  else
+    run.store(p);
 }
 
 // Sum over a team: 2^log lanes of a wavefront, or (WIDE) the workgroup.
@@ -696,7 +711,7 @@ __global__ void __launch_bounds__(256) group_norm_apply_kernel(GnCall k, StreamP
           const float d = to_f32(r.v[v]) - col.mean[v];
           out.v[v] = from_f32<T>(act_value<act.value, T>(fmaf(d, col.factor[v], col.b[v])));
         }
-        out.store(y - p * k.width);
+        store(k, out, y - p * k.width);
       });
     });
   }
@@ -808,7 +823,7 @@ __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan
               to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
           out.v[v] = from_f32<T>(fmaf(-d * col.rstd[v], s2[v], fmaf(dz, col.factor[v], -s1[v])));
         }
-        out.store(dx - p * k.width);
+        store(k, out, dx - p * k.width);
       });
     });
   }

@@ -302,7 +302,7 @@ extern "C" int tgs_group_norm_fwd(uint64_t samples, uint64_t pixels, uint32_t wi
   TGS_CHECK_ARG(x_pitch >= (int64_t)width || pixels == 1, "tgs_group_norm_fwd: pitch below width");
   GnCall k = {samples, pixels, width, groups, width / groups, activation,
               weight_dtype != dtype, x, nullptr, x_sample, x_pitch, 0, 0, weight, bias, eps, y,
-              (float2*)stats};
+              (float2*)stats, samples * pixels * width * size_of(dtype) >= ONCE_BYTES};
   HeldPlan held;
   if (gn_held(samples, pixels, width, groups, dtype, held)) {
     k.stats = nullptr;
@@ -347,7 +347,7 @@ extern "C" int tgs_group_norm_bwd(uint64_t samples, uint64_t pixels, uint32_t wi
                 "tgs_group_norm_bwd: the workspace starts on 8 bytes");
   GnCall k = {samples, pixels, width, groups, width / groups, activation,
               weight_dtype != dtype, x, dy, x_sample, x_pitch, dy_sample, dy_pitch, weight, bias,
-              eps, dx, (float2*)stats};
+              eps, dx, (float2*)stats, samples * pixels * width * size_of(dtype) >= ONCE_BYTES};
   const auto join = [&](uint32_t parts, const float* rows) {
     if (!sums) return;
     with_dtype(weight_dtype, "tgs_group_norm_bwd", [&](auto tag) {

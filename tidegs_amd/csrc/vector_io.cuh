@@ -38,6 +38,22 @@ __device__ __forceinline__ void store_bytes(void* p, const void* w) {
     *(uint16_t*)p = *(const uint16_t*)w;
   }
 }
+// The same, for values that nothing reads soon: they do not displace what the caches hold.
+template <int BYTES>
+__device__ __forceinline__ void store_bytes_once(void* p, const void* w) {
+  // (of two stores in an if and its else the compiler would make one, a plain one)
+  asm volatile("");
+  if constexpr (BYTES % 16 == 0) {
+#pragma unroll
+    for (int k = 0; k < BYTES / 16; ++k)
+      __builtin_nontemporal_store(((const u32x4*)w)[k], (u32x4_at1*)p + k);
+  } else if constexpr (BYTES == 8) {
+    __builtin_nontemporal_store(*(const u32x2*)w, (u32x2_at1*)p);
+  } else {
+    store_bytes<BYTES>(p, w);
+  }
+  asm volatile("");
+}
 
 // N values of T in registers.
 template <typename T, int N>
@@ -45,6 +61,9 @@ struct alignas(N * sizeof(T) >= 16 ? 16 : N * sizeof(T)) Run {
   T v[N];
   __device__ __forceinline__ void load(const T* p) { load_bytes<N * sizeof(T)>(v, p); }
   __device__ __forceinline__ void store(T* p) const { store_bytes<N * sizeof(T)>(p, v); }
+  __device__ __forceinline__ void store_once(T* p) const {
+    store_bytes_once<N * sizeof(T)>(p, v);
+  }
   // Makes the compiler take the values for new ones: what was computed from them is computed
   // again rather than kept in registers.
   __device__ __forceinline__ void forget() {
