@@ -109,7 +109,8 @@ __device__ __forceinline__ float column(const void* w, int wide, uint32_t c, flo
 // Stores of a second pass that reads what the first one left in the caches.  Large outputs go past
 // them, measured with y alone and y read by the next kernel (bfloat16, 64 channels, silu, us, plain
 // and past): 64 MB 66, 64 and 85.5, 86; 128 MB 94, 91.5 and 149, 147; 256 MB 187, 155 and 283, 262;
-// 512 MB 355, 325 and 536, 520.  Held groups, read once, lose by it (128 MB: 92, 102 with y read).
+// 512 MB 355, 325 and 536, 520.  Held groups, read once, lose by it (128 MB: 92, 102 with y read),
+// and so does dx (4 x 960x540x64, both directions: 411 past the caches, 399 plain).
 #define ONCE_BYTES (96ull << 20)
 
 template <typename T, int V>
@@ -823,7 +824,7 @@ __global__ void __launch_bounds__(256) group_norm_dx_kernel(GnCall k, StreamPlan
               to_f32(g.v[v]) * act_slope<act.value, T>(fmaf(d, col.factor[v], col.b[v]));
           out.v[v] = from_f32<T>(fmaf(-d * col.rstd[v], s2[v], fmaf(dz, col.factor[v], -s1[v])));
         }
-        store(k, out, dx - p * k.width);
+        out.store(dx - p * k.width);
       });
     });
   }
